@@ -12,7 +12,8 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.path.join(_PKG, "lib", "libexcalibur_b200.so")
 
 EXB_OK, EXB_ERR_BAD_ARG, EXB_ERR_UNSUPPORTED, EXB_ERR_CUDA, EXB_ERR_TIMEOUT, EXB_ERR_NOMEM = 0, -1, -2, -3, -4, -5
-EXB_F16, EXB_I8, EXB_F32, EXB_I32 = 0, 1, 2, 3
+EXB_F16, EXB_I8, EXB_F32, EXB_I32, EXB_BF16, EXB_E4M3 = 0, 1, 2, 3, 4, 5
+NORM_RMS, NORM_LAYER = 0, 1
 ACT_NONE, ACT_RELU, ACT_RELU6_QUIRK, ACT_SIGMOID, ACT_MISH, ACT_RELU6, ACT_SILU, ACT_HARDSWISH, ACT_PRELU = 0, 1, 3, 4, 5, 103, 104, 105, 106
 
 EXPORTED_SYMBOLS = [
@@ -24,6 +25,7 @@ EXPORTED_SYMBOLS = [
     "exb_binaryop_scalar_fwd", "exb_relu_fwd", "exb_activation_fwd", "exb_quantize_fwd",
     "exb_dequantize_fwd", "exb_concat_fwd", "exb_concat_nearest_fwd", "exb_interp_nearest_fwd", "exb_channel_affine_fwd",
     "exb_conv_weights_set_slopes", "exb_dw_weights_set_slopes", "exb_depth_to_space_nchw_f32", "exb_deconv_few_f32", "exb_image_f32_to_nhwc_norm", "exb_nchw_f32_to_nhwc4_padded_norm", "exb_nhwc_f16_split_heads_f32", "exb_hardsigmoid_fwd", "exb_softmax_channels_f32", "exb_binaryop_channel_bcast_fwd", "exb_nchw_f16_to_nhwc4_padded", "exb_nchw_f32_focus_to_nhwc_f16", "exb_channel_affine_prelu_fwd", "exb_hardswish_fwd", "exb_focus_fwd", "exb_prelu_fwd", "exb_depth_to_space_fwd", "exb_transpose_hw_f32",
+    "exb_quantize_blocks_fwd", "exb_fp8_matmul_fwd", "exb_residual_norm_fwd", "exb_token_logprobs_fwd",
 ]
 
 
@@ -47,6 +49,12 @@ class PoolDesc(C.Structure):
         "N", "H", "W", "C", "c_stride", "type", "kh", "kw", "stride_h", "stride_w", "pad_t", "pad_b",
         "pad_l", "pad_r", "global_pool", "pad_mode", "count_include_pad", "dtype", "out2_dtype")] + \
         [("out2_scale", C.c_float)]
+
+
+class NormDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64)] + [(n, C.c_int32) for n in ("C", "dtype", "out_dtype", "kind")] + \
+        [("eps", C.c_float), ("residual_scale", C.c_float)] + \
+        [(n, C.c_int64) for n in ("gate_rows", "h_stride", "x_stride", "gate_stride", "r_stride", "n_stride", "scale_stride")]
 
 
 class ExbError(RuntimeError):
@@ -121,6 +129,10 @@ def lib():
         L.exb_prelu_fwd.argtypes = [vp, vp, vp, vp, i32, i64, i32, i32, i64, i32, i32, vp]
         L.exb_depth_to_space_fwd.argtypes = [vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, vp]
         L.exb_transpose_hw_f32.argtypes = [vp, vp, vp, i64, i32, i32, vp]
+        L.exb_quantize_blocks_fwd.argtypes = [vp, vp, i32, i64, vp, i64, vp, i64, i64, i32, i32, vp]
+        L.exb_fp8_matmul_fwd.argtypes = [vp, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, i32, i64, i64, i32, i32, vp]
+        L.exb_residual_norm_fwd.argtypes = [vp, C.POINTER(NormDesc)] + [vp] * 11
+        L.exb_token_logprobs_fwd.argtypes = [vp, vp, i32, i64, i64, i32, f32, vp, i32, vp, vp, i32, vp, vp, vp]
         _LIB = L
     return _LIB
 
@@ -145,7 +157,8 @@ def _torch():
     global _TORCH
     if _TORCH is None:
         import torch
-        _DTYPES.update({EXB_F16: torch.float16, EXB_I8: torch.int8, EXB_F32: torch.float32, EXB_I32: torch.int32})
+        _DTYPES.update({EXB_F16: torch.float16, EXB_I8: torch.int8, EXB_F32: torch.float32, EXB_I32: torch.int32,
+                        EXB_BF16: torch.bfloat16, EXB_E4M3: torch.float8_e4m3fn})
         _DTYPES.update({v: k for k, v in list(_DTYPES.items())})
         _TORCH = torch
     return _TORCH
@@ -157,8 +170,9 @@ def torch_dtype(dt):
 
 
 def exb_dtype_of(tensor):
+    """The library's type of a tensor, or of a torch type."""
     _torch()
-    return _DTYPES[tensor.dtype]
+    return _DTYPES[getattr(tensor, "dtype", tensor)]
 
 
 def ptr(t):
@@ -670,3 +684,161 @@ def nhwc_to_nchw_f32(ctx, x, Cc=None, scale=1.0, y=None):
     check(lib().exb_nhwc_to_nchw_f32(ctx.handle, ptr(x), exb_dtype_of(x), ptr(y), N, Cc, H, W, cs, float(scale),
                                      cur_stream()))
     return y
+
+
+# ---- operators behind a decoder ------------------------------------------------------------------
+# Matrices are (rows, channels) with channels innermost; rows may be apart.  The library is told addresses and strides only, so
+# shapes, types and devices are checked here.
+
+def _need(cond, what):
+    if not cond:
+        raise ExbError(EXB_ERR_BAD_ARG, what)
+
+
+def _matrix(ctx, t, what, dtype=None, shape=None):
+    """Row stride of a (rows, channels) tensor on the context's device."""
+    _need(t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1), "%s has to be (rows, channels), channels innermost" % what)
+    _need(t.get_device() == ctx.device, "%s is not on the context's device" % what)
+    _need(dtype is None or t.dtype == dtype, "%s has to be %s" % (what, dtype))
+    _need(shape is None or t.shape == shape, "%s has to be %s" % (what, shape))
+    return t.stride(0) if t.shape[0] > 1 and t.shape[1] > 0 else max(t.shape[1], t.stride(0))
+
+
+def _parameter(ctx, t, n, what):
+    _need(t is None or (t.dtype == _TORCH.float32 and t.dim() == 1 and t.shape[0] == n and t.get_device() == ctx.device and t.is_contiguous()),
+          "%s has to be %d float32 on the context's device" % (what, n))
+
+
+def _e4m3_rows(like, rows, channels):
+    """Room for (rows, channels) of e4m3 whose rows start at multiples of 16 bytes."""
+    q = like.new_empty((rows, (channels + 15) // 16 * 16), dtype=_TORCH.float8_e4m3fn)
+    return q if channels % 16 == 0 else q[:, :channels]
+
+
+def _row_pitch(q, what):
+    _need(q.shape[0] <= 1 or q.stride(0) % 16 == 0, "rows of %s have to start at multiples of 16 bytes" % what)
+    return q.stride(0) if q.shape[0] > 1 else max(q.stride(0), (q.shape[1] + 15) // 16 * 16) // 16 * 16
+
+
+def quantize_blocks(ctx, x, block_rows=1, q=None, scales=None):
+    """(q, scales): x in e4m3 with a scale for each block_rows x 128 of it.  block_rows 1 (activations): scales are
+    (ceil(channels / 128), rows); 128 (weights): (ceil(rows / 128), ceil(channels / 128)).  q's rows start at multiples of 16 bytes."""
+    t = _torch()
+    xs = _matrix(ctx, x, "x")
+    rows, channels = x.shape
+    _need(block_rows in (1, 128), "block_rows has to be 1 or 128")
+    _need(x.dtype in _DTYPES, "x has a type that the library does not have")
+    blocks = (channels + 127) // 128
+    shape = (blocks, rows) if block_rows == 1 else ((rows + 127) // 128, blocks)
+    if q is None:
+        q = _e4m3_rows(x, rows, channels)
+    else:
+        _matrix(ctx, q, "q", t.float8_e4m3fn, x.shape)
+    if scales is None:
+        scales = x.new_empty(shape, dtype=t.float32)
+        ss = shape[1]
+    else:
+        ss = _matrix(ctx, scales, "scales", t.float32, shape)
+    rc = lib().exb_quantize_blocks_fwd(ctx._h, x.data_ptr(), _DTYPES[x.dtype], xs, q.data_ptr(), _row_pitch(q, "q"), scales.data_ptr(), ss, rows, channels,
+                                       block_rows, _stream())
+    if rc:
+        check(rc)
+    return q, scales
+
+
+def fp8_matmul(ctx, a, a_scales, w, w_scales, bias=None, out_dtype=EXB_F16, y=None):
+    """y (M, N) = a (M, K) @ w (N, K)^T (+ bias) of e4m3 matrices with the scales of quantize_blocks (a: single rows, w: 128 x 128)."""
+    t = _torch()
+    _matrix(ctx, a, "a", t.float8_e4m3fn)
+    _matrix(ctx, w, "w", t.float8_e4m3fn)
+    M, K = a.shape
+    N = w.shape[0]
+    _need(w.shape[1] == K, "a and w have %d and %d columns" % (K, w.shape[1]))
+    blocks = (K + 127) // 128
+    sa = _matrix(ctx, a_scales, "a_scales", t.float32, (blocks, M))
+    sw = _matrix(ctx, w_scales, "w_scales", t.float32, ((N + 127) // 128, blocks))
+    _parameter(ctx, bias, N, "bias")
+    if y is None:
+        y = a.new_empty((M, N), dtype=_DTYPES[out_dtype])
+        ys = N
+    else:
+        ys = _matrix(ctx, y, "y", _DTYPES[out_dtype], (M, N))
+    rc = lib().exb_fp8_matmul_fwd(ctx._h, a.data_ptr(), _row_pitch(a, "a"), a_scales.data_ptr(), sa, w.data_ptr(), _row_pitch(w, "w"), w_scales.data_ptr(),
+                                  sw, _address(bias), y.data_ptr(), out_dtype, ys, M, N, K, _stream())
+    if rc:
+        check(rc)
+    return y
+
+
+def residual_norm(ctx, h, x=None, post_weight=None, post_bias=None, gate=None, gate_rows=0, residual_scale=1.0, weight=None, bias=None,
+                  kind=NORM_RMS, eps=1e-5, quantized=False, r=None, n=None):
+    """r = x + residual_scale * gate * norm(h; post), n = norm(r; weight).  gate: (1, C), all rows alike (gate_rows 0), or a row for each
+    gate_rows rows.  Returns (r, n), or with quantized (r, q, scales) as quantize_blocks gives them; without a weight n is None."""
+    t = _torch()
+    dtype, shape = h.dtype, h.shape
+    hs = _matrix(ctx, h, "h")
+    _need(dtype in _DTYPES, "h has a type that the library does not have")
+    rows, Cc = shape
+    xs = gs = ns = ss = 0
+    if x is not None:
+        xs = _matrix(ctx, x, "x", dtype, shape)
+    if gate is not None:
+        need = -(-rows // gate_rows) if gate_rows > 0 else 1
+        gs = _matrix(ctx, gate, "gate", dtype)
+        _need(gate.shape[1] == Cc and gate.shape[0] >= need, "gate has to be (%d, %d)" % (need, Cc))
+    for p, what in ((post_weight, "post_weight"), (post_bias, "post_bias"), (weight, "weight"), (bias, "bias")):
+        if p is not None:
+            _parameter(ctx, p, Cc, what)
+    if r is None:
+        r = h.new_empty(shape)
+        rs = Cc
+    else:
+        rs = _matrix(ctx, r, "r", dtype, shape)
+    scales = None
+    if weight is not None:
+        if quantized:
+            if n is None:
+                n = _e4m3_rows(h, rows, Cc)
+            else:
+                _matrix(ctx, n, "n", t.float8_e4m3fn, shape)
+            ns, ss = _row_pitch(n, "n"), rows
+            scales = h.new_empty(((Cc + 127) // 128, rows), dtype=t.float32)
+        elif n is None:
+            n = h.new_empty(shape)
+            ns = Cc
+        else:
+            ns = _matrix(ctx, n, "n", dtype, shape)
+    else:
+        _need(n is None, "n without a weight")
+    dt = _DTYPES[dtype]
+    d = NormDesc(rows, Cc, dt, EXB_E4M3 if quantized else dt, kind, eps, residual_scale, gate_rows, hs, xs, gs, rs, ns, ss)
+    rc = lib().exb_residual_norm_fwd(ctx._h, C.byref(d), h.data_ptr(), _address(x), _address(post_weight), _address(post_bias), _address(gate),
+                                     _address(weight), _address(bias), r.data_ptr(), _address(n), _address(scales), _stream())
+    if rc:
+        check(rc)
+    return (r, n, scales) if quantized else (r, n)
+
+
+def token_logprobs(ctx, logits, tokens=None, top=0, scale=1.0):
+    """(logprobs, entropy, top_logprobs, top_tokens) of rows of logits: log probabilities of tokens (rows, given) int32, the
+    entropy (rows,), and the `top` most probable tokens with theirs (rows, top); None where nothing was asked for."""
+    t = _torch()
+    ls = _matrix(ctx, logits, "logits")
+    _need(logits.dtype in _DTYPES, "logits have a type that the library does not have")
+    rows, V = logits.shape
+    given = 0
+    lp = top_lp = top_tokens = None
+    if tokens is not None:
+        _matrix(ctx, tokens, "tokens", t.int32)
+        given = tokens.shape[1]
+        _need(tokens.shape[0] == rows and tokens.is_contiguous(), "tokens have to be (%d, given), contiguous" % rows)
+        lp = logits.new_empty((rows, given), dtype=t.float32)
+    entropy = logits.new_empty((rows,), dtype=t.float32)
+    if top > 0:
+        top_lp = logits.new_empty((rows, top), dtype=t.float32)
+        top_tokens = logits.new_empty((rows, top), dtype=t.int32)
+    rc = lib().exb_token_logprobs_fwd(ctx._h, logits.data_ptr(), _DTYPES[logits.dtype], ls, rows, V, scale, _address(tokens) if given else None, given,
+                                      _address(lp), entropy.data_ptr(), top, _address(top_lp), _address(top_tokens), _stream())
+    if rc:
+        check(rc)
+    return lp, entropy, top_lp, top_tokens

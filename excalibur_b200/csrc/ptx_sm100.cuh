@@ -397,6 +397,34 @@ __device__ __forceinline__ void tc_mma_ab(uint32_t d_tmem, uint32_t a_lo, uint32
     }
 }
 
+// The same for 8-bit floating point operands (kind::f8f6f4, the formats of the instruction descriptor: make_idesc(false, ..)
+// says e4m3 x e4m3 -> fp32), 32 bytes of K each, by one CTA or for a pair.
+template <bool kPair>
+__device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc, uint32_t accumulate,
+                                          uint32_t leader = 1u) {
+    if (kPair) {
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+            "mov.b64 da, {%1, %3};\n\t"
+            "mov.b64 db, {%2, %3};\n\t"
+            "setp.ne.b32 p, %5, 0;\n\t"
+            "setp.ne.b32 q, %6, 0;\n\t"
+            "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %4, p;\n\t}" ::"r"(d_tmem),
+            "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate), "r"(leader)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+            "mov.b64 da, {%1, %3};\n\t"
+            "mov.b64 db, {%2, %3};\n\t"
+            "setp.ne.b32 p, %5, 0;\n\t"
+            "setp.ne.b32 q, %6, 0;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %4, p;\n\t}" ::"r"(d_tmem),
+            "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate), "r"(leader)
+            : "memory");
+    }
+}
+
 // ---- TMA (tiled mode, destination in this CTA's shared memory, no multicast) -----------
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");

@@ -1,0 +1,219 @@
+// A block's result joins the residual stream and the next block's norm is taken of the sum, in one pass:
+//   u = norm(h) * post + post_bias,  r = x + residual_scale * gate * u,  n = norm(r) * weight + bias
+// A row stays in its threads' registers in fp32 from the loads of h, x and the gate to the stores of r and n (in the
+// activations' type, or as e4m3 with a scale for each 128 channels), so that every tensor crosses memory once; the sums of
+// the norms are the only thing its warps exchange.  Bound by memory with many rows, by the chain of loads, reductions and
+// stores with few.
+#include "rows_common.cuh"
+
+#include <type_traits>
+
+namespace exb {
+namespace {
+
+using namespace rows;
+
+struct NormArgs {
+    const void *h, *x, *gate;
+    const float *post_weight, *post_bias, *weight, *bias;
+    void *r, *n;
+    float* n_scales;
+    int64_t rows, gate_rows;
+    int64_t h_stride, x_stride, gate_stride, r_stride, n_stride, scale_stride;
+    int C, quantized;
+    float eps, residual_scale;
+};
+
+constexpr int kShare = 256;      // elements of a row that a warp holds at a time, 8 in each lane
+
+// Sum over the row's threads: its warp's lanes, then (through shared memory, in the same order everywhere) its warps.  The two
+// halves of s_sum take turns, so that one barrier is enough.
+template <bool kOneWarp>
+__device__ __forceinline__ float row_sum(float v, float (*s_sum)[32], int& turn) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (!kOneWarp) {
+        const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+        if (lane == 0) s_sum[turn][threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = lane < warps ? s_sum[turn][lane] : 0.f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        turn ^= 1;
+    }
+    return v;
+}
+
+// v = norm(v) * weight + bias over the row
+template <bool kLayer, bool kVec, bool kOneWarp, int kPer>
+__device__ __forceinline__ void normalise(float (&v)[kPer][8], int lane, int share0, int share_step, const NormArgs& a, const float* weight,
+                                          const float* bias, float (*s_sum)[32], int& turn) {
+    const float inv_c = 1.f / (float)a.C;
+    if constexpr (kLayer) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += v[i][j];
+        const float mean = row_sum<kOneWarp>(s, s_sum, turn) * inv_c;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {      // (what lies behind the row's end stays 0)
+            const int valid = a.C - (share0 + i * share_step) * kShare;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = (kVec ? lane * 8 : j * 32 + lane) < valid ? v[i][j] - mean : 0.f;
+        }
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fmaf(v[i][j], v[i][j], s);
+    const float k = rsqrtf(row_sum<kOneWarp>(s, s_sum, turn) * inv_c + a.eps);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int c0 = (share0 + i * share_step) * kShare, valid = a.C - c0;
+        float w[8];
+        load8<float, kVec>(weight + c0, valid, lane, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * k * w[j];
+        if (bias) {
+            load8<float, kVec>(bias + c0, valid, lane, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] += w[j];
+        }
+    }
+}
+
+// kOneWarp: every warp of the CTA has a row of its own; otherwise the CTA has one.  kPer: shares per warp.
+constexpr int max_threads(bool one_warp, int per) { return one_warp ? 256 : per == 1 ? 1024 : 512; }
+
+template <typename T, bool kLayer, bool kVec, bool kOneWarp, int kPer>
+__global__ void __launch_bounds__(max_threads(kOneWarp, kPer)) residual_norm_kernel(const __grid_constant__ NormArgs a) {
+    __shared__ float s_sum[2][32];
+    pdl_enter();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = kOneWarp ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x;
+    if (kOneWarp && row >= a.rows) return;
+    const int share0 = kOneWarp ? 0 : warp, share_step = kOneWarp ? 1 : (int)(blockDim.x >> 5);
+    int turn = 0;
+    const T* h = static_cast<const T*>(a.h) + row * a.h_stride;
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* g = static_cast<const T*>(a.gate) + (a.gate_rows ? row / a.gate_rows : 0) * a.gate_stride;
+    // everything is asked for before anything is waited for, as long as there are registers for it
+    constexpr bool kAhead = kPer <= 4;
+    float v[kPer][8], xv[kAhead ? kPer : 1][8], gv[kAhead ? kPer : 1][8];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int c0 = (share0 + i * share_step) * kShare, valid = a.C - c0;
+        load8<T, kVec>(h + c0, valid, lane, v[i]);
+        if (kAhead && a.x) load8<T, kVec>(x + c0, valid, lane, xv[kAhead ? i : 0]);
+        if (kAhead && a.gate) load8<T, kVec>(g + c0, valid, lane, gv[kAhead ? i : 0]);
+    }
+    if (a.post_weight) normalise<kLayer, kVec, kOneWarp, kPer>(v, lane, share0, share_step, a, a.post_weight, a.post_bias, s_sum, turn);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int c0 = (share0 + i * share_step) * kShare, valid = a.C - c0;
+        constexpr int kAll = kAhead ? 1 : 0;
+        if (!kAhead && a.x) load8<T, kVec>(x + c0, valid, lane, xv[0]);
+        if (!kAhead && a.gate) load8<T, kVec>(g + c0, valid, lane, gv[0]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (a.gate) v[i][j] *= gv[i * kAll][j];
+            v[i][j] = a.x ? fmaf(a.residual_scale, v[i][j], xv[i * kAll][j]) : a.residual_scale * v[i][j];
+        }
+        if (a.r) store8<T, kVec>(static_cast<T*>(a.r) + row * a.r_stride + c0, valid, lane, v[i]);
+    }
+    if (!a.n) return;
+    normalise<kLayer, kVec, kOneWarp, kPer>(v, lane, share0, share_step, a, a.weight, a.bias, s_sum, turn);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int share = share0 + i * share_step, c0 = share * kShare, valid = a.C - c0;
+        if (a.quantized)
+            quantize8<kVec>(v[i], valid, lane, static_cast<uint8_t*>(a.n) + row * a.n_stride + c0, a.n_scales + 2 * share * a.scale_stride + row, a.scale_stride);
+        else
+            store8<T, kVec>(static_cast<T*>(a.n) + row * a.n_stride + c0, valid, lane, v[i]);
+    }
+}
+
+template <typename T, bool kLayer, bool kVec>
+int launch(const exb_ctx* ctx, const NormArgs& a, cudaStream_t st) {
+    const int shares = (a.C + kShare - 1) / kShare;
+    auto go = [&](auto one, auto per) {
+        constexpr bool kOne = decltype(one)::value;
+        constexpr int kPer = decltype(per)::value;
+        const int warps = kOne ? 8 : (shares + kPer - 1) / kPer;
+        const int64_t grid = kOne ? (a.rows + warps - 1) / warps : a.rows;
+        launch_overlapped(ctx, residual_norm_kernel<T, kLayer, kVec, kOne, kPer>, dim3((unsigned)grid), dim3(32 * warps), st, a);
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    const bool many = a.rows > 2 * ctx->sm_count;
+    if (shares == 1) go(Yes(), std::integral_constant<int, 1>());
+    else if (shares == 2 && many) go(Yes(), std::integral_constant<int, 2>());
+    else if (shares <= (many ? 4 : 32)) go(No(), std::integral_constant<int, 1>());
+    else if (shares <= 32) go(No(), std::integral_constant<int, 2>());
+    else if (shares <= 64) go(No(), std::integral_constant<int, 4>());
+    else go(No(), std::integral_constant<int, 8>());
+    return after_launch("exb_residual_norm_fwd");
+}
+
+}  // namespace
+}  // namespace exb
+
+using namespace exb;
+
+extern "C" int exb_residual_norm_fwd(exb_ctx* ctx, const exb_norm_desc* d, const void* h, const void* x, const float* post_weight,
+                                     const float* post_bias, const void* gate, const float* weight, const float* bias, void* r, void* n,
+                                     float* n_scales, void* stream) {
+    EXB_REQUIRE(ctx != nullptr && d != nullptr, "exb_residual_norm_fwd: null context or descriptor");
+    const size_t es = rows::element_size(d->dtype);
+    EXB_REQUIRE(es != 0, "exb_residual_norm_fwd: dtype must be EXB_F16, EXB_BF16 or EXB_F32, got %d", d->dtype);
+    const bool quantized = d->out_dtype == EXB_E4M3;
+    EXB_REQUIRE(quantized || d->out_dtype == d->dtype, "exb_residual_norm_fwd: the norm is written in dtype or as EXB_E4M3, got %d", d->out_dtype);
+    EXB_REQUIRE(d->kind == EXB_NORM_RMS || d->kind == EXB_NORM_LAYER, "exb_residual_norm_fwd: norm %d is not known", d->kind);
+    EXB_REQUIRE(d->rows >= 0 && d->C >= 1, "exb_residual_norm_fwd: bad shape (%lld rows of %d)", (long long)d->rows, d->C);
+    EXB_REQUIRE(d->eps >= 0.f, "exb_residual_norm_fwd: eps must not be negative");
+    if (d->C > 32768 || d->rows > INT32_MAX)
+        return fail(EXB_ERR_UNSUPPORTED, "exb_residual_norm_fwd: at most 32768 channels and 2^31 - 1 rows, got %lld rows of %d", (long long)d->rows, d->C);
+    if (d->rows == 0) return EXB_OK;
+    EXB_REQUIRE(h && (r || n), "exb_residual_norm_fwd: null buffer");
+    EXB_REQUIRE(!n || weight, "exb_residual_norm_fwd: the norm has no weight");
+    EXB_REQUIRE(!post_bias || post_weight, "exb_residual_norm_fwd: a bias without its norm's weight");
+    EXB_REQUIRE(d->gate_rows >= 0, "exb_residual_norm_fwd: gate_rows must not be negative");
+    EXB_REQUIRE(d->h_stride >= d->C && (!x || d->x_stride >= d->C) && (!r || d->r_stride >= d->C) && (!n || d->n_stride >= d->C),
+                "exb_residual_norm_fwd: row strides smaller than the rows");
+    EXB_REQUIRE(!gate || d->gate_rows == 0 || d->gate_stride >= d->C, "exb_residual_norm_fwd: row stride of the gate smaller than its rows");
+    for (const void* p : {h, x, gate, static_cast<const void*>(r), static_cast<const void*>(quantized ? nullptr : n)})
+        EXB_REQUIRE(rows::aligned_to(p, es), "exb_residual_norm_fwd: a tensor is not aligned to its element");
+    for (const float* p : {post_weight, post_bias, weight, bias, static_cast<const float*>(n_scales)})
+        EXB_REQUIRE(rows::aligned_to(p, 4), "exb_residual_norm_fwd: a parameter is not aligned to its element");
+    if (n && quantized) {
+        EXB_REQUIRE(n_scales && d->scale_stride >= d->rows, "exb_residual_norm_fwd: null n_scales, or a scale stride smaller than the rows");
+        EXB_REQUIRE(aligned16(n) && d->n_stride % 16 == 0, "exb_residual_norm_fwd: e4m3 rows must start at multiples of 16 bytes");
+        EXB_REQUIRE(n != h && n != x, "exb_residual_norm_fwd: e4m3 rows cannot take the input's place");
+    }
+    EXB_REQUIRE(!r || r != n, "exb_residual_norm_fwd: r and n are the same buffer");
+    EXB_REQUIRE((r != h || d->r_stride == d->h_stride) && (!x || r != x || d->r_stride == d->x_stride) && (n != h || d->n_stride == d->h_stride) &&
+                    (!x || n != x || d->n_stride == d->x_stride),
+                "exb_residual_norm_fwd: a result in an input's place needs its stride");
+    NormArgs a;
+    a.h = h; a.x = x; a.gate = gate;
+    a.post_weight = post_weight; a.post_bias = post_bias; a.weight = weight; a.bias = bias;
+    a.r = r; a.n = n; a.n_scales = n_scales;
+    a.rows = d->rows; a.gate_rows = d->gate_rows;
+    a.h_stride = d->h_stride; a.x_stride = d->x_stride; a.gate_stride = d->gate_rows ? d->gate_stride : 0;
+    a.r_stride = d->r_stride; a.n_stride = d->n_stride; a.scale_stride = d->scale_stride;
+    a.C = d->C; a.quantized = quantized;
+    a.eps = d->eps; a.residual_scale = d->residual_scale;
+    bool vec = d->C % 8 == 0 && rows::vector_rows(h, d->h_stride, es) && rows::vector_rows(x, d->x_stride, es) &&
+               rows::vector_rows(gate, a.gate_stride, es) && rows::vector_rows(r, d->r_stride, es) && (quantized || rows::vector_rows(n, d->n_stride, es));
+    for (const float* p : {post_weight, post_bias, weight, bias}) vec = vec && aligned16(p);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int rc = EXB_OK;
+    rows::with_type(d->dtype, [&](auto t) {
+        using T = decltype(t);
+        if (d->kind == EXB_NORM_LAYER) rc = vec ? launch<T, true, true>(ctx, a, st) : launch<T, true, false>(ctx, a, st);
+        else rc = vec ? launch<T, false, true>(ctx, a, st) : launch<T, false, false>(ctx, a, st);
+    });
+    return rc;
+}

@@ -40,7 +40,9 @@ typedef enum exb_dtype {
     EXB_F16 = 0,  /* IEEE half, the reference's `unsigned short` tensors */
     EXB_I8 = 1,   /* signed char */
     EXB_F32 = 2,
-    EXB_I32 = 3   /* raw int32 accumulators (parity / debugging output of the int8 conv) */
+    EXB_I32 = 3,  /* raw int32 accumulators (parity / debugging output of the int8 conv) */
+    EXB_BF16 = 4, /* bfloat16: the operators behind a decoder only */
+    EXB_E4M3 = 5  /* 8-bit floating point, 4 exponent and 3 mantissa bits, largest value 448: the same */
 } exb_dtype;
 
 /* 0..5: conv key 9 of the reference (src/Excalibur/operation_general_conv.cpp:127-272);
@@ -468,6 +470,75 @@ EXB_API int exb_channel_affine_fwd(exb_ctx* ctx, const void* x, void* y, const f
                                    const float* add, int64_t outer, int C, int c_stride,
                                    int64_t inner, int dtype, int channel_last, int act,
                                    void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Operators behind a decoder: what turns its last hidden states into scores of tokens.  The reference has no counterpart;
+ * they follow the framework's tails (InnerProduct, Softmax) where the classes are a vocabulary's tokens.  Activations are
+ * [rows][C] with C innermost and a row stride in elements, in EXB_F16, EXB_BF16 or EXB_F32; parameters are fp32 device
+ * arrays; sums, norms and statistics are held in fp32.  All pointers are device pointers, aligned to their element unless
+ * said otherwise; 16-byte aligned rows (base and stride) are read in vectors.  rows == 0 does nothing.
+ *
+ * exb_quantize_blocks_fwd: 8-bit floating point with a scale for each block of block_rows x 128 elements, block_rows 1
+ * (activations) or 128 (weights):
+ *   scale = max(max |x| / 448, 2^-126), q = e4m3(x * (1 / scale)) (round to nearest even, saturating)
+ * so that q * scale stands for x.  A block's last columns and rows may be missing.  A NaN stays one in q; an infinity makes
+ * scale one, and every product with the block NaN.
+ * q: [rows][C] with q_stride >= C, a multiple of 16, and a 16-byte aligned base, as exb_fp8_matmul_fwd takes it (bytes
+ * between C and q_stride are left alone).  scales: block_rows 1: [ceil(C / 128)][rows], block_rows 128: [ceil(rows / 128)]
+ * [ceil(C / 128)]; scale_stride is the distance of the first index, in floats.
+ * ------------------------------------------------------------------------------------- */
+EXB_API int exb_quantize_blocks_fwd(exb_ctx* ctx, const void* x, int in_dtype, int64_t x_stride, uint8_t* q,
+                                    int64_t q_stride, float* scales, int64_t scale_stride, int64_t rows, int C,
+                                    int block_rows, void* stream);
+
+/* Matrix product of what exb_quantize_blocks_fwd writes:
+ *   y[m][n] = sum over blocks b of 128: a_scales[b][m] * w_scales[n / 128][b] * sum over k in b: a[m][k] * w[n][k]  (+ bias[n])
+ * a: [M][K] e4m3, a_scales [ceil(K / 128)][M]; w: [N][K] e4m3, w_scales [ceil(N / 128)][ceil(K / 128)]; bias: fp32 [N] or
+ * NULL; y: [M][N] in EXB_F16, EXB_BF16 or EXB_F32.  a and w: 16-byte aligned, strides multiples of 16 and >= K (what
+ * lies between K and the stride is not read).  Products and their sums are fp32, rounded once at the end; the order of a sum depends on M, N and K
+ * and the device, not on the run. */
+EXB_API int exb_fp8_matmul_fwd(exb_ctx* ctx, const uint8_t* a, int64_t a_stride, const float* a_scales,
+                               int64_t a_scale_stride, const uint8_t* w, int64_t w_stride, const float* w_scales,
+                               int64_t w_scale_stride, const float* bias, void* y, int y_dtype, int64_t y_stride,
+                               int64_t M, int N, int K, void* stream);
+
+/* A block's result joins the residual stream, and the next block's norm is taken of the sum:
+ *   u = post_weight ? norm(h) * post_weight + post_bias : h
+ *   r = x + residual_scale * gate * u            (x, gate: left out where NULL)
+ *   n = norm(r) * weight + bias                  (of the fp32 sum, before r is rounded)
+ *   norm(v) = v / sqrt(mean(v^2) + eps), with EXB_NORM_LAYER of v - mean(v) in v's place
+ * r is written in dtype, n in out_dtype: dtype itself, or EXB_E4M3 with n_scales as exb_quantize_blocks_fwd writes blocks
+ * of one row.  Biases are NULL where there is none.  Row i takes row i / gate_rows of the gate (dtype); gate_rows 0: all
+ * take row 0.  r or n may be NULL (not both): then it is not written, and weight and bias are not read without n.  r
+ * and n may each be h or x, in the same place with the same stride (not both the same one). */
+typedef enum exb_norm { EXB_NORM_RMS = 0, EXB_NORM_LAYER = 1 } exb_norm;
+typedef struct exb_norm_desc {
+    int64_t rows;
+    int32_t C;              /* 1..32768 */
+    int32_t dtype;          /* of h, x, gate and r */
+    int32_t out_dtype;      /* of n: dtype or EXB_E4M3 */
+    int32_t kind;           /* exb_norm, of both norms */
+    float eps;              /* >= 0 */
+    float residual_scale;
+    int64_t gate_rows;
+    int64_t h_stride, x_stride, gate_stride, r_stride, n_stride, scale_stride;      /* elements between rows (n_scales: between blocks) */
+} exb_norm_desc;
+EXB_API int exb_residual_norm_fwd(exb_ctx* ctx, const exb_norm_desc* d, const void* h, const void* x,
+                                  const float* post_weight, const float* post_bias, const void* gate,
+                                  const float* weight, const float* bias, void* r, void* n, float* n_scales,
+                                  void* stream);
+
+/* Scores of tokens from rows of V logits, z = scale * logits (scale between 1e-38 and 1e38: the reciprocal of a temperature):
+ *   lse = log sum exp z;  logprobs[i][j] = z[tokens[i][j]] - lse, j < n_given
+ *   entropy[i] = -sum p log p, p = exp(z - lse)
+ *   top_tokens[i][0..top): the tokens of the largest logits in falling order, equal ones by their index; top_logprobs: theirs
+ * Minus infinity masks a token: p = 0, it adds nothing to the entropy.  A row with nothing else has log probabilities of minus
+ * infinity and entropy 0; a row with a NaN or plus infinity has NaN everywhere (NaN sorts above plus infinity).  A
+ * given token below 0 is none: its log probability is 0; one of V or more is an error of the caller's: NaN.
+ * tokens: int32 [rows][n_given], top: 0..32 and at most V.  entropy may be NULL, and so may what n_given or top of 0 leave empty. */
+EXB_API int exb_token_logprobs_fwd(exb_ctx* ctx, const void* logits, int dtype, int64_t stride, int64_t rows, int V,
+                                   float scale, const int32_t* tokens, int n_given, float* logprobs, float* entropy,
+                                   int top, float* top_logprobs, int32_t* top_tokens, void* stream);
 
 #ifdef __cplusplus
 }
