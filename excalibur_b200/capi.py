@@ -688,59 +688,77 @@ def nhwc_to_nchw_f32(ctx, x, Cc=None, scale=1.0, y=None):
 
 # ---- operators behind a decoder ------------------------------------------------------------------
 # Matrices are (rows, channels) with channels innermost; rows may be apart.  The library is told addresses and strides only, so
-# shapes, types and devices are checked here.
+# shapes, types and devices are checked here.  A decode step makes such calls by the hundred and their kernels take 2 to 5 us:
+# the checks are plain comparisons, and a message is put together only for a call that is refused.
 
-def _need(cond, what):
-    if not cond:
-        raise ExbError(EXB_ERR_BAD_ARG, what)
+def _refuse(what, *args):
+    raise ExbError(EXB_ERR_BAD_ARG, what % args)
 
 
-def _matrix(ctx, t, what, dtype=None, shape=None):
+def _row_stride(t, device, what):
     """Row stride of a (rows, channels) tensor on the context's device."""
-    _need(t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1), "%s has to be (rows, channels), channels innermost" % what)
-    _need(t.get_device() == ctx.device, "%s is not on the context's device" % what)
-    _need(dtype is None or t.dtype == dtype, "%s has to be %s" % (what, dtype))
-    _need(shape is None or t.shape == shape, "%s has to be %s" % (what, shape))
-    return t.stride(0) if t.shape[0] > 1 and t.shape[1] > 0 else max(t.shape[1], t.stride(0))
+    if t.get_device() != device:
+        _refuse("%s is not on the context's device", what)
+    if t.is_contiguous() and t.dim() == 2:
+        return t.shape[1]
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        _refuse("%s has to be (rows, channels), channels innermost", what)
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
 
 
-def _parameter(ctx, t, n, what):
-    _need(t is None or (t.dtype == _TORCH.float32 and t.dim() == 1 and t.shape[0] == n and t.get_device() == ctx.device and t.is_contiguous()),
-          "%s has to be %d float32 on the context's device" % (what, n))
+def _byte_row_stride(q, device, what):
+    """The same of an e4m3 matrix, whose rows have to start at multiples of 16 bytes."""
+    if q.dtype is not _TORCH.float8_e4m3fn:
+        _refuse("%s has to be float8_e4m3fn", what)
+    stride = _row_stride(q, device, what)
+    if stride & 15:
+        if q.shape[0] > 1:
+            _refuse("rows of %s have to start at multiples of 16 bytes", what)
+        stride = (stride + 15) // 16 * 16
+    return stride
+
+
+def _parameter(t, device, n, what):
+    """Address of n float32, or None."""
+    if t is None:
+        return None
+    if t.dtype is not _TORCH.float32 or t.shape != (n,) or t.get_device() != device or not t.is_contiguous():
+        _refuse("%s has to be %d float32 on the context's device", what, n)
+    return t.data_ptr()
 
 
 def _e4m3_rows(like, rows, channels):
-    """Room for (rows, channels) of e4m3 whose rows start at multiples of 16 bytes."""
-    q = like.new_empty((rows, (channels + 15) // 16 * 16), dtype=_TORCH.float8_e4m3fn)
-    return q if channels % 16 == 0 else q[:, :channels]
-
-
-def _row_pitch(q, what):
-    _need(q.shape[0] <= 1 or q.stride(0) % 16 == 0, "rows of %s have to start at multiples of 16 bytes" % what)
-    return q.stride(0) if q.shape[0] > 1 else max(q.stride(0), (q.shape[1] + 15) // 16 * 16) // 16 * 16
+    """Room for (rows, channels) of e4m3 whose rows start at multiples of 16 bytes, and their distance."""
+    if channels & 15 == 0:
+        return _TORCH.empty_like(like, dtype=_TORCH.float8_e4m3fn), channels      # (half the time of new_empty)
+    pitch = (channels + 15) // 16 * 16
+    return like.new_empty((rows, pitch), dtype=_TORCH.float8_e4m3fn)[:, :channels], pitch
 
 
 def quantize_blocks(ctx, x, block_rows=1, q=None, scales=None):
     """(q, scales): x in e4m3 with a scale for each block_rows x 128 of it.  block_rows 1 (activations): scales are
     (ceil(channels / 128), rows); 128 (weights): (ceil(rows / 128), ceil(channels / 128)).  q's rows start at multiples of 16 bytes."""
-    t = _torch()
-    xs = _matrix(ctx, x, "x")
+    t = _TORCH or _torch()
+    device = ctx.device
+    xs = _row_stride(x, device, "x")
     rows, channels = x.shape
-    _need(block_rows in (1, 128), "block_rows has to be 1 or 128")
-    _need(x.dtype in _DTYPES, "x has a type that the library does not have")
+    dt = _DTYPES.get(x.dtype, -1)
     blocks = (channels + 127) // 128
     shape = (blocks, rows) if block_rows == 1 else ((rows + 127) // 128, blocks)
     if q is None:
-        q = _e4m3_rows(x, rows, channels)
+        q, qs = _e4m3_rows(x, rows, channels)
     else:
-        _matrix(ctx, q, "q", t.float8_e4m3fn, x.shape)
+        qs = _byte_row_stride(q, device, "q")
+        if q.shape != x.shape:
+            _refuse("q has to be of x's shape")
     if scales is None:
         scales = x.new_empty(shape, dtype=t.float32)
         ss = shape[1]
     else:
-        ss = _matrix(ctx, scales, "scales", t.float32, shape)
-    rc = lib().exb_quantize_blocks_fwd(ctx._h, x.data_ptr(), _DTYPES[x.dtype], xs, q.data_ptr(), _row_pitch(q, "q"), scales.data_ptr(), ss, rows, channels,
-                                       block_rows, _stream())
+        ss = _row_stride(scales, device, "scales")
+        if scales.dtype is not t.float32 or scales.shape != shape:
+            _refuse("scales have to be %s float32", shape)
+    rc = lib().exb_quantize_blocks_fwd(ctx._h, x.data_ptr(), dt, xs, q.data_ptr(), qs, scales.data_ptr(), ss, rows, channels, block_rows, _stream())
     if rc:
         check(rc)
     return q, scales
@@ -748,23 +766,30 @@ def quantize_blocks(ctx, x, block_rows=1, q=None, scales=None):
 
 def fp8_matmul(ctx, a, a_scales, w, w_scales, bias=None, out_dtype=EXB_F16, y=None):
     """y (M, N) = a (M, K) @ w (N, K)^T (+ bias) of e4m3 matrices with the scales of quantize_blocks (a: single rows, w: 128 x 128)."""
-    t = _torch()
-    _matrix(ctx, a, "a", t.float8_e4m3fn)
-    _matrix(ctx, w, "w", t.float8_e4m3fn)
+    t = _TORCH or _torch()
+    device, f32 = ctx.device, t.float32
+    ast = _byte_row_stride(a, device, "a")
+    wst = _byte_row_stride(w, device, "w")
     M, K = a.shape
-    N = w.shape[0]
-    _need(w.shape[1] == K, "a and w have %d and %d columns" % (K, w.shape[1]))
+    N, k = w.shape
+    if K != k:
+        _refuse("a and w have %d and %d columns", K, k)
     blocks = (K + 127) // 128
-    sa = _matrix(ctx, a_scales, "a_scales", t.float32, (blocks, M))
-    sw = _matrix(ctx, w_scales, "w_scales", t.float32, ((N + 127) // 128, blocks))
-    _parameter(ctx, bias, N, "bias")
+    sa = _row_stride(a_scales, device, "a_scales")
+    sw = _row_stride(w_scales, device, "w_scales")
+    if a_scales.dtype is not f32 or a_scales.shape != (blocks, M):
+        _refuse("a_scales have to be (%d, %d) float32", blocks, M)
+    if w_scales.dtype is not f32 or w_scales.shape != ((N + 127) // 128, blocks):
+        _refuse("w_scales have to be (%d, %d) float32", (N + 127) // 128, blocks)
     if y is None:
         y = a.new_empty((M, N), dtype=_DTYPES[out_dtype])
         ys = N
     else:
-        ys = _matrix(ctx, y, "y", _DTYPES[out_dtype], (M, N))
-    rc = lib().exb_fp8_matmul_fwd(ctx._h, a.data_ptr(), _row_pitch(a, "a"), a_scales.data_ptr(), sa, w.data_ptr(), _row_pitch(w, "w"), w_scales.data_ptr(),
-                                  sw, _address(bias), y.data_ptr(), out_dtype, ys, M, N, K, _stream())
+        ys = _row_stride(y, device, "y")
+        if y.dtype is not _DTYPES[out_dtype] or y.shape != (M, N):
+            _refuse("y has to be (%d, %d) %s", M, N, _DTYPES[out_dtype])
+    rc = lib().exb_fp8_matmul_fwd(ctx._h, a.data_ptr(), ast, a_scales.data_ptr(), sa, w.data_ptr(), wst, w_scales.data_ptr(), sw,
+                                  None if bias is None else _parameter(bias, device, N, "bias"), y.data_ptr(), out_dtype, ys, M, N, K, _stream())
     if rc:
         check(rc)
     return y
@@ -774,46 +799,55 @@ def residual_norm(ctx, h, x=None, post_weight=None, post_bias=None, gate=None, g
                   kind=NORM_RMS, eps=1e-5, quantized=False, r=None, n=None):
     """r = x + residual_scale * gate * norm(h; post), n = norm(r; weight).  gate: (1, C), all rows alike (gate_rows 0), or a row for each
     gate_rows rows.  Returns (r, n), or with quantized (r, q, scales) as quantize_blocks gives them; without a weight n is None."""
-    t = _torch()
-    dtype, shape = h.dtype, h.shape
-    hs = _matrix(ctx, h, "h")
-    _need(dtype in _DTYPES, "h has a type that the library does not have")
+    t = _TORCH or _torch()
+    device, dtype, shape = ctx.device, h.dtype, h.shape
+    hs = _row_stride(h, device, "h")
     rows, Cc = shape
+    dt = _DTYPES.get(dtype, -1)
     xs = gs = ns = ss = 0
     if x is not None:
-        xs = _matrix(ctx, x, "x", dtype, shape)
+        xs = _row_stride(x, device, "x")
+        if x.dtype is not dtype or x.shape != shape:
+            _refuse("x has to be of h's shape and type")
     if gate is not None:
+        gs = _row_stride(gate, device, "gate")
         need = -(-rows // gate_rows) if gate_rows > 0 else 1
-        gs = _matrix(ctx, gate, "gate", dtype)
-        _need(gate.shape[1] == Cc and gate.shape[0] >= need, "gate has to be (%d, %d)" % (need, Cc))
-    for p, what in ((post_weight, "post_weight"), (post_bias, "post_bias"), (weight, "weight"), (bias, "bias")):
-        if p is not None:
-            _parameter(ctx, p, Cc, what)
+        if gate.dtype is not dtype or gate.shape[1] != Cc or gate.shape[0] < need:
+            _refuse("gate has to be (%d, %d) of h's type", need, Cc)
     if r is None:
-        r = h.new_empty(shape)
+        r = t.empty_like(h)
         rs = Cc
     else:
-        rs = _matrix(ctx, r, "r", dtype, shape)
+        rs = _row_stride(r, device, "r")
+        if r.dtype is not dtype or r.shape != shape:
+            _refuse("r has to be of h's shape and type")
     scales = None
-    if weight is not None:
-        if quantized:
-            if n is None:
-                n = _e4m3_rows(h, rows, Cc)
-            else:
-                _matrix(ctx, n, "n", t.float8_e4m3fn, shape)
-            ns, ss = _row_pitch(n, "n"), rows
-            scales = h.new_empty(((Cc + 127) // 128, rows), dtype=t.float32)
-        elif n is None:
-            n = h.new_empty(shape)
-            ns = Cc
+    if weight is None:
+        if n is not None:
+            _refuse("n without a weight")
+    elif quantized:
+        if n is None:
+            n, ns = _e4m3_rows(h, rows, Cc)
         else:
-            ns = _matrix(ctx, n, "n", dtype, shape)
+            ns = _byte_row_stride(n, device, "n")
+            if n.shape != shape:
+                _refuse("n has to be of h's shape")
+        scales = h.new_empty(((Cc + 127) // 128, rows), dtype=t.float32)
+        ss = rows
+    elif n is None:
+        n = t.empty_like(h)
+        ns = Cc
     else:
-        _need(n is None, "n without a weight")
-    dt = _DTYPES[dtype]
+        ns = _row_stride(n, device, "n")
+        if n.dtype is not dtype or n.shape != shape:
+            _refuse("n has to be of h's shape and type")
     d = NormDesc(rows, Cc, dt, EXB_E4M3 if quantized else dt, kind, eps, residual_scale, gate_rows, hs, xs, gs, rs, ns, ss)
-    rc = lib().exb_residual_norm_fwd(ctx._h, C.byref(d), h.data_ptr(), _address(x), _address(post_weight), _address(post_bias), _address(gate),
-                                     _address(weight), _address(bias), r.data_ptr(), _address(n), _address(scales), _stream())
+    rc = lib().exb_residual_norm_fwd(ctx._h, d, h.data_ptr(), None if x is None else x.data_ptr(),
+                                     None if post_weight is None else _parameter(post_weight, device, Cc, "post_weight"),
+                                     None if post_bias is None else _parameter(post_bias, device, Cc, "post_bias"),
+                                     None if gate is None else gate.data_ptr(), None if weight is None else _parameter(weight, device, Cc, "weight"),
+                                     None if bias is None else _parameter(bias, device, Cc, "bias"), r.data_ptr(),
+                                     None if n is None else n.data_ptr(), None if scales is None else scales.data_ptr(), _stream())
     if rc:
         check(rc)
     return (r, n, scales) if quantized else (r, n)
@@ -822,23 +856,25 @@ def residual_norm(ctx, h, x=None, post_weight=None, post_bias=None, gate=None, g
 def token_logprobs(ctx, logits, tokens=None, top=0, scale=1.0):
     """(logprobs, entropy, top_logprobs, top_tokens) of rows of logits: log probabilities of tokens (rows, given) int32, the
     entropy (rows,), and the `top` most probable tokens with theirs (rows, top); None where nothing was asked for."""
-    t = _torch()
-    ls = _matrix(ctx, logits, "logits")
-    _need(logits.dtype in _DTYPES, "logits have a type that the library does not have")
+    t = _TORCH or _torch()
+    device, f32 = ctx.device, t.float32
+    ls = _row_stride(logits, device, "logits")
     rows, V = logits.shape
     given = 0
-    lp = top_lp = top_tokens = None
+    at = lp = top_lp = top_tokens = None
     if tokens is not None:
-        _matrix(ctx, tokens, "tokens", t.int32)
+        if tokens.dtype is not t.int32 or tokens.dim() != 2 or tokens.shape[0] != rows or tokens.get_device() != device or not tokens.is_contiguous():
+            _refuse("tokens have to be (%d, given) int32, contiguous, on the context's device", rows)
         given = tokens.shape[1]
-        _need(tokens.shape[0] == rows and tokens.is_contiguous(), "tokens have to be (%d, given), contiguous" % rows)
-        lp = logits.new_empty((rows, given), dtype=t.float32)
-    entropy = logits.new_empty((rows,), dtype=t.float32)
+        at = tokens.data_ptr()
+        lp = t.empty_like(tokens, dtype=f32)
+    entropy = logits.new_empty(rows, dtype=f32)
     if top > 0:
-        top_lp = logits.new_empty((rows, top), dtype=t.float32)
-        top_tokens = logits.new_empty((rows, top), dtype=t.int32)
-    rc = lib().exb_token_logprobs_fwd(ctx._h, logits.data_ptr(), _DTYPES[logits.dtype], ls, rows, V, scale, _address(tokens) if given else None, given,
-                                      _address(lp), entropy.data_ptr(), top, _address(top_lp), _address(top_tokens), _stream())
+        top_lp = logits.new_empty((rows, top), dtype=f32)
+        top_tokens = t.empty_like(top_lp, dtype=t.int32)
+    rc = lib().exb_token_logprobs_fwd(ctx._h, logits.data_ptr(), _DTYPES.get(logits.dtype, -1), ls, rows, V, scale, at, given, None if lp is None else lp.data_ptr(),
+                                      entropy.data_ptr(), top, None if top_lp is None else top_lp.data_ptr(), None if top_tokens is None else top_tokens.data_ptr(),
+                                      _stream())
     if rc:
         check(rc)
     return lp, entropy, top_lp, top_tokens
