@@ -116,10 +116,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_matmul_kernel(const __grid_co
         for (int b = 0; b < p.blocks; ++b) {
             const int buf = b & 1;
             const float s = row < p.M ? __ldg(p.a_scales + (int64_t)b * p.a_scale_stride + row) * __ldg(p.w_scales + (int64_t)(n0 / kBlk) * p.w_scale_stride + b) : 0.f;
-            if (!ptx::mbar_wait_bounded_warp(&tfull_bar[buf], (uint32_t)(b / 2) & 1u, &abort_flag, kMaxSpins)) {
+            if (!ptx::mbar_wait_bounded_uniform(tfull0 + buf * 8, (uint32_t)(b / 2) & 1u, &abort_flag, kMaxSpins)) {
                 ok = false;
                 break;
             }
+            __syncwarp();
             ptx::tc_fence_after_sync();
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * kTileN + half * 64);
 #pragma unroll
@@ -155,6 +156,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_matmul_kernel(const __grid_co
 // 512 cycles of MMA: 64 bytes per cycle and SM from L2 (a lone CTA's tile of 128 x 128 needs 128).  TMEM holds two accumulators of
 // 256 columns; a thread's sums are 128 registers.
 constexpr int kPairStages = 6;
+constexpr int kPairEpiWarps = 8;                 // two per TMEM lane quarter
+constexpr int kPairCols = 4 * 256 / kPairEpiWarps;      // of the accumulator's columns each
 constexpr int kPairM = 256, kPairN = 256;
 constexpr int kPairStageBytes = (kPairM + kPairN) / 2 * kBlk;      // of one of the two CTAs
 
@@ -178,20 +181,20 @@ __device__ __forceinline__ uint32_t result_pair(float a, float b) {
     return rows::float_to_pair(a, b, T());
 }
 
-// Columns [col, col + 128) of 32 rows from row0 on: sums in `acc` (a thread has a row), through shared memory to y in full lines.
+// Columns [col, col + kPairCols) of 32 rows from row0 on: sums in `acc` (a thread has a row), through shared memory to y in full lines.
 template <typename T>
-__device__ __forceinline__ void store_rows(f32x2 (&acc)[64], uint8_t* stage, T* y, int64_t y_stride, const float* bias, int row0, int col, int M, int N,
+__device__ __forceinline__ void store_rows(const float (&acc)[kPairCols], uint8_t* stage, T* y, int64_t y_stride, const float* bias, int row0, int col, int M, int N,
                                            bool vec, int lane) {
     constexpr int kPer = 16 / (int)sizeof(T), kCols = 8 * kPer;      // columns in a unit, in a pass
 #pragma unroll
-    for (int c0 = 0; c0 < 128; c0 += kCols) {
+    for (int c0 = 0; c0 < kPairCols; c0 += kCols) {
         if (col + c0 >= N) break;
         const int left = N - col - c0;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             float v[kPer];
 #pragma unroll
-            for (int j = 0; j < kPer; j += 2) unpack2(acc[(c0 + u * kPer + j) / 2], v[j], v[j + 1]);
+            for (int j = 0; j < kPer; ++j) v[j] = acc[c0 + u * kPer + j];
             if (bias) {
 #pragma unroll
                 for (int j = 0; j < kPer; ++j)
@@ -236,7 +239,7 @@ __device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int& m,
 }
 
 // Warp 0 loads, warp 1 issues the MMAs, two warpgroups keep the sums: 2 x 224 + 56 registers are the 3 x 168 of the launch.
-constexpr int kPairThreads = 384;
+constexpr int kPairThreads = 128 + kPairEpiWarps * 32;
 template <int kRegs> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 template <int kRegs> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 
@@ -258,7 +261,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
         }
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&tfull_bar[i], 1);
-            ptx::mbar_init(&tempty_bar[i], 2 * kEpiWarps);      // both CTAs' warps arrive at rank 0
+            ptx::mbar_init(&tempty_bar[i], 2 * kPairEpiWarps);      // both CTAs' warps arrive at rank 0
         }
         ptx::fence_mbar_init();
         ptx::tma_prefetch_desc(&p.tmA);
@@ -316,8 +319,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
             uint32_t phase = 0, acc_phase = 1;
             for (int t = first; t < total && ok; t += step) {
                 for (int b = 0; b < p.blocks; ++b) {
-                    if (!ptx::mbar_wait_bounded_uniform(tempty0 + buf * 8, acc_phase, &abort_flag, kMaxSpins) ||
-                        !ptx::mbar_wait_bounded_uniform(full0 + s * 8, phase, &abort_flag, kMaxSpins)) {
+                    // (the loads are ahead: what is waited for last is what comes last)
+                    if (!ptx::mbar_wait_bounded_uniform(full0 + s * 8, phase, &abort_flag, kMaxSpins) ||
+                        !ptx::mbar_wait_bounded_uniform(tempty0 + buf * 8, acc_phase, &abort_flag, kMaxSpins)) {
                         ok = false;
                         break;
                     }
@@ -341,9 +345,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
     }
     } else {
         more_registers<224>();
-        const int q = warp & 3, half = (warp >> 2) - 1;
+        const int q = warp & 3, part = (warp >> 2) - 1;
         uint8_t* stage = ring + kPairStages * kPairStageBytes + (warp - 4) * kStageOut;
-        const uint32_t taddr0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
+        const uint32_t taddr0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(part * kPairCols);
         const uint32_t tempty_lead = ptx::map_to_cta(tempty0, 0);
         bool ok = true;
         int buf = 0;
@@ -351,8 +355,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
         for (int t = first; t < total && ok; t += step) {
             int mt, nt;
             tile_at(t, p.m_tiles, p.n_tiles, mt, nt);
-            const int row = mt * kPairM + rank * 128 + q * 32 + lane, col = nt * kPairN + half * 128;
-            // this row's and this half's scales of the next two blocks are on their way while one is worked on
+            const int row = mt * kPairM + rank * 128 + q * 32 + lane, col = nt * kPairN + part * kPairCols;
+            // this row's and these columns' scales of the next two blocks are on their way while one is worked on
             const float* sa = p.a_scales + (row < p.M ? row : 0);
             const float* sw = p.w_scales + (int64_t)(col < p.N ? col / kBlk : 0) * p.w_scale_stride;
             float sa0 = __ldg(sa), sw0 = __ldg(sw), sa1 = 0.f, sw1 = 0.f;
@@ -360,38 +364,35 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
                 sa1 = __ldg(sa += p.a_scale_stride);
                 sw1 = __ldg(++sw);
             }
-            f32x2 acc[64];
+            float acc[kPairCols];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) acc[i] = 0;
+            for (int i = 0; i < kPairCols; ++i) acc[i] = 0.f;
             for (int b = 0; b < p.blocks; ++b) {
                 float sa2 = 0.f, sw2 = 0.f;
                 if (b + 2 < p.blocks) {
                     sa2 = __ldg(sa += p.a_scale_stride);
                     sw2 = __ldg(++sw);
                 }
-                if (!ptx::mbar_wait_bounded_warp(&tfull_bar[buf], acc_phase, &abort_flag, kMaxSpins)) {
+                if (!ptx::mbar_wait_bounded_uniform(tfull0 + buf * 8, acc_phase, &abort_flag, kMaxSpins)) {
                     ok = false;
                     break;
                 }
+                __syncwarp();      // (what follows needs the warp together)
                 ptx::tc_fence_after_sync();
                 const uint32_t taddr = taddr0 + (uint32_t)(buf * kPairN);
                 const float s = sa0 * sw0;
-                const f32x2 ss = pack2(s, s);
-                uint32_t raw[2][16];
-                ptx::tmem_ld_32x32b_x16(taddr, raw[0]);
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {      // 16 columns are read while 16 others are added
-                    ptx::tmem_ld_wait(raw[c & 1]);
-                    if (c < 7) {
-                        ptx::tmem_ld_32x32b_x16(taddr + (c + 1) * 16, raw[(c + 1) & 1]);
-                    } else {
+                for (int c = 0; c < kPairCols; c += 16) {
+                    uint32_t raw[16];
+                    ptx::tmem_ld_32x32b_x16(taddr + c, raw);
+                    ptx::tmem_ld_wait(raw);
+                    if (c + 16 == kPairCols) {
                         ptx::tc_fence_before_sync();
                         __syncwarp();
                         if (lane == 0) ptx::mbar_arrive_cluster_u32(tempty_lead + buf * 8);
                     }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        acc[c * 8 + j] = fma2(pack2(__uint_as_float(raw[c & 1][2 * j]), __uint_as_float(raw[c & 1][2 * j + 1])), ss, acc[c * 8 + j]);
+                    for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(__uint_as_float(raw[j]), s, acc[c + j]);
                 }
                 sa0 = sa1;
                 sw0 = sw1;
@@ -467,7 +468,7 @@ extern "C" int exb_fp8_matmul_fwd(exb_ctx* ctx, const uint8_t* a, int64_t a_stri
         const int tiles = p.m_tiles * p.n_tiles, places = ctx->sm_count / 2;
         if (int rc = raise_smem_limit(ctx, fp8_matmul_pair_kernel)) return rc;
         return launch_pdl_cluster(ctx, "fp8_matmul_pair_kernel", fp8_matmul_pair_kernel, dim3(2 * (tiles < places ? tiles : places)), dim3(kPairThreads), dim3(2),
-                                  (size_t)kPairStages * kPairStageBytes + kEpiWarps * kStageOut + 1024, static_cast<cudaStream_t>(stream), p);
+                                  (size_t)kPairStages * kPairStageBytes + kPairEpiWarps * kStageOut + 1024, static_cast<cudaStream_t>(stream), p);
     }
     MatmulParams p;
     if (int rc = encode(&p.tmA, a, M, K, a_stride, kTileM)) return rc;
