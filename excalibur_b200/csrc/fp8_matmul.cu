@@ -7,15 +7,12 @@
 #include "rows_common.cuh"
 #include "tensor_map.cuh"
 
+#include <type_traits>
+
 namespace exb {
 namespace {
 
 constexpr int kBlk = 128;                  // K block: bytes of a row in a stage, elements that share a scale
-constexpr int kTileM = 128, kTileN = 128;
-constexpr int kStages = 6;
-constexpr int kEpiWarps = 8;               // two per TMEM lane quarter, half of the columns each
-constexpr int kThreads = (2 + kEpiWarps) * 32;
-constexpr int kStageBytes = (kTileM + kTileN) * kBlk;
 constexpr uint32_t kMaxSpins = 1u << 21;
 
 struct MatmulParams {
@@ -23,7 +20,8 @@ struct MatmulParams {
     const float *a_scales, *w_scales, *bias;
     void* y;
     int64_t a_scale_stride, w_scale_stride, y_stride;
-    int M, N, blocks, y_dtype;
+    int M, N, blocks, y_dtype, vec;
+    int m_tiles, n_tiles, splits;
     uint32_t idesc;
     int* error;
 };
@@ -34,14 +32,56 @@ __device__ __forceinline__ void store_one(void* y, int dtype, int64_t at, float 
     else static_cast<float*>(y)[at] = v;
 }
 
-__global__ void __launch_bounds__(kThreads, 1) fp8_matmul_kernel(const __grid_constant__ MatmulParams p) {
+// Four neighbouring channels of a row.
+__device__ __forceinline__ void store_four(const MatmulParams& p, int m, int n, float (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (p.bias && n + j < p.N) v[j] += __ldg(p.bias + n + j);
+    const int64_t at = (int64_t)m * p.y_stride + n;
+    if (p.vec && n + 4 <= p.N) {
+        if (p.y_dtype == EXB_F32)
+            *reinterpret_cast<float4*>(static_cast<float*>(p.y) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + at) =
+                p.y_dtype == EXB_F16 ? make_uint2(rows::float_to_pair(v[0], v[1], __half()), rows::float_to_pair(v[2], v[3], __half()))
+                                     : make_uint2(rows::float_to_pair(v[0], v[1], __nv_bfloat16()), rows::float_to_pair(v[2], v[3], __nv_bfloat16()));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (n + j < p.N) store_one(p.y, p.y_dtype, at + j, v[j]);
+    }
+}
+
+// ---- few rows of a -----------------------------------------------------------------------------
+// Bound by the reading of w.  The roles of the operands are exchanged: w's rows are the MMA's 128 rows (lanes of TMEM), the rows of a its
+// kCols columns, so that a narrow product wastes no tensor work and a thread has one channel of all rows.  The K blocks of a
+// tile are divided over a cluster of up to 8 CTAs, so that enough of them ask for w at the same time.  Every CTA then finishes a
+// share of the columns: the others send it their parts in one bulk copy each, counted by a barrier of its own, and it sums them in
+// the order of the CTAs.  (Read out of the others' shared memory between cluster barriers the exchange took 3600 cycles for 16
+// columns and 8000 for 64.)
+constexpr int kFewBufs = 4;          // accumulators in turn: TMEM has room
+constexpr int kFewTable = 16;        // blocks whose scales are in shared memory at a time
+constexpr int few_stages(int cols) { return cols == 128 ? 4 : cols == 64 ? 3 : cols == 32 ? 4 : 5; }      // (two CTAs fit an SM up to 64 columns)
+constexpr int few_epi_warps(int cols) { return cols == 128 ? 8 : 4; }
+constexpr int few_stage_bytes(int cols) { return (128 + cols) * kBlk; }
+constexpr int few_smem(int cols) { return few_stages(cols) * few_stage_bytes(cols) + kFewTable * cols * 4 + cols * 512 + 1024; }
+
+template <int kCols>
+__global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ? 1 : 2) fp8_matmul_few_kernel(const __grid_constant__ MatmulParams p) {
+    constexpr int kStages = few_stages(kCols), kStageBytes = few_stage_bytes(kCols), kEpi = few_epi_warps(kCols);
+    constexpr int kMine = kCols * 4 / kEpi;      // columns of a warp
+    constexpr int kTmem = kFewBufs * kCols;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages], tfull_bar[2], tempty_bar[2];
+    __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages], tfull_bar[kFewBufs], tempty_bar[kFewBufs], recv_bar;
     __shared__ uint32_t tmem_base_smem;
     __shared__ int abort_flag;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* table = reinterpret_cast<float*>(ring + kStages * kStageBytes);      // [block][column]: a's scale x w's
+    float* recv = table + kFewTable * kCols;                                    // [CTA][column of the share][128]
+    float* part = reinterpret_cast<float*>(ring);                               // [column][128] behind the loop
     const int warp = ptx::uniform_warp(), lane = threadIdx.x & 31;
-    const int n0 = blockIdx.x * kTileN, m0 = blockIdx.y * kTileM;
+    const int rank = (int)blockIdx.x % p.splits, n0 = (int)blockIdx.x / p.splits * 128, m0 = blockIdx.y * kCols;
+    const int b0 = (int)((int64_t)rank * p.blocks / p.splits), nb = (int)((int64_t)(rank + 1) * p.blocks / p.splits) - b0;
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
         abort_flag = 0;
@@ -49,16 +89,17 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_matmul_kernel(const __grid_co
             ptx::mbar_init(&full_bar[s], 1);
             ptx::mbar_init(&empty_bar[s], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kFewBufs; ++i) {
             ptx::mbar_init(&tfull_bar[i], 1);
-            ptx::mbar_init(&tempty_bar[i], kEpiWarps);
+            ptx::mbar_init(&tempty_bar[i], kEpi);
         }
+        ptx::mbar_init(&recv_bar, 1);
         ptx::fence_mbar_init();
         ptx::tma_prefetch_desc(&p.tmA);
         ptx::tma_prefetch_desc(&p.tmW);
     }
     if (warp == 1) {
-        ptx::tmem_alloc(&tmem_base_smem, 2 * kTileN);
+        ptx::tmem_alloc(&tmem_base_smem, kTmem);
         ptx::tmem_relinquish();
     }
     ptx::tc_fence_before_sync();
@@ -67,87 +108,185 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_matmul_kernel(const __grid_co
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_smem, 0);
     const uint32_t ring0 = ptx::smem_u32(ring), full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
     const uint32_t tfull0 = ptx::smem_u32(tfull_bar), tempty0 = ptx::smem_u32(tempty_bar);
+    // columns that this CTA finishes: [rank * share, rank * share + mine)
+    const int cols = min(kCols, p.M - m0), share = (cols + p.splits - 1) / p.splits, mine = max(min(share, cols - rank * share), 0);
+    if (p.splits > 1) {      // every CTA runs and its barriers are initialised: waited for before the first part is sent
+        ptx::cluster_arrive();
+        if (threadIdx.x == 0) ptx::mbar_arrive_expect_tx(&recv_bar, (uint32_t)(mine * (p.splits - 1) * 512));
+        __syncwarp();
+    }
+    float acc[kMine];
+    bool ok = true;
     pdl_wait();
-    if (warp == 0) {
-        if (lane == 0) {
-            const uint64_t mapA = reinterpret_cast<uint64_t>(&p.tmA), mapW = reinterpret_cast<uint64_t>(&p.tmW);
-            bool ok = true;
-            for (int b = 0; b < p.blocks; ++b) {
-                const int s = b % kStages;
-                if (b >= kStages && !ptx::mbar_wait_bounded_u32(empty0 + s * 8, (uint32_t)(b / kStages - 1) & 1u, &abort_flag, kMaxSpins)) {
-                    ok = false;
-                    break;
-                }
-                ptx::mbar_arrive_expect_tx_u32(full0 + s * 8, kStageBytes);
-                ptx::tma_load_2d_u32(ring0 + s * kStageBytes, mapA, full0 + s * 8, b * kBlk, m0);
-                ptx::tma_load_2d_u32(ring0 + s * kStageBytes + kTileM * kBlk, mapW, full0 + s * 8, b * kBlk, n0);
+    if (warp == 0 || warp == 2) {      // a loading warp for each operand
+        const bool is_w = warp == 0;
+        const uint32_t leader = ptx::elect_one() ? 1u : 0u;
+        const uint64_t map = is_w ? reinterpret_cast<uint64_t>(&p.tmW) : reinterpret_cast<uint64_t>(&p.tmA);
+        const uint32_t dst = ring0 + (is_w ? 0 : 128 * kBlk);
+        const int row0 = is_w ? n0 : m0;
+        int s = 0;
+        uint32_t phase = 1;      // (a fresh barrier's previous phase counts as complete)
+        for (int b = 0; b < nb; ++b) {
+            if (b >= kStages && !ptx::mbar_wait_quick_uniform(empty0 + s * 8, phase, &abort_flag, kMaxSpins)) {
+                ok = false;
+                break;
             }
-            if (!ok) ptx::give_up(p.error, 1);
+            ptx::mbar_arrive_expect_tx_u32(full0 + s * 8, kStageBytes, is_w ? leader : 0u);
+            ptx::tma_load_2d_u32(dst + s * kStageBytes, map, full0 + s * 8, (b0 + b) * kBlk, row0, leader);
+            __syncwarp();      // (the elected lane may take a branch of its own; what follows is in registers of the whole warp)
+            if (++s == kStages) {
+                s = 0;
+                phase ^= 1u;
+            }
         }
+        if (!ok && lane == 0) ptx::give_up(p.error, 1);
         __syncwarp();
     } else if (warp == 1) {
         const uint32_t leader = ptx::elect_one() ? 1u : 0u;
         const uint64_t d0 = ptx::make_smem_desc(ring0, kBlk);
         const uint32_t desc_hi = (uint32_t)(d0 >> 32);
-        bool ok = true;
-        for (int b = 0; b < p.blocks; ++b) {
-            const int s = b % kStages, buf = b & 1;
-            if ((b >= 2 && !ptx::mbar_wait_bounded_uniform(tempty0 + buf * 8, (uint32_t)(b / 2 - 1) & 1u, &abort_flag, kMaxSpins)) ||
-                !ptx::mbar_wait_bounded_uniform(full0 + s * 8, (uint32_t)(b / kStages) & 1u, &abort_flag, kMaxSpins)) {
+        int s = 0, buf = 0;
+        uint32_t phase = 0, acc_phase = 1;
+        for (int b = 0; b < nb; ++b) {
+            if (!ptx::mbar_wait_quick_uniform(full0 + s * 8, phase, &abort_flag, kMaxSpins) ||
+                !ptx::mbar_wait_quick_uniform(tempty0 + buf * 8, acc_phase, &abort_flag, kMaxSpins)) {
                 ok = false;
                 break;
             }
             ptx::tc_fence_after_sync();
-            const uint32_t a_lo = (uint32_t)d0 + ((uint32_t)(s * kStageBytes) >> 4), w_lo = a_lo + ((kTileM * kBlk) >> 4);
+            const uint32_t w_lo = (uint32_t)d0 + ((uint32_t)(s * kStageBytes) >> 4), a_lo = w_lo + ((128 * kBlk) >> 4);
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
-                ptx::tc_mma_f8<false>(tmem_base + buf * kTileN, a_lo + 2 * ks, w_lo + 2 * ks, desc_hi, p.idesc, ks ? 1u : 0u, leader);
-            if (b + kStages < p.blocks) ptx::tc_commit_u32(empty0 + s * 8, leader);
+                ptx::tc_mma_f8<false>(tmem_base + buf * kCols, w_lo + 2 * ks, a_lo + 2 * ks, desc_hi, p.idesc, ks ? 1u : 0u, leader);
+            if (b + kStages < nb) ptx::tc_commit_u32(empty0 + s * 8, leader);
             ptx::tc_commit_u32(tfull0 + buf * 8, leader);
+            __syncwarp();
+            if (++s == kStages) {
+                s = 0;
+                phase ^= 1u;
+            }
+            if (++buf == kFewBufs) {
+                buf = 0;
+                acc_phase ^= 1u;
+            }
         }
         if (!ok) ptx::give_up(p.error, 2);
         __syncwarp();
     } else {
-        const int q = warp & 3, half = warp < 6 ? 0 : 1, row = m0 + q * 32 + lane, col = n0 + half * 64;
-        float acc[64];
+        const int q = warp & 3, c0 = warp < 7 ? 0 : kMine, et = (int)threadIdx.x - 96;
+        const float* sw = p.w_scales + (int64_t)(n0 / kBlk) * p.w_scale_stride + b0;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) acc[i] = 0.f;
-        bool ok = true;
-        for (int b = 0; b < p.blocks; ++b) {
-            const int buf = b & 1;
-            const float s = row < p.M ? __ldg(p.a_scales + (int64_t)b * p.a_scale_stride + row) * __ldg(p.w_scales + (int64_t)(n0 / kBlk) * p.w_scale_stride + b) : 0.f;
-            if (!ptx::mbar_wait_bounded_uniform(tfull0 + buf * 8, (uint32_t)(b / 2) & 1u, &abort_flag, kMaxSpins)) {
-                ok = false;
-                break;
+        for (int i = 0; i < kMine; ++i) acc[i] = 0.f;
+        int buf = 0;
+        uint32_t acc_phase = 0;
+        for (int b = 0; b < nb; ++b) {
+            if (b % kFewTable == 0) {
+                if (b) asm volatile("bar.sync 1, %0;" ::"n"(kEpi * 32) : "memory");
+                // a thread has one column; eight loads at a time are under way
+                constexpr int kStep = kEpi * 32 / kCols;
+                const int n = min(nb - b, kFewTable), c = et % kCols;
+                const float* sa = p.a_scales + (int64_t)(b0 + b) * p.a_scale_stride + m0 + c;
+                for (int k = et / kCols; k < n; k += 8 * kStep) {
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        v[j] = c < cols && k + j * kStep < n ? __ldg(sa + (int64_t)(k + j * kStep) * p.a_scale_stride) * __ldg(sw + b + k + j * kStep) : 0.f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (k + j * kStep < n) table[(k + j * kStep) * kCols + c] = v[j];
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(kEpi * 32) : "memory");
             }
-            __syncwarp();
+            // a warp that has given up still meets the others at their barrier
+            if (ok && !ptx::mbar_wait_quick_uniform(tfull0 + buf * 8, acc_phase, &abort_flag, kMaxSpins)) ok = false;
+            if (!ok) continue;
+            __syncwarp();      // (what follows needs the warp together)
             ptx::tc_fence_after_sync();
-            const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * kTileN + half * 64);
+            const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * kCols + c0);
+            const float4* s4 = reinterpret_cast<const float4*>(table + (b % kFewTable) * kCols + c0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int c = 0; c < kMine; c += 16) {
                 uint32_t raw[16];
-                ptx::tmem_ld_32x32b_x16(taddr + i * 16, raw);
-                ptx::tmem_ld_wait(raw);
+                ptx::tmem_ld_32x32b_x16(taddr + c, raw);
+                float4 s[4];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) acc[i * 16 + j] = fmaf(__uint_as_float(raw[j]), s, acc[i * 16 + j]);
+                for (int j = 0; j < 4; ++j) s[j] = s4[c / 4 + j];
+                ptx::tmem_ld_wait(raw);
+                if (c + 16 == kMine) {
+                    ptx::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive_u32(tempty0 + buf * 8);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    acc[c + 4 * j] = fmaf(__uint_as_float(raw[4 * j]), s[j].x, acc[c + 4 * j]);
+                    acc[c + 4 * j + 1] = fmaf(__uint_as_float(raw[4 * j + 1]), s[j].y, acc[c + 4 * j + 1]);
+                    acc[c + 4 * j + 2] = fmaf(__uint_as_float(raw[4 * j + 2]), s[j].z, acc[c + 4 * j + 2]);
+                    acc[c + 4 * j + 3] = fmaf(__uint_as_float(raw[4 * j + 3]), s[j].w, acc[c + 4 * j + 3]);
+                }
             }
-            ptx::tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive_u32(tempty0 + buf * 8);
+            if (++buf == kFewBufs) {
+                buf = 0;
+                acc_phase ^= 1u;
+            }
         }
         if (!ok && lane == 0) atomicExch(p.error, 3);
-        if (ok && row < p.M) {
-            const int64_t at = (int64_t)row * p.y_stride + col;
+        const int n = n0 + q * 32 + lane;
+        if (p.splits == 1) {
+            if (ok && n < p.N) {
+                const float bias = p.bias ? __ldg(p.bias + n) : 0.f;
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
-                if (col + i < p.N) store_one(p.y, p.y_dtype, at + i, p.bias ? acc[i] + __ldg(p.bias + col + i) : acc[i]);
+                for (int i = 0; i < kMine; ++i)
+                    if (m0 + c0 + i < p.M) store_one(p.y, p.y_dtype, (int64_t)(m0 + c0 + i) * p.y_stride + n, p.bias ? acc[i] + bias : acc[i]);
+            }
+        } else if (ok) {      // every MMA has read its operands: the parts take the ring's place
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) part[(c0 + i) * 128 + q * 32 + lane] = acc[i];
         }
+    }
+    if (p.splits > 1) {
+        __syncwarp();
+        ptx::cluster_wait();
+        if (warp >= 3) {
+            const int et = (int)threadIdx.x - 96, row = (et & 31) * 4;      // a thread has four channels of a column
+            if (ok) ptx::fence_proxy_async();
+            asm volatile("bar.sync 1, %0;" ::"n"(kEpi * 32) : "memory");      // (all of them, whatever their waits gave)
+            ok = ok && *static_cast<volatile int*>(&abort_flag) == 0;
+            // lane r of the first warp sends CTA r its columns
+            const int theirs = min(share, cols - lane * share);
+            if (ok && warp == 3 && lane < p.splits && lane != rank && theirs > 0)
+                ptx::copy_to_cta(ptx::map_to_cta(ptx::smem_u32(recv + rank * share * 128), (uint32_t)lane), ptx::smem_u32(part + lane * share * 128),
+                                 (uint32_t)(theirs * 512), ptx::map_to_cta(ptx::smem_u32(&recv_bar), (uint32_t)lane));
+            __syncwarp();
+            if (ok) ok = ptx::mbar_wait_quick_uniform(ptx::smem_u32(&recv_bar), 0, &abort_flag, kMaxSpins);
+            if (!ok && lane == 0) atomicExch(p.error, 3);
+            __syncwarp();
+            ptx::cluster_arrive();      // no CTA leaves while parts may still be on their way to it or from it
+            for (int c = et >> 5; ok && c < mine; c += kEpi) {
+                const float* own = part + (rank * share + c) * 128 + row;
+                float sum[4];
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+                    if (s < p.splits) {
+                        const float4 v = *reinterpret_cast<const float4*>(s == rank ? own : recv + (s * share + c) * 128 + row);
+                        sum[0] = s ? sum[0] + v.x : v.x;
+                        sum[1] = s ? sum[1] + v.y : v.y;
+                        sum[2] = s ? sum[2] + v.z : v.z;
+                        sum[3] = s ? sum[3] + v.w : v.w;
+                    }
+                store_four(p, m0 + rank * share + c, n0 + row, sum);
+            }
+        } else {
+            ptx::cluster_arrive();
+        }
+        __syncwarp();
+        ptx::cluster_wait();
     }
     ptx::tc_fence_before_sync();
     __syncthreads();
     if (warp == 1) {
         ptx::tc_fence_after_sync();
-        ptx::tmem_dealloc(tmem_base, 2 * kTileN);
+        ptx::tmem_dealloc(tmem_base, kTmem);
     }
 }
 
@@ -155,22 +294,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_matmul_kernel(const __grid_co
 // Tiles of 256 x 256 by pairs of CTAs, persistent.  Each CTA keeps 128 rows of a and half of w's rows of a stage, 32 KB for
 // 512 cycles of MMA: 64 bytes per cycle and SM from L2 (a lone CTA's tile of 128 x 128 needs 128).  TMEM holds two accumulators of
 // 256 columns; a thread's sums are 128 registers.
-constexpr int kPairStages = 6;
-constexpr int kPairEpiWarps = 8;                 // two per TMEM lane quarter
-constexpr int kPairCols = 4 * 256 / kPairEpiWarps;      // of the accumulator's columns each
-constexpr int kPairM = 256, kPairN = 256;
-constexpr int kPairStageBytes = (kPairM + kPairN) / 2 * kBlk;      // of one of the two CTAs
-
-struct PairParams {
-    CUtensorMap tmA, tmW;
-    const float *a_scales, *w_scales, *bias;
-    void* y;
-    int64_t a_scale_stride, w_scale_stride, y_stride;
-    int M, N, blocks, y_dtype, vec;
-    int m_tiles, n_tiles;
-    uint32_t idesc;
-    int* error;
-};
+constexpr int kPairM = 256;
+constexpr int kPairEpiWarps = 8;                 // two per TMEM lane quarter, half of the accumulator's columns each
+constexpr int pair_stage_bytes(int n) { return (kPairM + n) / 2 * kBlk; }      // of one of the two CTAs
+constexpr int pair_stages(int n) { return n == 256 ? 6 : 8; }
 
 // 32 rows x 128 bytes of results per warp, in units of 16 bytes that are XOR-ed with the row: a thread writes its row's units and
 // the warp reads whole rows, both without bank conflicts.
@@ -181,13 +308,13 @@ __device__ __forceinline__ uint32_t result_pair(float a, float b) {
     return rows::float_to_pair(a, b, T());
 }
 
-// Columns [col, col + kPairCols) of 32 rows from row0 on: sums in `acc` (a thread has a row), through shared memory to y in full lines.
-template <typename T>
-__device__ __forceinline__ void store_rows(const float (&acc)[kPairCols], uint8_t* stage, T* y, int64_t y_stride, const float* bias, int row0, int col, int M, int N,
+// Columns [col, col + kMine) of 32 rows from row0 on: sums in `acc` (a thread has a row), through shared memory to y in full lines.
+template <typename T, int kMine>
+__device__ __forceinline__ void store_rows(const float (&acc)[kMine], uint8_t* stage, T* y, int64_t y_stride, const float* bias, int row0, int col, int M, int N,
                                            bool vec, int lane) {
     constexpr int kPer = 16 / (int)sizeof(T), kCols = 8 * kPer;      // columns in a unit, in a pass
 #pragma unroll
-    for (int c0 = 0; c0 < kPairCols; c0 += kCols) {
+    for (int c0 = 0; c0 < kMine; c0 += kCols) {
         if (col + c0 >= N) break;
         const int left = N - col - c0;
 #pragma unroll
@@ -238,14 +365,16 @@ __device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int& m,
     m = first + r - n * size;
 }
 
-// Warp 0 loads, warp 1 issues the MMAs, two warpgroups keep the sums: 2 x 224 + 56 registers are the 3 x 168 of the launch.
+// Warps 0 and 2 load, warp 1 issues the MMAs, two warpgroups keep the sums: 2 x 224 + 56 registers are the 3 x 168 of the launch.
 constexpr int kPairThreads = 128 + kPairEpiWarps * 32;
 template <int kRegs> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 template <int kRegs> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 
-__global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const __grid_constant__ PairParams p) {
+template <int kPairN>
+__global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
+    constexpr int kPairStages = pair_stages(kPairN), kPairStageBytes = pair_stage_bytes(kPairN), kPairCols = kPairN / 2, kBufs = 512 / kPairN;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[kPairStages], empty_bar[kPairStages], tfull_bar[2], tempty_bar[2];
+    __shared__ __align__(8) uint64_t full_bar[kPairStages], empty_bar[kPairStages], tfull_bar[kBufs];
     __shared__ uint32_t tmem_base_smem;
     __shared__ int abort_flag;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -256,19 +385,16 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < kPairStages; ++s) {
-            ptx::mbar_init(&full_bar[s], 1);
+            ptx::mbar_init(&full_bar[s], 1 + 2 * kPairEpiWarps);
             ptx::mbar_init(&empty_bar[s], 1);
         }
-        for (int i = 0; i < 2; ++i) {
-            ptx::mbar_init(&tfull_bar[i], 1);
-            ptx::mbar_init(&tempty_bar[i], 2 * kPairEpiWarps);      // both CTAs' warps arrive at rank 0
-        }
+        for (int i = 0; i < kBufs; ++i) ptx::mbar_init(&tfull_bar[i], 1);
         ptx::fence_mbar_init();
         ptx::tma_prefetch_desc(&p.tmA);
         ptx::tma_prefetch_desc(&p.tmW);
     }
     if (warp == 1) {
-        ptx::tmem_alloc_pair(&tmem_base_smem, 2 * kPairN);
+        ptx::tmem_alloc_pair(&tmem_base_smem, 512);
         ptx::tmem_relinquish_pair();
     }
     ptx::tc_fence_before_sync();
@@ -277,128 +403,138 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
     ptx::tc_fence_after_sync();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_smem, 0);
     const uint32_t ring0 = ptx::smem_u32(ring), full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
-    const uint32_t tfull0 = ptx::smem_u32(tfull_bar), tempty0 = ptx::smem_u32(tempty_bar);
+    const uint32_t tfull0 = ptx::smem_u32(tfull_bar), full_lead = ptx::map_to_cta(full0, 0);
     pdl_wait();
     if (warp < 4) {
-    fewer_registers<56>();
-    if (warp == 0) {
-        if (lane == 0) {
-            const uint64_t mapA = reinterpret_cast<uint64_t>(&p.tmA), mapW = reinterpret_cast<uint64_t>(&p.tmW);
-            const uint32_t full_lead = ptx::map_to_cta(full0, 0);      // both CTAs' bytes are counted by rank 0
+        fewer_registers<56>();
+        // The MMAs of a block take 512 (256 columns) or 256 cycles, a wait for a barrier that is complete 90, a load 120 and more.  So
+        // the operands have a loading warp each (with one for both, its 560 cycles a block were what the kernel waited for), and the
+        // issuing warp has one wait per block: the epilogue warps' arrival that frees the accumulator of block g is counted by the
+        // barrier of the stage that block g + kBufs is loaded into.  (Lanes that look at a barrier each are no way out: one look at
+        // 12 barriers took 280 cycles.)
+        if (warp == 0 || warp == 2) {
+            const bool is_w = warp == 2;
+            const uint32_t leader = ptx::elect_one() ? 1u : 0u, counts = rank == 0 && !is_w ? leader : 0u;
+            const uint64_t map = is_w ? reinterpret_cast<uint64_t>(&p.tmW) : reinterpret_cast<uint64_t>(&p.tmA);
+            const uint32_t dst = ring0 + (is_w ? 128 * kBlk : 0);
             bool ok = true;
             int s = 0;
             uint32_t phase = 1;      // (a fresh barrier's previous phase counts as complete)
             for (int t = first; t < total && ok; t += step) {
                 int mt, nt;
                 tile_at(t, p.m_tiles, p.n_tiles, mt, nt);
-                const int m0 = mt * kPairM + rank * 128, n0 = nt * kPairN + rank * 128;
+                const int row0 = is_w ? nt * kPairN + rank * (kPairN / 2) : mt * kPairM + rank * 128;
                 for (int b = 0; b < p.blocks; ++b) {
-                    if (!ptx::mbar_wait_bounded_u32(empty0 + s * 8, phase, &abort_flag, kMaxSpins)) {
+                    if (!ptx::mbar_wait_quick_uniform(empty0 + s * 8, phase, &abort_flag, kMaxSpins)) {
                         ok = false;
                         break;
                     }
-                    if (rank == 0) ptx::mbar_arrive_expect_tx_u32(full0 + s * 8, 2 * kPairStageBytes);
-                    ptx::tma_load_2d_pair(ring0 + s * kPairStageBytes, mapA, full_lead + s * 8, b * kBlk, m0);
-                    ptx::tma_load_2d_pair(ring0 + s * kPairStageBytes + 128 * kBlk, mapW, full_lead + s * 8, b * kBlk, n0);
+                    // (both CTAs' bytes are counted by rank 0)
+                    ptx::mbar_arrive_expect_tx_u32(full0 + s * 8, 2 * kPairStageBytes, counts);
+                    ptx::tma_load_2d_pair(dst + s * kPairStageBytes, map, full_lead + s * 8, b * kBlk, row0, leader);
+                    __syncwarp();      // (see the other kernel's)
                     if (++s == kPairStages) {
                         s = 0;
                         phase ^= 1u;
                     }
                 }
             }
-            if (!ok) ptx::give_up(p.error, 1);
-        }
-        __syncwarp();
-    } else if (warp == 1) {
-        if (rank == 0) {      // issues for both
-            const uint32_t leader = ptx::elect_one() ? 1u : 0u;
-            const uint64_t d0 = ptx::make_smem_desc(ring0, kBlk);
-            const uint32_t desc_hi = (uint32_t)(d0 >> 32);
-            bool ok = true;
-            int s = 0, buf = 0;
-            uint32_t phase = 0, acc_phase = 1;
-            for (int t = first; t < total && ok; t += step) {
-                for (int b = 0; b < p.blocks; ++b) {
-                    // (the loads are ahead: what is waited for last is what comes last)
-                    if (!ptx::mbar_wait_bounded_uniform(full0 + s * 8, phase, &abort_flag, kMaxSpins) ||
-                        !ptx::mbar_wait_bounded_uniform(tempty0 + buf * 8, acc_phase, &abort_flag, kMaxSpins)) {
-                        ok = false;
-                        break;
-                    }
-                    ptx::tc_fence_after_sync();
-                    const uint32_t a_lo = (uint32_t)d0 + ((uint32_t)(s * kPairStageBytes) >> 4), w_lo = a_lo + ((128 * kBlk) >> 4);
+            if (!ok && lane == 0) ptx::give_up(p.error, 1);
+            __syncwarp();
+        } else if (warp == 1) {
+            if (rank == 0) {      // issues for both
+                const uint32_t leader = ptx::elect_one() ? 1u : 0u;
+                const uint64_t d0 = ptx::make_smem_desc(ring0, kBlk);
+                const uint32_t desc_hi = (uint32_t)(d0 >> 32);
+                bool ok = true;
+                int s = 0, buf = 0;
+                uint32_t phase = 0;
+                for (int t = first; t < total && ok; t += step) {
+                    for (int b = 0; b < p.blocks; ++b) {
+                        if (!ptx::mbar_wait_quick_uniform(full0 + s * 8, phase, &abort_flag, kMaxSpins)) {
+                            ok = false;
+                            break;
+                        }
+                        ptx::tc_fence_after_sync();
+                        const uint32_t a_lo = (uint32_t)d0 + ((uint32_t)(s * kPairStageBytes) >> 4), w_lo = a_lo + ((128 * kBlk) >> 4);
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks)
-                        ptx::tc_mma_f8<true>(tmem_base + buf * kPairN, a_lo + 2 * ks, w_lo + 2 * ks, desc_hi, p.idesc, ks ? 1u : 0u, leader);
-                    ptx::tc_commit_pair_u32(empty0 + s * 8, leader);
-                    ptx::tc_commit_pair_u32(tfull0 + buf * 8, leader);
-                    if (++s == kPairStages) {
-                        s = 0;
-                        phase ^= 1u;
+                        for (int ks = 0; ks < 4; ++ks)
+                            ptx::tc_mma_f8<true>(tmem_base + buf * kPairN, a_lo + 2 * ks, w_lo + 2 * ks, desc_hi, p.idesc, ks ? 1u : 0u, leader);
+                        ptx::tc_commit_pair_u32(tfull0 + buf * 8, leader);
+                        ptx::tc_commit_pair_u32(empty0 + s * 8, leader);
+                        __syncwarp();
+                        if (++s == kPairStages) {
+                            s = 0;
+                            phase ^= 1u;
+                        }
+                        if (++buf == kBufs) buf = 0;
                     }
-                    if (buf ^= 1; buf == 0) acc_phase ^= 1u;
                 }
+                if (!ok) ptx::give_up(p.error, 2);
             }
-            if (!ok) ptx::give_up(p.error, 2);
+            __syncwarp();
         }
-        __syncwarp();
-    }
     } else {
         more_registers<224>();
         const int q = warp & 3, part = (warp >> 2) - 1;
         uint8_t* stage = ring + kPairStages * kPairStageBytes + (warp - 4) * kStageOut;
         const uint32_t taddr0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(part * kPairCols);
-        const uint32_t tempty_lead = ptx::map_to_cta(tempty0, 0);
         bool ok = true;
-        int buf = 0;
+        int buf = 0, next = kBufs;      // accumulator, and the stage of the block that takes it next
         uint32_t acc_phase = 0;
+        if (lane < kBufs) ptx::mbar_arrive_cluster_u32(full_lead + lane * 8);      // all accumulators are free
+        __syncwarp();
         for (int t = first; t < total && ok; t += step) {
             int mt, nt;
             tile_at(t, p.m_tiles, p.n_tiles, mt, nt);
             const int row = mt * kPairM + rank * 128 + q * 32 + lane, col = nt * kPairN + part * kPairCols;
-            // this row's and these columns' scales of the next two blocks are on their way while one is worked on
+            // This row's and these columns' scales: two blocks' are on their way, each in registers of its own (a register that is
+            // moved has to be there first, and the loop would wait for memory in every block).
             const float* sa = p.a_scales + (row < p.M ? row : 0);
             const float* sw = p.w_scales + (int64_t)(col < p.N ? col / kBlk : 0) * p.w_scale_stride;
-            float sa0 = __ldg(sa), sw0 = __ldg(sw), sa1 = 0.f, sw1 = 0.f;
+            float a_scale[2] = {__ldg(sa), 0.f}, w_scale[2] = {__ldg(sw), 0.f};
             if (p.blocks > 1) {
-                sa1 = __ldg(sa += p.a_scale_stride);
-                sw1 = __ldg(++sw);
+                a_scale[1] = __ldg(sa += p.a_scale_stride);
+                w_scale[1] = __ldg(++sw);
             }
             float acc[kPairCols];
 #pragma unroll
             for (int i = 0; i < kPairCols; ++i) acc[i] = 0.f;
-            for (int b = 0; b < p.blocks; ++b) {
-                float sa2 = 0.f, sw2 = 0.f;
-                if (b + 2 < p.blocks) {
-                    sa2 = __ldg(sa += p.a_scale_stride);
-                    sw2 = __ldg(++sw);
-                }
-                if (!ptx::mbar_wait_bounded_uniform(tfull0 + buf * 8, acc_phase, &abort_flag, kMaxSpins)) {
-                    ok = false;
-                    break;
-                }
-                __syncwarp();      // (what follows needs the warp together)
-                ptx::tc_fence_after_sync();
-                const uint32_t taddr = taddr0 + (uint32_t)(buf * kPairN);
-                const float s = sa0 * sw0;
+            for (int b = 0; b < p.blocks && ok; b += 2) {
 #pragma unroll
-                for (int c = 0; c < kPairCols; c += 16) {
-                    uint32_t raw[16];
-                    ptx::tmem_ld_32x32b_x16(taddr + c, raw);
-                    ptx::tmem_ld_wait(raw);
-                    if (c + 16 == kPairCols) {
-                        ptx::tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) ptx::mbar_arrive_cluster_u32(tempty_lead + buf * 8);
+                for (int k = 0; k < 2; ++k) {
+                    if (b + k >= p.blocks) break;
+                    const float s = a_scale[k] * w_scale[k];
+                    if (b + k + 2 < p.blocks) {
+                        a_scale[k] = __ldg(sa += p.a_scale_stride);
+                        w_scale[k] = __ldg(++sw);
                     }
+                    if (!ptx::mbar_wait_quick_uniform(tfull0 + buf * 8, acc_phase, &abort_flag, kMaxSpins)) {
+                        ok = false;
+                        break;
+                    }
+                    __syncwarp();      // (what follows needs the warp together)
+                    ptx::tc_fence_after_sync();
+                    const uint32_t taddr = taddr0 + (uint32_t)(buf * kPairN);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(__uint_as_float(raw[j]), s, acc[c + j]);
+                    for (int c = 0; c < kPairCols; c += 16) {
+                        uint32_t raw[16];
+                        ptx::tmem_ld_32x32b_x16(taddr + c, raw);
+                        ptx::tmem_ld_wait(raw);
+                        if (c + 16 == kPairCols) {
+                            ptx::tc_fence_before_sync();
+                            __syncwarp();
+                            if (lane == 0) ptx::mbar_arrive_cluster_u32(full_lead + next * 8);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(__uint_as_float(raw[j]), s, acc[c + j]);
+                    }
+                    if (++next == kPairStages) next = 0;
+                    if (++buf == kBufs) {
+                        buf = 0;
+                        acc_phase ^= 1u;
+                    }
                 }
-                sa0 = sa1;
-                sw0 = sw1;
-                sa1 = sa2;
-                sw1 = sw2;
-                if (buf ^= 1; buf == 0) acc_phase ^= 1u;
             }
             if (!ok) break;
             const int row0 = row - lane;
@@ -413,8 +549,37 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
     ptx::cluster_sync();      // neither CTA leaves while its peer may still signal its barriers or read its TMEM
     if (warp == 1) {
         ptx::tc_fence_after_sync();
-        ptx::tmem_dealloc_pair(tmem_base, 2 * kPairN);
+        ptx::tmem_dealloc_pair(tmem_base, 512);
     }
+}
+
+// Which kernel and how it divides the product: the one whose time is least by what was measured of each (graph-captured calls, us):
+//  - few rows, up to 64 columns: the only one that does not compute rows that are not there;
+//  - few rows, 128 columns: 4.5 + 2 where K is divided + 0.58 for each K block that a CTA works on one after the other
+//    (128 x 14336 x 4096 21.6; 128 x 4096 x 4096 in four parts 11.1);
+//  - pairs with tiles of 128 columns: 4.5 + 0.335 a block (512 x 4096 x 4096 14.9, in 256 columns 18.1);
+//  - pairs with tiles of 256 columns: 5 + 0.43 a block (256 x 14336 x 4096 19.9, in 128 columns 25.5; 4096^3 67 and 81).
+struct Plan {
+    bool few;
+    int tile, splits;      // columns of a tile
+};
+Plan plan_for(int sms, int M, int N, int blocks) {
+    const int64_t n_tiles = ((int64_t)N + 127) / 128;
+    // parts of K: as many as there are places for, of at least two blocks each
+    auto parts = [&](int64_t tiles, int64_t places) {
+        int s = 1;
+        while (s < 8 && tiles * s * 2 <= places && s * 4 <= blocks) s *= 2;
+        return s;
+    };
+    if (M <= 64) return {true, M <= 16 ? 16 : M <= 32 ? 32 : 64, parts(n_tiles, 2 * sms)};
+    auto rounds = [](int64_t tiles, int64_t places) { return (double)((tiles + places - 1) / places); };
+    const int64_t few_tiles = ((int64_t)M + 127) / 128 * n_tiles, m_pairs = ((int64_t)M + kPairM - 1) / kPairM;
+    const int splits = parts(few_tiles, sms);
+    const double few = 4.5 + (splits > 1 ? 2.0 : 0.0) + 0.58 * rounds(few_tiles * splits, sms) * ((blocks + splits - 1) / splits);
+    const double pair128 = 4.5 + 0.335 * rounds(m_pairs * n_tiles, sms / 2) * blocks;
+    const double pair256 = 5.0 + 0.43 * rounds(m_pairs * (((int64_t)N + 255) / 256), sms / 2) * blocks;
+    if (few < pair128 && few < pair256 && few_tiles / n_tiles <= 65535) return {true, 128, splits};
+    return {false, pair128 < pair256 ? 128 : 256, 1};
 }
 
 // Rows of K bytes in boxes of 128 bytes x box_rows, 128-byte swizzle; zeros beyond the matrix.
@@ -452,35 +617,48 @@ extern "C" int exb_fp8_matmul_fwd(exb_ctx* ctx, const uint8_t* a, int64_t a_stri
                 "exb_fp8_matmul_fwd: the rows of a and w must start at multiples of 16 bytes");
     EXB_REQUIRE(rows::aligned_to(y, es) && rows::aligned_to(a_scales, 4) && rows::aligned_to(w_scales, 4) && rows::aligned_to(bias, 4),
                 "exb_fp8_matmul_fwd: y, scales or bias not aligned to its element");
-    if (M > 128) {
-        PairParams p;
-        if (int rc = encode(&p.tmA, a, M, K, a_stride, 128)) return rc;
-        if (int rc = encode(&p.tmW, w, N, K, w_stride, 128)) return rc;
-        p.a_scales = a_scales; p.w_scales = w_scales; p.bias = bias; p.y = y;
-        p.a_scale_stride = a_scale_stride; p.w_scale_stride = w_scale_stride; p.y_stride = y_stride;
-        p.M = (int)M; p.N = N; p.blocks = blocks; p.y_dtype = y_dtype;
-        p.vec = rows::vector_rows(y, y_stride, es);
-        p.m_tiles = (int)((M + kPairM - 1) / kPairM);
-        p.n_tiles = (N + kPairN - 1) / kPairN;
-        if ((int64_t)p.m_tiles * p.n_tiles > INT32_MAX / 2) return fail(EXB_ERR_UNSUPPORTED, "exb_fp8_matmul_fwd: %lld x %d is too large for one call", (long long)M, N);
-        p.idesc = ptx::make_idesc(false, kPairM, kPairN);
-        p.error = ctx->d_error;
-        const int tiles = p.m_tiles * p.n_tiles, places = ctx->sm_count / 2;
-        if (int rc = raise_smem_limit(ctx, fp8_matmul_pair_kernel)) return rc;
-        return launch_pdl_cluster(ctx, "fp8_matmul_pair_kernel", fp8_matmul_pair_kernel, dim3(2 * (tiles < places ? tiles : places)), dim3(kPairThreads), dim3(2),
-                                  (size_t)kPairStages * kPairStageBytes + kPairEpiWarps * kStageOut + 1024, static_cast<cudaStream_t>(stream), p);
-    }
     MatmulParams p;
-    if (int rc = encode(&p.tmA, a, M, K, a_stride, kTileM)) return rc;
-    if (int rc = encode(&p.tmW, w, N, K, w_stride, kTileN)) return rc;
     p.a_scales = a_scales; p.w_scales = w_scales; p.bias = bias; p.y = y;
     p.a_scale_stride = a_scale_stride; p.w_scale_stride = w_scale_stride; p.y_stride = y_stride;
     p.M = (int)M; p.N = N; p.blocks = blocks; p.y_dtype = y_dtype;
-    p.idesc = ptx::make_idesc(false, kTileM, kTileN);
+    p.vec = rows::vector_rows(y, y_stride, es);
     p.error = ctx->d_error;
-    const int64_t gy = (M + kTileM - 1) / kTileM;
-    if (gy > 65535) return fail(EXB_ERR_UNSUPPORTED, "exb_fp8_matmul_fwd: %lld rows are too many for one call", (long long)M);
-    if (int rc = raise_smem_limit(ctx, fp8_matmul_kernel)) return rc;
-    return launch_pdl(ctx, "fp8_matmul_kernel", fp8_matmul_kernel, dim3((N + kTileN - 1) / kTileN, (unsigned)gy), dim3(kThreads),
-                      (size_t)kStages * kStageBytes + 1024, static_cast<cudaStream_t>(stream), p);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const Plan plan = plan_for(ctx->sm_count, (int)M, N, blocks);
+    if ((int64_t)((M + 127) / 128) * ((N + 127) / 128) > INT32_MAX / 16)
+        return fail(EXB_ERR_UNSUPPORTED, "exb_fp8_matmul_fwd: %lld x %d is too large for one call", (long long)M, N);
+    if (plan.few) {
+        const int cols = plan.tile;
+        p.m_tiles = (int)((M + cols - 1) / cols);
+        p.n_tiles = (N + 127) / 128;
+        p.splits = plan.splits;
+        if (int rc = encode(&p.tmA, a, M, K, a_stride, cols)) return rc;
+        if (int rc = encode(&p.tmW, w, N, K, w_stride, 128)) return rc;
+        p.idesc = ptx::make_idesc(false, 128, (uint32_t)cols);
+        auto go = [&](auto c) {
+            constexpr int kCols = decltype(c)::value;
+            if (int rc = raise_smem_limit(ctx, fp8_matmul_few_kernel<kCols>)) return rc;
+            return launch_pdl_cluster(ctx, "fp8_matmul_few_kernel", fp8_matmul_few_kernel<kCols>, dim3((unsigned)p.n_tiles * p.splits, (unsigned)p.m_tiles),
+                                      dim3(96 + few_epi_warps(kCols) * 32), dim3(p.splits), (size_t)few_smem(kCols), st, p);
+        };
+        if (cols == 16) return go(std::integral_constant<int, 16>());
+        if (cols == 32) return go(std::integral_constant<int, 32>());
+        if (cols == 64) return go(std::integral_constant<int, 64>());
+        return go(std::integral_constant<int, 128>());
+    }
+    if (int rc = encode(&p.tmA, a, M, K, a_stride, 128)) return rc;
+    const int wide = plan.tile;
+    if (int rc = encode(&p.tmW, w, N, K, w_stride, wide / 2)) return rc;
+    p.m_tiles = (int)((M + kPairM - 1) / kPairM);
+    p.n_tiles = (N + wide - 1) / wide;
+    p.splits = 1;
+    p.idesc = ptx::make_idesc(false, kPairM, (uint32_t)wide);
+    const int tiles = p.m_tiles * p.n_tiles, places = ctx->sm_count / 2;
+    auto go = [&](auto c) {
+        constexpr int kN = decltype(c)::value;
+        if (int rc = raise_smem_limit(ctx, fp8_matmul_pair_kernel<kN>)) return rc;
+        return launch_pdl_cluster(ctx, "fp8_matmul_pair_kernel", fp8_matmul_pair_kernel<kN>, dim3(2 * (tiles < places ? tiles : places)), dim3(kPairThreads), dim3(2),
+                                  (size_t)pair_stages(kN) * pair_stage_bytes(kN) + kPairEpiWarps * kStageOut + 1024, st, p);
+    };
+    return wide == 256 ? go(std::integral_constant<int, 256>()) : go(std::integral_constant<int, 128>());
 }
