@@ -101,25 +101,38 @@ __global__ void __launch_bounds__(max_threads(kOneWarp, kPer)) residual_norm_ker
     const T* g = static_cast<const T*>(a.gate) + (a.gate_rows ? row / a.gate_rows : 0) * a.gate_stride;
     // everything is asked for before anything is waited for, as long as there are registers for it
     constexpr bool kAhead = kPer <= 4;
-    float v[kPer][8], xv[kAhead ? kPer : 1][8], gv[kAhead ? kPer : 1][8];
+    constexpr int kKept = kAhead ? kPer : 1;
+    float v[kPer][8];
+    Kept<T, kVec> hk[kPer], xk[kKept], gk[kKept];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int c0 = (share0 + i * share_step) * kShare, valid = a.C - c0;
-        load8<T, kVec>(h + c0, valid, lane, v[i]);
-        if (kAhead && a.x) load8<T, kVec>(x + c0, valid, lane, xv[kAhead ? i : 0]);
-        if (kAhead && a.gate) load8<T, kVec>(g + c0, valid, lane, gv[kAhead ? i : 0]);
+        hk[i].load(h + c0, valid, lane);
+        if (kAhead && a.x) xk[kAhead ? i : 0].load(x + c0, valid, lane);
+        if (kAhead && a.gate) gk[kAhead ? i : 0].load(g + c0, valid, lane);
     }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) hk[i].get(v[i]);
     if (a.post_weight) normalise<kLayer, kVec, kOneWarp, kPer>(v, lane, share0, share_step, a, a.post_weight, a.post_bias, s_sum, turn);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int c0 = (share0 + i * share_step) * kShare, valid = a.C - c0;
         constexpr int kAll = kAhead ? 1 : 0;
-        if (!kAhead && a.x) load8<T, kVec>(x + c0, valid, lane, xv[0]);
-        if (!kAhead && a.gate) load8<T, kVec>(g + c0, valid, lane, gv[0]);
+        if (!kAhead && a.x) xk[0].load(x + c0, valid, lane);
+        if (!kAhead && a.gate) gk[0].load(g + c0, valid, lane);
+        float o[8];
+        if (a.gate) {
+            gk[i * kAll].get(o);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (a.gate) v[i][j] *= gv[i * kAll][j];
-            v[i][j] = a.x ? fmaf(a.residual_scale, v[i][j], xv[i * kAll][j]) : a.residual_scale * v[i][j];
+            for (int j = 0; j < 8; ++j) v[i][j] *= o[j];
+        }
+        if (a.x) {
+            xk[i * kAll].get(o);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = fmaf(a.residual_scale, v[i][j], o[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] *= a.residual_scale;
         }
         if (a.r) store8<T, kVec>(static_cast<T*>(a.r) + row * a.r_stride + c0, valid, lane, v[i]);
     }

@@ -11,7 +11,7 @@
 // are put in order by counting for each how many are before it.  Logits and indexes make keys that are all different, so that
 // equal logits, masked ones among them, need nothing else.
 //
-// A row that the pass cannot answer (a NaN or plus infinity in it, nothing but masks of fp32's or bf16's lowest value, or more
+// A row that the pass cannot answer (a NaN or plus infinity in it, nothing but masks or logits at the type's lowest end, or more
 // elements from tau on than there is room for) is answered by slow_row: the maximum, the sums about it, and one pass per token.
 #include "ptx_sm100.cuh"
 #include "rows_common.cuh"
@@ -59,29 +59,66 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// The largest of a 16-byte vector of logits, NaN if one is.
-__device__ __forceinline__ float largest(const uint4& v, float) {
-    return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
-}
-__device__ __forceinline__ float largest(const uint4& v, __half) {
-    const __half2* h = reinterpret_cast<const __half2*>(&v);
-    const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-    return __half2float(__hmax_nan(__low2half(m), __high2half(m)));
-}
-__device__ __forceinline__ float largest(const uint4& v, __nv_bfloat16) {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-    return __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
-}
+// A 16-byte vector of logits: the largest of its parts (NaN if one is) kept packed, its elements, and these no lower than kLow (minus
+// infinity would make 0 * infinity of p * t).
 template <typename T>
-__device__ __forceinline__ void elements(const uint4& v, float (&x)[16 / sizeof(T)]) {
-    if constexpr (sizeof(T) == 4) {
-        x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
-    } else {
-        const float2 a = pair_to_float(v.x, T()), b = pair_to_float(v.y, T()), c = pair_to_float(v.z, T()), d = pair_to_float(v.w, T());
-        x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y; x[4] = c.x; x[5] = c.y; x[6] = d.x; x[7] = d.y;
+struct Vec;
+template <>
+struct Vec<float> {
+    static constexpr int kCount = 4;
+    static constexpr float kLow = -1e30f;
+    typedef float Max;
+    static __device__ __forceinline__ Max largest(const uint4& v) {
+        return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
     }
-}
+    static __device__ __forceinline__ Max larger(Max a, Max b) { return max_nan(a, b); }
+    static __device__ __forceinline__ float value(Max m) { return m; }
+    static __device__ __forceinline__ void elements(const uint4& v, float2 (&x)[2]) {
+        x[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+        x[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+    }
+    static __device__ __forceinline__ void bounded(const uint4& v, float2 (&x)[2]) {
+        elements(v, x);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) x[j] = make_float2(fmaxf(x[j].x, kLow), fmaxf(x[j].y, kLow));
+    }
+};
+template <typename T, typename T2>
+struct Vec16 {
+    static constexpr int kCount = 8;
+    typedef T2 Max;
+    static __device__ __forceinline__ T2 part(uint32_t v) { return *reinterpret_cast<const T2*>(&v); }
+    static __device__ __forceinline__ Max largest(const uint4& v) {
+        return __hmax2_nan(__hmax2_nan(part(v.x), part(v.y)), __hmax2_nan(part(v.z), part(v.w)));
+    }
+    static __device__ __forceinline__ Max larger(Max a, Max b) { return __hmax2_nan(a, b); }
+    static __device__ __forceinline__ float value(Max m) {
+        const float2 f = pair_to_float(*reinterpret_cast<const uint32_t*>(&m), T());
+        return max_nan(f.x, f.y);
+    }
+    static __device__ __forceinline__ void elements(const uint4& v, float2 (&x)[4]) {
+        x[0] = pair_to_float(v.x, T());
+        x[1] = pair_to_float(v.y, T());
+        x[2] = pair_to_float(v.z, T());
+        x[3] = pair_to_float(v.w, T());
+    }
+    static __device__ __forceinline__ void bounded_by(const uint4& v, uint32_t low, float2 (&x)[4]) {
+        const T2 l = part(low);
+        const T2 a = __hmax2(part(v.x), l), b = __hmax2(part(v.y), l), c = __hmax2(part(v.z), l), d = __hmax2(part(v.w), l);
+        elements(make_uint4(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b), *reinterpret_cast<const uint32_t*>(&c),
+                            *reinterpret_cast<const uint32_t*>(&d)), x);
+    }
+};
+template <>
+struct Vec<__half> : Vec16<__half, __half2> {
+    static constexpr float kLow = -65504.f;
+    static __device__ __forceinline__ void bounded(const uint4& v, float2 (&x)[4]) { bounded_by(v, 0xfbfffbffu, x); }
+};
+template <>
+struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16, __nv_bfloat162> {
+    static constexpr float kLow = -9.9e29f;      // (0xf149 is lower)
+    static __device__ __forceinline__ void bounded(const uint4& v, float2 (&x)[4]) { bounded_by(v, 0xf149f149u, x); }
+};
 
 // Sums about a thread's (or a row's) reference e, and its largest logit.
 struct alignas(16) Sums {
@@ -99,6 +136,105 @@ __device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
     return r;
 }
 
+constexpr int kAhead = 4;      // vectors that a thread works on at a time; as many are on their way
+
+// What a thread keeps of the logits that it has seen.
+template <typename T>
+struct Seen {
+    Sums r = {-INFINITY, 0.f, 0.f, -INFINITY};
+    float2 s2 = {0.f, 0.f}, w2 = {0.f, 0.f};      // on top of r.s and r.w
+    int at = -1;                                   // where r.m is: vector at, or the head's element (-1) or the tail's (-2)
+    bool any = false;
+    float c;
+
+    __device__ __forceinline__ void fold() {
+        r.s += s2.x + s2.y;
+        r.w += w2.x + w2.y;
+        s2 = w2 = make_float2(0.f, 0.f);
+    }
+    // a new largest logit: does e still serve?
+    __device__ __forceinline__ void rise(float v, int where) {
+        if (v != v) {
+            r.s = NAN;
+            return;
+        }
+        r.m = v;
+        at = where;
+        const float e = ceilf(v * c);
+        if (e > r.e + 4.f) {
+            if (r.e != -INFINITY) {
+                const float d = r.e - e, f = exp2_fast(d);
+                r.w = (r.w + d * r.s) * f;
+                r.s *= f;
+            }
+            r.e = e;
+        }
+    }
+    __device__ __forceinline__ void single(float v, int where) {
+        any = true;
+        if (!(v <= r.m)) rise(v, where);
+        if (r.m != -INFINITY) {
+            const float t = fmaxf(fmaf(v, c, -r.e), -200.f), p = exp2_fast(t);
+            r.s += p;
+            r.w = fmaf(p, t, r.w);
+        }
+    }
+    // n of the vectors are there, `step` apart from `first` on
+    __device__ __forceinline__ void vectors(const uint4 (&q)[kAhead], int n, int first, int step) {
+        typename Vec<T>::Max m = Vec<T>::largest(q[0]);
+#pragma unroll
+        for (int j = 1; j < kAhead; ++j)
+            if (j < n) m = Vec<T>::larger(m, Vec<T>::largest(q[j]));
+        const float top = Vec<T>::value(m);
+        if (!(top <= r.m)) {
+            fold();
+            int j = 0;
+            if (top == top)
+                while (j < kAhead - 1 && Vec<T>::value(Vec<T>::largest(j == 0 ? q[0] : j == 1 ? q[1] : q[2])) != top) ++j;
+            rise(top, first + j * step);
+        }
+        if (r.m == -INFINITY) return;      // nothing but masks so far
+        const float2 cc = make_float2(c, c), ee = make_float2(-r.e, -r.e);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            if (j >= n) break;
+            constexpr int kPairs = Vec<T>::kCount / 2;
+            float2 x[kPairs];
+            Vec<T>::bounded(q[j], x);
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                const float2 t = __ffma2_rn(x[k], cc, ee), p = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+                s2 = __fadd2_rn(s2, p);
+                w2 = __ffma2_rn(p, t, w2);
+            }
+        }
+    }
+    // all of this thread's share of the vectors: from `first` on every `step`-th below `end`
+    __device__ __forceinline__ void stream(const uint4* body, int first, int end, int step) {
+        int i = first;
+        if (i < end) {
+            if (!any) at = i;
+            any = true;
+        }
+        uint4 q[kAhead];
+        auto fetch = [&](int from) {
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (from + j * step < end) q[j] = __ldg(body + from + j * step);
+        };
+        if (i < end) fetch(i);
+        for (; i + (kAhead - 1) * step < end; i += kAhead * step) {
+            uint4 now[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) now[j] = q[j];
+            if (i + kAhead * step < end) fetch(i + kAhead * step);
+            vectors(now, kAhead, i, step);
+        }
+        if (i < end) vectors(q, (end - i + step - 1) / step, i, step);
+        fold();
+    }
+};
+
 constexpr int kSplitMax = 8;      // CTAs that share a row
 constexpr int kRoom = 512;        // elements from tau on that are put in order
 
@@ -115,15 +251,23 @@ struct Shared {
     float part_f[kThreads / 32];
 };
 
+// Barriers and reductions of the threads that work on a row: a CTA, or a warp (kThreads 32).
+template <int kThreads>
+__device__ __forceinline__ void sync() {
+    if constexpr (kThreads == 32) __syncwarp();
+    else __syncthreads();
+}
 template <int kThreads, typename F>
-__device__ __forceinline__ float block_reduce(float v, float* s_part, F op) {
+__device__ __forceinline__ float group_reduce(float v, float* s_part, F op) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = s_part[0];
-    for (int i = 1; i < kThreads / 32; ++i) v = op(v, s_part[i]);
+    if constexpr (kThreads > 32) {
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = s_part[0];
+        for (int i = 1; i < kThreads / 32; ++i) v = op(v, s_part[i]);
+    }
     return v;
 }
 
@@ -138,6 +282,12 @@ struct Row {
     }
 };
 
+// Whether the pass has answered the row: its sum is a number, and what was taken for kLow has added nothing to it.
+template <typename T>
+__device__ __forceinline__ bool row_known(const Sums& all, float c) {
+    return all.s > 0.f && all.s < INFINITY && fmaf(Vec<T>::kLow, c, -all.e) < -150.f;
+}
+
 template <typename T>
 __device__ __forceinline__ void write_given(const LogprobArgs& a, const T* x, int64_t row, const Row& r, int first, int step) {
     for (int j = first; j < a.n_given; j += step) {
@@ -147,40 +297,41 @@ __device__ __forceinline__ void write_given(const LogprobArgs& a, const T* x, in
 }
 
 template <typename T, int kThreads>
-__device__ __noinline__ void slow_row(const LogprobArgs& a, const T* x, int64_t row, Shared<kThreads>& sh, bool sums_known, Row r) {
+__device__ __noinline__ void slow_row(const LogprobArgs& a, const T* x, int64_t row, float* s_part, unsigned long long* s_best, bool sums_known, Row r) {
+    const int tid = kThreads == 32 ? threadIdx.x & 31 : threadIdx.x;
     if (!sums_known) {
         const float c = a.scale * kLog2e;
         float m = -INFINITY, s = 0.f, w = 0.f;
-        for (int i = threadIdx.x; i < a.V; i += kThreads) m = fmaxf(m, to_float<T>(x[i]));
-        m = block_reduce<kThreads>(m, sh.part_f, [](float u, float v) { return fmaxf(u, v); });
-        for (int i = threadIdx.x; i < a.V; i += kThreads) {
+        for (int i = tid; i < a.V; i += kThreads) m = fmaxf(m, to_float<T>(x[i]));
+        m = group_reduce<kThreads>(m, s_part, [](float u, float v) { return fmaxf(u, v); });
+        for (int i = tid; i < a.V; i += kThreads) {
             const float v = to_float<T>(x[i]), t = (v - m) * c, p = v == -INFINITY ? 0.f : exp2f(t);
             s += p;
             w += p == 0.f ? 0.f : p * t;
         }
-        s = block_reduce<kThreads>(s, sh.part_f, [](float u, float v) { return u + v; });
-        w = block_reduce<kThreads>(w, sh.part_f, [](float u, float v) { return u + v; });
+        s = group_reduce<kThreads>(s, s_part, [](float u, float v) { return u + v; });
+        w = group_reduce<kThreads>(w, s_part, [](float u, float v) { return u + v; });
         r.m = m;
         r.log_s = log2f(s);
         r.empty = !(s != 0.f);       // (a NaN anywhere makes s one)
         r.entropy = r.empty ? 0.f : (r.log_s - w / s) * kLn2;
-        if (threadIdx.x == 0 && a.entropy) a.entropy[row] = r.entropy;
-        write_given<T>(a, x, row, r, threadIdx.x, kThreads);
+        if (tid == 0 && a.entropy) a.entropy[row] = r.entropy;
+        write_given<T>(a, x, row, r, tid, kThreads);
     }
     unsigned long long last = ~0ull;
     for (int j = 0; j < a.top; ++j) {
         unsigned long long best = 0;
-        for (int i = threadIdx.x; i < a.V; i += kThreads) {
+        for (int i = tid; i < a.V; i += kThreads) {
             const unsigned long long k = key_of(to_float<T>(x[i]), i);
             if (k < last && k > best) best = k;
         }
-        __syncthreads();
-        if (threadIdx.x == 0) sh.tau = 0;
-        __syncthreads();
-        atomicMax(&sh.tau, best);
-        __syncthreads();
-        last = sh.tau;
-        if (threadIdx.x == 0) {
+        sync<kThreads>();
+        if (tid == 0) *s_best = 0;
+        sync<kThreads>();
+        atomicMax(s_best, best);
+        sync<kThreads>();
+        last = *static_cast<volatile unsigned long long*>(s_best);
+        if (tid == 0) {
             const int token = index_of(last);
             a.top_tokens[row * a.top + j] = token;
             a.top_logprobs[row * a.top + j] = r.logprob(to_float<T>(x[token]));
@@ -188,21 +339,137 @@ __device__ __noinline__ void slow_row(const LogprobArgs& a, const T* x, int64_t 
     }
 }
 
+// Where a row's whole 16-byte vectors are, and the single elements before (head) and behind them (tail).
+template <typename T>
+struct Parts {
+    int head, vecs, tail0;
+    const uint4* body;
+    __device__ __forceinline__ Parts(const T* x, int V) {
+        head = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T), V);
+        vecs = (V - head) / Vec<T>::kCount;
+        tail0 = head + vecs * Vec<T>::kCount;
+        body = reinterpret_cast<const uint4*>(x + head);
+    }
+};
+
+// The lanes' sums joined, in the same order in all of them.
+__device__ __forceinline__ Sums warp_sums(Sums all, int lane) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const Sums other = {__shfl_xor_sync(0xffffffffu, all.e, o), __shfl_xor_sync(0xffffffffu, all.s, o), __shfl_xor_sync(0xffffffffu, all.w, o),
+                            __shfl_xor_sync(0xffffffffu, all.m, o)};
+        all = (lane & o) ? joined(other, all) : joined(all, other);
+    }
+    return all;
+}
+
+// A warp's row each: short rows, whose exchange between warps would take longer than their reading.
+constexpr int kWarpRows = 4, kWarpRoom = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(kWarpRows * 32) token_logprobs_warp_kernel(const __grid_constant__ LogprobArgs a, int64_t n_rows) {
+    constexpr int kVec = Vec<T>::kCount;
+    __shared__ unsigned long long s_list[kWarpRows][kWarpRoom], s_best[kWarpRows];
+    __shared__ int s_n[kWarpRows];
+    pdl_enter();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = (int64_t)blockIdx.x * kWarpRows + warp;
+    if (row >= n_rows) return;
+    const T* x = static_cast<const T*>(a.logits) + row * a.stride;
+    const Parts<T> part(x, a.V);
+    const int n_tail = a.V - part.tail0;
+    if (lane == 0) s_n[warp] = 0;
+    Seen<T> seen;
+    seen.c = a.scale * kLog2e;
+    if (lane < part.head) seen.single(to_float<T>(x[lane]), -1);
+    seen.stream(part.body, lane, part.vecs, 32);
+    if (lane < n_tail) {
+        if (!seen.any) seen.at = -2;
+        seen.single(to_float<T>(x[part.tail0 + lane]), -2);
+    }
+    const Sums all = warp_sums(seen.r, lane);
+    Row out;
+    out.scale = a.scale;
+    out.m = all.m;
+    out.empty = false;
+    const bool known = row_known<T>(all, a.scale * kLog2e);
+    if (known) {
+        const float log_s = log2f(all.s);
+        out.entropy = (log_s - all.w / all.s) * kLn2;
+        out.log_s = log_s - fmaf(all.m, seen.c, -all.e);
+        if (lane == 0 && a.entropy) a.entropy[row] = out.entropy;
+        write_given<T>(a, x, row, out, lane, 32);
+    }
+    bool slow = !known;
+    if (known && a.top) {
+        // tau: the top-th largest of the lanes' largest, taken out one after the other
+        const int first_index = seen.at == -1 ? lane : seen.at == -2 ? part.tail0 + lane : part.head + seen.at * kVec;
+        const unsigned long long low = seen.any ? key_of(seen.r.m, first_index + (seen.at >= 0 ? kVec - 1 : 0)) : 0;
+        const unsigned long long high = seen.any ? key_of(seen.r.m, first_index) : 0;
+        uint32_t hi = (uint32_t)(low >> 32), lo = (uint32_t)low;
+        unsigned long long tau = 0;
+        for (int j = 0; j < a.top; ++j) {
+            const uint32_t m = __reduce_max_sync(0xffffffffu, hi);
+            if (m == 0) {      // fewer lanes than tokens: every element is one to look at
+                tau = 0;
+                break;
+            }
+            const uint32_t l = __reduce_max_sync(0xffffffffu, hi == m ? lo : 0u);
+            tau = (unsigned long long)m << 32 | l;
+            if (hi == m && lo == l) hi = 0;
+        }
+        auto offer = [&](float v, int index) {
+            const unsigned long long k = key_of(v, index);
+            if (k >= tau) {
+                const int n = atomicAdd(&s_n[warp], 1);
+                if (n < kWarpRoom) s_list[warp][n] = k;
+            }
+        };
+        __syncwarp();
+        for (uint32_t left = __ballot_sync(0xffffffffu, seen.any && high >= tau); left; left &= left - 1) {      // the warp reads one lane's elements again
+            const int t = __ffs(left) - 1;
+            if (lane == 0 && t < part.head) offer(to_float<T>(x[t]), t);
+            if (lane == 1 && t < n_tail) offer(to_float<T>(x[part.tail0 + t]), part.tail0 + t);
+            for (int j = t + lane * 32; j < part.vecs; j += 32 * 32) {
+                float2 v[kVec / 2];
+                Vec<T>::elements(__ldg(part.body + j), v);
+#pragma unroll
+                for (int k = 0; k < kVec / 2; ++k) {
+                    offer(v[k].x, part.head + j * kVec + 2 * k);
+                    offer(v[k].y, part.head + j * kVec + 2 * k + 1);
+                }
+            }
+        }
+        __syncwarp();
+        const int n = *static_cast<volatile int*>(&s_n[warp]);
+        slow = n > kWarpRoom;
+        for (int k = lane; k < n && !slow; k += 32) {
+            const unsigned long long mine = s_list[warp][k];
+            int before = 0;
+            for (int j = 0; j < n; ++j) before += s_list[warp][j] > mine;
+            if (before < a.top) {
+                a.top_tokens[row * a.top + before] = index_of(mine);
+                a.top_logprobs[row * a.top + before] = out.logprob(logit_of(mine));
+            }
+        }
+    }
+    if (slow) slow_row<T, 32>(a, x, row, nullptr, &s_best[warp], known, out);
+}
+
 // gridDim.x = rows * splits, the CTAs of a row are a cluster.
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
-    constexpr int kVec = 16 / sizeof(T), kAhead = 4;
+    constexpr int kVec = 16 / sizeof(T);
     __shared__ Shared<kThreads> sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.x / a.splits;
     const int rank = (int)(blockIdx.x - row * a.splits);
     const T* x = static_cast<const T*>(a.logits) + row * a.stride;
-    // Whole 16-byte vectors, of which this CTA has [lo, hi) and a thread every kThreads-th, and single elements before (head, with
-    // the first CTA) and behind them (tail, with the last).
-    const int head = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T), a.V);
-    const int vecs = (a.V - head) / kVec, tail0 = head + vecs * kVec;
+    // Of the row's vectors this CTA has [lo, hi) and a thread every kThreads-th; the head is with the first CTA, the tail with the last.
+    const Parts<T> part(x, a.V);
+    const int head = part.head, vecs = part.vecs, tail0 = part.tail0;
+    const uint4* body = part.body;
     const int lo = (int)((int64_t)rank * vecs / a.splits), hi = (int)((int64_t)(rank + 1) * vecs / a.splits);
-    const uint4* body = reinterpret_cast<const uint4*>(x + head);
     const int n_head = rank == 0 ? head : 0, n_tail = rank == a.splits - 1 ? a.V - tail0 : 0;
     const float c = a.scale * kLog2e;
     if (tid == 0) {
@@ -213,94 +480,17 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
     if (a.splits > 1) ptx::cluster_arrive();      // (waited for before anything is written into the first CTA)
     pdl_enter();
 
-    Sums r = {-INFINITY, 0.f, 0.f, -INFINITY};
-    int at = -1;      // where r.m is: vector at, or the head's element (-1) or the tail's (-2)
-    bool any = false;
-    // what a new largest logit means: whether e still serves
-    auto rise = [&](float v, int where) {
-        if (v != v) {
-            r.s = NAN;
-            return;
-        }
-        r.m = v;
-        at = where;
-        const float e = ceilf(v * c);
-        if (e > r.e + 4.f) {
-            if (r.e != -INFINITY) {
-                const float d = r.e - e, f = exp2_fast(d);
-                r.w = (r.w + d * r.s) * f;
-                r.s *= f;
-            }
-            r.e = e;
-        }
-    };
-    auto single = [&](float v, int where) {
-        any = true;
-        if (!(v <= r.m)) rise(v, where);
-        if (r.m != -INFINITY) {
-            const float t = fmaxf(fmaf(v, c, -r.e), -200.f), p = exp2_fast(t);
-            r.s += p;
-            r.w = fmaf(p, t, r.w);
-        }
-    };
-    if (tid < n_head) single(to_float<T>(x[tid]), -1);
-    f32x2 s2 = pack2(0.f, 0.f), w2 = s2;
-    auto fold = [&]() {
-        float u, v;
-        unpack2(s2, u, v);
-        r.s += u + v;
-        unpack2(w2, u, v);
-        r.w += u + v;
-        s2 = w2 = pack2(0.f, 0.f);
-    };
-    auto vector = [&](const uint4& q, int where) {
-        const float m = largest(q, T());
-        if (!(m <= r.m)) {
-            fold();
-            rise(m, where);
-        }
-        if (r.m == -INFINITY) return;      // nothing but masks so far
-        float v[kVec];
-        elements<T>(q, v);
-        const f32x2 cc = pack2(c, c), ee = pack2(-r.e, -r.e);
-#pragma unroll
-        for (int j = 0; j < kVec; j += 2) {
-            float t0, t1;
-            unpack2(fma2(pack2(v[j], v[j + 1]), cc, ee), t0, t1);
-            t0 = fmaxf(t0, -200.f);      // (p is 0 there and p * t has to be)
-            t1 = fmaxf(t1, -200.f);
-            const f32x2 p = pack2(exp2_fast(t0), exp2_fast(t1));
-            s2 = add2(s2, p);
-            w2 = fma2(p, pack2(t0, t1), w2);
-        }
-    };
-    int i = lo + tid;
-    if (i < hi) {
-        if (!any) at = i;
-        any = true;
-    }
-    for (; i + (kAhead - 1) * kThreads < hi; i += kAhead * kThreads) {
-        uint4 q[kAhead];
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) q[j] = __ldg(body + i + j * kThreads);
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) vector(q[j], i + j * kThreads);
-    }
-    for (; i < hi; i += kThreads) vector(__ldg(body + i), i);
-    fold();
+    Seen<T> seen;
+    seen.c = c;
+    if (tid < n_head) seen.single(to_float<T>(x[tid]), -1);
+    seen.stream(body, lo + tid, hi, kThreads);
     if (tid < n_tail) {
-        if (!any) at = -2;
-        single(to_float<T>(x[tail0 + tid]), -2);
+        if (!seen.any) seen.at = -2;
+        seen.single(to_float<T>(x[tail0 + tid]), -2);
     }
 
     // the block's sums, in a fixed order
-    Sums all = r;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Sums other = {__shfl_xor_sync(0xffffffffu, all.e, o), __shfl_xor_sync(0xffffffffu, all.s, o), __shfl_xor_sync(0xffffffffu, all.w, o),
-                            __shfl_xor_sync(0xffffffffu, all.m, o)};
-        all = (lane & o) ? joined(other, all) : joined(all, other);
-    }
+    Sums all = warp_sums(seen.r, lane);
     if (lane == 0) sh.part[warp] = all;
 
     if (a.splits > 1) {
@@ -311,8 +501,9 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
     int n_best = 0;
     if (a.top) {
         // The thread's largest as a key that is not above the true one (the vector's last index), and one that is not below it.
-        const int first_index = at == -1 ? tid : at == -2 ? tail0 + tid : head + at * kVec;
-        const unsigned long long low = any ? key_of(r.m, first_index + (at >= 0 ? kVec - 1 : 0)) : 0, high = any ? key_of(r.m, first_index) : 0;
+        const int first_index = seen.at == -1 ? tid : seen.at == -2 ? tail0 + tid : head + seen.at * kVec;
+        const unsigned long long low = seen.any ? key_of(seen.r.m, first_index + (seen.at >= 0 ? kVec - 1 : 0)) : 0;
+        const unsigned long long high = seen.any ? key_of(seen.r.m, first_index) : 0;
         // the top-th largest of the largest of 8 threads each: a first bound, so that few keys remain
         unsigned long long g = low;
 #pragma unroll
@@ -342,7 +533,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
         }
         __syncthreads();
         const unsigned long long tau = sh.tau;
-        if (any && high >= tau) sh.threads[atomicAdd(&sh.n_threads, 1)] = tid;
+        if (seen.any && high >= tau) sh.threads[atomicAdd(&sh.n_threads, 1)] = tid;
         if (tid == 0) sh.n_list = 0;
         __syncthreads();
         auto offer = [&](float v, int index) {
@@ -357,10 +548,13 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
             if (lane == 0 && t < n_head) offer(to_float<T>(x[t]), t);
             if (lane == 1 && t < n_tail) offer(to_float<T>(x[tail0 + t]), tail0 + t);
             for (int j = lo + t + lane * kThreads; j < hi; j += 32 * kThreads) {
-                float v[kVec];
-                elements<T>(__ldg(body + j), v);
+                float2 v[kVec / 2];
+                Vec<T>::elements(__ldg(body + j), v);
 #pragma unroll
-                for (int k = 0; k < kVec; ++k) offer(v[k], head + j * kVec + k);
+                for (int k = 0; k < kVec / 2; ++k) {
+                    offer(v[k].x, head + j * kVec + 2 * k);
+                    offer(v[k].y, head + j * kVec + 2 * k + 1);
+                }
             }
         }
         __syncthreads();
@@ -405,7 +599,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
     out.scale = a.scale;
     out.m = all.m;
     out.empty = false;
-    const bool known = all.s > 0.f && all.s < INFINITY;
+    const bool known = row_known<T>(all, a.scale * kLog2e);
     if (known) {
         const float log_s = log2f(all.s);
         out.entropy = (log_s - all.w / all.s) * kLn2;
@@ -414,7 +608,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
         write_given<T>(a, x, row, out, tid, kThreads);
     }
     if (!known || (a.top && too_many)) {
-        slow_row<T, kThreads>(a, x, row, sh, known, out);
+        slow_row<T, kThreads>(a, x, row, sh.part_f, &sh.tau, known, out);
         return;
     }
     if (a.top) {
@@ -452,7 +646,7 @@ extern "C" int exb_token_logprobs_fwd(exb_ctx* ctx, const void* logits, int dtyp
     const size_t es = rows::element_size(dtype);
     EXB_REQUIRE(es != 0, "exb_token_logprobs_fwd: logits must be EXB_F16, EXB_BF16 or EXB_F32, got %d", dtype);
     EXB_REQUIRE(n_rows >= 0 && V >= 1, "exb_token_logprobs_fwd: bad shape (%lld rows of %d)", (long long)n_rows, V);
-    EXB_REQUIRE(scale > 1e-38f && scale < 1e38f, "exb_token_logprobs_fwd: scale must be a positive number");
+    EXB_REQUIRE(scale > 1e-8f && scale < 1e8f, "exb_token_logprobs_fwd: scale must be a positive number between 1e-8 and 1e8");
     EXB_REQUIRE(n_given >= 0 && top >= 0, "exb_token_logprobs_fwd: n_given and top must not be negative");
     EXB_REQUIRE(top <= V, "exb_token_logprobs_fwd: %d of %d tokens asked for", top, V);
     if (top > kMaxTop) return fail(EXB_ERR_UNSUPPORTED, "exb_token_logprobs_fwd: at most %d of the most probable tokens, got %d", kMaxTop, top);
@@ -471,14 +665,23 @@ extern "C" int exb_token_logprobs_fwd(exb_ctx* ctx, const void* logits, int dtyp
     if (n_given == 0 && top == 0 && !entropy) return EXB_OK;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int64_t bytes = (int64_t)V * (int64_t)es;
-    const int threads = bytes <= 8192 ? 128 : bytes >= 131072 && n_rows <= ctx->sm_count ? 512 : 256;
+    int rc = EXB_OK;
+    // A warp for a row where that takes no longer than its CTA's exchange, or where there are rows for all warps.  (fp16, top 5:
+    // kWarpTimes)
+    if (bytes <= 8192 || (bytes <= 32768 && n_rows >= 8 * ctx->sm_count)) {
+        rows::with_type(dtype, [&](auto t) {
+            using T = decltype(t);
+            launch_overlapped(ctx, token_logprobs_warp_kernel<T>, dim3((unsigned)((n_rows + kWarpRows - 1) / kWarpRows)), dim3(kWarpRows * 32), st, a, n_rows);
+        });
+        return after_launch("token_logprobs_warp_kernel");
+    }
+    const int threads = bytes >= 131072 && n_rows <= ctx->sm_count ? 512 : 256;
     // a row is shared where there are too few of them, as long as each CTA has two vectors for a thread
     a.splits = 1;
     while (a.splits < kSplitMax && n_rows * a.splits * 2 <= 2 * ctx->sm_count && bytes >= (int64_t)a.splits * 2 * threads * 32) a.splits *= 2;
-    int rc = EXB_OK;
     rows::with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        rc = threads == 128 ? launch<T, 128>(ctx, a, n_rows, st) : threads == 256 ? launch<T, 256>(ctx, a, n_rows, st) : launch<T, 512>(ctx, a, n_rows, st);
+        rc = threads == 256 ? launch<T, 256>(ctx, a, n_rows, st) : launch<T, 512>(ctx, a, n_rows, st);
     });
     return rc;
 }

@@ -528,7 +528,7 @@ EXB_API int exb_residual_norm_fwd(exb_ctx* ctx, const exb_norm_desc* d, const vo
                                   const float* weight, const float* bias, void* r, void* n, float* n_scales,
                                   void* stream);
 
-/* Scores of tokens from rows of V logits, z = scale * logits (scale between 1e-38 and 1e38: the reciprocal of a temperature):
+/* Scores of tokens from rows of V logits, z = scale * logits (scale between 1e-8 and 1e8: the reciprocal of a temperature):
  *   lse = log sum exp z;  logprobs[i][j] = z[tokens[i][j]] - lse, j < n_given
  *   entropy[i] = -sum p log p, p = exp(z - lse)
  *   top_tokens[i][0..top): the tokens of the largest logits in falling order, equal ones by their index; top_logprobs: theirs
