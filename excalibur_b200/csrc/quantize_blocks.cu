@@ -14,8 +14,7 @@ constexpr int kTileRows = kThreads / 32 * kRowsPerWarp;       // a CTA's scales 
 constexpr int kShare = 2 * kBlock;
 
 // Blocks of one row.  CTA: kTileRows rows x 256 channels, a warp kRowsPerWarp of the rows.
-// kVec: rows in whole, aligned vectors.
-template <typename T, bool kVec>
+template <typename T, Layout kL>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, int64_t x_stride, uint8_t* __restrict__ q,
                                                                  int64_t q_stride, float* __restrict__ scales, int64_t scale_stride,
                                                                  int64_t rows, int C, int shares, Span span) {
@@ -23,23 +22,24 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int share = blockIdx.x % shares, c0 = share * kShare, valid = C - c0;
     const int64_t r0 = (int64_t)(blockIdx.x / shares) * kTileRows + warp * kRowsPerWarp;
-    float v[kRowsPerWarp][8];
-#pragma unroll
-    for (int i = 0; i < kRowsPerWarp; ++i) {
-        const T* at = x + (r0 + i) * x_stride + c0;
-        if constexpr (kVec) load8<T, true>(at, r0 + i < rows ? valid : 0, lane, v[i]);
-        else if (r0 + i < rows) load8_shifted<T>(at, valid, lane, span, v[i]);
-    }
+    Kept<T, kL> k[kRowsPerWarp];
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i)
-        if (r0 + i < rows) quantize8<true>(v[i], valid, lane, q + (r0 + i) * q_stride + c0, scales + 2 * share * scale_stride + r0 + i, scale_stride);
+        if (r0 + i < rows) k[i].load(x + (r0 + i) * x_stride + c0, valid, lane, span);
+#pragma unroll
+    for (int i = 0; i < kRowsPerWarp; ++i)
+        if (r0 + i < rows) {
+            float v[8];
+            k[i].get(v);
+            quantize8(v, k[i].amax(), valid, lane, q + (r0 + i) * q_stride + c0, scales + 2 * share * scale_stride + r0 + i, scale_stride);
+        }
 }
 
-// Blocks of 128 rows: a CTA has two neighbouring ones, its warps read shares of 256 channels of every 8th row.
+// Blocks of 128 rows: a CTA has two neighbouring ones, its warps read shares of 256 channels of every 16th row.
 constexpr int kTileWarps = 16, kTileSteps = kBlock / kTileWarps;
 
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kTileWarps * 32) quantize_tiles_kernel(const T* __restrict__ x, int64_t x_stride, uint8_t* __restrict__ q,
+template <typename T, Layout kL>
+__global__ void __launch_bounds__(kTileWarps * 32, sizeof(T) == 2 ? 2 : 1) quantize_tiles_kernel(const T* __restrict__ x, int64_t x_stride, uint8_t* __restrict__ q,
                                                                          int64_t q_stride, float* __restrict__ scales, int64_t scale_stride,
                                                                          int64_t rows, int C, int shares, Span span) {
     __shared__ float s_max[2][kTileWarps];
@@ -47,25 +47,16 @@ __global__ void __launch_bounds__(kTileWarps * 32) quantize_tiles_kernel(const T
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int share = blockIdx.x % shares, c0 = share * kShare, valid = C - c0;
     const int64_t rb = blockIdx.x / shares, r0 = rb * kBlock + warp;
-    float v[kTileSteps][8], m = 0.f;
+    Kept<T, kL> k[kTileSteps];
+    float m = 0.f;
 #pragma unroll
     for (int i = 0; i < kTileSteps; ++i) {
         const int64_t r = r0 + i * kTileWarps;
-        if constexpr (kVec) {
-            load8<T, true>(x + r * x_stride + c0, r < rows ? valid : 0, lane, v[i]);
-        } else {
-            if (r < rows) {
-                load8_shifted<T>(x + r * x_stride + c0, valid, lane, span, v[i]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-            }
-        }
+        if (r < rows) k[i].load(x + r * x_stride + c0, valid, lane, span);
+        else k[i].none();
     }
 #pragma unroll
-    for (int i = 0; i < kTileSteps; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[i][j]));
+    for (int i = 0; i < kTileSteps; ++i) m = fmaxf(m, k[i].amax());
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const int half = lane >> 4;
@@ -80,7 +71,9 @@ __global__ void __launch_bounds__(kTileWarps * 32) quantize_tiles_kernel(const T
     for (int i = 0; i < kTileSteps; ++i) {
         const int64_t r = r0 + i * kTileWarps;
         if (r >= rows) break;
-        store8_e4m3(q + r * q_stride + c0 + lane * 8, v[i], inv, valid - lane * 8);
+        float v[8];
+        k[i].get(v);
+        store8_e4m3(q + r * q_stride + c0 + lane * 8, v, inv, valid - lane * 8);
     }
 }
 
@@ -113,10 +106,10 @@ extern "C" int exb_quantize_blocks_fwd(exb_ctx* ctx, const void* x, int in_dtype
         const T* in = static_cast<const T*>(x);
         const rows::Span span = rows::span_of(x, n_rows, x_stride, C, es);
         if (block_rows == 1)
-            launch_overlapped(ctx, vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, dim3((unsigned)grid), dim3(kThreads), st, in, x_stride,
+            launch_overlapped(ctx, vec ? quantize_rows_kernel<T, rows::kVectors> : quantize_rows_kernel<T, rows::kShifted>, dim3((unsigned)grid), dim3(kThreads), st, in, x_stride,
                               q, q_stride, scales, scale_stride, n_rows, C, (int)shares, span);
         else
-            launch_overlapped(ctx, vec ? quantize_tiles_kernel<T, true> : quantize_tiles_kernel<T, false>, dim3((unsigned)grid), dim3(kTileWarps * 32), st, in,
+            launch_overlapped(ctx, vec ? quantize_tiles_kernel<T, rows::kVectors> : quantize_tiles_kernel<T, rows::kShifted>, dim3((unsigned)grid), dim3(kTileWarps * 32), st, in,
                               x_stride, q, q_stride, scales, scale_stride, n_rows, C, (int)shares, span);
     });
     return after_launch("exb_quantize_blocks_fwd");

@@ -45,7 +45,7 @@ __device__ __forceinline__ float row_sum(float v, float (*s_sum)[32], int& turn)
 }
 
 // v = norm(v) * weight + bias over the row
-template <bool kLayer, bool kVec, bool kOneWarp, int kPer>
+template <bool kLayer, Layout kL, bool kOneWarp, int kPer>
 __device__ __forceinline__ void normalise(float (&v)[kPer][8], int lane, int share0, int share_step, const NormArgs& a, const float* weight,
                                           const float* bias, float (*s_sum)[32], int& turn) {
     const float inv_c = 1.f / (float)a.C;
@@ -60,7 +60,7 @@ __device__ __forceinline__ void normalise(float (&v)[kPer][8], int lane, int sha
         for (int i = 0; i < kPer; ++i) {      // (what lies behind the row's end stays 0)
             const int valid = a.C - (share0 + i * share_step) * kShare;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = (kVec ? lane * 8 : j * 32 + lane) < valid ? v[i][j] - mean : 0.f;
+            for (int j = 0; j < 8; ++j) v[i][j] = (kL == kVectors ? lane * 8 : j * 32 + lane) < valid ? v[i][j] - mean : 0.f;
         }
     }
     float s = 0.f;
@@ -73,11 +73,11 @@ __device__ __forceinline__ void normalise(float (&v)[kPer][8], int lane, int sha
     for (int i = 0; i < kPer; ++i) {
         const int c0 = (share0 + i * share_step) * kShare, valid = a.C - c0;
         float w[8];
-        load8<float, kVec>(weight + c0, valid, lane, w);
+        load8_params<kL>(weight + c0, valid, lane, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * k * w[j];
         if (bias) {
-            load8<float, kVec>(bias + c0, valid, lane, w);
+            load8_params<kL>(bias + c0, valid, lane, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] += w[j];
         }
@@ -87,7 +87,7 @@ __device__ __forceinline__ void normalise(float (&v)[kPer][8], int lane, int sha
 // kOneWarp: every warp of the CTA has a row of its own; otherwise the CTA has one.  kPer: shares per warp.
 constexpr int max_threads(bool one_warp, int per) { return one_warp ? 256 : per == 1 ? 1024 : 512; }
 
-template <typename T, bool kLayer, bool kVec, bool kOneWarp, int kPer>
+template <typename T, bool kLayer, Layout kL, bool kOneWarp, int kPer>
 __global__ void __launch_bounds__(max_threads(kOneWarp, kPer)) residual_norm_kernel(const __grid_constant__ NormArgs a) {
     __shared__ float s_sum[2][32];
     pdl_enter();
@@ -103,23 +103,23 @@ __global__ void __launch_bounds__(max_threads(kOneWarp, kPer)) residual_norm_ker
     constexpr bool kAhead = kPer <= 4;
     constexpr int kKept = kAhead ? kPer : 1;
     float v[kPer][8];
-    Kept<T, kVec> hk[kPer], xk[kKept], gk[kKept];
+    Kept<T, kL> hk[kPer], xk[kKept], gk[kKept];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int c0 = (share0 + i * share_step) * kShare, valid = a.C - c0;
-        hk[i].load(h + c0, valid, lane);
-        if (kAhead && a.x) xk[kAhead ? i : 0].load(x + c0, valid, lane);
-        if (kAhead && a.gate) gk[kAhead ? i : 0].load(g + c0, valid, lane);
+        hk[i].load(h + c0, valid, lane, {});
+        if (kAhead && a.x) xk[kAhead ? i : 0].load(x + c0, valid, lane, {});
+        if (kAhead && a.gate) gk[kAhead ? i : 0].load(g + c0, valid, lane, {});
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) hk[i].get(v[i]);
-    if (a.post_weight) normalise<kLayer, kVec, kOneWarp, kPer>(v, lane, share0, share_step, a, a.post_weight, a.post_bias, s_sum, turn);
+    if (a.post_weight) normalise<kLayer, kL, kOneWarp, kPer>(v, lane, share0, share_step, a, a.post_weight, a.post_bias, s_sum, turn);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int c0 = (share0 + i * share_step) * kShare, valid = a.C - c0;
         constexpr int kAll = kAhead ? 1 : 0;
-        if (!kAhead && a.x) xk[0].load(x + c0, valid, lane);
-        if (!kAhead && a.gate) gk[0].load(g + c0, valid, lane);
+        if (!kAhead && a.x) xk[0].load(x + c0, valid, lane, {});
+        if (!kAhead && a.gate) gk[0].load(g + c0, valid, lane, {});
         float o[8];
         if (a.gate) {
             gk[i * kAll].get(o);
@@ -134,21 +134,24 @@ __global__ void __launch_bounds__(max_threads(kOneWarp, kPer)) residual_norm_ker
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] *= a.residual_scale;
         }
-        if (a.r) store8<T, kVec>(static_cast<T*>(a.r) + row * a.r_stride + c0, valid, lane, v[i]);
+        if (a.r) store8<T, kL>(static_cast<T*>(a.r) + row * a.r_stride + c0, valid, lane, v[i]);
     }
     if (!a.n) return;
-    normalise<kLayer, kVec, kOneWarp, kPer>(v, lane, share0, share_step, a, a.weight, a.bias, s_sum, turn);
+    normalise<kLayer, kL, kOneWarp, kPer>(v, lane, share0, share_step, a, a.weight, a.bias, s_sum, turn);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int share = share0 + i * share_step, c0 = share * kShare, valid = a.C - c0;
-        if (a.quantized)
-            quantize8<kVec>(v[i], valid, lane, static_cast<uint8_t*>(a.n) + row * a.n_stride + c0, a.n_scales + 2 * share * a.scale_stride + row, a.scale_stride);
-        else
-            store8<T, kVec>(static_cast<T*>(a.n) + row * a.n_stride + c0, valid, lane, v[i]);
+        if (a.quantized) {
+            uint8_t* q = static_cast<uint8_t*>(a.n) + row * a.n_stride + c0;
+            float* scale = a.n_scales + 2 * share * a.scale_stride + row;
+            if constexpr (kL == kVectors) quantize8(v[i], largest_of(v[i]), valid, lane, q, scale, a.scale_stride);
+            else quantize8_strided(v[i], valid, lane, q, scale, a.scale_stride);
+        } else
+            store8<T, kL>(static_cast<T*>(a.n) + row * a.n_stride + c0, valid, lane, v[i]);
     }
 }
 
-template <typename T, bool kLayer, bool kVec>
+template <typename T, bool kLayer, Layout kL>
 int launch(const exb_ctx* ctx, const NormArgs& a, cudaStream_t st) {
     const int shares = (a.C + kShare - 1) / kShare;
     auto go = [&](auto one, auto per) {
@@ -156,7 +159,7 @@ int launch(const exb_ctx* ctx, const NormArgs& a, cudaStream_t st) {
         constexpr int kPer = decltype(per)::value;
         const int warps = kOne ? 8 : (shares + kPer - 1) / kPer;
         const int64_t grid = kOne ? (a.rows + warps - 1) / warps : a.rows;
-        launch_overlapped(ctx, residual_norm_kernel<T, kLayer, kVec, kOne, kPer>, dim3((unsigned)grid), dim3(32 * warps), st, a);
+        launch_overlapped(ctx, residual_norm_kernel<T, kLayer, kL, kOne, kPer>, dim3((unsigned)grid), dim3(32 * warps), st, a);
     };
     using Yes = std::true_type;
     using No = std::false_type;
@@ -225,8 +228,8 @@ extern "C" int exb_residual_norm_fwd(exb_ctx* ctx, const exb_norm_desc* d, const
     int rc = EXB_OK;
     rows::with_type(d->dtype, [&](auto t) {
         using T = decltype(t);
-        if (d->kind == EXB_NORM_LAYER) rc = vec ? launch<T, true, true>(ctx, a, st) : launch<T, true, false>(ctx, a, st);
-        else rc = vec ? launch<T, false, true>(ctx, a, st) : launch<T, false, false>(ctx, a, st);
+        if (d->kind == EXB_NORM_LAYER) rc = vec ? launch<T, true, rows::kVectors>(ctx, a, st) : launch<T, true, rows::kStrided>(ctx, a, st);
+        else rc = vec ? launch<T, false, rows::kVectors>(ctx, a, st) : launch<T, false, rows::kStrided>(ctx, a, st);
     });
     return rc;
 }

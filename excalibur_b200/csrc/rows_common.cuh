@@ -3,6 +3,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace exb {
@@ -29,31 +31,28 @@ __device__ __forceinline__ uint32_t float_to_pair(float a, float b, __nv_bfloat1
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// A warp's share of a row is 256 consecutive elements, 8 of them in each lane: 8 neighbours in 16-byte vectors (kVec), or
-// every 32nd in single elements where rows start anywhere (8 loads of 32 neighbours each: 64 bytes a load, which still
-// is more than memory delivers).  `at`: the share's first element, `valid`: elements of the row from there on (<= 0: none).
-// With kVec the row's length is a multiple of 8.
-template <typename T, bool kVec>
-__device__ __forceinline__ void load8(const T* at, int valid, int lane, float (&v)[8]) {
-    if constexpr (kVec) {
+// A warp's share of a row is 256 consecutive elements.  `valid`: elements of the row from the share's first one on (<= 0: none).
+// How the lanes have them:
+//  kVectors: 8 neighbours each, in 16-byte vectors: rows that start at multiples of 16 bytes and are whole vectors long;
+//  kShifted: 8 neighbours each of rows that start anywhere, read in whole vectors and moved between lanes;
+//  kStrided: every 32nd, loaded and stored one by one (64 or 128 bytes an instruction): rows that start anywhere.
+enum Layout { kVectors, kShifted, kStrided };
+
+// fp32 parameters of the share's channels.
+template <Layout kL>
+__device__ __forceinline__ void load8_params(const float* at, int valid, int lane, float (&v)[8]) {
+    if constexpr (kL == kVectors) {
         if (lane * 8 < valid) {
-            const uint4* src = reinterpret_cast<const uint4*>(at + lane * 8);
-            if constexpr (sizeof(T) == 4) {
-                const uint4 a = src[0], b = src[1];
-                v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
-                v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
-            } else {
-                const uint4 a = src[0];
-                const float2 p0 = pair_to_float(a.x, T()), p1 = pair_to_float(a.y, T()), p2 = pair_to_float(a.z, T()), p3 = pair_to_float(a.w, T());
-                v[0] = p0.x; v[1] = p0.y; v[2] = p1.x; v[3] = p1.y; v[4] = p2.x; v[5] = p2.y; v[6] = p3.x; v[7] = p3.y;
-            }
+            const float4 a = __ldg(reinterpret_cast<const float4*>(at + lane * 8)), b = __ldg(reinterpret_cast<const float4*>(at + lane * 8) + 1);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = 0.f;
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j * 32 + lane < valid ? to_float<T>(at[j * 32 + lane]) : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = j * 32 + lane < valid ? __ldg(at + j * 32 + lane) : 0.f;
     }
 }
 
@@ -84,7 +83,7 @@ __device__ __forceinline__ uint4 load16_within(const uint8_t* at, const Span& sp
 // multiples of 16, and moved into place between neighbouring lanes.  About 20 instructions for 8 elements of 16 bits; eight loads
 // of single elements for each lane's 8 took 3.7 times the time of aligned rows (8192 x 14335 bf16 to e4m3: 200 us, 63 aligned).
 template <typename T>
-__device__ __forceinline__ void load8_shifted(const T* row_at, int valid, int lane, const Span& span, float (&v)[8]) {
+__device__ __forceinline__ void load8_shifted(const T* row_at, int valid, int lane, const Span& span, uint32_t (&out)[2 * sizeof(T)]) {
     constexpr int kWords = 8 * sizeof(T) / 4, kVecs = kWords / 4;      // of a lane
     const uintptr_t a = reinterpret_cast<uintptr_t>(row_at);
     const int o = (int)(a & 15);
@@ -115,53 +114,80 @@ __device__ __forceinline__ void load8_shifted(const T* row_at, int valid, int la
 #pragma unroll
         for (int i = 0; i < kWords + 1; ++i) x[i] = x[i + 1];
     }
-    if constexpr (sizeof(T) == 2) {
-        const int sh = (o & 2) * 8;
+    const int sh = sizeof(T) == 2 ? (o & 2) * 8 : 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = pair_to_float(__funnelshift_r(x[i], x[i + 1], sh), T());
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(x[i]);
-    }
+    for (int i = 0; i < kWords; ++i) out[i] = sizeof(T) == 2 ? __funnelshift_r(x[i], x[i + 1], sh) : x[i];
+    // behind the row's end: 0
+    constexpr int kPer = 4 / sizeof(T);
     if (lane * 8 + 8 > valid) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (lane * 8 + j >= valid) v[j] = 0.f;
+        for (int i = 0; i < kWords; ++i) {
+            const int left = valid - lane * 8 - i * kPer;
+            if (left <= 0) out[i] = 0;
+            else if (kPer == 2 && left == 1) out[i] &= 0xffffu;
+        }
     }
 }
 
-// The same, kept as it is in memory until it is needed: 4 registers for 8 elements of 16 bits in vectors.
-template <typename T, bool kVec>
+// A lane's 8 elements, kept as they are in memory until they are needed: 4 registers for 16-bit elements that are neighbours.
+template <typename T, Layout kL>
 struct Kept {
-    static constexpr bool kPacked = kVec && sizeof(T) == 2;
-    uint4 packed;
-    float v[kPacked ? 1 : 8];
-    __device__ __forceinline__ void load(const T* at, int valid, int lane) {
-        if constexpr (kPacked) {
-            packed = make_uint4(0, 0, 0, 0);
-            if (lane * 8 < valid) packed = *reinterpret_cast<const uint4*>(at + lane * 8);
+    static constexpr bool kPacked = sizeof(T) == 2 && kL != kStrided;
+    static constexpr int kWords = kPacked ? 4 : 8;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void none() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load(const T* at, int valid, int lane, const Span& span) {
+        if constexpr (kL == kVectors) {
+#pragma unroll
+            for (int i = 0; i < kWords / 4; ++i) {
+                uint4 q = make_uint4(0, 0, 0, 0);
+                if (lane * 8 < valid) q = reinterpret_cast<const uint4*>(at + lane * 8)[i];
+                w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+            }
+        } else if constexpr (kL == kShifted) {
+            load8_shifted<T>(at, valid, lane, span, w);
         } else {
-            load8<T, kVec>(at, valid, lane, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = j * 32 + lane < valid ? __float_as_uint(to_float<T>(at[j * 32 + lane])) : 0u;
         }
     }
     __device__ __forceinline__ void get(float (&o)[8]) const {
         if constexpr (kPacked) {
-            const float2 a = pair_to_float(packed.x, T()), b = pair_to_float(packed.y, T()), c = pair_to_float(packed.z, T()), d = pair_to_float(packed.w, T());
-            o[0] = a.x; o[1] = a.y; o[2] = b.x; o[3] = b.y; o[4] = c.x; o[5] = c.y; o[6] = d.x; o[7] = d.y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = pair_to_float(w[i], T());
+                o[2 * i] = f.x;
+                o[2 * i + 1] = f.y;
+            }
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = v[j];
+            for (int i = 0; i < 8; ++i) o[i] = __uint_as_float(w[i]);
+        }
+    }
+    // the largest magnitude; NaN are left out
+    __device__ __forceinline__ float amax() const {
+        if constexpr (kPacked) {
+            using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+            auto part = [&](int i) { return __habs2(*reinterpret_cast<const T2*>(&w[i])); };
+            const T2 m = __hmax2(__hmax2(part(0), part(1)), __hmax2(part(2), part(3)));
+            const float2 f = pair_to_float(*reinterpret_cast<const uint32_t*>(&m), T());
+            return fmaxf(f.x, f.y);
+        } else {
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(__uint_as_float(w[i])));
+            return m;
         }
     }
 };
 
-template <typename T, bool kVec>
+template <typename T, Layout kL>
 __device__ __forceinline__ void store8(T* at, int valid, int lane, const float (&v)[8]) {
-    if constexpr (kVec) {
+    static_assert(kL != kShifted, "results are written in vectors or one by one");
+    if constexpr (kL == kVectors) {
         if (lane * 8 < valid) {
             uint4* dst = reinterpret_cast<uint4*>(at + lane * 8);
             if constexpr (sizeof(T) == 4) {
@@ -204,37 +230,40 @@ __device__ __forceinline__ void store8_e4m3(uint8_t* q, const float (&v)[8], flo
     }
 }
 
-// The warp's share (two blocks of 128) of a row -> e4m3 and its blocks' scales.  fmaxf drops NaN: a block's scale comes from
-// its other values, the NaN itself goes into q.  kVec: 8 neighbours in each lane, else every 32nd.
-template <bool kVec>
-__device__ __forceinline__ void quantize8(const float (&v)[8], int valid, int lane, uint8_t* __restrict__ q, float* __restrict__ scale,
+// The warp's share of a row, neighbours in each lane (two blocks of 128, 16 lanes each) -> e4m3 and its blocks' scales; m: the lane's
+// largest magnitude.  fmaxf drops NaN: a block's scale comes from its other values, the NaN itself goes into q.
+__device__ __forceinline__ void quantize8(const float (&v)[8], float m, int valid, int lane, uint8_t* __restrict__ q, float* __restrict__ scale,
                                           int64_t scale_stride) {
-    if constexpr (kVec) {      // 16 lanes have a block
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float s = block_scale(m), inv = 1.f / s;
+    if (lane * 8 < valid) {
+        store8_e4m3(q + lane * 8, v, inv, valid - lane * 8);
+        if ((lane & 15) == 0) scale[(lane >> 4) * scale_stride] = s;
+    }
+}
+// The same of every 32nd element: a lane has four of each block.
+__device__ __forceinline__ void quantize8_strided(const float (&v)[8], int valid, int lane, uint8_t* __restrict__ q, float* __restrict__ scale,
+                                                  int64_t scale_stride) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
         float m = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
+        for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(v[4 * b + j]));
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const float s = block_scale(m), inv = 1.f / s;
-        if (lane * 8 < valid) {
-            store8_e4m3(q + lane * 8, v, inv, valid - lane * 8);
-            if ((lane & 15) == 0) scale[(lane >> 4) * scale_stride] = s;
-        }
-    } else {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            float m = 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(v[4 * b + j]));
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float s = block_scale(m), inv = 1.f / s;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (b * kBlock + j * 32 + lane < valid) q[b * kBlock + j * 32 + lane] = to_e4m3(v[4 * b + j] * inv);
-            if (lane == 0 && b * kBlock < valid) scale[b * scale_stride] = s;
-        }
+        for (int j = 0; j < 4; ++j)
+            if (b * kBlock + j * 32 + lane < valid) q[b * kBlock + j * 32 + lane] = to_e4m3(v[4 * b + j] * inv);
+        if (lane == 0 && b * kBlock < valid) scale[b * scale_stride] = s;
     }
+}
+__device__ __forceinline__ float largest_of(const float (&v)[8]) {
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
+    return m;
 }
 
 // ---- host ----------------------------------------------------------------------------------

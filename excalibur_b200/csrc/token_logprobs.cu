@@ -5,11 +5,12 @@
 // One pass over the row, bound by its reading.  A thread keeps an integer e near the largest value that it has seen, so that
 // x * scale * log2(e) - e is one multiply-add with one rounding and a change of e scales its sums by a power of two, exactly.
 //
-// The most probable tokens come out of the same pass: a thread also keeps its largest logit and the vector that has it.  The top-th
-// largest of these is a lower bound tau of the answer, and only the threads whose largest is not below tau can hold
-// anything that is not: about as many as tokens are asked for.  Their elements are read again (out of L2), those from tau on
-// are put in order by counting for each how many are before it.  Logits and indexes make keys that are all different, so that
-// equal logits, masked ones among them, need nothing else.
+// The most probable tokens come out of the same pass: a thread also keeps its largest logit.  The top-th largest of these (of groups
+// of 8 threads in a CTA) is a lower bound tau of the answer, and only threads whose largest is not below tau hold anything
+// that is not: about as many as tokens are asked for.  Their elements are read again (out of L2), those from tau on are put in
+// order by counting for each how many are before it.  Logits and indexes make keys that are all different.  Where there are too many
+// elements of equal value from tau on (masks, constant rows), the threads find out where their largest is, and the same
+// is done with keys.
 //
 // A row that the pass cannot answer (a NaN or plus infinity in it, nothing but masks or logits at the type's lowest end, or more
 // elements from tau on than there is room for) is answered by slow_row: the maximum, the sums about it, and one pass per token.
@@ -120,31 +121,50 @@ struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16, __nv_bfloat162> {
     static __device__ __forceinline__ void bounded(const uint4& v, float2 (&x)[4]) { bounded_by(v, 0xf149f149u, x); }
 };
 
-// Sums about a thread's (or a row's) reference e, and its largest logit.
+// Sums about a thread's (or a row's) reference e, and its largest logit (NaN if there is one).
 struct alignas(16) Sums {
     float e, s, w, m;
 };
-__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
-    // (a side without anything has s = w = 0 and e = -inf: its factor is 0, and the difference of two infinities is not taken)
-    Sums r;
-    r.e = fmaxf(a.e, b.e);
-    r.m = fmaxf(a.m, b.m);
-    const float da = a.e == r.e ? 0.f : fmaxf(a.e - r.e, -1000.f), db = b.e == r.e ? 0.f : fmaxf(b.e - r.e, -1000.f);
-    const float fa = exp2_fast(da), fb = exp2_fast(db);
-    r.s = a.s * fa + b.s * fb;
-    r.w = (a.w + da * a.s) * fa + (b.w + db * b.s) * fb;
+
+// The lanes' sums joined, alike in all lanes (a sum over pairs does not depend on their order).  A lane without anything has e = -inf.
+__device__ __forceinline__ Sums warp_sums(const Sums& a) {
+    Sums r = a;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        r.e = fmaxf(r.e, __shfl_xor_sync(0xffffffffu, r.e, o));
+        r.m = max_nan(r.m, __shfl_xor_sync(0xffffffffu, r.m, o));
+    }
+    const float d = a.e == r.e ? 0.f : fmaxf(a.e - r.e, -1000.f), f = exp2_fast(d);      // (not the difference of two infinities)
+    r.s = a.s * f;
+    r.w = fmaf(d, a.s, a.w) * f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+        r.w += __shfl_xor_sync(0xffffffffu, r.w, o);
+    }
     return r;
 }
 
-constexpr int kAhead = 4;      // vectors that a thread works on at a time; as many are on their way
 
-// What a thread keeps of the logits that it has seen.
+// Where a row's whole 16-byte vectors are, and the single elements before (head) and behind them (tail).
+template <typename T>
+struct Parts {
+    int head, vecs, tail0;
+    const uint4* body;
+    __device__ __forceinline__ Parts(const T* x, int V) {
+        head = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T), V);
+        vecs = (V - head) / Vec<T>::kCount;
+        tail0 = head + vecs * Vec<T>::kCount;
+        body = reinterpret_cast<const uint4*>(x + head);
+    }
+};
+
+// A thread's share of a row: every `step`-th of the vectors from `first` below `end`, and an element of the head and of the tail at most.
 template <typename T>
 struct Seen {
+    static constexpr int kAhead = sizeof(T) == 4 ? 8 : 4;      // vectors that are asked for at a time
     Sums r = {-INFINITY, 0.f, 0.f, -INFINITY};
     float2 s2 = {0.f, 0.f}, w2 = {0.f, 0.f};      // on top of r.s and r.w
-    int at = -1;                                   // where r.m is: vector at, or the head's element (-1) or the tail's (-2)
-    bool any = false;
     float c;
 
     __device__ __forceinline__ void fold() {
@@ -152,48 +172,40 @@ struct Seen {
         r.w += w2.x + w2.y;
         s2 = w2 = make_float2(0.f, 0.f);
     }
-    // a new largest logit: does e still serve?
-    __device__ __forceinline__ void rise(float v, int where) {
+    // the sums about another e: v is far above it (in most rows only the first vectors are)
+    __device__ __forceinline__ void rise(float v) {
+        fold();
         if (v != v) {
             r.s = NAN;
             return;
         }
-        r.m = v;
-        at = where;
         const float e = ceilf(v * c);
-        if (e > r.e + 4.f) {
-            if (r.e != -INFINITY) {
-                const float d = r.e - e, f = exp2_fast(d);
-                r.w = (r.w + d * r.s) * f;
-                r.s *= f;
-            }
-            r.e = e;
+        if (r.e != -INFINITY) {
+            const float d = r.e - e, f = exp2_fast(d);
+            r.w = (r.w + d * r.s) * f;
+            r.s *= f;
         }
+        r.e = e;
     }
-    __device__ __forceinline__ void single(float v, int where) {
-        any = true;
-        if (!(v <= r.m)) rise(v, where);
-        if (r.m != -INFINITY) {
+    __device__ __forceinline__ void single(float v) {
+        r.m = max_nan(r.m, v);
+        if (!(v * c <= r.e + 4.f)) rise(v);
+        if (r.e != -INFINITY) {
             const float t = fmaxf(fmaf(v, c, -r.e), -200.f), p = exp2_fast(t);
             r.s += p;
             r.w = fmaf(p, t, r.w);
         }
     }
-    // n of the vectors are there, `step` apart from `first` on
-    __device__ __forceinline__ void vectors(const uint4 (&q)[kAhead], int n, int first, int step) {
+    // n of the vectors are there
+    __device__ __forceinline__ void vectors(const uint4 (&q)[kAhead], int n) {
         typename Vec<T>::Max m = Vec<T>::largest(q[0]);
 #pragma unroll
         for (int j = 1; j < kAhead; ++j)
             if (j < n) m = Vec<T>::larger(m, Vec<T>::largest(q[j]));
         const float top = Vec<T>::value(m);
-        if (!(top <= r.m)) {
-            fold();
-            int j = 0;
-            if (top == top)
-                while (j < kAhead - 1 && Vec<T>::value(Vec<T>::largest(j == 0 ? q[0] : j == 1 ? q[1] : q[2])) != top) ++j;
-            rise(top, first + j * step);
-        }
-        if (r.m == -INFINITY) return;      // nothing but masks so far
+        r.m = max_nan(r.m, top);
+        if (!(top * c <= r.e + 4.f)) rise(top);
+        if (r.e == -INFINITY) return;      // nothing but masks so far
         const float2 cc = make_float2(c, c), ee = make_float2(-r.e, -r.e);
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
@@ -209,31 +221,85 @@ struct Seen {
             }
         }
     }
-    // all of this thread's share of the vectors: from `first` on every `step`-th below `end`
     __device__ __forceinline__ void stream(const uint4* body, int first, int end, int step) {
         int i = first;
-        if (i < end) {
-            if (!any) at = i;
-            any = true;
+        for (; i + (kAhead - 1) * step < end; i += kAhead * step) {
+            uint4 q[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) q[j] = __ldg(body + i + j * step);
+            vectors(q, kAhead);
         }
-        uint4 q[kAhead];
-        auto fetch = [&](int from) {
+        if (i < end) {
+            uint4 q[kAhead];
 #pragma unroll
             for (int j = 0; j < kAhead; ++j)
-                if (from + j * step < end) q[j] = __ldg(body + from + j * step);
-        };
-        if (i < end) fetch(i);
-        for (; i + (kAhead - 1) * step < end; i += kAhead * step) {
-            uint4 now[kAhead];
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) now[j] = q[j];
-            if (i + kAhead * step < end) fetch(i + kAhead * step);
-            vectors(now, kAhead, i, step);
+                if (i + j * step < end) q[j] = __ldg(body + i + j * step);
+            vectors(q, (end - i + step - 1) / step);
         }
-        if (i < end) vectors(q, (end - i + step - 1) / step, i, step);
         fold();
     }
 };
+
+// Key of a thread's largest logit (the first of equal ones); 0 where it has none.
+template <typename T>
+__device__ __noinline__ unsigned long long best_key(const T* x, const Parts<T>& part, int thread, int n_head, int n_tail, int first, int end, int step) {
+    unsigned long long best = 0;
+    auto look = [&](float v, int index) {
+        const unsigned long long k = key_of(v, index);
+        best = k > best ? k : best;
+    };
+    if (thread < n_head) look(to_float<T>(x[thread]), thread);
+    for (int i = first; i < end; i += step) {
+        float2 v[Vec<T>::kCount / 2];
+        Vec<T>::elements(__ldg(part.body + i), v);
+#pragma unroll
+        for (int k = 0; k < Vec<T>::kCount / 2; ++k) {
+            look(v[k].x, part.head + i * Vec<T>::kCount + 2 * k);
+            look(v[k].y, part.head + i * Vec<T>::kCount + 2 * k + 1);
+        }
+    }
+    if (thread < n_tail) look(to_float<T>(x[part.tail0 + thread]), part.tail0 + thread);
+    return best;
+}
+
+// The keys from tau on among a thread's elements go to the list, `lanes` lanes reading its vectors together.
+template <typename T>
+__device__ __forceinline__ void collect(const T* x, const Parts<T>& part, unsigned long long tau, int thread, int n_head, int n_tail, int first, int end, int step,
+                                        int lane, int lanes, unsigned long long* list, int* n_list, int room) {
+    const float low = tau >> 32 ? logit_of(tau) : -INFINITY;
+    auto offer = [&](float v, int index) {
+        if (!(v >= low)) return;
+        const unsigned long long k = key_of(v, index);
+        if (k >= tau) {
+            const int n = atomicAdd(n_list, 1);
+            if (n < room) list[n] = k;
+        }
+    };
+    if (lane == 0 && thread < n_head) offer(to_float<T>(x[thread]), thread);
+    for (int i = first + lane * step; i < end; i += lanes * step) {
+        const uint4 q = __ldg(part.body + i);
+        if (!(Vec<T>::value(Vec<T>::largest(q)) >= low)) continue;
+        float2 v[Vec<T>::kCount / 2];
+        Vec<T>::elements(q, v);
+#pragma unroll
+        for (int k = 0; k < Vec<T>::kCount / 2; ++k) {
+            offer(v[k].x, part.head + i * Vec<T>::kCount + 2 * k);
+            offer(v[k].y, part.head + i * Vec<T>::kCount + 2 * k + 1);
+        }
+    }
+    if (lane == 0 && thread < n_tail) offer(to_float<T>(x[part.tail0 + thread]), part.tail0 + thread);
+}
+
+// The n-th largest of the lanes' values (0: none); 0 if there are fewer.
+__device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
+    uint32_t m = 0;
+    for (int j = 0; j < n; ++j) {
+        m = __reduce_max_sync(0xffffffffu, v);
+        const uint32_t who = __ballot_sync(0xffffffffu, v == m);
+        if ((int)(threadIdx.x & 31) == __ffs(who) - 1) v = 0;
+    }
+    return m;
+}
 
 constexpr int kSplitMax = 8;      // CTAs that share a row
 constexpr int kRoom = 512;        // elements from tau on that are put in order
@@ -243,7 +309,7 @@ struct Shared {
     Sums part[kThreads / 32];
     Sums row[kSplitMax];                                   // (of the cluster's CTAs, in the first one)
     unsigned long long best[kSplitMax][kMaxTop];           // the same: their best, in order
-    unsigned long long group[kThreads / 8];
+    uint32_t largest[kThreads / 8];                        // of 8 threads each
     unsigned long long list[kRoom > kThreads ? kRoom : kThreads];
     int threads[kThreads];
     unsigned long long tau;
@@ -339,36 +405,11 @@ __device__ __noinline__ void slow_row(const LogprobArgs& a, const T* x, int64_t 
     }
 }
 
-// Where a row's whole 16-byte vectors are, and the single elements before (head) and behind them (tail).
-template <typename T>
-struct Parts {
-    int head, vecs, tail0;
-    const uint4* body;
-    __device__ __forceinline__ Parts(const T* x, int V) {
-        head = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T), V);
-        vecs = (V - head) / Vec<T>::kCount;
-        tail0 = head + vecs * Vec<T>::kCount;
-        body = reinterpret_cast<const uint4*>(x + head);
-    }
-};
-
-// The lanes' sums joined, in the same order in all of them.
-__device__ __forceinline__ Sums warp_sums(Sums all, int lane) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Sums other = {__shfl_xor_sync(0xffffffffu, all.e, o), __shfl_xor_sync(0xffffffffu, all.s, o), __shfl_xor_sync(0xffffffffu, all.w, o),
-                            __shfl_xor_sync(0xffffffffu, all.m, o)};
-        all = (lane & o) ? joined(other, all) : joined(all, other);
-    }
-    return all;
-}
-
 // A warp's row each: short rows, whose exchange between warps would take longer than their reading.
 constexpr int kWarpRows = 4, kWarpRoom = 128;
 
 template <typename T>
 __global__ void __launch_bounds__(kWarpRows * 32) token_logprobs_warp_kernel(const __grid_constant__ LogprobArgs a, int64_t n_rows) {
-    constexpr int kVec = Vec<T>::kCount;
     __shared__ unsigned long long s_list[kWarpRows][kWarpRoom], s_best[kWarpRows];
     __shared__ int s_n[kWarpRows];
     pdl_enter();
@@ -378,21 +419,17 @@ __global__ void __launch_bounds__(kWarpRows * 32) token_logprobs_warp_kernel(con
     const T* x = static_cast<const T*>(a.logits) + row * a.stride;
     const Parts<T> part(x, a.V);
     const int n_tail = a.V - part.tail0;
-    if (lane == 0) s_n[warp] = 0;
     Seen<T> seen;
     seen.c = a.scale * kLog2e;
-    if (lane < part.head) seen.single(to_float<T>(x[lane]), -1);
+    if (lane < part.head) seen.single(to_float<T>(x[lane]));
     seen.stream(part.body, lane, part.vecs, 32);
-    if (lane < n_tail) {
-        if (!seen.any) seen.at = -2;
-        seen.single(to_float<T>(x[part.tail0 + lane]), -2);
-    }
-    const Sums all = warp_sums(seen.r, lane);
+    if (lane < n_tail) seen.single(to_float<T>(x[part.tail0 + lane]));
+    const Sums all = warp_sums(seen.r);
     Row out;
     out.scale = a.scale;
     out.m = all.m;
     out.empty = false;
-    const bool known = row_known<T>(all, a.scale * kLog2e);
+    const bool known = row_known<T>(all, seen.c);
     if (known) {
         const float log_s = log2f(all.s);
         out.entropy = (log_s - all.w / all.s) * kLn2;
@@ -402,54 +439,45 @@ __global__ void __launch_bounds__(kWarpRows * 32) token_logprobs_warp_kernel(con
     }
     bool slow = !known;
     if (known && a.top) {
-        // tau: the top-th largest of the lanes' largest, taken out one after the other
-        const int first_index = seen.at == -1 ? lane : seen.at == -2 ? part.tail0 + lane : part.head + seen.at * kVec;
-        const unsigned long long low = seen.any ? key_of(seen.r.m, first_index + (seen.at >= 0 ? kVec - 1 : 0)) : 0;
-        const unsigned long long high = seen.any ? key_of(seen.r.m, first_index) : 0;
-        uint32_t hi = (uint32_t)(low >> 32), lo = (uint32_t)low;
-        unsigned long long tau = 0;
-        for (int j = 0; j < a.top; ++j) {
-            const uint32_t m = __reduce_max_sync(0xffffffffu, hi);
-            if (m == 0) {      // fewer lanes than tokens: every element is one to look at
-                tau = 0;
-                break;
-            }
-            const uint32_t l = __reduce_max_sync(0xffffffffu, hi == m ? lo : 0u);
-            tau = (unsigned long long)m << 32 | l;
-            if (hi == m && lo == l) hi = 0;
-        }
-        auto offer = [&](float v, int index) {
-            const unsigned long long k = key_of(v, index);
-            if (k >= tau) {
-                const int n = atomicAdd(&s_n[warp], 1);
-                if (n < kWarpRoom) s_list[warp][n] = k;
-            }
-        };
-        __syncwarp();
-        for (uint32_t left = __ballot_sync(0xffffffffu, seen.any && high >= tau); left; left &= left - 1) {      // the warp reads one lane's elements again
-            const int t = __ffs(left) - 1;
-            if (lane == 0 && t < part.head) offer(to_float<T>(x[t]), t);
-            if (lane == 1 && t < n_tail) offer(to_float<T>(x[part.tail0 + t]), part.tail0 + t);
-            for (int j = t + lane * 32; j < part.vecs; j += 32 * 32) {
-                float2 v[kVec / 2];
-                Vec<T>::elements(__ldg(part.body + j), v);
-#pragma unroll
-                for (int k = 0; k < kVec / 2; ++k) {
-                    offer(v[k].x, part.head + j * kVec + 2 * k);
-                    offer(v[k].y, part.head + j * kVec + 2 * k + 1);
+        const bool any = lane < part.head || lane < part.vecs || lane < n_tail;
+        const uint32_t mine = any ? order_of(seen.r.m) : 0;
+        unsigned long long tau = (unsigned long long)nth_largest(mine, a.top) << 32;
+        bool looked = any && mine >= tau >> 32;
+        int n;
+        for (int tries = 0;; ++tries) {
+            if (lane == 0) s_n[warp] = 0;
+            __syncwarp();
+            if (part.vecs <= 32 * 8) {      // each lane reads its own few vectors again, otherwise the warp one lane's after the other
+                if (looked) collect<T>(x, part, tau, lane, part.head, n_tail, lane, part.vecs, 32, 0, 1, s_list[warp], &s_n[warp], kWarpRoom);
+            } else {
+                for (uint32_t left = __ballot_sync(0xffffffffu, looked); left; left &= left - 1) {
+                    const int t = __ffs(left) - 1;
+                    collect<T>(x, part, tau, t, part.head, n_tail, t, part.vecs, 32, lane, 32, s_list[warp], &s_n[warp], kWarpRoom);
                 }
             }
+            __syncwarp();
+            n = *static_cast<volatile int*>(&s_n[warp]);
+            __syncwarp();
+            if (n <= kWarpRoom || tries) break;
+            // too many of equal value: the same with keys
+            const unsigned long long key = best_key<T>(x, part, lane, part.head, n_tail, lane, part.vecs, 32);
+            unsigned long long left = key;
+            tau = 0;
+            for (int j = 0; j < a.top; ++j) {
+                const uint32_t h = __reduce_max_sync(0xffffffffu, (uint32_t)(left >> 32)), l = __reduce_max_sync(0xffffffffu, (uint32_t)(left >> 32) == h ? (uint32_t)left : 0u);
+                tau = (unsigned long long)h << 32 | l;
+                if (left == tau) left = 0;
+            }
+            looked = key != 0 && key >= tau;
         }
-        __syncwarp();
-        const int n = *static_cast<volatile int*>(&s_n[warp]);
         slow = n > kWarpRoom;
         for (int k = lane; k < n && !slow; k += 32) {
-            const unsigned long long mine = s_list[warp][k];
+            const unsigned long long mine_ = s_list[warp][k];
             int before = 0;
-            for (int j = 0; j < n; ++j) before += s_list[warp][j] > mine;
+            for (int j = 0; j < n; ++j) before += s_list[warp][j] > mine_;
             if (before < a.top) {
-                a.top_tokens[row * a.top + before] = index_of(mine);
-                a.top_logprobs[row * a.top + before] = out.logprob(logit_of(mine));
+                a.top_tokens[row * a.top + before] = index_of(mine_);
+                a.top_logprobs[row * a.top + before] = out.logprob(logit_of(mine_));
             }
         }
     }
@@ -459,7 +487,6 @@ __global__ void __launch_bounds__(kWarpRows * 32) token_logprobs_warp_kernel(con
 // gridDim.x = rows * splits, the CTAs of a row are a cluster.
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
-    constexpr int kVec = 16 / sizeof(T);
     __shared__ Shared<kThreads> sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.x / a.splits;
@@ -482,102 +509,89 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
 
     Seen<T> seen;
     seen.c = c;
-    if (tid < n_head) seen.single(to_float<T>(x[tid]), -1);
+    if (tid < n_head) seen.single(to_float<T>(x[tid]));
     seen.stream(body, lo + tid, hi, kThreads);
-    if (tid < n_tail) {
-        if (!seen.any) seen.at = -2;
-        seen.single(to_float<T>(x[tail0 + tid]), -2);
-    }
+    if (tid < n_tail) seen.single(to_float<T>(x[tail0 + tid]));
 
-    // the block's sums, in a fixed order
-    Sums all = warp_sums(seen.r, lane);
+    Sums all = warp_sums(seen.r);
     if (lane == 0) sh.part[warp] = all;
-
+    const bool any = tid < n_head || lo + tid < hi || tid < n_tail;
+    const uint32_t mine = any ? order_of(seen.r.m) : 0;
+    if (a.top) {
+        uint32_t g = mine;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if ((lane & 7) == 0) sh.largest[tid >> 3] = g;
+    }
     if (a.splits > 1) {
         __syncwarp();
         ptx::cluster_wait();
     }
+    __syncthreads();
     bool too_many = false;
     int n_best = 0;
     if (a.top) {
-        // The thread's largest as a key that is not above the true one (the vector's last index), and one that is not below it.
-        const int first_index = seen.at == -1 ? tid : seen.at == -2 ? tail0 + tid : head + seen.at * kVec;
-        const unsigned long long low = seen.any ? key_of(seen.r.m, first_index + (seen.at >= 0 ? kVec - 1 : 0)) : 0;
-        const unsigned long long high = seen.any ? key_of(seen.r.m, first_index) : 0;
-        // the top-th largest of the largest of 8 threads each: a first bound, so that few keys remain
-        unsigned long long g = low;
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
-            const unsigned long long other = __shfl_xor_sync(0xffffffffu, g, o);
-            g = other > g ? other : g;
-        }
-        if ((lane & 7) == 0) sh.group[tid >> 3] = g;
-        __syncthreads();
-        if (tid < kThreads / 8) {
-            const unsigned long long mine = sh.group[tid];
-            int before = 0;
-#pragma unroll 8
-            for (int j = 0; j < kThreads / 8; ++j) before += sh.group[j] > mine;
-            if (mine && before == a.top - 1) sh.tau = mine;
+        if (warp == 0) {      // (with 64 groups a lane has the larger of two: the bound is lower, and serves all the same)
+            uint32_t g = sh.largest[lane];
+            if constexpr (kThreads == 512) g = max(g, sh.largest[lane + 32]);
+            g = nth_largest(g, a.top);
+            if (lane == 0) sh.tau = (unsigned long long)g << 32;
         }
         __syncthreads();
-        const unsigned long long tau1 = sh.tau;
-        if (low && low >= tau1) sh.list[atomicAdd(&sh.n_list, 1)] = low;      // (no more than there are threads)
-        __syncthreads();
-        const int n1 = sh.n_list;
-        for (int k = tid; k < n1; k += kThreads) {      // the bound itself: the top-th largest of the threads'
-            const unsigned long long mine = sh.list[k];
-            int before = 0;
-            for (int j = 0; j < n1; ++j) before += sh.list[j] > mine;
-            if (before == a.top - 1) sh.tau = mine;
-        }
-        __syncthreads();
-        const unsigned long long tau = sh.tau;
-        if (seen.any && high >= tau) sh.threads[atomicAdd(&sh.n_threads, 1)] = tid;
-        if (tid == 0) sh.n_list = 0;
-        __syncthreads();
-        auto offer = [&](float v, int index) {
-            const unsigned long long k = key_of(v, index);
-            if (k >= tau) {
-                const int n = atomicAdd(&sh.n_list, 1);
-                if (n < kRoom) sh.list[n] = k;
-            }
-        };
-        for (int w = warp; w < sh.n_threads; w += kThreads / 32) {      // a warp reads one thread's elements again
-            const int t = sh.threads[w];
-            if (lane == 0 && t < n_head) offer(to_float<T>(x[t]), t);
-            if (lane == 1 && t < n_tail) offer(to_float<T>(x[tail0 + t]), tail0 + t);
-            for (int j = lo + t + lane * kThreads; j < hi; j += 32 * kThreads) {
-                float2 v[kVec / 2];
-                Vec<T>::elements(__ldg(body + j), v);
-#pragma unroll
-                for (int k = 0; k < kVec / 2; ++k) {
-                    offer(v[k].x, head + j * kVec + 2 * k);
-                    offer(v[k].y, head + j * kVec + 2 * k + 1);
+        unsigned long long tau = sh.tau;
+        bool looked = any && mine >= tau >> 32;
+        int n;
+        for (int tries = 0;; ++tries) {
+            if (looked) sh.threads[atomicAdd(&sh.n_threads, 1)] = tid;
+            __syncthreads();
+            const int n_threads = sh.n_threads;
+            // (all threads for a bound that few tokens are above: masks)
+            if (tries || n_threads <= kThreads / 2) {
+                for (int w = warp; w < n_threads; w += kThreads / 32) {
+                    const int t = sh.threads[w];
+                    collect<T>(x, part, tau, t, n_head, n_tail, lo + t, hi, kThreads, lane, 32, sh.list, &sh.n_list, kRoom);
                 }
+                __syncthreads();
+                n = sh.n_list;
+            } else {
+                n = kRoom + 1;
             }
+            if (n <= kRoom || tries) break;
+            // too many of equal value: the top-th largest of the threads' keys, by way of that of groups of 8
+            const unsigned long long key = best_key<T>(x, part, tid, n_head, n_tail, lo + tid, hi, kThreads);
+            __syncthreads();
+            sh.list[tid] = key;
+            if (tid == 0) {
+                sh.n_threads = 0;
+                sh.tau = 0;
+            }
+            __syncthreads();
+            int before = 0;
+            for (int j = 0; j < kThreads; ++j) before += sh.list[j] > key;
+            if (key && before == a.top - 1) sh.tau = key;
+            __syncthreads();
+            tau = sh.tau;
+            looked = key != 0 && key >= tau;
+            if (tid == 0) sh.n_list = 0;
         }
-        __syncthreads();
-        const int n = sh.n_list;
         too_many = n > kRoom;
         n_best = min(n, a.top);
         if (!too_many) {
             unsigned long long* to = a.splits > 1 ? nullptr : sh.best[0];
             for (int k = tid; k < n; k += kThreads) {
-                const unsigned long long mine = sh.list[k];
+                const unsigned long long key = sh.list[k];
                 int before = 0;
-                for (int j = 0; j < n; ++j) before += sh.list[j] > mine;
+                for (int j = 0; j < n; ++j) before += sh.list[j] > key;
                 if (before < a.top) {
-                    if (to) to[before] = mine;
-                    else ptx::st_cta_u64(ptx::map_to_cta(ptx::smem_u32(&sh.best[rank][before]), 0), mine);
+                    if (to) to[before] = key;
+                    else ptx::st_cta_u64(ptx::map_to_cta(ptx::smem_u32(&sh.best[rank][before]), 0), key);
                 }
             }
             if (a.splits > 1 && tid >= n_best && tid < a.top) ptx::st_cta_u64(ptx::map_to_cta(ptx::smem_u32(&sh.best[rank][tid]), 0), 0);
         }
     }
-    __syncthreads();
-    all = sh.part[0];
-    for (int w = 1; w < kThreads / 32; ++w) all = joined(all, sh.part[w]);
+    // (the warps' sums, in every warp for itself)
+    all = warp_sums(lane < kThreads / 32 ? sh.part[lane] : Sums{-INFINITY, 0.f, 0.f, -INFINITY});
     if (a.splits > 1) {      // the first CTA finishes the row
         if (tid == 0) {
             const uint32_t to = ptx::map_to_cta(ptx::smem_u32(&sh.row[rank]), 0);
@@ -588,12 +602,8 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
         __syncwarp();
         ptx::cluster_sync();
         if (rank) return;
-        all = sh.row[0];
-        too_many = sh.too_many[0] != 0;
-        for (int k = 1; k < a.splits; ++k) {
-            all = joined(all, sh.row[k]);
-            too_many = too_many || sh.too_many[k] != 0;
-        }
+        all = warp_sums(lane < a.splits ? sh.row[lane] : Sums{-INFINITY, 0.f, 0.f, -INFINITY});
+        too_many = __any_sync(0xffffffffu, lane < a.splits && sh.too_many[lane] != 0);
     }
     Row out;
     out.scale = a.scale;
@@ -612,6 +622,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
         return;
     }
     if (a.top) {
+        if (a.splits == 1) __syncthreads();
         const int n = a.splits * a.top;
         for (int k = tid; k < n; k += kThreads) {
             const unsigned long long mine = sh.best[k / a.top][k % a.top];
