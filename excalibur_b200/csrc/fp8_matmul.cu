@@ -599,10 +599,12 @@ int encode(CUtensorMap* map, const uint8_t* base, int64_t rows, int K, int64_t s
 
 using namespace exb;
 
-extern "C" int exb_fp8_matmul_fwd(exb_ctx* ctx, const uint8_t* a, int64_t a_stride, const float* a_scales, int64_t a_scale_stride,
-                                  const uint8_t* w, int64_t w_stride, const float* w_scales, int64_t w_scale_stride, const float* bias, void* y,
-                                  int y_dtype, int64_t y_stride, int64_t M, int N, int K, void* stream) {
-    EXB_REQUIRE(ctx != nullptr, "exb_fp8_matmul_fwd: null context");
+extern "C" int exb_fp8_matmul_fwd(exb_ctx* ctx, const exb_matmul_desc* d, const uint8_t* a, const float* a_scales, const uint8_t* w,
+                                  const float* w_scales, const float* bias, void* y, void* stream) {
+    EXB_REQUIRE(ctx != nullptr && d != nullptr, "exb_fp8_matmul_fwd: null context or descriptor");
+    const int64_t M = d->M, a_stride = d->a_stride, a_scale_stride = d->a_scale_stride, w_stride = d->w_stride, w_scale_stride = d->w_scale_stride,
+                  y_stride = d->y_stride;
+    const int N = d->N, K = d->K, y_dtype = d->y_dtype;
     const size_t es = rows::element_size(y_dtype);
     EXB_REQUIRE(es != 0, "exb_fp8_matmul_fwd: y must be EXB_F16, EXB_BF16 or EXB_F32, got %d", y_dtype);
     EXB_REQUIRE(M >= 0 && N >= 1 && K >= 1, "exb_fp8_matmul_fwd: bad shape (%lld x %d x %d)", (long long)M, N, K);

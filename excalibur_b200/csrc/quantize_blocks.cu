@@ -82,9 +82,10 @@ __global__ void __launch_bounds__(kTileWarps * 32, sizeof(T) == 2 ? 2 : 1) quant
 
 using namespace exb;
 
-extern "C" int exb_quantize_blocks_fwd(exb_ctx* ctx, const void* x, int in_dtype, int64_t x_stride, uint8_t* q, int64_t q_stride,
-                                       float* scales, int64_t scale_stride, int64_t n_rows, int C, int block_rows, void* stream) {
-    EXB_REQUIRE(ctx != nullptr, "exb_quantize_blocks_fwd: null context");
+extern "C" int exb_quantize_blocks_fwd(exb_ctx* ctx, const exb_blocks_desc* d, const void* x, uint8_t* q, float* scales, void* stream) {
+    EXB_REQUIRE(ctx != nullptr && d != nullptr, "exb_quantize_blocks_fwd: null context or descriptor");
+    const int in_dtype = d->in_dtype, C = d->C, block_rows = d->block_rows;
+    const int64_t n_rows = d->rows, x_stride = d->x_stride, q_stride = d->q_stride, scale_stride = d->scale_stride;
     const size_t es = rows::element_size(in_dtype);
     EXB_REQUIRE(es != 0, "exb_quantize_blocks_fwd: x must be EXB_F16, EXB_BF16 or EXB_F32, got %d", in_dtype);
     EXB_REQUIRE(n_rows >= 0 && C >= 1, "exb_quantize_blocks_fwd: bad shape (%lld rows of %d)", (long long)n_rows, C);

@@ -650,10 +650,12 @@ int launch(const exb_ctx* ctx, LogprobArgs& a, int64_t n_rows, cudaStream_t st) 
 
 using namespace exb;
 
-extern "C" int exb_token_logprobs_fwd(exb_ctx* ctx, const void* logits, int dtype, int64_t stride, int64_t n_rows, int V, float scale,
-                                      const int32_t* tokens, int n_given, float* logprobs, float* entropy, int top, float* top_logprobs,
-                                      int32_t* top_tokens, void* stream) {
-    EXB_REQUIRE(ctx != nullptr, "exb_token_logprobs_fwd: null context");
+extern "C" int exb_token_logprobs_fwd(exb_ctx* ctx, const exb_logprobs_desc* d, const void* logits, const int32_t* tokens, float* logprobs,
+                                      float* entropy, float* top_logprobs, int32_t* top_tokens, void* stream) {
+    EXB_REQUIRE(ctx != nullptr && d != nullptr, "exb_token_logprobs_fwd: null context or descriptor");
+    const int64_t n_rows = d->rows, stride = d->stride;
+    const int dtype = d->dtype, V = d->V, n_given = d->n_given, top = d->top;
+    const float scale = d->scale;
     const size_t es = rows::element_size(dtype);
     EXB_REQUIRE(es != 0, "exb_token_logprobs_fwd: logits must be EXB_F16, EXB_BF16 or EXB_F32, got %d", dtype);
     EXB_REQUIRE(n_rows >= 0 && V >= 1, "exb_token_logprobs_fwd: bad shape (%lld rows of %d)", (long long)n_rows, V);

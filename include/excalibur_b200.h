@@ -487,9 +487,16 @@ EXB_API int exb_channel_affine_fwd(exb_ctx* ctx, const void* x, void* y, const f
  * between C and q_stride are left alone).  scales: block_rows 1: [ceil(C / 128)][rows], block_rows 128: [ceil(rows / 128)]
  * [ceil(C / 128)]; scale_stride is the distance of the first index, in floats.
  * ------------------------------------------------------------------------------------- */
-EXB_API int exb_quantize_blocks_fwd(exb_ctx* ctx, const void* x, int in_dtype, int64_t x_stride, uint8_t* q,
-                                    int64_t q_stride, float* scales, int64_t scale_stride, int64_t rows, int C,
-                                    int block_rows, void* stream);
+typedef struct exb_blocks_desc {
+    int64_t rows;
+    int32_t C;
+    int32_t in_dtype;       /* of x */
+    int32_t block_rows;     /* 1 or 128 */
+    int32_t reserved;       /* 0 */
+    int64_t x_stride, q_stride, scale_stride;
+} exb_blocks_desc;
+EXB_API int exb_quantize_blocks_fwd(exb_ctx* ctx, const exb_blocks_desc* d, const void* x, uint8_t* q, float* scales,
+                                    void* stream);
 
 /* Matrix product of what exb_quantize_blocks_fwd writes:
  *   y[m][n] = sum over blocks b of 128: a_scales[b][m] * w_scales[n / 128][b] * sum over k in b: a[m][k] * w[n][k]  (+ bias[n])
@@ -497,10 +504,15 @@ EXB_API int exb_quantize_blocks_fwd(exb_ctx* ctx, const void* x, int in_dtype, i
  * NULL; y: [M][N] in EXB_F16, EXB_BF16 or EXB_F32.  a and w: 16-byte aligned, strides multiples of 16 and >= K (what
  * lies between K and the stride is not read).  Products and their sums are fp32, rounded once at the end; the order of a sum depends on M, N and K
  * and the device, not on the run. */
-EXB_API int exb_fp8_matmul_fwd(exb_ctx* ctx, const uint8_t* a, int64_t a_stride, const float* a_scales,
-                               int64_t a_scale_stride, const uint8_t* w, int64_t w_stride, const float* w_scales,
-                               int64_t w_scale_stride, const float* bias, void* y, int y_dtype, int64_t y_stride,
-                               int64_t M, int N, int K, void* stream);
+typedef struct exb_matmul_desc {
+    int64_t M;
+    int32_t N, K;
+    int32_t y_dtype;
+    int32_t reserved;       /* 0 */
+    int64_t a_stride, a_scale_stride, w_stride, w_scale_stride, y_stride;
+} exb_matmul_desc;
+EXB_API int exb_fp8_matmul_fwd(exb_ctx* ctx, const exb_matmul_desc* d, const uint8_t* a, const float* a_scales,
+                               const uint8_t* w, const float* w_scales, const float* bias, void* y, void* stream);
 
 /* A block's result joins the residual stream, and the next block's norm is taken of the sum:
  *   u = post_weight ? norm(h) * post_weight + post_bias : h
@@ -536,9 +548,17 @@ EXB_API int exb_residual_norm_fwd(exb_ctx* ctx, const exb_norm_desc* d, const vo
  * infinity and entropy 0; a row with a NaN or plus infinity has NaN everywhere (NaN sorts above plus infinity).  A
  * given token below 0 is none: its log probability is 0; one of V or more is an error of the caller's: NaN.
  * tokens: int32 [rows][n_given], top: 0..32 and at most V.  entropy may be NULL, and so may what n_given or top of 0 leave empty. */
-EXB_API int exb_token_logprobs_fwd(exb_ctx* ctx, const void* logits, int dtype, int64_t stride, int64_t rows, int V,
-                                   float scale, const int32_t* tokens, int n_given, float* logprobs, float* entropy,
-                                   int top, float* top_logprobs, int32_t* top_tokens, void* stream);
+typedef struct exb_logprobs_desc {
+    int64_t rows, stride;   /* of logits */
+    int32_t V;
+    int32_t dtype;          /* of logits */
+    int32_t n_given, top;
+    float scale;
+    int32_t reserved;       /* 0 */
+} exb_logprobs_desc;
+EXB_API int exb_token_logprobs_fwd(exb_ctx* ctx, const exb_logprobs_desc* d, const void* logits, const int32_t* tokens,
+                                   float* logprobs, float* entropy, float* top_logprobs, int32_t* top_tokens,
+                                   void* stream);
 
 #ifdef __cplusplus
 }

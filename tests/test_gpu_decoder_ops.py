@@ -553,14 +553,31 @@ def test_refusals(ctx):
             call()
         assert e.value.code in (capi.EXB_ERR_BAD_ARG, capi.EXB_ERR_UNSUPPORTED), i
     ctx.sync_check()
-    # null buffers, at the C entries
-    L = capi.lib()
-    h = ctx.handle
-    assert L.exb_quantize_blocks_fwd(h, None, capi.EXB_F32, 256, q.data_ptr(), 256, s.data_ptr(), 8, 8, 256, 1, None) == capi.EXB_ERR_BAD_ARG
-    assert L.exb_quantize_blocks_fwd(None, x.data_ptr(), capi.EXB_F32, 256, q.data_ptr(), 256, s.data_ptr(), 8, 8, 256, 1, None) == capi.EXB_ERR_BAD_ARG
-    assert L.exb_quantize_blocks_fwd(h, x.data_ptr(), capi.EXB_F32, 255, q.data_ptr(), 256, s.data_ptr(), 8, 8, 256, 1, None) == capi.EXB_ERR_BAD_ARG
-    assert L.exb_fp8_matmul_fwd(h, q.data_ptr(), 256, s.data_ptr(), 8, w.data_ptr(), 256, sw.data_ptr(), 2, None, None, capi.EXB_F16, 8, 8, 8, 256, None) == capi.EXB_ERR_BAD_ARG
-    assert L.exb_fp8_matmul_fwd(h, q.data_ptr(), 256, s.data_ptr(), 8, w.data_ptr(), 256, sw.data_ptr(), 2, None, x.data_ptr(), capi.EXB_F16, 8, 8, 8, 0, None) == capi.EXB_ERR_BAD_ARG
-    assert L.exb_residual_norm_fwd(h, None, x.data_ptr(), *[None] * 10) == capi.EXB_ERR_BAD_ARG
-    assert L.exb_token_logprobs_fwd(h, None, capi.EXB_F32, 256, 8, 256, 1.0, None, 0, None, s.data_ptr(), 0, None, None, None) == capi.EXB_ERR_BAD_ARG
-    assert L.exb_token_logprobs_fwd(h, x.data_ptr(), capi.EXB_F32, 256, 8, 256, 1.0, None, 1, None, None, 0, None, None, None) == capi.EXB_ERR_BAD_ARG
+    # null buffers and descriptors, at the C entries
+    import ctypes as C
+    L, h, E = capi.lib(), ctx.handle, capi.EXB_ERR_BAD_ARG
+    xp, qp, sp, wp, swp = (v.data_ptr() for v in (x, q, s, w, sw))
+
+    def blocks(**k):
+        return C.byref(capi.BlocksDesc(**{**dict(rows=8, C=256, in_dtype=capi.EXB_F32, block_rows=1, x_stride=256, q_stride=256, scale_stride=8), **k}))
+    assert L.exb_quantize_blocks_fwd(h, blocks(), None, qp, sp, None) == E
+    assert L.exb_quantize_blocks_fwd(None, blocks(), xp, qp, sp, None) == E
+    assert L.exb_quantize_blocks_fwd(h, None, xp, qp, sp, None) == E
+    for k in (dict(x_stride=255), dict(q_stride=200), dict(q_stride=264), dict(scale_stride=7), dict(rows=-1), dict(C=0), dict(in_dtype=capi.EXB_I8)):
+        assert L.exb_quantize_blocks_fwd(h, blocks(**k), xp, qp, sp, None) == E, k
+
+    def matmul(**k):
+        return C.byref(capi.MatmulDesc(**{**dict(M=8, N=8, K=256, y_dtype=capi.EXB_F16, a_stride=256, a_scale_stride=8, w_stride=256, w_scale_stride=2, y_stride=8), **k}))
+    assert L.exb_fp8_matmul_fwd(h, matmul(), qp, sp, wp, swp, None, None, None) == E
+    assert L.exb_fp8_matmul_fwd(h, None, qp, sp, wp, swp, None, xp, None) == E
+    for k in (dict(K=0), dict(N=0), dict(M=-1), dict(a_stride=240), dict(w_stride=250), dict(y_stride=7), dict(w_scale_stride=1), dict(y_dtype=capi.EXB_I8)):
+        assert L.exb_fp8_matmul_fwd(h, matmul(**k), qp, sp, wp, swp, None, xp, None) == E, k
+    assert L.exb_residual_norm_fwd(h, None, xp, *[None] * 10) == E
+
+    def scores(**k):
+        return C.byref(capi.LogprobsDesc(**{**dict(rows=8, stride=256, V=256, dtype=capi.EXB_F32, n_given=0, top=0, scale=1.0), **k}))
+    assert L.exb_token_logprobs_fwd(h, scores(), None, None, None, sp, None, None, None) == E
+    assert L.exb_token_logprobs_fwd(h, None, xp, None, None, sp, None, None, None) == E
+    for k in (dict(n_given=1), dict(top=1), dict(stride=255), dict(V=0), dict(rows=-1), dict(scale=-1.0), dict(top=-1), dict(dtype=capi.EXB_I32)):
+        assert L.exb_token_logprobs_fwd(h, scores(**k), xp, None, None, sp, None, None, None) == E, k
+    ctx.sync_check()
