@@ -62,7 +62,7 @@ __device__ __forceinline__ void store_four(const MatmulParams& p, int m, int n, 
 constexpr int kFewBufs = 4;          // accumulators in turn: TMEM has room
 constexpr int kFewTable = 16;        // blocks whose scales are in shared memory at a time
 constexpr int few_stages(int cols) { return cols == 128 ? 4 : cols == 64 ? 3 : cols == 32 ? 4 : 5; }      // (two CTAs fit an SM up to 64 columns)
-constexpr int few_epi_warps(int cols) { return cols == 128 ? 8 : 4; }
+constexpr int few_epi_warps(int cols) { return cols >= 64 ? 8 : 4; }
 constexpr int few_stage_bytes(int cols) { return (128 + cols) * kBlk; }
 constexpr int few_smem(int cols) { return few_stages(cols) * few_stage_bytes(cols) + kFewTable * cols * 4 + cols * 512 + 1024; }
 
