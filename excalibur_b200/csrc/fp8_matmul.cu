@@ -62,7 +62,7 @@ __device__ __forceinline__ void store_four(const MatmulParams& p, int m, int n, 
 constexpr int kFewBufs = 4;          // accumulators in turn: TMEM has room
 constexpr int kFewTable = 16;        // blocks whose scales are in shared memory at a time
 constexpr int few_stages(int cols) { return cols == 128 ? 4 : cols == 64 ? 3 : cols == 32 ? 4 : 5; }      // (two CTAs fit an SM up to 64 columns)
-constexpr int few_epi_warps(int cols) { return cols >= 64 ? 8 : 4; }
+constexpr int few_epi_warps(int cols) { return cols == 128 ? 16 : cols == 64 ? 8 : 4; }
 constexpr int few_stage_bytes(int cols) { return (128 + cols) * kBlk; }
 constexpr int few_smem(int cols) { return few_stages(cols) * few_stage_bytes(cols) + kFewTable * cols * 4 + cols * 512 + 1024; }
 
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
         if (!ok) ptx::give_up(p.error, 2);
         __syncwarp();
     } else {
-        const int q = warp & 3, c0 = warp < 7 ? 0 : kMine, et = (int)threadIdx.x - 96;
+        const int q = warp & 3, c0 = ((warp - 3) >> 2) * kMine, et = (int)threadIdx.x - 96;
         const float* sw = p.w_scales + (int64_t)(n0 / kBlk) * p.w_scale_stride + b0;
 #pragma unroll
         for (int i = 0; i < kMine; ++i) acc[i] = 0.f;
@@ -308,20 +308,20 @@ __device__ __forceinline__ uint32_t result_pair(float a, float b) {
     return rows::float_to_pair(a, b, T());
 }
 
-// Columns [col, col + kMine) of 32 rows from row0 on: sums in `acc` (a thread has a row), through shared memory to y in full lines.
-template <typename T, int kMine>
-__device__ __forceinline__ void store_rows(const float (&acc)[kMine], uint8_t* stage, T* y, int64_t y_stride, const float* bias, int row0, int col, int M, int N,
+// Columns [col, col + 2 * kPairs) of 32 rows from row0 on: sums in `acc` (a thread has a row), through shared memory to y in full lines.
+template <typename T, int kPairs>
+__device__ __forceinline__ void store_rows(const float2 (&acc)[kPairs], uint8_t* stage, T* y, int64_t y_stride, const float* bias, int row0, int col, int M, int N,
                                            bool vec, int lane) {
     constexpr int kPer = 16 / (int)sizeof(T), kCols = 8 * kPer;      // columns in a unit, in a pass
 #pragma unroll
-    for (int c0 = 0; c0 < kMine; c0 += kCols) {
+    for (int c0 = 0; c0 < 2 * kPairs; c0 += kCols) {
         if (col + c0 >= N) break;
         const int left = N - col - c0;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             float v[kPer];
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) v[j] = acc[c0 + u * kPer + j];
+            for (int j = 0; j < kPer; ++j) v[j] = j & 1 ? acc[(c0 + u * kPer + j) / 2].y : acc[(c0 + u * kPer + j) / 2].x;
             if (bias) {
 #pragma unroll
                 for (int j = 0; j < kPer; ++j)
@@ -497,9 +497,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
                 a_scale[1] = __ldg(sa += p.a_scale_stride);
                 w_scale[1] = __ldg(++sw);
             }
-            float acc[kPairCols];
+            float2 acc[kPairCols / 2];
 #pragma unroll
-            for (int i = 0; i < kPairCols; ++i) acc[i] = 0.f;
+            for (int i = 0; i < kPairCols / 2; ++i) acc[i] = make_float2(0.f, 0.f);
             for (int b = 0; b < p.blocks && ok; b += 2) {
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -527,7 +527,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
                             if (lane == 0) ptx::mbar_arrive_cluster_u32(full_lead + next * 8);
                         }
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(__uint_as_float(raw[j]), s, acc[c + j]);
+                        for (int j = 0; j < 8; ++j)
+                            acc[c / 2 + j] = __ffma2_rn(make_float2(__uint_as_float(raw[2 * j]), __uint_as_float(raw[2 * j + 1])), make_float2(s, s), acc[c / 2 + j]);
                     }
                     if (++next == kPairStages) next = 0;
                     if (++buf == kBufs) {
@@ -555,8 +556,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
 
 // Which kernel and how it divides the product: the one whose time is least by what was measured of each (graph-captured calls, us):
 //  - few rows, up to 64 columns: the only one that does not compute rows that are not there;
-//  - few rows, 128 columns: 4.5 + 2 where K is divided + 0.58 for each K block that a CTA works on one after the other
-//    (128 x 14336 x 4096 21.6; 128 x 4096 x 4096 in four parts 11.1);
+//  - few rows, 128 columns: 4.5 + 2 where K is divided + 0.53 for each K block that a CTA works on one after the other
+//    (128 x 8192 x 4096 in two parts 14.9, 128 x 4096 x 4096 in four 10.8);
 //  - pairs with tiles of 128 columns: 4.5 + 0.335 a block (512 x 4096 x 4096 14.9, in 256 columns 18.1);
 //  - pairs with tiles of 256 columns: 5 + 0.43 a block (256 x 14336 x 4096 19.9, in 128 columns 25.5; 4096^3 67 and 81).
 struct Plan {
@@ -575,7 +576,7 @@ Plan plan_for(int sms, int M, int N, int blocks) {
     auto rounds = [](int64_t tiles, int64_t places) { return (double)((tiles + places - 1) / places); };
     const int64_t few_tiles = ((int64_t)M + 127) / 128 * n_tiles, m_pairs = ((int64_t)M + kPairM - 1) / kPairM;
     const int splits = parts(few_tiles, sms);
-    const double few = 4.5 + (splits > 1 ? 2.0 : 0.0) + 0.58 * rounds(few_tiles * splits, sms) * ((blocks + splits - 1) / splits);
+    const double few = 4.5 + (splits > 1 ? 2.0 : 0.0) + 0.53 * rounds(few_tiles * splits, sms) * ((blocks + splits - 1) / splits);
     const double pair128 = 4.5 + 0.335 * rounds(m_pairs * n_tiles, sms / 2) * blocks;
     const double pair256 = 5.0 + 0.43 * rounds(m_pairs * (((int64_t)N + 255) / 256), sms / 2) * blocks;
     if (few < pair128 && few < pair256 && few_tiles / n_tiles <= 65535) return {true, 128, splits};

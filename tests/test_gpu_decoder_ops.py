@@ -581,3 +581,41 @@ def test_refusals(ctx):
     for k in (dict(n_given=1), dict(top=1), dict(stride=255), dict(V=0), dict(rows=-1), dict(scale=-1.0), dict(top=-1), dict(dtype=capi.EXB_I32)):
         assert L.exb_token_logprobs_fwd(h, scores(**k), xp, None, None, sp, None, None, None) == E, k
     ctx.sync_check()
+
+
+# ---- together ------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,C,V", [(1, 512, 4001), (70, 1000, 1000), (300, 256, 9000)])
+def test_token_head(ctx, rows, C, V):
+    """Norm, e4m3, product and log probabilities one after the other: each against 64 bits on what the one before it wrote."""
+    torch, capi = _mods()
+    from excalibur_b200.token_head import TokenHead
+    g = _gen(rows)
+    rand = lambda *s: torch.randn(s, device="cuda", generator=g)  # noqa: E731
+    w = 1 + 0.1 * rand(C)
+    head = TokenHead(ctx, rand(V, C).half() * 0.1, w, residual_scale=0.5)
+    h, x = rand(rows, C).half(), rand(rows, C).half()
+    tokens = torch.randint(0, V, (rows, 2), device="cuda", generator=g).int()
+    r, logits = head.logits(h, x, out_dtype=capi.EXB_F32)
+    r2, q, s = capi.residual_norm(ctx, h, x, residual_scale=0.5, weight=w, quantized=True)
+    ctx.sync_check()
+    assert torch.equal(r, r2)
+    _check_product(logits, q, s, head.weights, head.scales, None, "float32")
+    given, entropy, best, best_tokens = head.scores(h, x, tokens, top=5, temperature=2.0, out_dtype=capi.EXB_F32)
+    again = capi.token_logprobs(ctx, logits, tokens, top=5, scale=0.5)
+    ctx.sync_check()
+    assert all(torch.equal(a, b) for a, b in zip((given, entropy, best, best_tokens), again))
+    _check_logprobs(ctx, logits, tokens, 5, 0.5)
+    # and the whole against the same without 8 bits: e4m3 is off by 2^-4 of each factor at most, which random signs average out
+    ref = (x.double() + 0.5 * h.double())
+    ref = ref * (ref.square().mean(1, keepdim=True) + 1e-5).rsqrt() * w.double()
+    full = ref @ (_dequantized(head.weights, head.scales, 128)).t()
+    assert ((logits.double() - full).norm() / full.norm()) < 0.04
+
+
+def test_token_head_example_runs(ctx, capsys, monkeypatch):
+    from excalibur_b200 import token_head
+    monkeypatch.setattr("sys.argv", ["token_head", "--rows", "3", "--channels", "256", "--vocab", "1000", "--top", "2"])
+    token_head.main()
+    lines = capsys.readouterr().out.strip().split("\n")
+    assert len(lines) == 3 and all(" best " in line for line in lines)
