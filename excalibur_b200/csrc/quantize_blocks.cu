@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i)
         if (r0 + i < rows) {
-            float v[8];
+            float2 v[4];
             k[i].get(v);
             quantize8(v, k[i].amax(), valid, lane, q + (r0 + i) * q_stride + c0, scales + 2 * share * scale_stride + r0 + i, scale_stride);
         }
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kTileWarps * 32, sizeof(T) == 2 ? 2 : 1) quant
     for (int i = 0; i < kTileSteps; ++i) {
         const int64_t r = r0 + i * kTileWarps;
         if (r >= rows) break;
-        float v[8];
+        float2 v[4];
         k[i].get(v);
         store8_e4m3(q + r * q_stride + c0 + lane * 8, v, inv, valid - lane * 8);
     }

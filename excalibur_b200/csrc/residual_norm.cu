@@ -44,42 +44,47 @@ __device__ __forceinline__ float row_sum(float v, float (*s_sum)[32], int& turn)
     return v;
 }
 
-// v = norm(v) * weight + bias over the row
+// v = norm(v) * weight + bias over the row.  Elements go in pairs, two to an instruction: 40 and more instructions an element are what
+// the fused form with both norms, a gate and e4m3 is bound by.
 template <bool kLayer, Layout kL, bool kOneWarp, int kPer>
-__device__ __forceinline__ void normalise(float (&v)[kPer][8], int lane, int share0, int share_step, const NormArgs& a, const float* weight,
+__device__ __forceinline__ void normalise(float2 (&v)[kPer][4], int lane, int share0, int share_step, const NormArgs& a, const float* weight,
                                           const float* bias, float (*s_sum)[32], int& turn) {
     const float inv_c = 1.f / (float)a.C;
     if constexpr (kLayer) {
-        float s = 0.f;
+        float2 s = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s += v[i][j];
-        const float mean = row_sum<kOneWarp>(s, s_sum, turn) * inv_c;
+            for (int j = 0; j < 4; ++j) s = __fadd2_rn(s, v[i][j]);
+        const float mean = row_sum<kOneWarp>(s.x + s.y, s_sum, turn) * inv_c;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {      // (what lies behind the row's end stays 0)
             const int valid = a.C - (share0 + i * share_step) * kShare;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = (kL == kVectors ? lane * 8 : j * 32 + lane) < valid ? v[i][j] - mean : 0.f;
+            for (int j = 0; j < 4; ++j) {
+                v[i][j].x = (kL == kVectors ? lane * 8 : 2 * j * 32 + lane) < valid ? v[i][j].x - mean : 0.f;
+                v[i][j].y = (kL == kVectors ? lane * 8 : (2 * j + 1) * 32 + lane) < valid ? v[i][j].y - mean : 0.f;
+            }
         }
     }
-    float s = 0.f;
+    float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s = fmaf(v[i][j], v[i][j], s);
-    const float k = rsqrtf(row_sum<kOneWarp>(s, s_sum, turn) * inv_c + a.eps);
+        for (int j = 0; j < 4; ++j) s = __ffma2_rn(v[i][j], v[i][j], s);
+    const float k = rsqrtf(row_sum<kOneWarp>(s.x + s.y, s_sum, turn) * inv_c + a.eps);
+    const float2 kk = make_float2(k, k);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int c0 = (share0 + i * share_step) * kShare, valid = a.C - c0;
-        float w[8];
+        float2 w[4];
         load8_params<kL>(weight + c0, valid, lane, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * k * w[j];
+        for (int j = 0; j < 4; ++j) v[i][j] = __fmul2_rn(__fmul2_rn(v[i][j], kk), w[j]);
         if (bias) {
             load8_params<kL>(bias + c0, valid, lane, w);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] += w[j];
+            for (int j = 0; j < 4; ++j) v[i][j] = __fadd2_rn(v[i][j], w[j]);
         }
     }
 }
@@ -102,7 +107,7 @@ __global__ void __launch_bounds__(max_threads(kOneWarp, kPer)) residual_norm_ker
     // everything is asked for before anything is waited for, as long as there are registers for it
     constexpr bool kAhead = kPer <= 4;
     constexpr int kKept = kAhead ? kPer : 1;
-    float v[kPer][8];
+    float2 v[kPer][4];
     Kept<T, kL> hk[kPer], xk[kKept], gk[kKept];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -120,19 +125,20 @@ __global__ void __launch_bounds__(max_threads(kOneWarp, kPer)) residual_norm_ker
         constexpr int kAll = kAhead ? 1 : 0;
         if (!kAhead && a.x) xk[0].load(x + c0, valid, lane, {});
         if (!kAhead && a.gate) gk[0].load(g + c0, valid, lane, {});
-        float o[8];
+        float2 o[4];
+        const float2 scale = make_float2(a.residual_scale, a.residual_scale);
         if (a.gate) {
             gk[i * kAll].get(o);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] *= o[j];
+            for (int j = 0; j < 4; ++j) v[i][j] = __fmul2_rn(v[i][j], o[j]);
         }
         if (a.x) {
             xk[i * kAll].get(o);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = fmaf(a.residual_scale, v[i][j], o[j]);
+            for (int j = 0; j < 4; ++j) v[i][j] = __ffma2_rn(scale, v[i][j], o[j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] *= a.residual_scale;
+            for (int j = 0; j < 4; ++j) v[i][j] = __fmul2_rn(v[i][j], scale);
         }
         if (a.r) store8<T, kL>(static_cast<T*>(a.r) + row * a.r_stride + c0, valid, lane, v[i]);
     }

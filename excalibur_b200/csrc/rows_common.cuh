@@ -40,19 +40,22 @@ enum Layout { kVectors, kShifted, kStrided };
 
 // fp32 parameters of the share's channels.
 template <Layout kL>
-__device__ __forceinline__ void load8_params(const float* at, int valid, int lane, float (&v)[8]) {
+__device__ __forceinline__ void load8_params(const float* at, int valid, int lane, float2 (&v)[4]) {
     if constexpr (kL == kVectors) {
         if (lane * 8 < valid) {
             const float4 a = __ldg(reinterpret_cast<const float4*>(at + lane * 8)), b = __ldg(reinterpret_cast<const float4*>(at + lane * 8) + 1);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+            v[0] = make_float2(a.x, a.y);
+            v[1] = make_float2(a.z, a.w);
+            v[2] = make_float2(b.x, b.y);
+            v[3] = make_float2(b.z, b.w);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = 0.f;
+            for (int j = 0; j < 4; ++j) v[j] = make_float2(0.f, 0.f);
         }
     } else {
+        auto one = [&](int j) { return j * 32 + lane < valid ? __ldg(at + j * 32 + lane) : 0.f; };
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j * 32 + lane < valid ? __ldg(at + j * 32 + lane) : 0.f;
+        for (int j = 0; j < 4; ++j) v[j] = make_float2(one(2 * j), one(2 * j + 1));
     }
 }
 
@@ -154,17 +157,11 @@ struct Kept {
             for (int j = 0; j < 8; ++j) w[j] = j * 32 + lane < valid ? __float_as_uint(to_float<T>(at[j * 32 + lane])) : 0u;
         }
     }
-    __device__ __forceinline__ void get(float (&o)[8]) const {
-        if constexpr (kPacked) {
+    __device__ __forceinline__ void get(float2 (&o)[4]) const {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = pair_to_float(w[i], T());
-                o[2 * i] = f.x;
-                o[2 * i + 1] = f.y;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = __uint_as_float(w[i]);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (kPacked) o[i] = pair_to_float(w[i], T());
+            else o[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
         }
     }
     // the largest magnitude; NaN are left out
@@ -185,23 +182,25 @@ struct Kept {
 };
 
 template <typename T, Layout kL>
-__device__ __forceinline__ void store8(T* at, int valid, int lane, const float (&v)[8]) {
+__device__ __forceinline__ void store8(T* at, int valid, int lane, const float2 (&v)[4]) {
     static_assert(kL != kShifted, "results are written in vectors or one by one");
     if constexpr (kL == kVectors) {
         if (lane * 8 < valid) {
-            uint4* dst = reinterpret_cast<uint4*>(at + lane * 8);
             if constexpr (sizeof(T) == 4) {
-                dst[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-                dst[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+                float4* dst = reinterpret_cast<float4*>(at + lane * 8);
+                dst[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+                dst[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
             } else {
-                dst[0] = make_uint4(float_to_pair(v[0], v[1], T()), float_to_pair(v[2], v[3], T()), float_to_pair(v[4], v[5], T()),
-                                    float_to_pair(v[6], v[7], T()));
+                *reinterpret_cast<uint4*>(at + lane * 8) = make_uint4(float_to_pair(v[0].x, v[0].y, T()), float_to_pair(v[1].x, v[1].y, T()),
+                                                                      float_to_pair(v[2].x, v[2].y, T()), float_to_pair(v[3].x, v[3].y, T()));
             }
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j * 32 + lane < valid) at[j * 32 + lane] = from_float<T>(v[j]);
+        for (int j = 0; j < 4; ++j) {
+            if (2 * j * 32 + lane < valid) at[2 * j * 32 + lane] = from_float<T>(v[j].x);
+            if ((2 * j + 1) * 32 + lane < valid) at[(2 * j + 1) * 32 + lane] = from_float<T>(v[j].y);
+        }
     }
 }
 
@@ -212,15 +211,16 @@ constexpr float kE4m3Max = 448.f;
 constexpr float kSmallestScale = 1.17549435e-38f;
 
 __device__ __forceinline__ float block_scale(float amax) { return fmaxf(amax / kE4m3Max, kSmallestScale); }
-__device__ __forceinline__ uint32_t to_e4m3x2(float a, float b) {
-    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint32_t to_e4m3x4(float2 a, float2 b) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3);
+    return __byte_perm(lo, hi, 0x5410);
 }
 __device__ __forceinline__ uint8_t to_e4m3(float a) { return (uint8_t)__nv_cvt_float_to_fp8(a, __NV_SATFINITE, __NV_E4M3); }
 
 // 8 neighbours, of which `valid` are the row's.
-__device__ __forceinline__ void store8_e4m3(uint8_t* q, const float (&v)[8], float inv, int valid) {
-    const uint32_t lo = to_e4m3x2(v[0] * inv, v[1] * inv) | to_e4m3x2(v[2] * inv, v[3] * inv) << 16;
-    const uint32_t hi = to_e4m3x2(v[4] * inv, v[5] * inv) | to_e4m3x2(v[6] * inv, v[7] * inv) << 16;
+__device__ __forceinline__ void store8_e4m3(uint8_t* q, const float2 (&v)[4], float inv, int valid) {
+    const float2 ii = make_float2(inv, inv);
+    const uint32_t lo = to_e4m3x4(__fmul2_rn(v[0], ii), __fmul2_rn(v[1], ii)), hi = to_e4m3x4(__fmul2_rn(v[2], ii), __fmul2_rn(v[3], ii));
     if (valid >= 8) {
         *reinterpret_cast<uint2*>(q) = make_uint2(lo, hi);
     } else {
@@ -232,7 +232,7 @@ __device__ __forceinline__ void store8_e4m3(uint8_t* q, const float (&v)[8], flo
 
 // The warp's share of a row, neighbours in each lane (two blocks of 128, 16 lanes each) -> e4m3 and its blocks' scales; m: the lane's
 // largest magnitude.  fmaxf drops NaN: a block's scale comes from its other values, the NaN itself goes into q.
-__device__ __forceinline__ void quantize8(const float (&v)[8], float m, int valid, int lane, uint8_t* __restrict__ q, float* __restrict__ scale,
+__device__ __forceinline__ void quantize8(const float2 (&v)[4], float m, int valid, int lane, uint8_t* __restrict__ q, float* __restrict__ scale,
                                           int64_t scale_stride) {
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -243,26 +243,27 @@ __device__ __forceinline__ void quantize8(const float (&v)[8], float m, int vali
     }
 }
 // The same of every 32nd element: a lane has four of each block.
-__device__ __forceinline__ void quantize8_strided(const float (&v)[8], int valid, int lane, uint8_t* __restrict__ q, float* __restrict__ scale,
+__device__ __forceinline__ void quantize8_strided(const float2 (&v)[4], int valid, int lane, uint8_t* __restrict__ q, float* __restrict__ scale,
                                                   int64_t scale_stride) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
+        const float u[4] = {v[2 * b].x, v[2 * b].y, v[2 * b + 1].x, v[2 * b + 1].y};
         float m = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(v[4 * b + j]));
+        for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(u[j]));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const float s = block_scale(m), inv = 1.f / s;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (b * kBlock + j * 32 + lane < valid) q[b * kBlock + j * 32 + lane] = to_e4m3(v[4 * b + j] * inv);
+            if (b * kBlock + j * 32 + lane < valid) q[b * kBlock + j * 32 + lane] = to_e4m3(u[j] * inv);
         if (lane == 0 && b * kBlock < valid) scale[b * scale_stride] = s;
     }
 }
-__device__ __forceinline__ float largest_of(const float (&v)[8]) {
+__device__ __forceinline__ float largest_of(const float2 (&v)[4]) {
     float m = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
+    for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(fabsf(v[j].x), fabsf(v[j].y)));
     return m;
 }
 
