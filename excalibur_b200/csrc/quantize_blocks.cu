@@ -22,14 +22,16 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int share = blockIdx.x % shares, c0 = share * kShare, valid = C - c0;
     const int64_t r0 = (int64_t)(blockIdx.x / shares) * kTileRows + warp * kRowsPerWarp;
+    const bool inside = r0 >= 8 && r0 + kRowsPerWarp <= rows - 8;
     Kept<T, kL> k[kRowsPerWarp];
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i)
-        if (r0 + i < rows) k[i].load(x + (r0 + i) * x_stride + c0, valid, lane, span);
+        if (r0 + i < rows) k[i].load(x + (r0 + i) * x_stride + c0, valid, lane, span, inside);
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i)
         if (r0 + i < rows) {
             float2 v[4];
+            k[i].settle(x + (r0 + i) * x_stride + c0, valid, lane);
             k[i].get(v);
             quantize8(v, k[i].amax(), valid, lane, q + (r0 + i) * q_stride + c0, scales + 2 * share * scale_stride + r0 + i, scale_stride);
         }
@@ -47,16 +49,20 @@ __global__ void __launch_bounds__(kTileWarps * 32, sizeof(T) == 2 ? 2 : 1) quant
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int share = blockIdx.x % shares, c0 = share * kShare, valid = C - c0;
     const int64_t rb = blockIdx.x / shares, r0 = rb * kBlock + warp;
+    const bool inside = rb > 0 && (rb + 1) * kBlock <= rows - 8;
     Kept<T, kL> k[kTileSteps];
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < kTileSteps; ++i) {
         const int64_t r = r0 + i * kTileWarps;
-        if (r < rows) k[i].load(x + r * x_stride + c0, valid, lane, span);
+        if (r < rows) k[i].load(x + r * x_stride + c0, valid, lane, span, inside);
         else k[i].none();
     }
 #pragma unroll
-    for (int i = 0; i < kTileSteps; ++i) m = fmaxf(m, k[i].amax());
+    for (int i = 0; i < kTileSteps; ++i) {
+        k[i].settle(x + (r0 + i * kTileWarps) * x_stride + c0, valid, lane);
+        m = fmaxf(m, k[i].amax());
+    }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const int half = lane >> 4;

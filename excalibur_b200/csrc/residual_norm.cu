@@ -112,9 +112,9 @@ __global__ void __launch_bounds__(max_threads(kOneWarp, kPer)) residual_norm_ker
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int c0 = (share0 + i * share_step) * kShare, valid = a.C - c0;
-        hk[i].load(h + c0, valid, lane, {});
-        if (kAhead && a.x) xk[kAhead ? i : 0].load(x + c0, valid, lane, {});
-        if (kAhead && a.gate) gk[kAhead ? i : 0].load(g + c0, valid, lane, {});
+        hk[i].load(h + c0, valid, lane);
+        if (kAhead && a.x) xk[kAhead ? i : 0].load(x + c0, valid, lane);
+        if (kAhead && a.gate) gk[kAhead ? i : 0].load(g + c0, valid, lane);
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) hk[i].get(v[i]);
@@ -123,8 +123,8 @@ __global__ void __launch_bounds__(max_threads(kOneWarp, kPer)) residual_norm_ker
     for (int i = 0; i < kPer; ++i) {
         const int c0 = (share0 + i * share_step) * kShare, valid = a.C - c0;
         constexpr int kAll = kAhead ? 1 : 0;
-        if (!kAhead && a.x) xk[0].load(x + c0, valid, lane, {});
-        if (!kAhead && a.gate) gk[0].load(g + c0, valid, lane, {});
+        if (!kAhead && a.x) xk[0].load(x + c0, valid, lane);
+        if (!kAhead && a.gate) gk[0].load(g + c0, valid, lane);
         float2 o[4];
         const float2 scale = make_float2(a.residual_scale, a.residual_scale);
         if (a.gate) {

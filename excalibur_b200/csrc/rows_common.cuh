@@ -83,30 +83,33 @@ __device__ __forceinline__ uint4 load16_within(const uint8_t* at, const Span& sp
 }
 
 // A warp's share of 256 elements, 8 neighbours in each lane, of a row that starts anywhere: whole 16-byte vectors are read, at
-// multiples of 16, and moved into place between neighbouring lanes.  About 20 instructions for 8 elements of 16 bits; eight loads
-// of single elements for each lane's 8 took 3.7 times the time of aligned rows (8192 x 14335 bf16 to e4m3: 200 us, 63 aligned).
+// multiples of 16 (fetch), and then moved into place between neighbouring lanes (settle).  Two steps, so that several rows can be
+// asked for before the first is there.  Eight loads of single elements for each lane's 8 took 3.2 times the time of aligned rows
+// (8192 x 14335 bf16 to e4m3: 200 us, 63 aligned), both steps at once for each row 1.7 times.
+// inside: no 16 bytes that hold some of the row reach out of the span (rows that have 8 others before and behind them).
 template <typename T>
-__device__ __forceinline__ void load8_shifted(const T* row_at, int valid, int lane, const Span& span, uint32_t (&out)[2 * sizeof(T)]) {
-    constexpr int kWords = 8 * sizeof(T) / 4, kVecs = kWords / 4;      // of a lane
+__device__ __forceinline__ void fetch8_shifted(const T* row_at, int valid, int lane, const Span& span, bool inside, uint32_t (&x)[2 * sizeof(T) + 4]) {
+    constexpr int kWords = 2 * sizeof(T), kVecs = kWords / 4;          // of a lane
     const uintptr_t a = reinterpret_cast<uintptr_t>(row_at);
     const int o = (int)(a & 15);
     const uint8_t* base = reinterpret_cast<const uint8_t*>(a - o);
     const int bytes = o + min(valid, 256) * (int)sizeof(T);            // needed from base on
-    uint32_t x[kWords + 4];
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
+    for (int i = 0; i <= kVecs; ++i) {      // (what follows the last lane's own vectors, it reads itself)
         const int at = (lane * kVecs + i) * 16;
-        const uint4 q = at < bytes ? load16_within<sizeof(T)>(base + at, span) : make_uint4(0, 0, 0, 0);
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (at < bytes && (i < kVecs || lane == 31)) q = inside ? __ldg(reinterpret_cast<const uint4*>(base + at)) : load16_within<sizeof(T)>(base + at, span);
         x[4 * i] = q.x; x[4 * i + 1] = q.y; x[4 * i + 2] = q.z; x[4 * i + 3] = q.w;
     }
-    uint4 last = make_uint4(0, 0, 0, 0);
-    if (lane == 31 && 32 * kVecs * 16 < bytes) last = load16_within<sizeof(T)>(base + 32 * kVecs * 16, span);
-    x[kWords] = __shfl_down_sync(0xffffffffu, x[0], 1);
-    x[kWords + 1] = __shfl_down_sync(0xffffffffu, x[1], 1);
-    x[kWords + 2] = __shfl_down_sync(0xffffffffu, x[2], 1);
-    x[kWords + 3] = __shfl_down_sync(0xffffffffu, x[3], 1);
-    if (lane == 31) {
-        x[kWords] = last.x; x[kWords + 1] = last.y; x[kWords + 2] = last.z; x[kWords + 3] = last.w;
+}
+template <typename T>
+__device__ __forceinline__ void settle8_shifted(const T* row_at, int valid, int lane, uint32_t (&x)[2 * sizeof(T) + 4]) {
+    constexpr int kWords = 2 * sizeof(T);
+    const int o = (int)(reinterpret_cast<uintptr_t>(row_at) & 15);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t next = __shfl_down_sync(0xffffffffu, x[i], 1);
+        if (lane < 31) x[kWords + i] = next;
     }
     // by o bytes: two words, one word, half a word
     if (o & 8) {
@@ -117,17 +120,19 @@ __device__ __forceinline__ void load8_shifted(const T* row_at, int valid, int la
 #pragma unroll
         for (int i = 0; i < kWords + 1; ++i) x[i] = x[i + 1];
     }
-    const int sh = sizeof(T) == 2 ? (o & 2) * 8 : 0;
+    if constexpr (sizeof(T) == 2) {
+        const int sh = (o & 2) * 8;
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) out[i] = sizeof(T) == 2 ? __funnelshift_r(x[i], x[i + 1], sh) : x[i];
+        for (int i = 0; i < kWords; ++i) x[i] = __funnelshift_r(x[i], x[i + 1], sh);
+    }
     // behind the row's end: 0
     constexpr int kPer = 4 / sizeof(T);
     if (lane * 8 + 8 > valid) {
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {
             const int left = valid - lane * 8 - i * kPer;
-            if (left <= 0) out[i] = 0;
-            else if (kPer == 2 && left == 1) out[i] &= 0xffffu;
+            if (left <= 0) x[i] = 0;
+            else if (kPer == 2 && left == 1) x[i] &= 0xffffu;
         }
     }
 }
@@ -137,12 +142,12 @@ template <typename T, Layout kL>
 struct Kept {
     static constexpr bool kPacked = sizeof(T) == 2 && kL != kStrided;
     static constexpr int kWords = kPacked ? 4 : 8;
-    uint32_t w[kWords];
+    uint32_t w[kWords + (kL == kShifted ? 4 : 0)];
     __device__ __forceinline__ void none() {
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = 0;
+        for (uint32_t& v : w) v = 0;
     }
-    __device__ __forceinline__ void load(const T* at, int valid, int lane, const Span& span) {
+    __device__ __forceinline__ void load(const T* at, int valid, int lane, const Span& span = {}, bool inside = false) {
         if constexpr (kL == kVectors) {
 #pragma unroll
             for (int i = 0; i < kWords / 4; ++i) {
@@ -151,11 +156,15 @@ struct Kept {
                 w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
             }
         } else if constexpr (kL == kShifted) {
-            load8_shifted<T>(at, valid, lane, span, w);
+            fetch8_shifted<T>(at, valid, lane, span, inside, w);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) w[j] = j * 32 + lane < valid ? __float_as_uint(to_float<T>(at[j * 32 + lane])) : 0u;
         }
+    }
+    // (for rows that start anywhere, before anything is taken; by the whole warp)
+    __device__ __forceinline__ void settle(const T* at, int valid, int lane) {
+        if constexpr (kL == kShifted) settle8_shifted<T>(at, valid, lane, w);
     }
     __device__ __forceinline__ void get(float2 (&o)[4]) const {
 #pragma unroll
