@@ -762,8 +762,9 @@ def quantize_blocks(ctx, x, block_rows=1, q=None, scales=None):
     (ceil(channels / 128), rows); 128 (weights): (ceil(rows / 128), ceil(channels / 128)).  q's rows start at multiples of 16 bytes."""
     t = _TORCH or _torch()
     device = ctx.device
-    xs = _row_stride(x, device, "x")
-    rows, channels = x.shape
+    shape = x.shape
+    xs = shape[-1] if x.is_contiguous() and x.get_device() == device and len(shape) == 2 else _row_stride(x, device, "x")
+    rows, channels = shape
     s1 = (channels + 127) // 128
     if block_rows == 1:
         s0, s1 = s1, rows
@@ -773,7 +774,7 @@ def quantize_blocks(ctx, x, block_rows=1, q=None, scales=None):
         q, qs = _e4m3_rows(x, rows, channels)
     else:
         qs = _byte_row_stride(q, device, "q")
-        if q.shape != x.shape:
+        if q.shape != shape:
             _refuse("q has to be of x's shape")
     if scales is None:
         scales = x.new_empty(s0, s1, dtype=t.float32)
@@ -800,8 +801,8 @@ def fp8_matmul(ctx, a, a_scales, w, w_scales, bias=None, out_dtype=EXB_F16, y=No
     if K != k:
         _refuse("a and w have %d and %d columns", K, k)
     blocks = (K + 127) // 128
-    sa = _row_stride(a_scales, device, "a_scales")
-    sw = _row_stride(w_scales, device, "w_scales")
+    sa = M if a_scales.is_contiguous() and a_scales.get_device() == device else _row_stride(a_scales, device, "a_scales")
+    sw = blocks if w_scales.is_contiguous() and w_scales.get_device() == device else _row_stride(w_scales, device, "w_scales")
     if a_scales.dtype is not f32 or a_scales.shape != (blocks, M):
         _refuse("a_scales have to be (%d, %d) float32", blocks, M)
     if w_scales.dtype is not f32 or w_scales.shape != ((N + 127) // 128, blocks):
@@ -826,13 +827,13 @@ def residual_norm(ctx, h, x=None, post_weight=None, post_bias=None, gate=None, g
     gate_rows rows.  Returns (r, n), or with quantized (r, q, scales) as quantize_blocks gives them; without a weight n is None."""
     t = _TORCH or _torch()
     device, dtype, shape = ctx.device, h.dtype, h.shape
-    hs = _row_stride(h, device, "h")
+    hs = shape[-1] if h.is_contiguous() and h.get_device() == device and len(shape) == 2 else _row_stride(h, device, "h")
     rows, Cc = shape
     dt = _DTYPES.get(dtype, -1)
     xs = gs = ns = ss = 0
     xp = gp = np_ = sp = None
     if x is not None:
-        xs = _row_stride(x, device, "x")
+        xs = Cc if x.is_contiguous() and x.get_device() == device else _row_stride(x, device, "x")
         if x.dtype is not dtype or x.shape != shape:
             _refuse("x has to be of h's shape and type")
         xp = x.data_ptr()
@@ -887,8 +888,9 @@ def token_logprobs(ctx, logits, tokens=None, top=0, scale=1.0):
     entropy (rows,), and the `top` most probable tokens with theirs (rows, top); None where nothing was asked for."""
     t = _TORCH or _torch()
     device, f32 = ctx.device, t.float32
-    ls = _row_stride(logits, device, "logits")
-    rows, V = logits.shape
+    shape = logits.shape
+    ls = shape[-1] if logits.is_contiguous() and logits.get_device() == device and len(shape) == 2 else _row_stride(logits, device, "logits")
+    rows, V = shape
     given = 0
     lp = top_lp = top_tokens = tokens_p = lp_p = top_p = top_tokens_p = None
     if tokens is not None:

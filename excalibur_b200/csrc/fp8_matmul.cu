@@ -33,10 +33,7 @@ __device__ __forceinline__ void store_one(void* y, int dtype, int64_t at, float 
 }
 
 // Four neighbouring channels of a row.
-__device__ __forceinline__ void store_four(const MatmulParams& p, int m, int n, float (&v)[4]) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (p.bias && n + j < p.N) v[j] += __ldg(p.bias + n + j);
+__device__ __forceinline__ void store_four(const MatmulParams& p, int m, int n, const float (&v)[4]) {
     const int64_t at = (int64_t)m * p.y_stride + n;
     if (p.vec && n + 4 <= p.N) {
         if (p.y_dtype == EXB_F32)
@@ -175,8 +172,10 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
     } else {
         const int q = warp & 3, c0 = ((warp - 3) >> 2) * kMine, et = (int)threadIdx.x - 96;
         const float* sw = p.w_scales + (int64_t)(n0 / kBlk) * p.w_scale_stride + b0;
+        const int n = n0 + q * 32 + lane;
+        const float start = p.bias && rank == 0 && n < p.N ? __ldg(p.bias + n) : 0.f;      // (asked for before there is anything to add)
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) acc[i] = 0.f;
+        for (int i = 0; i < kMine; ++i) acc[i] = start;
         int buf = 0;
         uint32_t acc_phase = 0;
         for (int b = 0; b < nb; ++b) {
@@ -184,16 +183,16 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
                 if (b) asm volatile("bar.sync 1, %0;" ::"n"(kEpi * 32) : "memory");
                 // a thread has one column; eight loads at a time are under way
                 constexpr int kStep = kEpi * 32 / kCols;
-                const int n = min(nb - b, kFewTable), c = et % kCols;
+                const int rows = min(nb - b, kFewTable), c = et % kCols;
                 const float* sa = p.a_scales + (int64_t)(b0 + b) * p.a_scale_stride + m0 + c;
-                for (int k = et / kCols; k < n; k += 8 * kStep) {
+                for (int k = et / kCols; k < rows; k += 8 * kStep) {
                     float v[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        v[j] = c < cols && k + j * kStep < n ? __ldg(sa + (int64_t)(k + j * kStep) * p.a_scale_stride) * __ldg(sw + b + k + j * kStep) : 0.f;
+                        v[j] = c < cols && k + j * kStep < rows ? __ldg(sa + (int64_t)(k + j * kStep) * p.a_scale_stride) * __ldg(sw + b + k + j * kStep) : 0.f;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (k + j * kStep < n) table[(k + j * kStep) * kCols + c] = v[j];
+                        if (k + j * kStep < rows) table[(k + j * kStep) * kCols + c] = v[j];
                 }
                 asm volatile("bar.sync 1, %0;" ::"n"(kEpi * 32) : "memory");
             }
@@ -231,13 +230,11 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
             }
         }
         if (!ok && lane == 0) atomicExch(p.error, 3);
-        const int n = n0 + q * 32 + lane;
         if (p.splits == 1) {
             if (ok && n < p.N) {
-                const float bias = p.bias ? __ldg(p.bias + n) : 0.f;
 #pragma unroll
                 for (int i = 0; i < kMine; ++i)
-                    if (m0 + c0 + i < p.M) store_one(p.y, p.y_dtype, (int64_t)(m0 + c0 + i) * p.y_stride + n, p.bias ? acc[i] + bias : acc[i]);
+                    if (m0 + c0 + i < p.M) store_one(p.y, p.y_dtype, (int64_t)(m0 + c0 + i) * p.y_stride + n, acc[i]);
             }
         } else if (ok) {      // every MMA has read its operands: the parts take the ring's place
 #pragma unroll
@@ -310,8 +307,8 @@ __device__ __forceinline__ uint32_t result_pair(float a, float b) {
 
 // Columns [col, col + 2 * kPairs) of 32 rows from row0 on: sums in `acc` (a thread has a row), through shared memory to y in full lines.
 template <typename T, int kPairs>
-__device__ __forceinline__ void store_rows(const float2 (&acc)[kPairs], uint8_t* stage, T* y, int64_t y_stride, const float* bias, int row0, int col, int M, int N,
-                                           bool vec, int lane) {
+__device__ __forceinline__ void store_rows(const float2 (&acc)[kPairs], uint8_t* stage, T* y, int64_t y_stride, int row0, int col, int M, int N, bool vec,
+                                           int lane) {
     constexpr int kPer = 16 / (int)sizeof(T), kCols = 8 * kPer;      // columns in a unit, in a pass
 #pragma unroll
     for (int c0 = 0; c0 < 2 * kPairs; c0 += kCols) {
@@ -322,11 +319,6 @@ __device__ __forceinline__ void store_rows(const float2 (&acc)[kPairs], uint8_t*
             float v[kPer];
 #pragma unroll
             for (int j = 0; j < kPer; ++j) v[j] = j & 1 ? acc[(c0 + u * kPer + j) / 2].y : acc[(c0 + u * kPer + j) / 2].x;
-            if (bias) {
-#pragma unroll
-                for (int j = 0; j < kPer; ++j)
-                    if (u * kPer + j < left) v[j] += __ldg(bias + col + c0 + u * kPer + j);
-            }
             uint4 o;
             if constexpr (sizeof(T) == 4)
                 o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
@@ -365,7 +357,8 @@ __device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int& m,
     m = first + r - n * size;
 }
 
-// Warps 0 and 2 load, warp 1 issues the MMAs, two warpgroups keep the sums: 2 x 224 + 56 registers are the 3 x 168 of the launch.
+// Warps 0 and 2 load, warp 1 issues the MMAs, two warpgroups keep the sums: 2 x 224 + 56 registers (2 x 176 + 152 with
+// 128 columns) are the 3 x 168 of the launch.
 constexpr int kPairThreads = 128 + kPairEpiWarps * 32;
 template <int kRegs> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 template <int kRegs> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
@@ -406,7 +399,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
     const uint32_t tfull0 = ptx::smem_u32(tfull_bar), full_lead = ptx::map_to_cta(full0, 0);
     pdl_wait();
     if (warp < 4) {
-        fewer_registers<56>();
+        fewer_registers<kPairN == 256 ? 56 : 152>();
         // The MMAs of a block take 512 (256 columns) or 256 cycles, a wait for a barrier that is complete 90, a load 120 and more.  So
         // the operands have a loading warp each (with one for both, its 560 cycles a block were what the kernel waited for), and the
         // issuing warp has one wait per block: the epilogue warps' arrival that frees the accumulator of block g is counted by the
@@ -475,7 +468,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
             __syncwarp();
         }
     } else {
-        more_registers<224>();
+        more_registers<kPairN == 256 ? 224 : 176>();
         const int q = warp & 3, part = (warp >> 2) - 1;
         uint8_t* stage = ring + kPairStages * kPairStageBytes + (warp - 4) * kStageOut;
         const uint32_t taddr0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(part * kPairCols);
@@ -500,6 +493,13 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
             float2 acc[kPairCols / 2];
 #pragma unroll
             for (int i = 0; i < kPairCols / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+            if (p.bias) {      // (while the first block is on its way)
+#pragma unroll
+                for (int i = 0; i < kPairCols / 2; ++i) {
+                    if (col + 2 * i < p.N) acc[i].x = __ldg(p.bias + col + 2 * i);
+                    if (col + 2 * i + 1 < p.N) acc[i].y = __ldg(p.bias + col + 2 * i + 1);
+                }
+            }
             for (int b = 0; b < p.blocks && ok; b += 2) {
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -526,9 +526,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
                             __syncwarp();
                             if (lane == 0) ptx::mbar_arrive_cluster_u32(full_lead + next * 8);
                         }
+                        // (two sums at an instruction save power, 1 % of 8192^3 under the cap; with 128 columns, where the loop's length
+                        // counts, one at a time is faster: 512 x 4096 x 4096 14.9 us, 16.6 in twos)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            acc[c / 2 + j] = __ffma2_rn(make_float2(__uint_as_float(raw[2 * j]), __uint_as_float(raw[2 * j + 1])), make_float2(s, s), acc[c / 2 + j]);
+                        for (int j = 0; j < 8; ++j) {
+                            const float u = __uint_as_float(raw[2 * j]), v = __uint_as_float(raw[2 * j + 1]);
+                            float2& to = acc[c / 2 + j];
+                            if constexpr (kPairN == 256) to = __ffma2_rn(make_float2(u, v), make_float2(s, s), to);
+                            else to = make_float2(fmaf(u, s, to.x), fmaf(v, s, to.y));
+                        }
                     }
                     if (++next == kPairStages) next = 0;
                     if (++buf == kBufs) {
@@ -539,9 +545,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
             }
             if (!ok) break;
             const int row0 = row - lane;
-            if (p.y_dtype == EXB_F16) store_rows(acc, stage, static_cast<__half*>(p.y), p.y_stride, p.bias, row0, col, p.M, p.N, p.vec, lane);
-            else if (p.y_dtype == EXB_BF16) store_rows(acc, stage, static_cast<__nv_bfloat16*>(p.y), p.y_stride, p.bias, row0, col, p.M, p.N, p.vec, lane);
-            else store_rows(acc, stage, static_cast<float*>(p.y), p.y_stride, p.bias, row0, col, p.M, p.N, p.vec, lane);
+            if (p.y_dtype == EXB_F16) store_rows(acc, stage, static_cast<__half*>(p.y), p.y_stride, row0, col, p.M, p.N, p.vec, lane);
+            else if (p.y_dtype == EXB_BF16) store_rows(acc, stage, static_cast<__nv_bfloat16*>(p.y), p.y_stride, row0, col, p.M, p.N, p.vec, lane);
+            else store_rows(acc, stage, static_cast<float*>(p.y), p.y_stride, row0, col, p.M, p.N, p.vec, lane);
         }
         if (!ok && lane == 0) atomicExch(p.error, 3);
     }
