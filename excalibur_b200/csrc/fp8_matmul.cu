@@ -15,6 +15,9 @@ namespace {
 constexpr int kBlk = 128;                  // K block: bytes of a row in a stage, elements that share a scale
 constexpr uint32_t kMaxSpins = 1u << 21;
 
+// kTmemOrder: a kernel whose CTAs took TMEM while they wait for the previous kernel could take what CTAs of that one, started but not
+// that far, still need, and both would wait for good.  So TMEM is taken behind griddepcontrol.wait, and the next kernel is let in
+// (griddepcontrol.launch_dependents) only behind that.
 struct MatmulParams {
     CUtensorMap tmA, tmW;
     const float *a_scales, *w_scales, *bias;
@@ -79,7 +82,6 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
     const int warp = ptx::uniform_warp(), lane = threadIdx.x & 31;
     const int rank = (int)blockIdx.x % p.splits, n0 = (int)blockIdx.x / p.splits * 128, m0 = blockIdx.y * kCols;
     const int b0 = (int)((int64_t)rank * p.blocks / p.splits), nb = (int)((int64_t)(rank + 1) * p.blocks / p.splits) - b0;
-    pdl_launch_dependents();
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < kStages; ++s) {
@@ -95,14 +97,7 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
         ptx::tma_prefetch_desc(&p.tmA);
         ptx::tma_prefetch_desc(&p.tmW);
     }
-    if (warp == 1) {
-        ptx::tmem_alloc(&tmem_base_smem, kTmem);
-        ptx::tmem_relinquish();
-    }
-    ptx::tc_fence_before_sync();
     __syncthreads();
-    ptx::tc_fence_after_sync();
-    const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_smem, 0);
     const uint32_t ring0 = ptx::smem_u32(ring), full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
     const uint32_t tfull0 = ptx::smem_u32(tfull_bar), tempty0 = ptx::smem_u32(tempty_bar);
     // columns that this CTA finishes: [rank * share, rank * share + mine)
@@ -115,6 +110,20 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
     float acc[kMine];
     bool ok = true;
     pdl_wait();
+    // TMEM is taken when the previous kernel is done, and the next one may start when it is taken (see kTmemOrder).  The loads do not wait
+    // for it.
+    uint32_t tmem_base = 0;
+    if (warp != 0 && warp != 2) {
+        if (warp == 1) {
+            ptx::tmem_alloc(&tmem_base_smem, kTmem);
+            ptx::tmem_relinquish();
+            ptx::tc_fence_before_sync();
+        }
+        asm volatile("bar.sync 2, %0;" ::"n"(kEpi * 32 + 32) : "memory");
+        ptx::tc_fence_after_sync();
+        tmem_base = __shfl_sync(0xffffffffu, tmem_base_smem, 0);
+        pdl_launch_dependents();
+    }
     if (warp == 0 || warp == 2) {      // a loading warp for each operand
         const bool is_w = warp == 0;
         const uint32_t leader = ptx::elect_one() ? 1u : 0u;
@@ -374,7 +383,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
     const int warp = ptx::uniform_warp(), lane = threadIdx.x & 31;
     const int rank = (int)__shfl_sync(0xffffffffu, ptx::cluster_ctarank(), 0);
     const int total = p.m_tiles * p.n_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
-    pdl_launch_dependents();
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < kPairStages; ++s) {
@@ -386,6 +394,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
         ptx::tma_prefetch_desc(&p.tmA);
         ptx::tma_prefetch_desc(&p.tmW);
     }
+    pdl_wait();      // (before TMEM is taken: see kTmemOrder)
     if (warp == 1) {
         ptx::tmem_alloc_pair(&tmem_base_smem, 512);
         ptx::tmem_relinquish_pair();
@@ -394,10 +403,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
     __syncthreads();
     ptx::cluster_sync();
     ptx::tc_fence_after_sync();
+    pdl_launch_dependents();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_smem, 0);
     const uint32_t ring0 = ptx::smem_u32(ring), full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
     const uint32_t tfull0 = ptx::smem_u32(tfull_bar), full_lead = ptx::map_to_cta(full0, 0);
-    pdl_wait();
     if (warp < 4) {
         fewer_registers<kPairN == 256 ? 56 : 152>();
         // The MMAs of a block take 512 (256 columns) or 256 cycles, a wait for a barrier that is complete 90, a load 120 and more.  So

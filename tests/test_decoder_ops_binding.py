@@ -39,3 +39,16 @@ def test_calls_without_a_context_are_refused():
     assert L.exb_residual_norm_fwd(None, *[None] * 12) == capi.EXB_ERR_BAD_ARG
     assert L.exb_token_logprobs_fwd(None, d, None, None, None, None, None, None, None) == capi.EXB_ERR_BAD_ARG
     assert "null context" in capi.last_error()
+
+
+def test_tensor_memory_is_taken_between_the_two_launch_controls():
+    """A kernel that holds tensor memory while it waits for the previous one could keep from that one what it still needs: waited for
+    first, taken, and only then the next kernel is let in.  No run shows it: the window is a fraction of a microsecond."""
+    import re
+    text = open(os.path.join(ROOT, "excalibur_b200", "csrc", "fp8_matmul.cu")).read()
+    kernels = re.findall(r"__global__ .*?\n}\n", text, re.S)
+    assert len(kernels) == 2
+    for body in kernels:
+        wait, alloc, let_in = (body.index(w) for w in ("pdl_wait();", "ptx::tmem_alloc", "pdl_launch_dependents();"))
+        assert wait < alloc < let_in
+        assert all(body.count(w) == 1 for w in ("pdl_wait();", "ptx::tmem_alloc", "pdl_launch_dependents();"))
