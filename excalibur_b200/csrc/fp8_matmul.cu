@@ -305,53 +305,81 @@ constexpr int kPairEpiWarps = 8;                 // two per TMEM lane quarter, h
 constexpr int pair_stage_bytes(int n) { return (kPairM + n) / 2 * kBlk; }      // of one of the two CTAs
 constexpr int pair_stages(int n) { return n == 256 ? 6 : 8; }
 
-// 32 rows x 128 bytes of results per warp, in units of 16 bytes that are XOR-ed with the row: a thread writes its row's units and
-// the warp reads whole rows, both without bank conflicts.
+// Results of 32 rows x up to 128 bytes per warp, in units of 16 bytes that are XOR-ed with the row: a thread writes its row's units
+// and the warp reads whole rows, both without bank conflicts.
 constexpr int kStageOut = 32 * 128;
 
-template <typename T>
-__device__ __forceinline__ uint32_t result_pair(float a, float b) {
-    return rows::float_to_pair(a, b, T());
-}
-
-// Columns [col, col + 2 * kPairs) of 32 rows from row0 on: sums in `acc` (a thread has a row), through shared memory to y in full lines.
+// Columns [col, col + 2 * kPairs) of 32 rows from row0 on: sums in `acc` (a thread has a row), through shared memory to y in whole vectors.
 template <typename T, int kPairs>
 __device__ __forceinline__ void store_rows(const float2 (&acc)[kPairs], uint8_t* stage, T* y, int64_t y_stride, int row0, int col, int M, int N, bool vec,
                                            int lane) {
-    constexpr int kPer = 16 / (int)sizeof(T), kCols = 8 * kPer;      // columns in a unit, in a pass
+    constexpr int kPer = 16 / (int)sizeof(T);                                                   // columns in a unit,
+    constexpr int kUnits = 2 * kPairs / kPer < 8 ? 2 * kPairs / kPer : 8, kCols = kUnits * kPer;      // units and columns in a pass
+    constexpr int kRows = 32 / kUnits;                                                          // rows that the warp writes at a time
+    const int sub = lane / kUnits, u = lane % kUnits;
+    auto unit = [&](int r, int i) { return reinterpret_cast<uint4*>(stage + r * 128 + ((i ^ (r & 7)) << 4)); };
+    auto element = [&](int r, int e) { return reinterpret_cast<const T*>(unit(r, e / kPer))[e % kPer]; };
 #pragma unroll
     for (int c0 = 0; c0 < 2 * kPairs; c0 += kCols) {
         if (col + c0 >= N) break;
         const int left = N - col - c0;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            float v[kPer];
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) v[j] = j & 1 ? acc[(c0 + u * kPer + j) / 2].y : acc[(c0 + u * kPer + j) / 2].x;
-            uint4 o;
+        for (int i = 0; i < kUnits; ++i) {
+            const float2* v = acc + (c0 + i * kPer) / 2;
             if constexpr (sizeof(T) == 4)
-                o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                *unit(lane, i) = make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
             else
-                o = make_uint4(result_pair<T>(v[0], v[1]), result_pair<T>(v[2], v[3]), result_pair<T>(v[4], v[5]), result_pair<T>(v[6], v[7]));
-            *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = o;
+                *unit(lane, i) = make_uint4(rows::float_to_pair(v[0].x, v[0].y, T()), rows::float_to_pair(v[1].x, v[1].y, T()),
+                                            rows::float_to_pair(v[2].x, v[2].y, T()), rows::float_to_pair(v[3].x, v[3].y, T()));
         }
         __syncwarp();
-        T* out = y + col + c0;
-        if (vec && left >= kCols) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + (lane >> 3), u = lane & 7;
-                const uint4 o = *reinterpret_cast<const uint4*>(stage + r * 128 + ((u ^ (r & 7)) << 4));
-                if (row0 + r < M) *reinterpret_cast<uint4*>(out + (int64_t)(row0 + r) * y_stride + u * kPer) = o;
-            }
-        } else {
+        T* out = y + (int64_t)row0 * y_stride + col + c0;
+        if (left < kCols) {
             for (int r = 0; r < 32 && row0 + r < M; ++r) {
 #pragma unroll
-                for (int c = 0; c < kCols; c += 32) {
-                    const int cc = c + lane;
-                    const T o = *reinterpret_cast<const T*>(stage + r * 128 + (((cc / kPer) ^ (r & 7)) << 4) + (cc % kPer) * sizeof(T));
-                    if (cc < left) out[(int64_t)(row0 + r) * y_stride + cc] = o;
+                for (int c = lane; c < kCols; c += 32)
+                    if (c < left) out[r * y_stride + c] = element(r, c);
+            }
+        } else if (vec) {
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const int r = i * kRows + sub;
+                if (row0 + r < M) *reinterpret_cast<uint4*>(out + r * y_stride + u * kPer) = *unit(r, u);
+            }
+        } else {
+            // Rows that start anywhere: kUnits - 1 vectors at multiples of 16 bytes, put together of two units each, and 16 bytes before
+            // and behind them element by element.  (Element by element 4048 x 7313 x 264 took 51.8 us.)
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const int r = i * kRows + sub;
+                if (row0 + r >= M) continue;
+                T* to = out + r * y_stride;
+                const int o = (int)((16 - (reinterpret_cast<uintptr_t>(to) & 15)) & 15);      // bytes before the first multiple of 16
+                if (o == 0) {
+                    *reinterpret_cast<uint4*>(to + u * kPer) = *unit(r, u);
+                    continue;
                 }
+                if (u < kUnits - 1) {
+                    const uint4 a = *unit(r, u), b = *unit(r, u + 1);
+                    uint32_t x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                    if (o & 8) {
+#pragma unroll
+                        for (int k = 0; k < 6; ++k) x[k] = x[k + 2];
+                    }
+                    if (o & 4) {
+#pragma unroll
+                        for (int k = 0; k < 5; ++k) x[k] = x[k + 1];
+                    }
+                    const int sh = (o & 2) * 8;
+                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(to) + o + u * 16) =
+                        make_uint4(__funnelshift_r(x[0], x[1], sh), __funnelshift_r(x[1], x[2], sh), __funnelshift_r(x[2], x[3], sh), __funnelshift_r(x[3], x[4], sh));
+                }
+#pragma unroll
+                for (int k = 0; k < kPer; k += kUnits)      // as many elements before the first vector and behind the last as a unit has
+                    if (k + u < kPer) {
+                        const int e = (k + u) * (int)sizeof(T) < o ? k + u : kCols - kPer + k + u;
+                        to[e] = element(r, e);
+                    }
             }
         }
         __syncwarp();
