@@ -27,14 +27,20 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i)
         if (r0 + i < rows) k[i].load(x + (r0 + i) * x_stride + c0, valid, lane, span, inside);
+    float m[kRowsPerWarp];
 #pragma unroll
-    for (int i = 0; i < kRowsPerWarp; ++i)
-        if (r0 + i < rows) {
-            float2 v[4];
-            k[i].settle(x + (r0 + i) * x_stride + c0, valid, lane);
-            k[i].get(v);
-            quantize8(v, k[i].amax(), valid, lane, q + (r0 + i) * q_stride + c0, scales + 2 * share * scale_stride + r0 + i, scale_stride);
-        }
+    for (int i = 0; i < kRowsPerWarp; ++i) {
+        if (r0 + i < rows) k[i].settle(x + (r0 + i) * x_stride + c0, valid, lane);
+        else k[i].none();
+        m[i] = k[i].amax();
+    }
+    quantize_shares<kRowsPerWarp>(
+        [&](int i, float2(&v)[4]) { k[i].get(v); }, m, lane, scale_stride,
+        [&](int i, int& n) {
+            n = r0 + i < rows ? valid : 0;
+            return q + (r0 + i) * q_stride + c0;
+        },
+        [&](int i) { return scales + 2 * share * scale_stride + r0 + i; });
 }
 
 // Blocks of 128 rows: a CTA has two neighbouring ones, its warps read shares of 256 channels of every 16th row.

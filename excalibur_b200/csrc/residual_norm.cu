@@ -144,16 +144,37 @@ __global__ void __launch_bounds__(max_threads(kOneWarp, kPer)) residual_norm_ker
     }
     if (!a.n) return;
     normalise<kLayer, kL, kOneWarp, kPer>(v, lane, share0, share_step, a, a.weight, a.bias, s_sum, turn);
+    if (a.quantized) {
+        uint8_t* q = static_cast<uint8_t*>(a.n) + row * a.n_stride;
+        if constexpr (kL == kVectors) {
+            float m[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) m[i] = largest_of(v[i]);
+            quantize_shares<kPer>(
+                [&](int i, float2(&o)[4]) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[j] = v[i][j];
+                },
+                m, lane, a.scale_stride,
+                [&](int i, int& n) {
+                    const int c0 = (share0 + i * share_step) * kShare;
+                    n = a.C - c0;
+                    return q + c0;
+                },
+                [&](int i) { return a.n_scales + 2 * (share0 + i * share_step) * a.scale_stride + row; });
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int share = share0 + i * share_step, c0 = share * kShare;
+                quantize8_strided(v[i], a.C - c0, lane, q + c0, a.n_scales + 2 * share * a.scale_stride + row, a.scale_stride);
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const int share = share0 + i * share_step, c0 = share * kShare, valid = a.C - c0;
-        if (a.quantized) {
-            uint8_t* q = static_cast<uint8_t*>(a.n) + row * a.n_stride + c0;
-            float* scale = a.n_scales + 2 * share * a.scale_stride + row;
-            if constexpr (kL == kVectors) quantize8(v[i], largest_of(v[i]), valid, lane, q, scale, a.scale_stride);
-            else quantize8_strided(v[i], valid, lane, q, scale, a.scale_stride);
-        } else
-            store8<T, kL>(static_cast<T*>(a.n) + row * a.n_stride + c0, valid, lane, v[i]);
+        const int c0 = (share0 + i * share_step) * kShare;
+        store8<T, kL>(static_cast<T*>(a.n) + row * a.n_stride + c0, a.C - c0, lane, v[i]);
     }
 }
 

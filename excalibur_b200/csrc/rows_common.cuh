@@ -239,16 +239,40 @@ __device__ __forceinline__ void store8_e4m3(uint8_t* q, const float2 (&v)[4], fl
     }
 }
 
-// The warp's share of a row, neighbours in each lane (two blocks of 128, 16 lanes each) -> e4m3 and its blocks' scales; m: the lane's
-// largest magnitude.  fmaxf drops NaN: a block's scale comes from its other values, the NaN itself goes into q.
-__device__ __forceinline__ void quantize8(const float2 (&v)[4], float m, int valid, int lane, uint8_t* __restrict__ q, float* __restrict__ scale,
-                                          int64_t scale_stride) {
+// kN values of each lane, kN a power of two up to 16: the largest of value number lane % kN over the 16 lanes of a block.  Each step
+// hands half of the values to the neighbour that keeps them, so that 4 values take 5 exchanges instead of 16.  fmaxf drops NaN.
+template <int kN>
+__device__ __forceinline__ float largest_of_block(float (&m)[kN], int lane) {
+    int step = 1;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float s = block_scale(m), inv = 1.f / s;
-    if (lane * 8 < valid) {
-        store8_e4m3(q + lane * 8, v, inv, valid - lane * 8);
-        if ((lane & 15) == 0) scale[(lane >> 4) * scale_stride] = s;
+    for (int n = kN; n > 1; n /= 2, step *= 2) {
+        const bool odd = (lane & step) != 0;
+#pragma unroll
+        for (int j = 0; j < n / 2; ++j) {
+            const float keep = odd ? m[2 * j + 1] : m[2 * j], give = odd ? m[2 * j] : m[2 * j + 1];
+            m[j] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, step));
+        }
+    }
+    for (; step < 16; step *= 2) m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], step));
+    return m[0];
+}
+
+// kN shares (two blocks of 128 each, 16 lanes a block, 8 neighbours a lane) -> e4m3 and their blocks' scales.  m: each lane's largest
+// magnitudes; a block's scale comes from its numbers, a NaN itself goes into q.  A scale costs two IEEE divisions, 40 instructions
+// where a share's 8 elements cost 60: lane i works out that of share i % kN, for all lanes of its block.
+// values(i, v): the lane's elements of share i; q_at(i, valid): where it goes and how many elements it has (0: none); scale_at(i): where its first block's scale goes.
+template <int kN, typename V, typename Q, typename S>
+__device__ __forceinline__ void quantize_shares(V&& values, float (&m)[kN], int lane, int64_t scale_stride, Q&& q_at, S&& scale_at) {
+    const float s = block_scale(largest_of_block<kN>(m, lane)), inv = 1.f / s;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        int valid;      // of the share's elements
+        uint8_t* q = q_at(i, valid);
+        const float each = __shfl_sync(0xffffffffu, inv, (lane & 16) + i);
+        float2 v[4];
+        values(i, v);
+        if (lane * 8 < valid) store8_e4m3(q + lane * 8, v, each, valid - lane * 8);
+        if ((lane & 15) == i && (lane >> 4) * kBlock < valid) scale_at(i)[(lane >> 4) * scale_stride] = s;
     }
 }
 // The same of every 32nd element: a lane has four of each block.
