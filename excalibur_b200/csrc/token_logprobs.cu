@@ -145,7 +145,6 @@ __device__ __forceinline__ Sums warp_sums(const Sums& a) {
     return r;
 }
 
-
 // Where a row's whole 16-byte vectors are, and the single elements before (head) and behind them (tail).
 template <typename T>
 struct Parts {
@@ -162,7 +161,8 @@ struct Parts {
 // A thread's share of a row: every `step`-th of the vectors from `first` below `end`, and an element of the head and of the tail at most.
 template <typename T>
 struct Seen {
-    static constexpr int kAhead = sizeof(T) == 4 ? 8 : 6;      // vectors that are asked for at a time (16 bits: 4, 6 and 8 took 47.8, 47.1 and 49.8 us for 2048 rows of 50001)
+    // vectors that are asked for at a time (16 bits: 4, 6 and 8 took 47.8, 47.1 and 49.8 us for 2048 rows of 50001)
+    static constexpr int kAhead = sizeof(T) == 4 ? 8 : 6;
     Sums r = {-INFINITY, 0.f, 0.f, -INFINITY};
     float2 s2 = {0.f, 0.f}, w2 = {0.f, 0.f};      // on top of r.s and r.w
     float c;
@@ -301,7 +301,8 @@ __device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
     return m;
 }
 
-constexpr int kSplitMax = 8;      // CTAs that share a row
+constexpr int kSplitMax = 8;      // CTAs of kWide threads that share a row
+constexpr int kWide = 512, kNarrow = 256;
 constexpr int kRoom = 512;        // elements from tau on that are put in order
 
 template <int kThreads>
@@ -484,27 +485,28 @@ __global__ void __launch_bounds__(kWarpRows * 32) token_logprobs_warp_kernel(con
     if (slow) slow_row<T, 32>(a, x, row, nullptr, &s_best[warp], known, out);
 }
 
-// gridDim.x = rows * splits, the CTAs of a row are a cluster.
+// gridDim.x = rows * splits, the CTAs of a row are a cluster (kNarrow threads: one CTA a row).
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
     __shared__ Shared<kThreads> sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t row = blockIdx.x / a.splits;
-    const int rank = (int)(blockIdx.x - row * a.splits);
+    const int splits = kThreads == kWide ? a.splits : 1;
+    const int64_t row = blockIdx.x / splits;
+    const int rank = (int)(blockIdx.x - row * splits);
     const T* x = static_cast<const T*>(a.logits) + row * a.stride;
     // Of the row's vectors this CTA has [lo, hi) and a thread every kThreads-th; the head is with the first CTA, the tail with the last.
     const Parts<T> part(x, a.V);
     const int head = part.head, vecs = part.vecs, tail0 = part.tail0;
     const uint4* body = part.body;
-    const int lo = (int)((int64_t)rank * vecs / a.splits), hi = (int)((int64_t)(rank + 1) * vecs / a.splits);
-    const int n_head = rank == 0 ? head : 0, n_tail = rank == a.splits - 1 ? a.V - tail0 : 0;
+    const int lo = (int)((int64_t)rank * vecs / splits), hi = (int)((int64_t)(rank + 1) * vecs / splits);
+    const int n_head = rank == 0 ? head : 0, n_tail = rank == splits - 1 ? a.V - tail0 : 0;
     const float c = a.scale * kLog2e;
     if (tid == 0) {
         sh.n_list = 0;
         sh.n_threads = 0;
         sh.tau = 0;
     }
-    if (a.splits > 1) ptx::cluster_arrive();      // (waited for before anything is written into the first CTA)
+    if (splits > 1) ptx::cluster_arrive();      // (waited for before anything is written into the first CTA)
     pdl_enter();
 
     Seen<T> seen;
@@ -523,7 +525,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
         for (int o = 4; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
         if ((lane & 7) == 0) sh.largest[tid >> 3] = g;
     }
-    if (a.splits > 1) {
+    if (splits > 1) {
         __syncwarp();
         ptx::cluster_wait();
     }
@@ -533,7 +535,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
     if (a.top) {
         if (warp == 0) {      // (with 64 groups a lane has the larger of two: the bound is lower, and serves all the same)
             uint32_t g = sh.largest[lane];
-            if constexpr (kThreads == 512) g = max(g, sh.largest[lane + 32]);
+            if constexpr (kThreads == kWide) g = max(g, sh.largest[lane + 32]);
             g = nth_largest(g, a.top);
             if (lane == 0) sh.tau = (unsigned long long)g << 32;
         }
@@ -577,7 +579,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
         too_many = n > kRoom;
         n_best = min(n, a.top);
         if (!too_many) {
-            unsigned long long* to = a.splits > 1 ? nullptr : sh.best[0];
+            unsigned long long* to = splits > 1 ? nullptr : sh.best[0];
             for (int k = tid; k < n; k += kThreads) {
                 const unsigned long long key = sh.list[k];
                 int before = 0;
@@ -587,12 +589,12 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
                     else ptx::st_cta_u64(ptx::map_to_cta(ptx::smem_u32(&sh.best[rank][before]), 0), key);
                 }
             }
-            if (a.splits > 1 && tid >= n_best && tid < a.top) ptx::st_cta_u64(ptx::map_to_cta(ptx::smem_u32(&sh.best[rank][tid]), 0), 0);
+            if (splits > 1 && tid >= n_best && tid < a.top) ptx::st_cta_u64(ptx::map_to_cta(ptx::smem_u32(&sh.best[rank][tid]), 0), 0);
         }
     }
     // (the warps' sums, in every warp for itself)
     all = warp_sums(lane < kThreads / 32 ? sh.part[lane] : Sums{-INFINITY, 0.f, 0.f, -INFINITY});
-    if (a.splits > 1) {      // the first CTA finishes the row
+    if (splits > 1) {      // the first CTA finishes the row
         if (tid == 0) {
             const uint32_t to = ptx::map_to_cta(ptx::smem_u32(&sh.row[rank]), 0);
             ptx::st_cta_u64(to, (unsigned long long)__float_as_uint(all.s) << 32 | __float_as_uint(all.e));
@@ -602,8 +604,8 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
         __syncwarp();
         ptx::cluster_sync();
         if (rank) return;
-        all = warp_sums(lane < a.splits ? sh.row[lane] : Sums{-INFINITY, 0.f, 0.f, -INFINITY});
-        too_many = __any_sync(0xffffffffu, lane < a.splits && sh.too_many[lane] != 0);
+        all = warp_sums(lane < splits ? sh.row[lane] : Sums{-INFINITY, 0.f, 0.f, -INFINITY});
+        too_many = __any_sync(0xffffffffu, lane < splits && sh.too_many[lane] != 0);
     }
     Row out;
     out.scale = a.scale;
@@ -622,14 +624,14 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
         return;
     }
     if (a.top) {
-        if (a.splits == 1) __syncthreads();
-        const int n = a.splits * a.top;
+        if (splits == 1) __syncthreads();
+        const int n = splits * a.top;
         for (int k = tid; k < n; k += kThreads) {
             const unsigned long long mine = sh.best[k / a.top][k % a.top];
             int before = 0;
-            if (a.splits == 1) before = k;
+            if (splits == 1) before = k;
             else
-                for (int j = 0; j < a.splits; ++j)
+                for (int j = 0; j < splits; ++j)
                     for (int l = 0; l < a.top; ++l) before += sh.best[j][l] > mine;
             if (before < a.top && mine) {
                 a.top_tokens[row * a.top + before] = index_of(mine);
@@ -679,22 +681,28 @@ extern "C" int exb_token_logprobs_fwd(exb_ctx* ctx, const exb_logprobs_desc* d, 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int64_t bytes = (int64_t)V * (int64_t)es;
     int rc = EXB_OK;
-    // A warp for a row where that takes no longer than its CTA's exchange, or where there are rows for all warps.  (fp16, top 5:
-    // kWarpTimes)
-    if (bytes <= 8192 || (bytes <= 32768 && n_rows >= 8 * ctx->sm_count)) {
+    // A warp for a row where a CTA's exchange between warps takes longer than the reading, and where there are rows for all warps.  (fp16,
+    // top 5, us with a warp and with a CTA for a row.  64 rows of 200: 3.3 and 13.2, of 1000: 4.4 and 4.2, of 2000: 5.7 and 4.4, of 8000:
+    // 8.1 and 5.3.  1184 rows of 2000: 11.1 and 10.2, of 4000: 14.3 and 11.0; 1776 of 2000: 7.6 and 14.5, of 8000: 13.7 and 17.3;
+    // 8192 of 4000: 23.7 and 60; 2368 of 16000: 31.8 and 28.0.)
+    if (bytes <= 2048 || (bytes <= 16384 && n_rows >= 12 * ctx->sm_count)) {
         rows::with_type(dtype, [&](auto t) {
             using T = decltype(t);
             launch_overlapped(ctx, token_logprobs_warp_kernel<T>, dim3((unsigned)((n_rows + kWarpRows - 1) / kWarpRows)), dim3(kWarpRows * 32), st, a, n_rows);
         });
         return after_launch("token_logprobs_warp_kernel");
     }
-    const int threads = bytes >= 131072 && n_rows <= ctx->sm_count ? 512 : 256;
-    // a row is shared where there are too few of them, as long as each CTA has two vectors for a thread
+    // Two CTAs of 512 threads fill an SM, four of 256.  As long as all rows have their CTAs at once the wide ones are the faster (fp16, us
+    // with 512 and 256: 148 rows of 50000 9.0 and 9.9, 296 of them 11.1 and 17.0, 296 of 8000 6.1 and 7.3, of 131072 18.7 and 32.1);
+    // with more rows the narrow ones leave less of a last wave empty (444 of 16000: 11.8 and 9.9, 2048 of 50000: 64.6 and 45.7).
+    const bool wide = bytes >= 16384 && n_rows <= 2 * ctx->sm_count;
+    // Fewer rows than SMs are shared by the CTAs of a cluster as long as each has three vectors for a thread (in 1, 2, 4, 8 parts: one row of
+    // 131072 9.6, 8.0, 6.9, 6.6; 32 of them 14.5, 12.0, 10.2, 11.1; 74 12.8, 10.5, 15.7, 19.3; one row of 20000 4.7, 5.4, 5.5, 5.9).
     a.splits = 1;
-    while (a.splits < kSplitMax && n_rows * a.splits * 2 <= 2 * ctx->sm_count && bytes >= (int64_t)a.splits * 2 * threads * 32) a.splits *= 2;
+    while (wide && a.splits < kSplitMax && n_rows * a.splits * 2 <= ctx->sm_count && bytes >= (int64_t)a.splits * 2 * kWide * 48) a.splits *= 2;
     rows::with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        rc = threads == 256 ? launch<T, 256>(ctx, a, n_rows, st) : launch<T, 512>(ctx, a, n_rows, st);
+        rc = wide ? launch<T, kWide>(ctx, a, n_rows, st) : launch<T, kNarrow>(ctx, a, n_rows, st);
     });
     return rc;
 }
