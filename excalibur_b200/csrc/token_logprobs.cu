@@ -290,15 +290,21 @@ __device__ __forceinline__ void collect(const T* x, const Parts<T>& part, unsign
     if (lane == 0 && thread < n_tail) offer(to_float<T>(x[part.tail0 + thread]), part.tail0 + thread);
 }
 
-// The n-th largest of the lanes' values (0: none); 0 if there are fewer.
+// The n-th largest (1..32) of the lanes' values (0: none); 0 if there are fewer.  Each lane counts the larger ones, in 32 exchanges that
+// need not wait for each other; the n-th is the smallest of those with fewer than n.
 __device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
-    uint32_t m = 0;
-    for (int j = 0; j < n; ++j) {
-        m = __reduce_max_sync(0xffffffffu, v);
-        const uint32_t who = __ballot_sync(0xffffffffu, v == m);
-        if ((int)(threadIdx.x & 31) == __ffs(who) - 1) v = 0;
-    }
-    return m;
+    int larger = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) larger += __shfl_sync(0xffffffffu, v, j) > v;
+    return __reduce_min_sync(0xffffffffu, larger < n ? v : 0xffffffffu);
+}
+
+// How many of n keys are before (above) one.
+__device__ __forceinline__ int count_before(const unsigned long long* keys, int n, unsigned long long key) {
+    int before = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) before += keys[j] > key;
+    return before;
 }
 
 constexpr int kSplitMax = 8;      // CTAs of kWide threads that share a row
@@ -309,7 +315,7 @@ template <int kThreads>
 struct Shared {
     Sums part[kThreads / 32];
     Sums row[kSplitMax];                                   // (of the cluster's CTAs, in the first one)
-    unsigned long long best[kSplitMax][kMaxTop];           // the same: their best, in order
+    unsigned long long best[kSplitMax * kMaxTop];         // the same: the `top` best of each, in order
     uint32_t largest[kThreads / 8];                        // of 8 threads each
     unsigned long long list[kRoom > kThreads ? kRoom : kThreads];
     int threads[kThreads];
@@ -474,8 +480,7 @@ __global__ void __launch_bounds__(kWarpRows * 32) token_logprobs_warp_kernel(con
         slow = n > kWarpRoom;
         for (int k = lane; k < n && !slow; k += 32) {
             const unsigned long long mine_ = s_list[warp][k];
-            int before = 0;
-            for (int j = 0; j < n; ++j) before += s_list[warp][j] > mine_;
+            const int before = count_before(s_list[warp], n, mine_);
             if (before < a.top) {
                 a.top_tokens[row * a.top + before] = index_of(mine_);
                 a.top_logprobs[row * a.top + before] = out.logprob(logit_of(mine_));
@@ -568,8 +573,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
                 sh.tau = 0;
             }
             __syncthreads();
-            int before = 0;
-            for (int j = 0; j < kThreads; ++j) before += sh.list[j] > key;
+            const int before = count_before(sh.list, kThreads, key);
             if (key && before == a.top - 1) sh.tau = key;
             __syncthreads();
             tau = sh.tau;
@@ -579,17 +583,16 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
         too_many = n > kRoom;
         n_best = min(n, a.top);
         if (!too_many) {
-            unsigned long long* to = splits > 1 ? nullptr : sh.best[0];
+            unsigned long long* to = splits > 1 ? nullptr : sh.best;
             for (int k = tid; k < n; k += kThreads) {
                 const unsigned long long key = sh.list[k];
-                int before = 0;
-                for (int j = 0; j < n; ++j) before += sh.list[j] > key;
+                const int before = count_before(sh.list, n, key);
                 if (before < a.top) {
                     if (to) to[before] = key;
-                    else ptx::st_cta_u64(ptx::map_to_cta(ptx::smem_u32(&sh.best[rank][before]), 0), key);
+                    else ptx::st_cta_u64(ptx::map_to_cta(ptx::smem_u32(&sh.best[rank * a.top + before]), 0), key);
                 }
             }
-            if (splits > 1 && tid >= n_best && tid < a.top) ptx::st_cta_u64(ptx::map_to_cta(ptx::smem_u32(&sh.best[rank][tid]), 0), 0);
+            if (splits > 1 && tid >= n_best && tid < a.top) ptx::st_cta_u64(ptx::map_to_cta(ptx::smem_u32(&sh.best[rank * a.top + tid]), 0), 0);
         }
     }
     // (the warps' sums, in every warp for itself)
@@ -627,12 +630,8 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
         if (splits == 1) __syncthreads();
         const int n = splits * a.top;
         for (int k = tid; k < n; k += kThreads) {
-            const unsigned long long mine = sh.best[k / a.top][k % a.top];
-            int before = 0;
-            if (splits == 1) before = k;
-            else
-                for (int j = 0; j < splits; ++j)
-                    for (int l = 0; l < a.top; ++l) before += sh.best[j][l] > mine;
+            const unsigned long long mine = sh.best[k];
+            const int before = splits == 1 ? k : count_before(sh.best, n, mine);
             if (before < a.top && mine) {
                 a.top_tokens[row * a.top + before] = index_of(mine);
                 a.top_logprobs[row * a.top + before] = out.logprob(logit_of(mine));
