@@ -235,6 +235,7 @@ extern "C" int exb_residual_norm_fwd(exb_ctx* ctx, const exb_norm_desc* d, const
         EXB_REQUIRE(aligned16(n) && d->n_stride % 16 == 0, "exb_residual_norm_fwd: e4m3 rows must start at multiples of 16 bytes");
         EXB_REQUIRE(n != h && n != x, "exb_residual_norm_fwd: e4m3 rows cannot take the input's place");
     }
+    EXB_REQUIRE(!gate || (gate != r && gate != n), "exb_residual_norm_fwd: a result cannot take the gate's place");
     EXB_REQUIRE(!r || r != n, "exb_residual_norm_fwd: r and n are the same buffer");
     EXB_REQUIRE((r != h || d->r_stride == d->h_stride) && (!x || r != x || d->r_stride == d->x_stride) && (n != h || d->n_stride == d->h_stride) &&
                     (!x || n != x || d->n_stride == d->x_stride),

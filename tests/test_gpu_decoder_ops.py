@@ -170,6 +170,20 @@ def test_fp8_matmul(ctx, M, N, K, dtype):
     assert torch.equal(y, again)
 
 
+@pytest.mark.parametrize("M,N,K,dtype", [
+    (1, 130, 1290, "float32"),      # parts of K that divide neither it nor the rows: 5 of 11 blocks,
+    (9, 130, 1750, "bfloat16"),     # 7 of 14,
+    (16, 4300, 1800, "float16"),    # 7, where each CTA gets 3 columns of 6 others at most,
+    (15, 4900, 1540, "float32"),    # 6,
+    (33, 6100, 1300, "float16"),    # 5,
+    (50, 9001, 777, "bfloat16"),    # 3,
+    (131, 2400, 800, "float32"),    # 3 of tiles of 128 columns,
+    (100, 2500, 1700, "float16"),   # 6
+])
+def test_fp8_matmul_in_uneven_parts(ctx, M, N, K, dtype):
+    test_fp8_matmul(ctx, M, N, K, dtype)
+
+
 @pytest.mark.parametrize("M,N,K", [(3, 200, 300), (70, 200, 300), (300, 700, 1000), (600, 1100, 300)])
 def test_fp8_matmul_takes_strides_and_writes_nothing_else(ctx, M, N, K):
     torch, capi = _mods()
@@ -215,6 +229,21 @@ def test_fp8_matmul_with_extreme_scales(ctx, M):
     keep = [i for i in range(M) if i != M // 2]
     if keep:
         _check_product(y[keep], a[keep], sa[:, keep], w, sw, None, "float32")
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_residual_norm_refuses_the_gate_as_a_result(ctx, quantized):
+    """A gate that several rows share would be read by one row after another has written it."""
+    torch, capi = _mods()
+    h = torch.randn((4, 256), device="cuda").half()
+    gate = torch.randn((4, 256), device="cuda").half()
+    w = torch.ones(256, device="cuda")
+    with pytest.raises(capi.ExbError):
+        capi.residual_norm(ctx, h, gate=gate, weight=w, quantized=quantized, r=gate)
+    if not quantized:
+        with pytest.raises(capi.ExbError):
+            capi.residual_norm(ctx, h, gate=gate, weight=w, n=gate)
+    ctx.sync_check()
 
 
 def test_fp8_matmul_on_another_stream_and_in_a_graph(ctx):
