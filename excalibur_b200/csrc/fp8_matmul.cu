@@ -7,6 +7,7 @@
 #include "rows_common.cuh"
 #include "tensor_map.cuh"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace exb {
@@ -64,7 +65,9 @@ constexpr int kFewTable = 16;        // blocks whose scales are in shared memory
 constexpr int few_stages(int cols) { return cols == 128 ? 4 : cols == 64 ? 3 : cols == 32 ? 4 : 5; }      // (two CTAs fit an SM up to 64 columns)
 constexpr int few_epi_warps(int cols) { return cols == 128 ? 16 : cols == 64 ? 8 : 4; }
 constexpr int few_stage_bytes(int cols) { return (128 + cols) * kBlk; }
-constexpr int few_smem(int cols) { return few_stages(cols) * few_stage_bytes(cols) + kFewTable * cols * 4 + cols * 512 + 1024; }
+// (columns that a CTA gets, of 16 by 7 CTAs: 3 from each of 6 others)
+constexpr int few_received(int cols) { return cols == 16 ? 18 : cols; }
+constexpr int few_smem(int cols) { return few_stages(cols) * few_stage_bytes(cols) + kFewTable * cols * 4 + few_received(cols) * 512 + 1024; }
 
 template <int kCols>
 __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ? 1 : 2) fp8_matmul_few_kernel(const __grid_constant__ MatmulParams p) {
@@ -77,7 +80,7 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
     __shared__ int abort_flag;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float* table = reinterpret_cast<float*>(ring + kStages * kStageBytes);      // [block][column]: a's scale x w's
-    float* recv = table + kFewTable * kCols;                                    // [CTA][column of the share][128]
+    float* recv = table + kFewTable * kCols;                                    // [CTA, without this one][column of the share][128]
     float* part = reinterpret_cast<float*>(ring);                               // [column][128] behind the loop
     const int warp = ptx::uniform_warp(), lane = threadIdx.x & 31;
     const int rank = (int)blockIdx.x % p.splits, n0 = (int)blockIdx.x / p.splits * 128, m0 = blockIdx.y * kCols;
@@ -261,7 +264,7 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
             // lane r of the first warp sends CTA r its columns
             const int theirs = min(share, cols - lane * share);
             if (ok && warp == 3 && lane < p.splits && lane != rank && theirs > 0)
-                ptx::copy_to_cta(ptx::map_to_cta(ptx::smem_u32(recv + rank * share * 128), (uint32_t)lane), ptx::smem_u32(part + lane * share * 128),
+                ptx::copy_to_cta(ptx::map_to_cta(ptx::smem_u32(recv + (rank - (rank > lane)) * theirs * 128), (uint32_t)lane), ptx::smem_u32(part + lane * share * 128),
                                  (uint32_t)(theirs * 512), ptx::map_to_cta(ptx::smem_u32(&recv_bar), (uint32_t)lane));
             __syncwarp();
             if (ok) ok = ptx::mbar_wait_quick_uniform(ptx::smem_u32(&recv_bar), 0, &abort_flag, kMaxSpins);
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
 #pragma unroll
                 for (int s = 0; s < 8; ++s)
                     if (s < p.splits) {
-                        const float4 v = *reinterpret_cast<const float4*>(s == rank ? own : recv + (s * share + c) * 128 + row);
+                        const float4 v = *reinterpret_cast<const float4*>(s == rank ? own : recv + ((s - (s > rank)) * mine + c) * 128 + row);
                         sum[0] = s ? sum[0] + v.x : v.x;
                         sum[1] = s ? sum[1] + v.y : v.y;
                         sum[2] = s ? sum[2] + v.z : v.z;
@@ -599,8 +602,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_matmul_pair_kernel(const 
 
 // Which kernel and how it divides the product: the one whose time is least by what was measured of each (graph-captured calls, us):
 //  - few rows, up to 64 columns: the only one that does not compute rows that are not there;
-//  - few rows, 128 columns: 4.5 + 2 where K is divided + 0.53 for each K block that a CTA works on one after the other
-//    (128 x 8192 x 4096 in two parts 14.9, 128 x 4096 x 4096 in four 10.8);
+//  - few rows, 128 columns: 5 + 2.2 where K is divided + 0.42 for each K block that a CTA works on one after the other
+//    (131 x 2432 x 9088 in one part 34.4, in two 20.8, in three 16.6; 512 x 1024 x 8192 in four 13.4);
 //  - pairs with tiles of 128 columns: 4.5 + 0.335 a block (512 x 4096 x 4096 14.9, in 256 columns 18.1);
 //  - pairs with tiles of 256 columns: 5 + 0.43 a block (256 x 14336 x 4096 19.9, in 128 columns 25.5; 4096^3 67 and 81).
 struct Plan {
@@ -609,17 +612,20 @@ struct Plan {
 };
 Plan plan_for(int sms, int M, int N, int blocks) {
     const int64_t n_tiles = ((int64_t)N + 127) / 128;
-    // parts of K: as many as there are places for, of at least two blocks each
-    auto parts = [&](int64_t tiles, int64_t places) {
-        int s = 1;
-        while (s < 8 && tiles * s * 2 <= places && s * 4 <= blocks) s *= 2;
-        return s;
+    // Parts of K, of at least two blocks each.  Clusters of several CTAs do not fill the SMs to the last: up to nine tenths are counted on.
+    // Up to 64 columns an SM has room for two CTAs; they are only used, and up to 1.65 an SM, where one each would leave a fifth
+    // of the SMs out (1 row, K = 4096, N = 4096 in 4 parts 6.0, in 8 6.7; N = 6144 in 3 parts 7.6, in 5 7.4, in 6 10.4; 64 rows, N = 4096 8.7 and
+    // 9.7, N = 6144 12.3, 10.6 and 15.7).
+    auto parts = [&](int64_t tiles, bool two) {
+        auto within = [&](int64_t places) { return std::max<int64_t>(1, std::min<int64_t>({8, places / tiles, blocks / 2})); };
+        const int64_t s = within(sms * 9 / 10);
+        return (int)(two && tiles * s * 5 < sms * 4 ? within(sms * 33 / 20) : s);
     };
-    if (M <= 64) return {true, M <= 16 ? 16 : M <= 32 ? 32 : 64, parts(n_tiles, 2 * sms)};
+    if (M <= 64) return {true, M <= 16 ? 16 : M <= 32 ? 32 : 64, parts(n_tiles, true)};
     auto rounds = [](int64_t tiles, int64_t places) { return (double)((tiles + places - 1) / places); };
     const int64_t few_tiles = ((int64_t)M + 127) / 128 * n_tiles, m_pairs = ((int64_t)M + kPairM - 1) / kPairM;
-    const int splits = parts(few_tiles, sms);
-    const double few = 4.5 + (splits > 1 ? 2.0 : 0.0) + 0.53 * rounds(few_tiles * splits, sms) * ((blocks + splits - 1) / splits);
+    const int splits = parts(few_tiles, false);
+    const double few = 5.0 + (splits > 1 ? 2.2 : 0.0) + 0.42 * rounds(few_tiles * splits, sms) * ((blocks + splits - 1) / splits);
     const double pair128 = 4.5 + 0.335 * rounds(m_pairs * n_tiles, sms / 2) * blocks;
     const double pair256 = 5.0 + 0.43 * rounds(m_pairs * (((int64_t)N + 255) / 256), sms / 2) * blocks;
     if (few < pair128 && few < pair256 && few_tiles / n_tiles <= 65535) return {true, 128, splits};
