@@ -90,7 +90,7 @@ __device__ __forceinline__ void normalise(float2 (&v)[kPer][4], int lane, int sh
 }
 
 // kOneWarp: every warp of the CTA has a row of its own; otherwise the CTA has one.  kPer: shares per warp.
-constexpr int max_threads(bool one_warp, int per) { return one_warp ? 256 : per == 1 ? 1024 : 512; }
+constexpr int max_threads(bool one_warp, int per) { return one_warp || per == 1 ? 256 : 512; }
 
 template <typename T, bool kLayer, Layout kL, bool kOneWarp, int kPer>
 __global__ void __launch_bounds__(max_threads(kOneWarp, kPer)) residual_norm_kernel(const __grid_constant__ NormArgs a) {
@@ -190,10 +190,14 @@ int launch(const exb_ctx* ctx, const NormArgs& a, cudaStream_t st) {
     };
     using Yes = std::true_type;
     using No = std::false_type;
-    const bool many = a.rows > 2 * ctx->sm_count;
+    // Up to two shares a warp has the row and no warp waits for another (bf16, us, with a warp and with a CTA for a row: 1 x 512 1.40 and 1.61,
+    // 1024 x 512 3.4 and 3.6, 32768 x 512 21.5 and 34.4).  Wider rows have as many warps as they have shares while those are few (8192 x 1280
+    // with a share for a warp 14.6, with two 15.8), then half as many, which exchange their sums sooner (8192 wide: 64 rows 3.6, in
+    // single shares 3.8, in four 3.9; 2048 rows 25.7, 26.2, 27.6; 4096 x 4096 with everything 29.2, 30.9, 31.0; one row of 4096 1.93, 1.86).
+    // A CTA has 16 warps, so that a thread may have 128 registers: four shares for a warp beyond 8192, eight beyond 16384.
     if (shares == 1) go(Yes(), std::integral_constant<int, 1>());
-    else if (shares == 2 && many) go(Yes(), std::integral_constant<int, 2>());
-    else if (shares <= (many ? 4 : 32)) go(No(), std::integral_constant<int, 1>());
+    else if (shares == 2) go(Yes(), std::integral_constant<int, 2>());
+    else if (shares <= 8) go(No(), std::integral_constant<int, 1>());
     else if (shares <= 32) go(No(), std::integral_constant<int, 2>());
     else if (shares <= 64) go(No(), std::integral_constant<int, 4>());
     else go(No(), std::integral_constant<int, 8>());
