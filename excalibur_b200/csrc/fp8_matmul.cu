@@ -60,6 +60,8 @@ __device__ __forceinline__ void store_four(const MatmulParams& p, int m, int n, 
 // share of the columns: the others send it their parts in one bulk copy each, counted by a barrier of its own, and it sums them in
 // the order of the CTAs.  (Read out of the others' shared memory between cluster barriers the exchange took 3600 cycles for 16
 // columns and 8000 for 64.)
+// 1 x 4096 x 4096 takes 6.0 us, 1 x 14336 x 4096 12.4 (4730 GB/s), 64 x 14336 x 4096 16.4 (3710 GB/s): about 3 us of start, exchange and
+// end, and w at 5 TB/s or so between them.  Without w's latency to hide (131 x 2432 x 9088, 16.6) the 0.42 us of a K block are what counts.
 constexpr int kFewBufs = 4;          // accumulators in turn: TMEM has room
 constexpr int kFewTable = 16;        // blocks whose scales are in shared memory at a time
 constexpr int few_stages(int cols) { return cols == 128 ? 4 : cols == 64 ? 3 : cols == 32 ? 4 : 5; }      // (two CTAs fit an SM up to 64 columns)
@@ -302,7 +304,11 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
 // ---- CTA pairs ---------------------------------------------------------------------------------
 // Tiles of 256 x 256 by pairs of CTAs, persistent.  Each CTA keeps 128 rows of a and half of w's rows of a stage, 32 KB for
 // 512 cycles of MMA: 64 bytes per cycle and SM from L2 (a lone CTA's tile of 128 x 128 needs 128).  TMEM holds two accumulators of
-// 256 columns; a thread's sums are 128 registers.
+// 256 columns; a thread's sums are 128 registers.  8192^3 takes 441 to 458 us (2400 to 2490 TFLOP/s) from a cool GPU and 543 (2020
+// TFLOP/s) when repeated for seconds, where the power limit sets the clock; 4096^3 67.  Bound by the epilogue: a block's read out of
+// TMEM and its multiply-adds take 800 cycles, the MMAs 512 of these (the tensor pipe is active 58 % of 4096^3).  K is not divided
+// between pairs: clusters of two pairs took 131 x 2432 x 9088 in 18.8 us where the kernel above takes 16.6, and 1695 x 3315 x 9300,
+// which leaves most of a second wave empty, in 92 instead of 70 (a CTA's start costs more than the wave).
 constexpr int kPairM = 256;
 constexpr int kPairEpiWarps = 8;                 // two per TMEM lane quarter, half of the accumulator's columns each
 constexpr int pair_stage_bytes(int n) { return (kPairM + n) / 2 * kBlk; }      // of one of the two CTAs
@@ -351,7 +357,8 @@ __device__ __forceinline__ void store_rows(const float2 (&acc)[kPairs], uint8_t*
             }
         } else {
             // Rows that start anywhere: kUnits - 1 vectors at multiples of 16 bytes, put together of two units each, and 16 bytes before
-            // and behind them element by element.  (Element by element 4048 x 7313 x 264 took 51.8 us.)
+            // and behind them element by element.  (4048 x 7313 x 264 takes
+            // 42.9 us, element by element 51.8, and 4048 x 7312 x 264 29: sectors that two passes write a part of each are what is left.)
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
                 const int r = i * kRows + sub;

@@ -3,7 +3,9 @@
 // A row stays in its threads' registers in fp32 from the loads of h, x and the gate to the stores of r and n (in the
 // activations' type, or as e4m3 with a scale for each 128 channels), so that every tensor crosses memory once; the sums of
 // the norms are the only thing its warps exchange.  Bound by memory with many rows, by the chain of loads, reductions and
-// stores with few.
+// stores with few.  4096 x 4096 bf16 takes 23.3 us (5760 GB/s), with both norms, a gate and e4m3 29.2 (4030 GB/s: 37 instructions an
+// element are issued 60 % of the time), one row 1.95, 3152 x 1000 fp16 with a gate's rows 6.9; rows that start anywhere (4096 x 1001,
+// 9.1) are loaded and stored in single elements.
 #include "rows_common.cuh"
 
 #include <type_traits>
@@ -44,8 +46,8 @@ __device__ __forceinline__ float row_sum(float v, float (*s_sum)[32], int& turn)
     return v;
 }
 
-// v = norm(v) * weight + bias over the row.  Elements go in pairs, two to an instruction: 40 and more instructions an element are what
-// the fused form with both norms, a gate and e4m3 is bound by.
+// v = norm(v) * weight + bias over the row.  Elements go in pairs, two to an instruction: the number of instructions is
+// what the form with both norms, a gate and e4m3 is bound by.
 template <bool kLayer, Layout kL, bool kOneWarp, int kPer>
 __device__ __forceinline__ void normalise(float2 (&v)[kPer][4], int lane, int share0, int share_step, const NormArgs& a, const float* weight,
                                           const float* bias, float (*s_sum)[32], int& turn) {

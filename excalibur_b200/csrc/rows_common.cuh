@@ -84,8 +84,8 @@ __device__ __forceinline__ uint4 load16_within(const uint8_t* at, const Span& sp
 
 // A warp's share of 256 elements, 8 neighbours in each lane, of a row that starts anywhere: whole 16-byte vectors are read, at
 // multiples of 16 (fetch), and then moved into place between neighbouring lanes (settle).  Two steps, so that several rows can be
-// asked for before the first is there.  Eight loads of single elements for each lane's 8 took 3.2 times the time of aligned rows
-// (8192 x 14335 bf16 to e4m3: 200 us, 63 aligned), both steps at once for each row 1.7 times.
+// asked for before the first is there.  Eight loads of single elements for each lane's 8 took three and a half times as long as aligned rows
+// (8192 x 14335 bf16 to e4m3: 200 us; 56 aligned, 86 this way), both steps at once for each row 110 us.
 // inside: no 16 bytes that hold some of the row reach out of the span (rows that have 8 others before and behind them).
 template <typename T>
 __device__ __forceinline__ void fetch8_shifted(const T* row_at, int valid, int lane, const Span& span, bool inside, uint32_t (&x)[2 * sizeof(T) + 4]) {
