@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
 // 512 cycles of MMA: 64 bytes per cycle and SM from L2 (a lone CTA's tile of 128 x 128 needs 128).  TMEM holds two accumulators of
 // 256 columns; a thread's sums are 128 registers.  8192^3 takes 441 to 458 us (2400 to 2490 TFLOP/s) from a cool GPU and 543 (2020
 // TFLOP/s) when repeated for seconds, where the power limit sets the clock; 4096^3 67.  Bound by the epilogue: a block's read out of
-// TMEM and its multiply-adds take 800 cycles, the MMAs 512 of these (the tensor pipe is active 58 % of 4096^3).  K is not divided
+// TMEM and its multiply-adds take 800 cycles, the MMAs 512 of these (the tensor pipe is active 59 % of 4096^3).  K is not divided
 // between pairs: clusters of two pairs took 131 x 2432 x 9088 in 18.8 us where the kernel above takes 16.6, and 1695 x 3315 x 9300,
 // which leaves most of a second wave empty, in 92 instead of 70 (a CTA's start costs more than the wave).
 constexpr int kPairM = 256;
