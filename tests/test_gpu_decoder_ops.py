@@ -439,13 +439,8 @@ def test_token_logprobs(ctx, rows, V, dtype):
         _check_logprobs(ctx, _rows(x, pad, offset), tokens, top, scale)
 
 
-@pytest.mark.parametrize("V", [40, 1000, 5001, 40000])
-@pytest.mark.parametrize("dtype", DTYPES)
-def test_token_logprobs_with_masks(ctx, V, dtype):
-    """Rows of which the mask leaves nothing, one or a few tokens, masks of the type's lowest value, rows of equal values, and values that are no numbers."""
-    torch, capi = _mods()
-    t = getattr(torch, dtype)
-    g = _gen(V)
+def _masked_rows(torch, V, t, g):
+    """16 rows: masks that leave nothing, one or a few tokens, the type's lowest value, equal values, and values that are no numbers."""
     low = torch.finfo(t).min
     x = torch.randn((16, V), device="cuda", generator=g) * 4
     x[0] = -math.inf
@@ -472,13 +467,37 @@ def test_token_logprobs_with_masks(ctx, V, dtype):
     x[14, -1] = low
     x[15] = low
     x[15, 7] = torch.finfo(t).max
-    x = x.to(t)
+    return x.to(t)
+
+
+@pytest.mark.parametrize("V", [40, 1000, 5001, 40000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_token_logprobs_with_masks(ctx, V, dtype):
+    """Rows of which the mask leaves nothing, one or a few tokens, masks of the type's lowest value, rows of equal values, and values that are no numbers."""
+    torch, capi = _mods()
+    t = getattr(torch, dtype)
+    g = _gen(V)
+    x = _masked_rows(torch, V, t, g)
     tokens = torch.stack([torch.randint(0, V, (16,), device="cuda", generator=g), torch.full((16,), 5, device="cuda"), torch.full((16,), -1, device="cuda"),
                           torch.full((16,), V, device="cuda"), torch.full((16,), V // 3, device="cuda")], 1).int()
     for scale in (1.0, 2.0, 0.5):
         for top in (0, 1, 5, 20, 32):
             for pad, offset in ((0, 0), (1, 1)):
                 _check_logprobs(ctx, _rows(x, pad, offset), tokens, top, scale)
+
+
+@pytest.mark.parametrize("rows,V", [(1792, 500), (1792, 2500), (1792, 8000), (304, 12001), (80, 30000)])
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_token_logprobs_with_masks_in_many_rows(ctx, rows, V, dtype):
+    """The same rows often enough that a warp has one each (in 16 bits up to 8192 tokens), or a narrow CTA; between them rows without masks."""
+    torch, capi = _mods()
+    t = getattr(torch, dtype)
+    g = _gen(rows + V)
+    x = (torch.randn((rows, V), device="cuda", generator=g) * 4).to(t)
+    x[::2] = _masked_rows(torch, V, t, g).repeat(-(-rows // 32), 1)[: (rows + 1) // 2]
+    tokens = torch.randint(-1, V + 1, (rows, 2), device="cuda", generator=g).int()
+    for top, scale, (pad, offset) in ((0, 1.0, (0, 0)), (5, 0.7, (1, 1)), (32, 1.3, (0, 0))):
+        _check_logprobs(ctx, _rows(x, pad, offset), tokens, top, scale)
 
 
 def test_token_logprobs_differences_in_huge_logits(ctx):
