@@ -37,11 +37,11 @@ struct LogprobArgs {
     float scale;
 };
 
-// Logits in an order of unsigned numbers: both zeros alike, NaN above infinity.  With the index behind it (the lower one is the larger
-// key) no two keys are alike.
+// Logits in an order of unsigned numbers: both zeros alike, all NaN alike and above infinity.  With the index behind it (the lower one
+// is the larger key) no two keys are alike, and none is 0 or all ones: a search may start from either.
 __device__ __forceinline__ uint32_t order_of(float x) {
     const uint32_t b = __float_as_uint(x + 0.f);
-    return x != x ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+    return x != x ? 0xfffffffeu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ unsigned long long key_of(float x, int index) { return (unsigned long long)order_of(x) << 32 | (uint32_t)~index; }
 
@@ -393,7 +393,7 @@ __device__ __noinline__ void slow_row(const LogprobArgs& a, const T* x, int64_t 
         if (tid == 0 && a.entropy) a.entropy[row] = r.entropy;
         write_given<T>(a, x, row, r, tid, kThreads);
     }
-    unsigned long long last = ~0ull;
+    unsigned long long last = ~0ull;      // (above every key; top <= V, so that each pass finds one)
     for (int j = 0; j < a.top; ++j) {
         unsigned long long best = 0;
         for (int i = tid; i < a.V; i += kThreads) {

@@ -1,0 +1,37 @@
+"""The operators behind a decoder where they can go wrong at the ends: values that are no numbers in the log probabilities."""
+import math
+
+import pytest
+
+from tests.test_gpu_decoder_ops import DTYPES, _check_logprobs, _gen, _mods, _rows
+
+pytestmark = pytest.mark.gpu
+
+
+def _tokens(torch, rows, V, given, g):
+    return torch.randint(0, V, (rows, given), device="cuda", generator=g).int()
+
+
+# ---- token log probabilities ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,V", [(8, 1), (8, 2), (8, 32), (8, 200), (8, 1000), (8, 5001), (8, 40000), (2, 131072), (1800, 2500), (400, 12001)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_token_logprobs_with_a_nan_at_the_first_token(ctx, rows, V, dtype):
+    """NaN sorts above plus infinity and equal ones by their index, the first token's too; as many tokens as there are may be asked for."""
+    torch, capi = _mods()
+    g = _gen(rows + V)
+    x = (torch.randn((rows, V), device="cuda", generator=g) * 3).to(getattr(torch, dtype))
+    x[0::8, 0] = math.nan
+    x[1::8] = math.nan
+    x[2::8, 0] = -math.nan
+    x[2::8, V - 1] = math.nan
+    x[3::8] = -math.inf
+    x[3::8, 0] = math.nan
+    x[4::8, 0] = math.inf
+    x[5::8, V // 2] = math.nan
+    x[6::8] = -math.inf
+    x[6::8, V - 1] = -math.nan
+    tokens = _tokens(torch, rows, V, 2, g)
+    for top in sorted({1, min(V, 5), min(V, 32)}):
+        for pad, offset in ((0, 0), (1, 1)):
+            _check_logprobs(ctx, _rows(x, pad, offset), tokens, top, 0.7)
