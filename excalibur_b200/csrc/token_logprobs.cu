@@ -183,7 +183,7 @@ struct Seen {
         }
         const float e = ceilf(v * c);
         if (r.e != -INFINITY) {
-            const float d = r.e - e, f = exp2_fast(d);
+            const float d = fmaxf(r.e - e, -1000.f), f = exp2_fast(d);      // (0 from there on; d * s has to stay a number)
             r.w = (r.w + d * r.s) * f;
             r.s *= f;
         }

@@ -1,4 +1,4 @@
-"""The operators behind a decoder where they can go wrong at the ends: values that are no numbers in the log probabilities."""
+"""The operators behind a decoder where they can go wrong at the ends: values that are no numbers and huge logits in the log probabilities."""
 import math
 
 import pytest
@@ -35,3 +35,15 @@ def test_token_logprobs_with_a_nan_at_the_first_token(ctx, rows, V, dtype):
     for top in sorted({1, min(V, 5), min(V, 32)}):
         for pad, offset in ((0, 0), (1, 1)):
             _check_logprobs(ctx, _rows(x, pad, offset), tokens, top, 0.7)
+
+@pytest.mark.parametrize("rows,V", [(6, 900), (6, 40000), (2, 131072), (1800, 2500), (400, 12001)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_token_logprobs_of_a_huge_logit_behind_others(ctx, rows, V, dtype):
+    """A thread that has added up small logits meets one near the type's end: its row's other tokens are nothing, and the entropy is 0."""
+    torch, capi = _mods()
+    x = torch.zeros((rows, V), device="cuda", dtype=getattr(torch, dtype))
+    at = torch.arange(rows, device="cuda") * 997 % (V // 3) + V * 2 // 3
+    x[torch.arange(rows, device="cuda"), at] = 2.0 ** 123      # (exact times log2 e, so that the one pass answers it)
+    tokens = torch.stack([at, at * 0], 1).int()
+    for scale in (0.5, 1.0, 2.0):
+        _check_logprobs(ctx, x, tokens, 3, scale)
