@@ -357,10 +357,11 @@ struct Row {
     }
 };
 
-// Whether the pass has answered the row: its sum is a number, and what was taken for kLow has added nothing to it.
+// Whether the pass has answered the row: its sums are numbers (the products in w are not where scaled logits lie further apart than fp32
+// reaches), and what was taken for kLow has added nothing to them.
 template <typename T>
 __device__ __forceinline__ bool row_known(const Sums& all, float c) {
-    return all.s > 0.f && all.s < INFINITY && fmaf(Vec<T>::kLow, c, -all.e) < -150.f;
+    return all.s > 0.f && all.s < INFINITY && fabsf(all.w) < INFINITY && fmaf(Vec<T>::kLow, c, -all.e) < -150.f;
 }
 
 template <typename T>

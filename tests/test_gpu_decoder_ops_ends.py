@@ -47,3 +47,14 @@ def test_token_logprobs_of_a_huge_logit_behind_others(ctx, rows, V, dtype):
     tokens = torch.stack([at, at * 0], 1).int()
     for scale in (0.5, 1.0, 2.0):
         _check_logprobs(ctx, x, tokens, 3, scale)
+
+@pytest.mark.parametrize("rows,V", [(3, 900), (3, 40000), (2, 131072), (1800, 2500), (400, 12001)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_token_logprobs_of_logits_further_apart_than_fp32_reaches(ctx, rows, V, dtype):
+    """Distances that are no fp32 number any more at a large scale: those tokens are nothing, and the entropy is 0, not NaN."""
+    torch, capi = _mods()
+    x = torch.full((rows, V), torch.finfo(getattr(torch, dtype)).min, device="cuda", dtype=getattr(torch, dtype))
+    x[1::2] = -9e29
+    x[:, V // 2] = 2.0 ** 101
+    tokens = torch.tensor([[V // 2, 0]], device="cuda").repeat(rows, 1).int()
+    _check_logprobs(ctx, x, tokens, 3, 9e7)
