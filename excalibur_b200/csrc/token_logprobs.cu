@@ -181,6 +181,7 @@ struct Seen {
             r.s = NAN;
             return;
         }
+        if (v <= Vec<T>::kLow) return;      // masks by a low value are masks: a reference down there would overflow what is taken for kLow
         const float e = ceilf(v * c);
         if (r.e != -INFINITY) {
             const float d = fmaxf(r.e - e, -1000.f), f = exp2_fast(d);      // (0 from there on; d * s has to stay a number)

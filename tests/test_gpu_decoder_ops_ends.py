@@ -1,4 +1,5 @@
-"""The operators behind a decoder where they can go wrong at the ends: values that are no numbers and huge logits in the log probabilities."""
+"""The operators behind a decoder where they can go wrong at the ends: values that are no numbers, masks and huge logits in the log
+probabilities."""
 import math
 
 import pytest
@@ -58,3 +59,25 @@ def test_token_logprobs_of_logits_further_apart_than_fp32_reaches(ctx, rows, V, 
     x[:, V // 2] = 2.0 ** 101
     tokens = torch.tensor([[V // 2, 0]], device="cuda").repeat(rows, 1).int()
     _check_logprobs(ctx, x, tokens, 3, 9e7)
+
+@pytest.mark.parametrize("rows,V", [(3, 900), (1800, 2500), (3, 40000), (2, 131072), (400, 20001)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_token_logprobs_masked_with_low_values_take_the_same_way(ctx, rows, V, dtype):
+    """Masks of the type's lowest value, or of one that is low enough, are answered by the same sums in the same order as minus infinity,
+    whatever the scale and however many of a thread's tokens are masked: equal bits."""
+    torch, capi = _mods()
+    t = getattr(torch, dtype)
+    g = _gen(V)
+    x = (torch.randn((rows, V), device="cuda", generator=g) * 4).to(t)
+    mask = torch.rand((rows, V), device="cuda", generator=g) < 0.6
+    mask[:, V // 5: V * 3 // 5] = True
+    mask[1:, : V // 5] = True
+    tokens = torch.arange(V - 3, V, device="cuda").repeat(rows, 1).int()
+    mask[:, V - 3:] = False
+    want = {s: capi.token_logprobs(ctx, x.masked_fill(mask, -math.inf), tokens, top=5, scale=s) for s in (0.3, 0.5, 1.0, 1.5)}
+    for low in (torch.finfo(t).min,) + (() if dtype == "float16" else (-2e30, -1e38)):
+        for scale, w in want.items():
+            got = capi.token_logprobs(ctx, x.masked_fill(mask, low), tokens, top=5, scale=scale)
+            ctx.sync_check()
+            assert all(torch.equal(a, b) for a, b in zip(got, w)), (low, scale)
+    _check_logprobs(ctx, x.masked_fill(mask, torch.finfo(t).min), tokens, 5, 0.5)
