@@ -61,6 +61,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
 // A 16-byte vector of logits: the largest of its parts (NaN if one is) kept packed, its elements, and these no lower than kLow (minus
 // infinity would make 0 * infinity of p * t).
@@ -347,14 +352,16 @@ __device__ __forceinline__ float group_reduce(float v, float* s_part, F op) {
     return v;
 }
 
-// What is written of a row whose sums are known: s and w about e, with the largest logit m.
+// What is written of a row whose sums are known: s and w about e, with the largest logit m.  The sum, its logarithm and the distance of
+// m from e are rounded each for itself: where one token has nearly everything, that comes out up to 1.2e-7 beyond 0 more often than not, and the exponential
+// of such a log probability above 1, so both are kept in their range.
 struct Row {
     float m, log_s, entropy;      // log_s: log2 of the sum about m
     bool empty;
     float scale;
     __device__ __forceinline__ float logprob(float v) const {
         // (halves: the distance of fp32's two ends is no fp32 number)
-        return empty ? -INFINITY : (0.5f * v - 0.5f * m) * (2.f * scale) - log_s * kLn2;
+        return empty ? -INFINITY : min_nan((0.5f * v - 0.5f * m) * (2.f * scale) - log_s * kLn2, 0.f);
     }
 };
 
@@ -443,7 +450,7 @@ __global__ void __launch_bounds__(kWarpRows * 32) token_logprobs_warp_kernel(con
     const bool known = row_known<T>(all, seen.c);
     if (known) {
         const float log_s = log2f(all.s);
-        out.entropy = (log_s - all.w / all.s) * kLn2;
+        out.entropy = max_nan((log_s - all.w / all.s) * kLn2, 0.f);
         out.log_s = log_s - fmaf(all.m, seen.c, -all.e);
         if (lane == 0 && a.entropy) a.entropy[row] = out.entropy;
         write_given<T>(a, x, row, out, lane, 32);
@@ -621,7 +628,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_c
     const bool known = row_known<T>(all, a.scale * kLog2e);
     if (known) {
         const float log_s = log2f(all.s);
-        out.entropy = (log_s - all.w / all.s) * kLn2;
+        out.entropy = max_nan((log_s - all.w / all.s) * kLn2, 0.f);
         out.log_s = log_s - fmaf(all.m, c, -all.e);
         if (tid == 0 && a.entropy) a.entropy[row] = out.entropy;
         write_given<T>(a, x, row, out, tid, kThreads);

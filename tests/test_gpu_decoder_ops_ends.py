@@ -81,3 +81,20 @@ def test_token_logprobs_masked_with_low_values_take_the_same_way(ctx, rows, V, d
             ctx.sync_check()
             assert all(torch.equal(a, b) for a, b in zip(got, w)), (low, scale)
     _check_logprobs(ctx, x.masked_fill(mask, torch.finfo(t).min), tokens, 5, 0.5)
+
+@pytest.mark.parametrize("rows,V", [(2000, 40), (64, 1000), (1800, 2500), (100, 40000), (16, 131072)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_token_logprobs_stay_in_their_range(ctx, rows, V, dtype):
+    """No log probability above 0 and no entropy below it, in rows of which a mask leaves one token, or of which one has nearly everything."""
+    torch, capi = _mods()
+    g = _gen(V)
+    at = torch.randint(0, V, (rows, 1), device="cuda", generator=g)
+    own = torch.randn((rows, 1), device="cuda", generator=g) * 10
+    for others in (torch.full((rows, V), -math.inf, device="cuda"), torch.randn((rows, V), device="cuda", generator=g) - 60):
+        x = others.scatter(1, at, own).to(getattr(torch, dtype))
+        for scale in (0.7, 1.0, 1.3):
+            lp, entropy, best, tokens = capi.token_logprobs(ctx, x, at.int(), top=1, scale=scale)
+            ctx.sync_check()
+            assert (lp <= 0).all() and (best <= 0).all() and (entropy >= 0).all()
+            assert torch.equal(tokens, at.int())
+        _check_logprobs(ctx, x, at.int(), 2, 1.3)
