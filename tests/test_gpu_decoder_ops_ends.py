@@ -4,7 +4,7 @@ import math
 
 import pytest
 
-from tests.test_gpu_decoder_ops import DTYPES, _check_logprobs, _gen, _mods, _rows
+from tests.test_gpu_decoder_ops import DTYPES, _check_logprobs, _gen, _masked_rows, _mods, _rows
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +98,41 @@ def test_token_logprobs_stay_in_their_range(ctx, rows, V, dtype):
             assert (lp <= 0).all() and (best <= 0).all() and (entropy >= 0).all()
             assert torch.equal(tokens, at.int())
         _check_logprobs(ctx, x, at.int(), 2, 1.3)
+
+@pytest.mark.parametrize("V", [129, 200, 256, 262])
+def test_token_logprobs_of_short_rows_with_many_alternatives(ctx, V):
+    """Rows of so few tokens that not every lane of a warp holds some, and as many alternatives as lanes that do or more: answered in one
+    go like others, where a pass over the row for each alternative took ten times as long."""
+    torch, capi = _mods()
+    rows = 8192
+    x = torch.randn((rows, V), device="cuda", generator=_gen(V)).half()
+    tokens = torch.zeros((rows, 1), device="cuda", dtype=torch.int32)
+    _check_logprobs(ctx, x, tokens, 32, 1.0)
+
+    def least(top):
+        times = []
+        for _ in range(12):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(10):
+                capi.token_logprobs(ctx, x, tokens, top=top)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+    assert least(32) < 4 * least(10)
+
+
+@pytest.mark.parametrize("V", [130, 200, 262, 500, 600])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_token_logprobs_of_short_rows_with_masks_and_many_alternatives(ctx, V, dtype):
+    """Equal logits among more candidates than are put in order at once: the lower indexes come first."""
+    torch, capi = _mods()
+    g = _gen(V)
+    x = _masked_rows(torch, V, getattr(torch, dtype), g)
+    x[11] = torch.randint(0, 3, (V,), device="cuda", generator=g)
+    x[12, 1::2] = 0.5
+    tokens = _tokens(torch, 16, V, 2, g)
+    for top in (15, 24, 32):
+        for pad, offset in ((0, 0), (1, 1)):
+            _check_logprobs(ctx, _rows(x, pad, offset), tokens, top, 0.9)
