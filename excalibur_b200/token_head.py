@@ -18,9 +18,10 @@ class TokenHead:
         self.norm_weight, self.post_weight = norm_weight, post_weight
         self.weights, self.scales = capi.quantize_blocks(ctx, vocab_weights, block_rows=128)
 
-    def logits(self, h, x, gate=None, gate_rows=0, out_dtype=capi.EXB_F16):
+    def logits(self, h, x, gate=None, gate_rows=0, out_dtype=capi.EXB_F32):
         """The last block's result h (rows, channels) joins the residual stream x, and the norm of the sum is multiplied with the
-        vocabulary.  Returns (residual stream, logits)."""
+        vocabulary.  Returns (residual stream, logits).  Logits are fp32 unless told otherwise: in fp16 one between 16 and 32 is off by up
+        to 2^-7, its log probability with it, and one above 65504 is infinite."""
         r, q, s = capi.residual_norm(self.ctx, h, x, post_weight=self.post_weight, gate=gate, gate_rows=gate_rows, residual_scale=self.residual_scale,
                                      weight=self.norm_weight, kind=self.kind, eps=self.eps, quantized=True)
         return r, capi.fp8_matmul(self.ctx, q, s, self.weights, self.scales, out_dtype=out_dtype)

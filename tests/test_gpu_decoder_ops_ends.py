@@ -1,10 +1,10 @@
 """The operators behind a decoder where they can go wrong at the ends: values that are no numbers, masks and huge logits in the log
-probabilities."""
+probabilities, and large logits on the way to them."""
 import math
 
 import pytest
 
-from tests.test_gpu_decoder_ops import DTYPES, _check_logprobs, _gen, _masked_rows, _mods, _rows
+from tests.test_gpu_decoder_ops import DTYPES, _check_logprobs, _gen, _masked_rows, _mods, _ref_logprobs, _rows
 
 pytestmark = pytest.mark.gpu
 
@@ -136,3 +136,21 @@ def test_token_logprobs_of_short_rows_with_masks_and_many_alternatives(ctx, V, d
     for top in (15, 24, 32):
         for pad, offset in ((0, 0), (1, 1)):
             _check_logprobs(ctx, _rows(x, pad, offset), tokens, top, 0.9)
+
+
+# ---- together ------------------------------------------------------------------------------------------------------------
+
+def test_token_head_keeps_logits_in_fp32(ctx):
+    """Log probabilities are as good as their logits: unless told otherwise these are fp32, where fp16 would end at 65504."""
+    torch, capi = _mods()
+    from excalibur_b200.token_head import TokenHead
+    g = _gen(11)
+    C, V = 256, 500
+    head = TokenHead(ctx, torch.randn((V, C), device="cuda", generator=g) * 1e4, torch.ones(C, device="cuda"))
+    h, x = torch.randn((4, C), device="cuda", generator=g), torch.zeros((4, C), device="cuda")
+    _, logits = head.logits(h, x)
+    assert logits.dtype == torch.float32 and float(logits.abs().max()) > 65504
+    given, entropy, best, tokens = head.scores(h, x, torch.zeros((4, 1), device="cuda", dtype=torch.int32), top=3, temperature=1e4)
+    ctx.sync_check()
+    assert all(torch.isfinite(v).all() for v in (given, entropy, best))
+    assert torch.equal(tokens, _ref_logprobs(logits, torch.zeros((4, 1), device="cuda", dtype=torch.int32), 3, 1e-4)[3])
