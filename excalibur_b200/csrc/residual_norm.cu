@@ -239,13 +239,25 @@ extern "C" int exb_residual_norm_fwd(exb_ctx* ctx, const exb_norm_desc* d, const
     if (n && quantized) {
         EXB_REQUIRE(n_scales && d->scale_stride >= d->rows, "exb_residual_norm_fwd: null n_scales, or a scale stride smaller than the rows");
         EXB_REQUIRE(aligned16(n) && d->n_stride % 16 == 0, "exb_residual_norm_fwd: e4m3 rows must start at multiples of 16 bytes");
-        EXB_REQUIRE(n != h && n != x, "exb_residual_norm_fwd: e4m3 rows cannot take the input's place");
     }
-    EXB_REQUIRE(!gate || (gate != r && gate != n), "exb_residual_norm_fwd: a result cannot take the gate's place");
-    EXB_REQUIRE(!r || r != n, "exb_residual_norm_fwd: r and n are the same buffer");
-    EXB_REQUIRE((r != h || d->r_stride == d->h_stride) && (!x || r != x || d->r_stride == d->x_stride) && (n != h || d->n_stride == d->h_stride) &&
-                    (!x || n != x || d->n_stride == d->x_stride),
-                "exb_residual_norm_fwd: a result in an input's place needs its stride");
+    {
+        // r and n may take h's or x's own place, where a row's threads read it before they write it; over any other input, or part of one, a
+        // row would be read after another has written it.
+        const int64_t gates = d->gate_rows ? (d->rows - 1) / d->gate_rows + 1 : 1;
+        const int64_t blocks = (d->C + rows::kBlock - 1) / rows::kBlock;
+        const rows::Place in[] = {rows::place_of(h, d->rows, d->C, d->h_stride, es),     rows::place_of(x, d->rows, d->C, d->x_stride, es),
+                                  rows::place_of(gate, gates, d->C, d->gate_stride, es), rows::place_of(post_weight, 1, d->C, d->C, 4),
+                                  rows::place_of(post_bias, 1, d->C, d->C, 4),           rows::place_of(n ? weight : nullptr, 1, d->C, d->C, 4),
+                                  rows::place_of(n ? bias : nullptr, 1, d->C, d->C, 4)};
+        const rows::Place out[] = {rows::place_of(r, d->rows, d->C, d->r_stride, es), rows::place_of(n, d->rows, d->C, d->n_stride, quantized ? 1 : es),
+                                   rows::place_of(n && quantized ? n_scales : nullptr, blocks, d->rows, d->scale_stride, 4)};
+        for (int i = 0; i < 3; ++i) {
+            for (int j = 0; j < 7; ++j)
+                EXB_REQUIRE(!rows::overlap(out[i], in[j]) || (i < 2 && j < 2 && rows::same_place(out[i], in[j])),
+                            "exb_residual_norm_fwd: a result lies over an input (r and n may take the place of h or x, with its stride)");
+            for (int j = 0; j < i; ++j) EXB_REQUIRE(!rows::overlap(out[i], out[j]), "exb_residual_norm_fwd: results lie over each other");
+        }
+    }
     NormArgs a;
     a.h = h; a.x = x; a.gate = gate;
     a.post_weight = post_weight; a.post_bias = post_bias; a.weight = weight; a.bias = bias;

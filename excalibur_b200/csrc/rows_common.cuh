@@ -306,6 +306,41 @@ inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<u
 // Whether rows at this base and stride can be read in 16-byte vectors (a missing tensor can).
 inline bool vector_rows(const void* p, int64_t stride, size_t es) { return !p || (aligned16(p) && stride * (int64_t)es % 16 == 0); }
 
+// Where a matrix lies: `rows` times `width` bytes, `stride` bytes apart (a missing tensor: no rows).
+struct Place {
+    const uint8_t* at;
+    int64_t rows, width, stride;
+};
+inline Place place_of(const void* p, int64_t rows, int64_t C, int64_t stride, size_t es) {
+    // (a single row's distance to the next means nothing)
+    return {static_cast<const uint8_t*>(p), p ? rows : 0, C * (int64_t)es, (rows > 1 ? stride : C) * (int64_t)es};
+}
+inline bool same_place(const Place& a, const Place& b) { return a.at == b.at && a.rows == b.rows && a.width == b.width && a.stride == b.stride; }
+
+// Whether two matrices share a byte.  Those that lie next to each other in the rows of a wider one do not.  Almost all calls are answered by
+// the two ends or by equal strides; otherwise each row of the shorter one is looked for among the other's.
+inline bool overlap(const Place& a, const Place& b) {
+    if (a.rows == 0 || b.rows == 0) return false;
+    auto end = [](const Place& p) { return p.at + (p.rows - 1) * p.stride + p.width; };
+    if (a.at >= end(b) || b.at >= end(a)) return false;
+    const Place &few = a.rows <= b.rows ? a : b, &many = a.rows <= b.rows ? b : a;
+    // the last row of `many` that starts at `d` bytes from its first one or before
+    auto before = [&](int64_t d) { return d >= 0 ? d / many.stride : -((-d + many.stride - 1) / many.stride); };
+    const int64_t d = few.at - many.at;
+    if (few.stride == many.stride) {      // row i of `few` lies m bytes behind row q + i of `many`
+        const int64_t q = before(d), m = d - q * many.stride;
+        auto both = [&](int64_t shift) { return shift < many.rows && shift + few.rows > 0; };
+        return (m < many.width && both(q)) || (m + few.width > many.stride && both(q + 1));
+    }
+    for (int64_t i = 0; i < few.rows; ++i) {
+        const int64_t at = d + i * few.stride;
+        int64_t row = before(at + few.width - 1);
+        if (row >= many.rows) row = many.rows - 1;
+        if (row >= 0 && row * many.stride + many.width > at) return true;
+    }
+    return false;
+}
+
 // fn(T()) for the element type
 template <typename F>
 inline void with_type(int dtype, F&& fn) {

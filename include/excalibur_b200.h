@@ -522,7 +522,8 @@ EXB_API int exb_fp8_matmul_fwd(exb_ctx* ctx, const exb_matmul_desc* d, const uin
  * r is written in dtype, n in out_dtype: dtype itself, or EXB_E4M3 with n_scales as exb_quantize_blocks_fwd writes blocks
  * of one row.  Biases are NULL where there is none.  Row i takes row i / gate_rows of the gate (dtype); gate_rows 0: all
  * take row 0.  r or n may be NULL (not both): then it is not written, and weight and bias are not read without n.  r
- * and n may each be h or x, in the same place with the same stride (not both the same one). */
+ * and n may each be h or x, in the same place with the same stride (not both the same one); results that share memory with
+ * an input or with each other in any other way are refused. */
 typedef enum exb_norm { EXB_NORM_RMS = 0, EXB_NORM_LAYER = 1 } exb_norm;
 typedef struct exb_norm_desc {
     int64_t rows;

@@ -1,5 +1,5 @@
 """The operators behind a decoder where they can go wrong at the ends: values that are no numbers, masks and huge logits in the log
-probabilities, and large logits on the way to them."""
+probabilities, large logits on the way to them, results that lie over inputs."""
 import math
 
 import pytest
@@ -154,3 +154,79 @@ def test_token_head_keeps_logits_in_fp32(ctx):
     ctx.sync_check()
     assert all(torch.isfinite(v).all() for v in (given, entropy, best))
     assert torch.equal(tokens, _ref_logprobs(logits, torch.zeros((4, 1), device="cuda", dtype=torch.int32), 3, 1e-4)[3])
+
+
+# ---- results over inputs -------------------------------------------------------------------------------------------------
+
+def _refused(capi, calls):
+    for i, call in enumerate(calls):
+        with pytest.raises(capi.ExbError) as e:
+            call()
+        assert e.value.code == capi.EXB_ERR_BAD_ARG, i
+
+
+def test_residual_norm_refuses_results_over_inputs(ctx):
+    """A result may take h's or x's own place; over any other part of an input, or over another result, some rows would be read after
+    they were written."""
+    torch, capi = _mods()
+    C = 256
+    w = torch.ones(C, device="cuda")
+    buf = torch.randn((12, C), device="cuda")
+    h, x, wide = torch.randn((8, C), device="cuda"), buf[:8], torch.randn((8, 4 * C), device="cuda")
+    flat = buf.view(-1)
+    as_bytes = buf.view(torch.float8_e4m3fn)
+    _refused(capi, [
+        lambda: capi.residual_norm(ctx, h, x, gate=x[3:4], weight=w, r=x),
+        lambda: capi.residual_norm(ctx, h, x, gate=x[2:6], gate_rows=2, weight=w, r=x),
+        lambda: capi.residual_norm(ctx, h, x, gate=x[7:8], weight=w, n=x),
+        lambda: capi.residual_norm(ctx, h, x, r=buf[1:9]),
+        lambda: capi.residual_norm(ctx, h, x, r=buf[4:12]),
+        lambda: capi.residual_norm(ctx, x, h, weight=w, n=buf[2:10]),
+        lambda: capi.residual_norm(ctx, h, x, r=flat[1:1 + 8 * C].view(8, C)),
+        lambda: capi.residual_norm(ctx, h, x, r=buf.as_strided((8, C), (C + 8, 1))),
+        lambda: capi.residual_norm(ctx, h, x, weight=w, r=wide[:, :C], n=wide[:, C // 2: C // 2 + C]),
+        lambda: capi.residual_norm(ctx, h, x, weight=w, r=wide.view(-1)[:8 * C].view(8, C), n=wide[:, C:2 * C]),
+        lambda: capi.residual_norm(ctx, wide[:, :C], wide[:, C:2 * C], r=wide[:, C - 8:2 * C - 8]),
+        lambda: capi.residual_norm(ctx, wide[:, :C], h, r=wide.as_strided((8, C), (4 * C - 8, 1), 3 * C + 8)),
+        lambda: capi.residual_norm(ctx, h, x, weight=x[0], r=x),
+        lambda: capi.residual_norm(ctx, h, x, post_weight=x[7], weight=w, n=x),
+        lambda: capi.residual_norm(ctx, h, x, weight=w, quantized=True, n=as_bytes[:8, :C]),
+        lambda: capi.residual_norm(ctx, h, x, weight=w, quantized=True, r=wide[:, :C], n=wide.view(torch.float8_e4m3fn)[:, C:2 * C]),
+    ])
+    ctx.sync_check()
+
+
+def test_residual_norm_takes_columns_of_a_wider_matrix(ctx):
+    """Inputs and results that lie next to each other in the rows of one matrix share no element, and h's and x's own places stay open."""
+    torch, capi = _mods()
+    g = _gen(21)
+    for C in (256, 250):
+        w = torch.rand(C, device="cuda", generator=g)
+        h, x, gate = (torch.randn((9, C), device="cuda", generator=g) for _ in range(3))
+        want = capi.residual_norm(ctx, h, x, gate=gate, gate_rows=1, weight=w)
+        wide = torch.zeros((9, 5 * C), device="cuda")
+        parts = [wide[:, i * C:(i + 1) * C] for i in range(5)]
+        for v, p in zip((h, x, gate), parts):
+            p.copy_(v)
+        r, n = capi.residual_norm(ctx, parts[0], parts[1], gate=parts[2], gate_rows=1, weight=w, r=parts[3], n=parts[4])
+        ctx.sync_check()
+        assert torch.equal(r, want[0]) and torch.equal(n, want[1]) and torch.equal(parts[0], h) and torch.equal(parts[2], gate)
+        r, n = capi.residual_norm(ctx, parts[0], parts[1], gate=parts[2], gate_rows=1, weight=w, r=parts[1], n=parts[0])
+        ctx.sync_check()
+        assert torch.equal(r, want[0]) and torch.equal(n, want[1]) and torch.equal(parts[2], gate)
+        # one row: its distance to the next does not matter
+        one = torch.stack([h[0], x[0], torch.zeros_like(x[0])])
+        r, _ = capi.residual_norm(ctx, one[0:1], one[1:2], r=one[2:3])
+        r2, _ = capi.residual_norm(ctx, h[:1], x[:1])
+        ctx.sync_check()
+        assert torch.equal(r, r2)
+        both = x[:1].clone()
+        capi.residual_norm(ctx, h[:1], both, r=both)
+        ctx.sync_check()
+        assert torch.equal(both, r2)
+        # x and h the same
+        same = h.clone()
+        capi.residual_norm(ctx, same, same, r=same)
+        r3, _ = capi.residual_norm(ctx, h, h)
+        ctx.sync_check()
+        assert torch.equal(same, r3)
