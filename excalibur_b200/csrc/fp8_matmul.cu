@@ -676,6 +676,10 @@ extern "C" int exb_fp8_matmul_fwd(exb_ctx* ctx, const exb_matmul_desc* d, const 
                 "exb_fp8_matmul_fwd: the rows of a and w must start at multiples of 16 bytes");
     EXB_REQUIRE(rows::aligned_to(y, es) && rows::aligned_to(a_scales, 4) && rows::aligned_to(w_scales, 4) && rows::aligned_to(bias, 4),
                 "exb_fp8_matmul_fwd: y, scales or bias not aligned to its element");
+    const rows::Place in[] = {rows::place_of(a, M, K, a_stride, 1), rows::place_of(a_scales, blocks, M, a_scale_stride, 4), rows::place_of(w, N, K, w_stride, 1),
+                              rows::place_of(w_scales, (N - 1) / kBlk + 1, blocks, w_scale_stride, 4), rows::place_of(bias, 1, N, N, 4)};
+    const rows::Place out[] = {rows::place_of(y, M, N, y_stride, es)};
+    EXB_REQUIRE(!rows::results_overlap(out, in), "exb_fp8_matmul_fwd: y lies over an input");
     MatmulParams p;
     p.a_scales = a_scales; p.w_scales = w_scales; p.bias = bias; p.y = y;
     p.a_scale_stride = a_scale_stride; p.w_scale_stride = w_scale_stride; p.y_stride = y_stride;

@@ -111,6 +111,11 @@ extern "C" int exb_quantize_blocks_fwd(exb_ctx* ctx, const exb_blocks_desc* d, c
     EXB_REQUIRE(scale_stride >= (block_rows == 1 ? n_rows : blocks), "exb_quantize_blocks_fwd: scale stride %lld is too small", (long long)scale_stride);
     EXB_REQUIRE(rows::aligned_to(x, es) && rows::aligned_to(scales, 4), "exb_quantize_blocks_fwd: x or scales not aligned to its element");
     EXB_REQUIRE(aligned16(q) && q_stride % 16 == 0, "exb_quantize_blocks_fwd: q and its row stride must be multiples of 16 bytes");
+    const rows::Place in[] = {rows::place_of(x, n_rows, C, x_stride, es)};
+    const rows::Place out[] = {rows::place_of(q, n_rows, C, q_stride, 1),
+                               block_rows == 1 ? rows::place_of(scales, blocks, n_rows, scale_stride, 4)
+                                               : rows::place_of(scales, (n_rows - 1) / 128 + 1, blocks, scale_stride, 4)};
+    EXB_REQUIRE(!rows::results_overlap(out, in), "exb_quantize_blocks_fwd: a result lies over x or over the other result");
     const int64_t shares = (blocks + 1) / 2;
     const int64_t grid = (block_rows == 1 ? (n_rows + kTileRows - 1) / kTileRows : (n_rows + 127) / 128) * shares;
     if (grid > INT32_MAX) return fail(EXB_ERR_UNSUPPORTED, "exb_quantize_blocks_fwd: %lld rows of %d are too many for one call", (long long)n_rows, C);

@@ -341,6 +341,18 @@ inline bool overlap(const Place& a, const Place& b) {
     return false;
 }
 
+// Whether one of the results shares a byte with an input or with another result.
+template <int kOut, int kIn>
+inline bool results_overlap(const Place (&out)[kOut], const Place (&in)[kIn]) {
+    for (int i = 0; i < kOut; ++i) {
+        for (const Place& p : in)
+            if (overlap(out[i], p)) return true;
+        for (int j = 0; j < i; ++j)
+            if (overlap(out[i], out[j])) return true;
+    }
+    return false;
+}
+
 // fn(T()) for the element type
 template <typename F>
 inline void with_type(int dtype, F&& fn) {

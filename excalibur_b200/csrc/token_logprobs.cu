@@ -712,6 +712,10 @@ extern "C" int exb_token_logprobs_fwd(exb_ctx* ctx, const exb_logprobs_desc* d, 
     for (const void* p : {static_cast<const void*>(tokens), static_cast<const void*>(logprobs), static_cast<const void*>(entropy),
                           static_cast<const void*>(top_logprobs), static_cast<const void*>(top_tokens)})
         EXB_REQUIRE(rows::aligned_to(p, 4), "exb_token_logprobs_fwd: a buffer is not aligned to its element");
+    const rows::Place in[] = {rows::place_of(logits, n_rows, V, stride, es), rows::place_of(n_given ? tokens : nullptr, n_rows, n_given, n_given, 4)};
+    const rows::Place out[] = {rows::place_of(n_given ? logprobs : nullptr, n_rows, n_given, n_given, 4), rows::place_of(entropy, 1, n_rows, n_rows, 4),
+                               rows::place_of(top ? top_logprobs : nullptr, n_rows, top, top, 4), rows::place_of(top ? top_tokens : nullptr, n_rows, top, top, 4)};
+    EXB_REQUIRE(!rows::results_overlap(out, in), "exb_token_logprobs_fwd: a result lies over an input or another result");
     LogprobArgs a;
     a.logits = logits; a.tokens = tokens; a.logprobs = logprobs; a.entropy = entropy; a.top_logprobs = top_logprobs; a.top_tokens = top_tokens;
     a.stride = stride; a.V = V; a.n_given = n_given; a.top = top; a.scale = scale;

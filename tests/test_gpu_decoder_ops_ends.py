@@ -230,3 +230,49 @@ def test_residual_norm_takes_columns_of_a_wider_matrix(ctx):
         r3, _ = capi.residual_norm(ctx, h, h)
         ctx.sync_check()
         assert torch.equal(same, r3)
+
+
+def test_other_results_over_inputs_are_refused(ctx):
+    torch, capi = _mods()
+    x = torch.randn((8, 256), device="cuda")
+    as_bytes, floats = x.view(torch.float8_e4m3fn), torch.zeros(4096, device="cuda")
+    _refused(capi, [
+        lambda: capi.quantize_blocks(ctx, x, q=as_bytes[:, :256]),
+        lambda: capi.quantize_blocks(ctx, x, q=as_bytes[:, 512:768]),
+        lambda: capi.quantize_blocks(ctx, x, 128, q=as_bytes[:, 768:1024]),
+        lambda: capi.quantize_blocks(ctx, x, scales=x[:2, :8]),
+        lambda: capi.quantize_blocks(ctx, x, q=floats[:512].view(torch.float8_e4m3fn).view(8, 256), scales=floats[500:516].view(2, 8)),
+    ])
+    # 8 bits between the columns of a wider matrix share nothing with them
+    wide = torch.zeros((8, 1024), device="cuda")
+    wide[:, :256] = x
+    q, s = capi.quantize_blocks(ctx, wide[:, :256], q=wide.view(torch.float8_e4m3fn)[:, 2048:2304], scales=wide[:2, 300:308])
+    want_q, want_s = capi.quantize_blocks(ctx, x)
+    ctx.sync_check()
+    assert torch.equal(q.view(torch.uint8), want_q.view(torch.uint8)) and torch.equal(s, want_s) and torch.equal(wide[:, :256], x)
+
+    w, sw = capi.quantize_blocks(ctx, x, 128)
+    a, sa = want_q, want_s
+    bias = torch.zeros(8, device="cuda")
+    half = capi.EXB_F16
+    L, st, addr = capi.lib(), None, lambda t: t.data_ptr()  # noqa: E731
+
+    def matmul(y_at, ys=8):
+        d = capi.MatmulDesc(M=8, N=8, K=256, y_dtype=half, a_stride=256, a_scale_stride=8, w_stride=256, w_scale_stride=2, y_stride=ys)
+        import ctypes
+        return L.exb_fp8_matmul_fwd(ctx.handle, ctypes.byref(d), addr(a), addr(sa), addr(w), addr(sw), addr(bias), y_at, st)
+    for at in (addr(a), addr(a) + 8 * 256 - 16, addr(w) + 512, addr(sa) + 32, addr(sw), addr(bias) + 16):
+        assert matmul(at) == capi.EXB_ERR_BAD_ARG
+
+    logits, tokens = torch.randn((4, 64), device="cuda"), torch.zeros((4, 2), device="cuda", dtype=torch.int32)
+    out = torch.zeros(256, device="cuda")
+
+    def scores(lp=addr(out), entropy=addr(out) + 64, top_lp=addr(out) + 128, top_tokens=addr(out) + 256):
+        import ctypes
+        d = capi.LogprobsDesc(rows=4, stride=64, V=64, dtype=capi.EXB_F32, n_given=2, top=3, scale=1.0)
+        return L.exb_token_logprobs_fwd(ctx.handle, ctypes.byref(d), addr(logits), addr(tokens), lp, entropy, top_lp, top_tokens, st)
+    assert scores() == capi.EXB_OK
+    for k in (dict(lp=addr(logits)), dict(lp=addr(tokens)), dict(entropy=addr(logits) + 4 * 255), dict(top_lp=addr(tokens) + 28), dict(top_tokens=addr(logits) + 100),
+              dict(entropy=addr(out) + 28), dict(top_lp=addr(out) + 76), dict(top_tokens=addr(out) + 172), dict(lp=addr(out) + 256 + 44)):
+        assert scores(**k) == capi.EXB_ERR_BAD_ARG, k
+    ctx.sync_check()
