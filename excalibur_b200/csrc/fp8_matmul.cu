@@ -668,6 +668,7 @@ extern "C" int exb_fp8_matmul_fwd(exb_ctx* ctx, const exb_matmul_desc* d, const 
     if (M > INT32_MAX - 256 || N > INT32_MAX - 256 || K > INT32_MAX - 256)
         return fail(EXB_ERR_UNSUPPORTED, "exb_fp8_matmul_fwd: %lld x %d x %d is too large for one call", (long long)M, N, K);
     if (M == 0) return EXB_OK;
+    if (int rc = rows::check_device(ctx, "exb_fp8_matmul_fwd")) return rc;
     EXB_REQUIRE(a && a_scales && w && w_scales && y, "exb_fp8_matmul_fwd: null buffer");
     const int blocks = (K + kBlk - 1) / kBlk;
     EXB_REQUIRE(a_stride >= K && w_stride >= K && y_stride >= N, "exb_fp8_matmul_fwd: row strides smaller than the rows");

@@ -105,6 +105,7 @@ extern "C" int exb_quantize_blocks_fwd(exb_ctx* ctx, const exb_blocks_desc* d, c
     EXB_REQUIRE(n_rows >= 0 && C >= 1, "exb_quantize_blocks_fwd: bad shape (%lld rows of %d)", (long long)n_rows, C);
     EXB_REQUIRE(block_rows == 1 || block_rows == 128, "exb_quantize_blocks_fwd: blocks have 1 or 128 rows, got %d", block_rows);
     if (n_rows == 0) return EXB_OK;
+    if (int rc = rows::check_device(ctx, "exb_quantize_blocks_fwd")) return rc;
     EXB_REQUIRE(x && q && scales, "exb_quantize_blocks_fwd: null buffer");
     const int64_t blocks = ((int64_t)C + rows::kBlock - 1) / rows::kBlock;
     EXB_REQUIRE(x_stride >= C && q_stride >= C, "exb_quantize_blocks_fwd: row strides smaller than the rows");

@@ -225,6 +225,7 @@ extern "C" int exb_residual_norm_fwd(exb_ctx* ctx, const exb_norm_desc* d, const
     if (d->C > 32768 || d->rows > INT32_MAX)
         return fail(EXB_ERR_UNSUPPORTED, "exb_residual_norm_fwd: at most 32768 channels and 2^31 - 1 rows, got %lld rows of %d", (long long)d->rows, d->C);
     if (d->rows == 0) return EXB_OK;
+    if (int rc = rows::check_device(ctx, "exb_residual_norm_fwd")) return rc;
     EXB_REQUIRE(h && (r || n), "exb_residual_norm_fwd: null buffer");
     EXB_REQUIRE(!n || weight, "exb_residual_norm_fwd: the norm has no weight");
     EXB_REQUIRE(!post_bias || post_weight, "exb_residual_norm_fwd: a bias without its norm's weight");

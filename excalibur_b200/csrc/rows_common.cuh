@@ -353,6 +353,15 @@ inline bool results_overlap(const Place (&out)[kOut], const Place (&in)[kIn]) {
     return false;
 }
 
+// A launch goes to the calling thread's current device, whatever the context's and the addresses': on another one it would read memory that is
+// not there.
+inline int check_device(const exb_ctx* ctx, const char* what) {
+    int device;
+    EXB_CUDA_TRY(cudaGetDevice(&device));
+    EXB_REQUIRE(device == ctx->device, "%s: the context is for device %d, the current device is %d", what, ctx->device, device);
+    return EXB_OK;
+}
+
 // fn(T()) for the element type
 template <typename F>
 inline void with_type(int dtype, F&& fn) {

@@ -706,6 +706,7 @@ extern "C" int exb_token_logprobs_fwd(exb_ctx* ctx, const exb_logprobs_desc* d, 
     if (n_rows > INT32_MAX / 16 || V > (1 << 30))
         return fail(EXB_ERR_UNSUPPORTED, "exb_token_logprobs_fwd: %lld rows of %d are too many for one call", (long long)n_rows, V);
     if (n_rows == 0) return EXB_OK;
+    if (int rc = rows::check_device(ctx, "exb_token_logprobs_fwd")) return rc;
     EXB_REQUIRE(logits && (n_given == 0 || (tokens && logprobs)) && (top == 0 || (top_logprobs && top_tokens)), "exb_token_logprobs_fwd: null buffer");
     EXB_REQUIRE(stride >= V, "exb_token_logprobs_fwd: row stride smaller than the rows");
     EXB_REQUIRE(rows::aligned_to(logits, es), "exb_token_logprobs_fwd: logits not aligned to their element");

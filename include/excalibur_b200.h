@@ -477,7 +477,8 @@ EXB_API int exb_channel_affine_fwd(exb_ctx* ctx, const void* x, void* y, const f
  * [rows][C] with C innermost and a row stride in elements, in EXB_F16, EXB_BF16 or EXB_F32; parameters are fp32 device
  * arrays; sums, norms and statistics are held in fp32.  All pointers are device pointers, aligned to their element unless
  * said otherwise; 16-byte aligned rows (base and stride) are read in vectors.  rows == 0 does nothing.  Results must not share
- * memory with inputs or with each other, unless said otherwise: such calls are refused.
+ * memory with inputs or with each other, unless said otherwise: such calls are refused, and so are calls of a thread whose
+ * current device is not the context's.
  *
  * exb_quantize_blocks_fwd: 8-bit floating point with a scale for each block of block_rows x 128 elements, block_rows 1
  * (activations) or 128 (weights):

@@ -1,5 +1,5 @@
 """The operators behind a decoder where they can go wrong at the ends: values that are no numbers, masks and huge logits in the log
-probabilities, large logits on the way to them, results that lie over inputs."""
+probabilities, large logits on the way to them, results that lie over inputs, another device."""
 import math
 
 import pytest
@@ -275,4 +275,33 @@ def test_other_results_over_inputs_are_refused(ctx):
     for k in (dict(lp=addr(logits)), dict(lp=addr(tokens)), dict(entropy=addr(logits) + 4 * 255), dict(top_lp=addr(tokens) + 28), dict(top_tokens=addr(logits) + 100),
               dict(entropy=addr(out) + 28), dict(top_lp=addr(out) + 76), dict(top_tokens=addr(out) + 172), dict(lp=addr(out) + 256 + 44)):
         assert scores(**k) == capi.EXB_ERR_BAD_ARG, k
+    ctx.sync_check()
+
+
+# ---- another device ------------------------------------------------------------------------------------------------------
+
+def test_a_context_of_another_device_than_the_current_one_is_refused(ctx):
+    """A launch goes to the calling thread's current device, whatever the context's and the tensors': these have to be the same."""
+    import ctypes as C
+    torch, capi = _mods()
+    # the context as it would be on the next device: its first field is the device
+    other = (C.c_int32 * 10).from_buffer_copy((C.c_int32 * 10).from_address(C.cast(ctx.handle, C.c_void_p).value))
+    assert other[0] == ctx.device == torch.cuda.current_device()
+    other[0] += 1
+    x = torch.randn((8, 256), device="cuda")
+    q, s = capi.quantize_blocks(ctx, x)
+    w, sw = capi.quantize_blocks(ctx, x, 128)
+    out, L = torch.zeros_like(x), capi.lib()
+    blocks = capi.BlocksDesc(rows=8, C=256, in_dtype=capi.EXB_F32, block_rows=1, x_stride=256, q_stride=256, scale_stride=8)
+    matmul = capi.MatmulDesc(M=8, N=8, K=256, y_dtype=capi.EXB_F16, a_stride=256, a_scale_stride=8, w_stride=256, w_scale_stride=2, y_stride=8)
+    norm = capi.NormDesc(rows=8, C=256, dtype=capi.EXB_F32, out_dtype=capi.EXB_F32, kind=0, eps=1e-5, residual_scale=1.0, h_stride=256, r_stride=256)
+    scores = capi.LogprobsDesc(rows=8, stride=256, V=256, dtype=capi.EXB_F32, n_given=0, top=0, scale=1.0)
+    X, Q, S, W, SW, Y = (t.data_ptr() for t in (x, q, s, w, sw, out))
+    for handle, want in ((C.byref(other), capi.EXB_ERR_BAD_ARG), (ctx.handle, capi.EXB_OK)):
+        assert L.exb_quantize_blocks_fwd(handle, C.byref(blocks), X, Q, S, None) == want
+        assert L.exb_fp8_matmul_fwd(handle, C.byref(matmul), Q, S, W, SW, None, Y, None) == want
+        assert L.exb_residual_norm_fwd(handle, C.byref(norm), X, None, None, None, None, None, None, Y, None, None, None) == want
+        assert L.exb_token_logprobs_fwd(handle, C.byref(scores), X, None, None, Y, None, None, None) == want
+        if want != capi.EXB_OK:
+            assert "current device" in capi.last_error()
     ctx.sync_check()
