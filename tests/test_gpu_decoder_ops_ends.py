@@ -1,10 +1,11 @@
 """The operators behind a decoder where they can go wrong at the ends: values that are no numbers, masks and huge logits in the log
-probabilities, large logits on the way to them, results that lie over inputs, another device."""
+probabilities, large logits on the way to them, scales at fp32's ends and wide vocabularies in the product, results that lie over inputs,
+another device."""
 import math
 
 import pytest
 
-from tests.test_gpu_decoder_ops import DTYPES, _check_logprobs, _gen, _masked_rows, _mods, _ref_logprobs, _rows
+from tests.test_gpu_decoder_ops import DTYPES, _check_logprobs, _check_product, _gen, _masked_rows, _mods, _ref_logprobs, _rows
 
 pytestmark = pytest.mark.gpu
 
@@ -136,6 +137,40 @@ def test_token_logprobs_of_short_rows_with_masks_and_many_alternatives(ctx, V, d
     for top in (15, 24, 32):
         for pad, offset in ((0, 0), (1, 1)):
             _check_logprobs(ctx, _rows(x, pad, offset), tokens, top, 0.9)
+
+
+# ---- the product ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("M", [1, 2, 16, 17, 64])
+def test_fp8_matmul_of_few_rows_with_extreme_scales(ctx, M):
+    """Scales that span the range of fp32 between blocks, and zero blocks, with nothing infinite: every row is right."""
+    torch, capi = _mods()
+    g = _gen(M)
+    N, K = 300, 640
+    x = torch.randn((M, K), device="cuda", generator=g)
+    v = torch.randn((N, K), device="cuda", generator=g)
+    x[:, :128] *= 1e18
+    x[:, 128:256] *= 1e-18
+    x[:, 256:384] = 0
+    v[:, :128] *= 1e-18
+    v[:, 128:256] *= 1e18
+    a, sa = capi.quantize_blocks(ctx, x)
+    w, sw = capi.quantize_blocks(ctx, v, 128)
+    y = capi.fp8_matmul(ctx, a, sa, w, sw, None, capi.EXB_F32)
+    ctx.sync_check()
+    _check_product(y, a, sa, w, sw, None, "float32")
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 128256, 300), (16, 70001, 260), (64, 131072, 128), (70, 66000, 200), (300, 131071, 150)])
+def test_fp8_matmul_with_a_vocabulary(ctx, M, N, K):
+    torch, capi = _mods()
+    g = _gen(N)
+    a, sa = capi.quantize_blocks(ctx, torch.randn((M, K), device="cuda", generator=g).half())
+    w, sw = capi.quantize_blocks(ctx, torch.randn((N, K), device="cuda", generator=g).half() * 0.05, 128)
+    for dtype in ("float32", "bfloat16"):
+        y = capi.fp8_matmul(ctx, a, sa, w, sw, None, capi.exb_dtype_of(getattr(torch, dtype)))
+        ctx.sync_check()
+        _check_product(y, a, sa, w, sw, None, dtype)
 
 
 # ---- together ------------------------------------------------------------------------------------------------------------
