@@ -357,8 +357,8 @@ __device__ __forceinline__ void store_rows(const float2 (&acc)[kPairs], uint8_t*
             }
         } else {
             // Rows that start anywhere: kUnits - 1 vectors at multiples of 16 bytes, put together of two units each, and 16 bytes before
-            // and behind them element by element.  (4048 x 7313 x 264 takes
-            // 42.9 us, element by element 51.8, and 4048 x 7312 x 264 29: sectors that two passes write a part of each are what is left.)
+            // and behind them element by element.  (fp16, 4048 x 7313 x 264 takes
+            // 42.9 us, element by element 51.8, and 4048 x 7312 x 264 29: sectors that two passes write a part of each are the difference.)
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
                 const int r = i * kRows + sub;

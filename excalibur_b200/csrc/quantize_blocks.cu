@@ -2,7 +2,7 @@
 // of 128 rows).  One pass over the input: a block's values stay in registers between its maximum and their conversion.
 // Bound by memory: 2 (or 4) bytes in and 1 out for each element.  bf16, single rows: 8192 x 14336 in 56 us (6350 GB/s), 64 x 4096 in
 // 1.7; rows of 14335, which are moved into place between lanes, 86 us.  Blocks of 128 rows: 4096 x 14336 in 29.8 us (5980 GB/s),
-// rows of 14337 in 53.
+// rows of 14337 in 53.  fp32, 4096 x 14336: single rows 43.4 us (6770 GB/s), blocks of 128 rows 49.3 (5960 GB/s).
 #include "rows_common.cuh"
 
 namespace exb {

@@ -3,9 +3,10 @@
 // A row stays in its threads' registers in fp32 from the loads of h, x and the gate to the stores of r and n (in the
 // activations' type, or as e4m3 with a scale for each 128 channels), so that every tensor crosses memory once; the sums of
 // the norms are the only thing its warps exchange.  Bound by memory with many rows, by the chain of loads, reductions and
-// stores with few.  4096 x 4096 bf16 takes 23.3 us (5760 GB/s), with both norms, a gate and e4m3 29.2 (4030 GB/s: 37 instructions an
-// element are issued 60 % of the time), one row 1.95, 3152 x 1000 fp16 with a gate's rows 6.9; rows that start anywhere (4096 x 1001,
-// 9.1) are loaded and stored in single elements.
+// stores with few.  4096 x 4096 bf16 takes 23.3 us (5760 GB/s), fp32 42.5 (6320 GB/s), bf16 with both norms, a gate and e4m3 29.2
+// (4030 GB/s), one row 1.95, 3152 x 1000 fp16 with a gate's rows 6.9; rows that start anywhere (4096 x 1001, 9.1) are loaded and stored in
+// single elements.  With everything no unit is full (62 % of the issue slots, 46 % of the warps): a quarter of the stalls are waits for a row's
+// loads, as many for the exchanges between lanes and warps in its reductions.
 #include "rows_common.cuh"
 
 #include <type_traits>
