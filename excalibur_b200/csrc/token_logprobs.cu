@@ -2,9 +2,9 @@
 //
 // z = scale * x, p = exp(z - lse), lse = log sum exp z.  With any e, t = x * scale * log2(e) - e, s = sum 2^t, w = sum 2^t * t:
 //   log p(v) = ln 2 * (t_v - log2 s),  entropy = ln 2 * (log2 s - w / s).
-// One pass over the row, bound by its reading and, in 16 bits, by the latency of its loads (46 to 49 % of the issue slots are used, 40 to 46 % of
-// the warps' stalls are waits for logits, and a CTA's loads drain at its row's end): 2048 rows of 50001 fp16 take 45.5 us with the
-// top 5 (4500 GB/s), 38.7 without, 52.8 with 20; 1024 rows of 50000 fp32 40.4 (5070 GB/s); one row of 131072 fp32 with 20 7.7.
+// One pass over the row, bound by its reading and, in 16 bits, by the latency of its loads (46 to 49 % of the issue slots are used, 40 to
+// 46 % of the warps' stalls are waits for logits, and a CTA's loads drain at its row's end): 2048 rows of 50001 fp16 take 46.2 us with the
+// top 5 (4430 GB/s), 40.7 without, 54.7 with 20; 1024 rows of 50000 fp32 without 36.4 (5630 GB/s); one row of 131072 fp32 with 20 7.9.
 // A thread keeps an integer e near the largest value that it has seen, so that x * scale * log2(e) - e is one multiply-add with one
 // rounding and a change of e scales its sums by a power of two, exactly.
 //
