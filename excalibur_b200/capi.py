@@ -27,6 +27,7 @@ EXPORTED_SYMBOLS = [
     "exb_dequantize_fwd", "exb_concat_fwd", "exb_concat_nearest_fwd", "exb_interp_nearest_fwd", "exb_channel_affine_fwd",
     "exb_conv_weights_set_slopes", "exb_dw_weights_set_slopes", "exb_depth_to_space_nchw_f32", "exb_deconv_few_f32", "exb_image_f32_to_nhwc_norm", "exb_nchw_f32_to_nhwc4_padded_norm", "exb_nhwc_f16_split_heads_f32", "exb_hardsigmoid_fwd", "exb_softmax_channels_f32", "exb_binaryop_channel_bcast_fwd", "exb_nchw_f16_to_nhwc4_padded", "exb_nchw_f32_focus_to_nhwc_f16", "exb_channel_affine_prelu_fwd", "exb_hardswish_fwd", "exb_focus_fwd", "exb_prelu_fwd", "exb_depth_to_space_fwd", "exb_transpose_hw_f32",
     "exb_quantize_blocks_fwd", "exb_fp8_matmul_fwd", "exb_residual_norm_fwd", "exb_token_logprobs_fwd",
+    "exb_quantize_rows_fwd", "exb_int8_matmul_fwd", "exb_grouped_matmul_fwd",
 ]
 
 
@@ -73,11 +74,28 @@ class LogprobsDesc(C.Structure):
         [("scale", C.c_float), ("reserved", C.c_int32)]
 
 
+class RowsDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64)] + [(n, C.c_int32) for n in ("C", "in_dtype")] + [(n, C.c_int64) for n in ("x_stride", "q_stride")]
+
+
+class Int8Desc(C.Structure):
+    _fields_ = [("M", C.c_int64)] + [(n, C.c_int32) for n in ("N", "K", "y_dtype", "reserved")] + \
+        [(n, C.c_int64) for n in ("a_stride", "w_stride", "y_stride")]
+
+
+class GroupedDesc(C.Structure):
+    _fields_ = [("M", C.c_int64)] + [(n, C.c_int32) for n in ("N", "K", "dtype", "y_dtype", "experts", "reserved")] + \
+        [(n, C.c_int64) for n in ("a_stride", "w_stride", "expert_stride", "y_stride")]
+
+
 # The same layouts as bytes: packing costs 0.2 us, a ctypes structure 0.8, and an argument of its own 0.1 each.
 _pack_norm = struct.Struct("@q4i2f7q").pack
 _pack_blocks = struct.Struct("@q4i3q").pack
 _pack_matmul = struct.Struct("@q4i5q").pack
 _pack_logprobs = struct.Struct("@2q4ifi").pack
+_pack_rows = struct.Struct("@q2i2q").pack
+_pack_int8 = struct.Struct("@q4i3q").pack
+_pack_grouped = struct.Struct("@q6i4q").pack
 
 
 class ExbError(RuntimeError):
@@ -156,6 +174,9 @@ def lib():
         L.exb_fp8_matmul_fwd.argtypes = [vp] * 9
         L.exb_residual_norm_fwd.argtypes = [vp] * 13
         L.exb_token_logprobs_fwd.argtypes = [vp] * 9
+        L.exb_quantize_rows_fwd.argtypes = [vp] * 6
+        L.exb_int8_matmul_fwd.argtypes = [vp] * 9
+        L.exb_grouped_matmul_fwd.argtypes = [vp] * 10
         _LIB = L
     return _LIB
 
@@ -910,3 +931,132 @@ def token_logprobs(ctx, logits, tokens=None, top=0, scale=1.0):
     if rc:
         check(rc)
     return lp, entropy, top_lp, top_tokens
+
+
+# ---- decoding in 8-bit integers, by experts and with beams -----------------------------------------
+def _int8_row_stride(q, device, what):
+    """Row stride of an 8-bit integer matrix, whose rows have to start at multiples of 16 bytes."""
+    if q.dtype is not _TORCH.int8:
+        _refuse("%s has to be int8", what)
+    stride = _row_stride(q, device, what)
+    if stride & 15:
+        if q.shape[0] > 1:
+            _refuse("rows of %s have to start at multiples of 16 bytes", what)
+        stride = (stride + 15) // 16 * 16
+    return stride
+
+
+def quantize_rows(ctx, x, q=None, scales=None):
+    """(q, scales): x (rows, channels) in 8-bit integers with a scale for each row; scales are (rows,).  q's rows start at multiples of 16 bytes."""
+    t = _TORCH or _torch()
+    device, shape = ctx.device, x.shape
+    xs = shape[-1] if x.is_contiguous() and x.get_device() == device and len(shape) == 2 else _row_stride(x, device, "x")
+    rows, channels = shape
+    if q is None:
+        qs = (channels + 15) & -16
+        q = x.new_empty(rows, qs, dtype=t.int8)
+        if qs != channels:
+            q = q.as_strided((rows, channels), (qs, 1))
+    else:
+        qs = _int8_row_stride(q, device, "q")
+        if q.shape != shape:
+            _refuse("q has to be of x's shape")
+    if scales is None:
+        scales = x.new_empty(rows, dtype=t.float32)
+        sp = scales.data_ptr()
+    else:
+        sp = _parameter(scales, device, rows, "scales")
+    rc = lib().exb_quantize_rows_fwd(ctx._h, _pack_rows(rows, channels, _DTYPES.get(x.dtype, -1), xs, qs), x.data_ptr(), q.data_ptr(), sp, _stream())
+    if rc:
+        check(rc)
+    return q, scales
+
+
+def int8_matmul(ctx, a, a_scales, w, w_scales, bias=None, out_dtype=EXB_F16, y=None):
+    """y (M, N) = a (M, K) @ w (N, K)^T (+ bias) of 8-bit integers, each row of a and each of w with its scale, as quantize_rows gives them."""
+    t = _TORCH or _torch()
+    device = ctx.device
+    ast = _int8_row_stride(a, device, "a")
+    wst = _int8_row_stride(w, device, "w")
+    M, K = a.shape
+    N, k = w.shape
+    if K != k:
+        _refuse("a and w have %d and %d columns", K, k)
+    if y is None:
+        y = a.new_empty(M, N, dtype=_DTYPES[out_dtype])
+        ys = N
+    else:
+        ys = _row_stride(y, device, "y")
+        if y.dtype is not _DTYPES[out_dtype] or y.shape != (M, N):
+            _refuse("y has to be (%d, %d) %s", M, N, _DTYPES[out_dtype])
+    rc = lib().exb_int8_matmul_fwd(ctx._h, _pack_int8(M, N, K, out_dtype, 0, ast, wst, ys), a.data_ptr(), _parameter(a_scales, device, M, "a_scales"),
+                                   w.data_ptr(), _parameter(w_scales, device, N, "w_scales"),
+                                   None if bias is None else _parameter(bias, device, N, "bias"), y.data_ptr(), _stream())
+    if rc:
+        check(rc)
+    return y
+
+
+def _expert_parameter(p, device, experts, n, what):
+    """Address of a float32 for each expert and channel."""
+    if p.dtype is not _TORCH.float32 or p.shape != (experts, n) or p.get_device() != device or not p.is_contiguous():
+        _refuse("%s has to be (%d, %d) float32, contiguous, on the context's device", what, experts, n)
+    return p.data_ptr()
+
+
+def grouped_matmul(ctx, a, w, ends, a_scales=None, w_scales=None, bias=None, out_dtype=None, y=None):
+    """Rows of a (M, K) that are sorted by expert, each times its expert's weights: y (M, N) = a[m] @ w[e]^T (+ bias[e]) for rows from ends[e - 1]
+    to before ends[e].  w: (experts, N, K); ends: (experts,) int32 on the device.  fp16 or bf16, or int8 with a_scales (M,) and w_scales
+    (experts, N).  bias: (experts, N) float32.  y is of a's type unless told otherwise (fp16 for int8); its rows from the last end on are left as they were."""
+    t = _TORCH or _torch()
+    device, dtype = ctx.device, a.dtype
+    dt = _DTYPES.get(dtype, -1)
+    whole = dt == EXB_I8
+    ast = _int8_row_stride(a, device, "a") if whole else _row_stride(a, device, "a")
+    if w.dim() != 3 or w.dtype is not dtype or w.get_device() != device:
+        _refuse("w has to be (experts, N, K) of a's type on the context's device")
+    M, K = a.shape
+    E, N, k = w.shape
+    if K != k:
+        _refuse("a and w have %d and %d columns", K, k)
+    if w.is_contiguous():
+        wst, est = K, N * K
+    else:
+        if K > 1 and w.stride(2) != 1:
+            _refuse("w has to be (experts, N, K), K innermost")
+        est, wst = w.stride(0), w.stride(1)
+    each = 16 // dtype.itemsize if dt in (EXB_I8, EXB_F16, EXB_BF16) else _refuse("a has to be int8, float16 or bfloat16")
+    if ast % each and M == 1:
+        ast = (ast + each - 1) // each * each
+    if N == 1:
+        wst = max(wst, K)
+        wst = (wst + each - 1) // each * each
+    if E == 1:
+        est = N * wst
+    if ast % each or wst % each or est % each:
+        _refuse("rows of a and w have to start at multiples of 16 bytes")
+    if ends.dtype is not t.int32 or ends.dim() != 1 or ends.shape[0] != E or ends.get_device() != device or not ends.is_contiguous():
+        _refuse("ends have to be %d int32 on the context's device", E)
+    sa = sw = b = None
+    if whole:
+        if a_scales is None or w_scales is None:
+            _refuse("8-bit integers have scales")
+        sa, sw = _parameter(a_scales, device, M, "a_scales"), _expert_parameter(w_scales, device, E, N, "w_scales")
+    elif a_scales is not None or w_scales is not None:
+        _refuse("%s has no scales", dtype)
+    if bias is not None:
+        b = _expert_parameter(bias, device, E, N, "bias")
+    if out_dtype is None:
+        out_dtype = EXB_F16 if whole else dt
+    if y is None:
+        y = a.new_empty(M, N, dtype=_DTYPES[out_dtype])
+        ys = N
+    else:
+        ys = _row_stride(y, device, "y")
+        if y.dtype is not _DTYPES[out_dtype] or y.shape != (M, N):
+            _refuse("y has to be (%d, %d) %s", M, N, _DTYPES[out_dtype])
+    rc = lib().exb_grouped_matmul_fwd(ctx._h, _pack_grouped(M, N, K, dt, out_dtype, E, 0, ast, wst, est, ys), a.data_ptr(), sa, w.data_ptr(), sw, ends.data_ptr(), b,
+                                      y.data_ptr(), _stream())
+    if rc:
+        check(rc)
+    return y

@@ -1,0 +1,708 @@
+// Matrix products whose sums stay in TMEM over all of K: 8-bit integers with a scale for each row of a and each row of w, and products grouped
+// by expert of 8-bit integers, fp16 or bf16:
+//   y[m][n] = a_scales[m] * w_scales[e][n] * sum_k a[m][k] * w[e][n][k]  (+ bias[e][n]),   ends[e - 1] <= m < ends[e]
+// (fp16 and bf16 without scales).  Sums of 8-bit integers are int32, exact; of fp16 and bf16 fp32.  An operand's rows are loaded in K blocks of
+// 128 bytes, alike for all types, so the kernels differ in the kind of their MMAs and in what becomes of a sum.
+#include "matmul_common.cuh"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace exb {
+namespace {
+
+using namespace product;
+
+enum Kind { kInt8, kHalf, kBfloat };
+
+struct ProductParams {
+    CUtensorMap tmA, tmW;      // a: {bytes of K, rows}; w: {bytes of K, rows, experts}
+    const float *a_scales, *w_scales, *bias;
+    const int32_t* ends;
+    void* y;
+    int64_t y_stride;
+    int M, N, blocks, experts, y_dtype, vec;      // experts 0: all rows are one's, and there are no ends
+    int n_tiles, splits;
+    uint32_t idesc;
+    int* error;
+};
+
+// ---- which rows are whose ------------------------------------------------------------------------
+// Where each expert's rows end, and its tiles (kRows rows by one of n_tiles).  Ends come from the device and nobody has looked at them: one
+// below those before it counts as theirs, one beyond the rows as their number, so that no row is two experts' and none is out of range.
+template <int kRows>
+__device__ __forceinline__ void list_experts(const ProductParams& p, int2* table, int lane) {
+    int end = 0, tiles = 0;
+    for (int e0 = 0; e0 < p.experts; e0 += 32) {
+        int v = e0 + lane < p.experts ? min(max(p.ends[e0 + lane], 0), p.M) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v = max(v, u);
+        }
+        v = max(v, end);
+        const int before = __shfl_up_sync(0xffffffffu, v, 1);
+        int t = (v - (lane ? before : end) + kRows - 1) / kRows * p.n_tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, t, o);
+            if (lane >= o) t += u;
+        }
+        t += tiles;
+        if (e0 + lane < p.experts) table[e0 + lane] = make_int2(v, t);
+        end = __shfl_sync(0xffffffffu, v, 31);
+        tiles = __shfl_sync(0xffffffffu, t, 31);
+    }
+}
+
+// An expert's rows, and the number of a tile among its tiles.
+struct Share {
+    int expert, begin, end, tile;
+};
+template <int kRows>
+__device__ __forceinline__ int all_tiles(const ProductParams& p, const int2* table) {
+    return p.experts ? table[p.experts - 1].y : (p.M + kRows - 1) / kRows * p.n_tiles;
+}
+__device__ __forceinline__ Share share_of(const ProductParams& p, const int2* table, int tile) {
+    if (!p.experts) return {0, 0, p.M, tile};
+    int lo = 0, hi = p.experts - 1;      // the first with more tiles up to its end than that
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (table[mid].y > tile) hi = mid;
+        else lo = mid + 1;
+    }
+    const int2 before = lo ? table[lo - 1] : make_int2(0, 0);
+    return {lo, before.x, table[lo].x, tile - before.y};
+}
+
+template <Kind kKind>
+__device__ __forceinline__ float sum_of(uint32_t raw) {
+    return kKind == kInt8 ? (float)(int)raw : __uint_as_float(raw);
+}
+
+// ---- few rows of a group -------------------------------------------------------------------------
+// Bound by the reading of w.  The roles of the operands are exchanged: w's rows are the MMA's 128 rows (lanes of TMEM), the rows of a its
+// kCols columns, so that a narrow product wastes no tensor work and a thread has one channel of all rows.  With enough tiles for all
+// SMs a CTA works on one after the other, the next one's loads under way while it stores (two accumulators in turn).  With fewer, the K blocks
+// of a tile are divided over a cluster of up to 8 CTAs, so that enough of them ask for w at the same time; every CTA then
+// finishes a share of the columns: the others send it their sums in one bulk copy each, counted by a barrier of its own.
+constexpr int few_stages(int cols) { return cols == 128 ? 4 : cols == 64 ? 3 : cols == 32 ? 4 : 5; }      // (two CTAs fit an SM up to 64 columns)
+constexpr int few_epi_warps(int cols) { return cols == 128 ? 16 : cols == 64 ? 8 : 4; }                   // up to 32 columns each
+constexpr int few_stage_bytes(int cols) { return (128 + cols) * kBlk; }
+// (columns that a CTA gets, of 16 by 7 CTAs: 3 from each of 6 others)
+constexpr int few_received(int cols) { return cols == 16 ? 18 : cols; }
+constexpr int few_smem(int cols) { return few_stages(cols) * few_stage_bytes(cols) + few_received(cols) * 512 + 1024; }
+
+template <Kind kKind, int kCols>
+__global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ? 1 : 2) product_few_kernel(const __grid_constant__ ProductParams p) {
+    constexpr int kStages = few_stages(kCols), kStageBytes = few_stage_bytes(kCols), kEpi = few_epi_warps(kCols);
+    constexpr int kMine = kCols * 4 / kEpi;      // columns of a warp
+    constexpr int kTmem = 2 * kCols;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages], tfull_bar[2], tempty_bar[2], recv_bar;
+    __shared__ uint32_t tmem_base_smem;
+    __shared__ int abort_flag;
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint32_t* part = reinterpret_cast<uint32_t*>(ring);                  // [column][128] behind the loop
+    uint32_t* recv = part + kStages * kStageBytes / 4;                   // [CTA, without this one][column of the share][128]
+    int2* table = reinterpret_cast<int2*>(recv + few_received(kCols) * 128);
+    const int warp = ptx::uniform_warp(), lane = threadIdx.x & 31;
+    const int rank = (int)blockIdx.x % p.splits, first = (int)blockIdx.x / p.splits, step = (int)gridDim.x / p.splits;
+    const int b0 = (int)((int64_t)rank * p.blocks / p.splits), nb = (int)((int64_t)(rank + 1) * p.blocks / p.splits) - b0;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < kStages; ++s) {
+            ptx::mbar_init(&full_bar[s], 2);
+            ptx::mbar_init(&empty_bar[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&tfull_bar[i], 1);
+            ptx::mbar_init(&tempty_bar[i], kEpi);
+        }
+        ptx::mbar_init(&recv_bar, 1);
+        ptx::fence_mbar_init();
+        ptx::tma_prefetch_desc(&p.tmA);
+        ptx::tma_prefetch_desc(&p.tmW);
+    }
+    __syncthreads();
+    if (p.splits > 1) ptx::cluster_arrive();      // every CTA runs and its barriers are initialised: waited for before the first part is sent
+    pdl_wait();
+    if (p.experts) {
+        if (warp == 0) list_experts<kCols>(p, table, lane);
+        __syncthreads();
+    }
+    // TMEM is taken when the previous kernel is done, and the next one may start when it is taken (see kTmemOrder).  The loads do not wait
+    // for it.
+    uint32_t tmem_base = 0;
+    if (warp != 0 && warp != 2) {
+        if (warp == 1) {
+            ptx::tmem_alloc(&tmem_base_smem, kTmem);
+            ptx::tmem_relinquish();
+            ptx::tc_fence_before_sync();
+        }
+        asm volatile("bar.sync 2, %0;" ::"n"(kEpi * 32 + 32) : "memory");
+        ptx::tc_fence_after_sync();
+        tmem_base = __shfl_sync(0xffffffffu, tmem_base_smem, 0);
+        pdl_launch_dependents();
+    }
+    const uint32_t ring0 = ptx::smem_u32(ring), full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
+    const uint32_t tfull0 = ptx::smem_u32(tfull_bar), tempty0 = ptx::smem_u32(tempty_bar);
+    const int total = all_tiles<kCols>(p, table);
+    bool ok = true;
+    auto tile_of = [&](int t, Share& s, int& m0, int& n0) {      // (an expert's tiles of the same rows of w follow one another)
+        s = share_of(p, table, t);
+        const int columns = (s.end - s.begin + kCols - 1) / kCols, n = s.tile / columns;
+        m0 = s.begin + (s.tile - n * columns) * kCols;
+        n0 = n * 128;
+    };
+    if (warp == 0 || warp == 2) {      // a loading warp for each operand
+        const bool is_w = warp == 0;
+        const uint32_t leader = ptx::elect_one() ? 1u : 0u;
+        int s = 0;
+        uint32_t phase = 1;      // (a fresh barrier's previous phase counts as complete)
+        for (int t = first; t < total && ok; t += step) {
+            Share of;
+            int m0, n0;
+            tile_of(t, of, m0, n0);
+            for (int b = 0; b < nb; ++b) {
+                if (!ptx::mbar_wait_quick_uniform(empty0 + s * 8, phase, &abort_flag, kMaxSpins)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t dst = ring0 + s * kStageBytes;
+                if (is_w) {
+                    ptx::mbar_arrive_expect_tx_u32(full0 + s * 8, 128 * kBlk, leader);
+                    ptx::tma_load_3d_u32(dst, reinterpret_cast<uint64_t>(&p.tmW), full0 + s * 8, (b0 + b) * kBlk, n0, of.expert, leader);
+                } else {
+                    ptx::mbar_arrive_expect_tx_u32(full0 + s * 8, kCols * kBlk, leader);
+                    ptx::tma_load_2d_u32(dst + 128 * kBlk, reinterpret_cast<uint64_t>(&p.tmA), full0 + s * 8, (b0 + b) * kBlk, m0, leader);
+                }
+                __syncwarp();      // (the elected lane may take a branch of its own; what follows is in registers of the whole warp)
+                if (++s == kStages) {
+                    s = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        if (!ok && lane == 0) ptx::give_up(p.error, 1);
+        __syncwarp();
+    } else if (warp == 1) {
+        const uint32_t leader = ptx::elect_one() ? 1u : 0u;
+        const uint64_t d0 = ptx::make_smem_desc(ring0, kBlk);
+        const uint32_t desc_hi = (uint32_t)(d0 >> 32);
+        int s = 0, buf = 0;
+        uint32_t phase = 0, acc_phase = 1;
+        for (int t = first; t < total && ok; t += step) {
+            if (!ptx::mbar_wait_quick_uniform(tempty0 + buf * 8, acc_phase, &abort_flag, kMaxSpins)) {
+                ok = false;
+                break;
+            }
+            ptx::tc_fence_after_sync();
+            for (int b = 0; b < nb; ++b) {
+                if (!ptx::mbar_wait_quick_uniform(full0 + s * 8, phase, &abort_flag, kMaxSpins)) {
+                    ok = false;
+                    break;
+                }
+                ptx::tc_fence_after_sync();
+                const uint32_t w_lo = (uint32_t)d0 + ((uint32_t)(s * kStageBytes) >> 4), a_lo = w_lo + ((128 * kBlk) >> 4);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                    ptx::tc_mma_lohi<kKind == kInt8>(tmem_base + buf * kCols, w_lo + 2 * ks, a_lo + 2 * ks, desc_hi, p.idesc, b | ks ? 1u : 0u, leader);
+                ptx::tc_commit_u32(empty0 + s * 8, leader);
+                __syncwarp();
+                if (++s == kStages) {
+                    s = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (!ok) break;
+            ptx::tc_commit_u32(tfull0 + buf * 8, leader);
+            __syncwarp();
+            if (++buf == 2) {
+                buf = 0;
+                acc_phase ^= 1u;
+            }
+        }
+        if (!ok) ptx::give_up(p.error, 2);
+        __syncwarp();
+    } else {
+        const int q = warp & 3, c0 = ((warp - 3) >> 2) * kMine;
+        int buf = 0;
+        uint32_t acc_phase = 0;
+        for (int t = first; t < total; t += step) {
+            Share of;
+            int m0, n0;
+            tile_of(t, of, m0, n0);
+            const int n = n0 + q * 32 + lane, rows = of.end - m0;
+            // (asked for before there is anything to scale) this channel's scale and bias, and each row's scale in a lane of its own
+            float ws = 1.f, as = 1.f, start = 0.f;
+            if (p.splits == 1) {
+                if (kKind == kInt8) {
+                    ws = n < p.N ? p.w_scales[(int64_t)of.expert * p.N + n] : 0.f;
+                    as = lane < kMine && c0 + lane < rows ? p.a_scales[m0 + c0 + lane] : 0.f;
+                }
+                if (p.bias && n < p.N) start = p.bias[(int64_t)of.expert * p.N + n];
+            }
+            if (!ptx::mbar_wait_quick_uniform(tfull0 + buf * 8, acc_phase, &abort_flag, kMaxSpins)) {
+                ok = false;
+                break;
+            }
+            __syncwarp();      // (what follows needs the warp together)
+            ptx::tc_fence_after_sync();
+            const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * kCols + c0);
+            uint32_t raw[kMine / 16][16];
+#pragma unroll
+            for (int c = 0; c < kMine; c += 16) ptx::tmem_ld_32x32b_x16(taddr + c, raw[c / 16]);
+#pragma unroll
+            for (int c = 0; c < kMine; c += 16) ptx::tmem_ld_wait(raw[c / 16]);
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_u32(tempty0 + buf * 8);
+            if (p.splits == 1) {
+#pragma unroll
+                for (int c = 0; c < kMine; ++c) {
+                    if (c0 + c >= rows) break;
+                    float v = sum_of<kKind>(raw[c / 16][c % 16]);
+                    v = kKind == kInt8 ? fmaf(v, __shfl_sync(0xffffffffu, as, c % 32) * ws, start) : v + start;
+                    if (n < p.N) store_one(p.y, p.y_dtype, (int64_t)(m0 + c0 + c) * p.y_stride + n, v);
+                }
+            } else {      // every MMA has read its operands: the sums take the ring's place
+#pragma unroll
+                for (int c = 0; c < kMine; ++c) part[(c0 + c) * 128 + q * 32 + lane] = raw[c / 16][c % 16];
+            }
+            if (++buf == 2) {
+                buf = 0;
+                acc_phase ^= 1u;
+            }
+        }
+        if (!ok && lane == 0) atomicExch(p.error, 3);
+    }
+    if (p.splits > 1) {      // (a cluster has one tile at most)
+        __syncwarp();
+        ptx::cluster_wait();
+        if (warp >= 3 && first < total) {
+            Share of;
+            int m0, n0;
+            tile_of(first, of, m0, n0);
+            // columns that this CTA finishes: [rank * share, rank * share + mine)
+            const int cols = min(kCols, of.end - m0), share = (cols + p.splits - 1) / p.splits, mine = max(min(share, cols - rank * share), 0);
+            const int et = (int)threadIdx.x - 96, row = (et & 31) * 4, n = n0 + row;      // a thread has four channels of a column
+            if (et == 0) ptx::mbar_arrive_expect_tx(&recv_bar, (uint32_t)(mine * (p.splits - 1) * 512));
+            if (ok) ptx::fence_proxy_async();
+            asm volatile("bar.sync 1, %0;" ::"n"(kEpi * 32) : "memory");      // (all of them, whatever their waits gave)
+            ok = ok && *static_cast<volatile int*>(&abort_flag) == 0;
+            // lane r of the first warp sends CTA r its columns
+            const int theirs = min(share, cols - lane * share);
+            if (ok && warp == 3 && lane < p.splits && lane != rank && theirs > 0)
+                ptx::copy_to_cta(ptx::map_to_cta(ptx::smem_u32(recv + (rank - (rank > lane)) * theirs * 128), (uint32_t)lane), ptx::smem_u32(part + lane * share * 128),
+                                 (uint32_t)(theirs * 512), ptx::map_to_cta(ptx::smem_u32(&recv_bar), (uint32_t)lane));
+            __syncwarp();
+            float ws[4] = {1.f, 1.f, 1.f, 1.f}, start[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n + j < p.N) {
+                    if (kKind == kInt8) ws[j] = p.w_scales[(int64_t)of.expert * p.N + n + j];
+                    if (p.bias) start[j] = p.bias[(int64_t)of.expert * p.N + n + j];
+                }
+            if (ok) ok = ptx::mbar_wait_quick_uniform(ptx::smem_u32(&recv_bar), 0, &abort_flag, kMaxSpins);
+            if (!ok && lane == 0) atomicExch(p.error, 3);
+            __syncwarp();
+            ptx::cluster_arrive();      // no CTA leaves while parts may still be on their way to it or from it
+            for (int c = et >> 5; ok && c < mine; c += kEpi) {
+                const int m = m0 + rank * share + c;
+                const float as = kKind == kInt8 ? p.a_scales[m] : 1.f;
+                const uint32_t* own = part + (rank * share + c) * 128 + row;
+                uint32_t sum[4];
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+                    if (s < p.splits) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(s == rank ? own : recv + ((s - (s > rank)) * mine + c) * 128 + row);
+                        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            sum[j] = !s ? u[j] : kKind == kInt8 ? sum[j] + u[j] : __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(u[j]));
+                    }
+                float v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = kKind == kInt8 ? fmaf(sum_of<kKind>(sum[j]), as * ws[j], start[j]) : sum_of<kKind>(sum[j]) + start[j];
+                store_four(p.y, p.y_dtype, p.y_stride, p.N, p.vec, m, n, v);
+            }
+        } else {
+            ptx::cluster_arrive();
+        }
+        __syncwarp();
+        ptx::cluster_wait();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc(tmem_base, kTmem);
+    }
+}
+
+// ---- CTA pairs ---------------------------------------------------------------------------------
+// Tiles of 256 rows of a by 256 or 128 of w by pairs of CTAs, persistent.  Each CTA keeps 128 rows of a and half of w's rows of a stage.  TMEM holds
+// two accumulators: the epilogue warps read one out, scale and store it while the MMAs fill the other.
+constexpr int kPairM = 256;
+constexpr int kPairEpiWarps = 8;                 // two per TMEM lane quarter, half of the accumulator's columns each
+constexpr int pair_stage_bytes(int n) { return (kPairM + n) / 2 * kBlk; }      // of one of the two CTAs
+constexpr int pair_stages(int n) { return n == 256 ? 5 : 7; }
+constexpr int pair_scale_bytes(int n) { return kPairEpiWarps * n * 4; }         // each warp's columns' scales and biases
+constexpr int pair_smem(int n) { return pair_stages(n) * pair_stage_bytes(n) + kPairEpiWarps * kStageOut + pair_scale_bytes(n) + 1024; }
+constexpr int kPairThreads = 128 + kPairEpiWarps * 32;
+
+template <Kind kKind, int kPairN>
+__global__ void __launch_bounds__(kPairThreads, 1) product_pair_kernel(const __grid_constant__ ProductParams p) {
+    constexpr int kStages = pair_stages(kPairN), kStageBytes = pair_stage_bytes(kPairN), kPairCols = kPairN / 2;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages], tfull_bar[2], tempty_bar[2];
+    __shared__ uint32_t tmem_base_smem;
+    __shared__ int abort_flag;
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* out = ring + kStages * kStageBytes;
+    float* scales = reinterpret_cast<float*>(out + kPairEpiWarps * kStageOut);
+    int2* table = reinterpret_cast<int2*>(scales + pair_scale_bytes(kPairN) / 4);
+    const int warp = ptx::uniform_warp(), lane = threadIdx.x & 31;
+    const int rank = (int)__shfl_sync(0xffffffffu, ptx::cluster_ctarank(), 0);
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < kStages; ++s) {
+            ptx::mbar_init(&full_bar[s], 2);
+            ptx::mbar_init(&empty_bar[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&tfull_bar[i], 1);
+            ptx::mbar_init(&tempty_bar[i], 2 * kPairEpiWarps);
+        }
+        ptx::fence_mbar_init();
+        ptx::tma_prefetch_desc(&p.tmA);
+        ptx::tma_prefetch_desc(&p.tmW);
+    }
+    pdl_wait();      // (before TMEM is taken: see kTmemOrder)
+    if (warp == 1) {
+        ptx::tmem_alloc_pair(&tmem_base_smem, 2 * kPairN);
+        ptx::tmem_relinquish_pair();
+    } else if (warp == 0 && p.experts) {
+        list_experts<kPairM>(p, table, lane);
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_sync();
+    ptx::tc_fence_after_sync();
+    pdl_launch_dependents();
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_smem, 0);
+    const uint32_t ring0 = ptx::smem_u32(ring), full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
+    const uint32_t tfull0 = ptx::smem_u32(tfull_bar), tempty0 = ptx::smem_u32(tempty_bar);
+    const int total = all_tiles<kPairM>(p, table);
+    auto tile_of = [&](int t, Share& s, int& m0, int& n0) {
+        s = share_of(p, table, t);
+        int m, n;
+        tile_at(s.tile, (s.end - s.begin + kPairM - 1) / kPairM, p.n_tiles, m, n);
+        m0 = s.begin + m * kPairM;
+        n0 = n * kPairN;
+    };
+    if (warp == 0 || warp == 2) {      // a loading warp for each operand
+        const bool is_w = warp == 2;
+        const uint32_t leader = ptx::elect_one() ? 1u : 0u, counts = rank == 0 ? leader : 0u;
+        const uint32_t full_lead = ptx::map_to_cta(full0, 0);
+        bool ok = true;
+        int s = 0;
+        uint32_t phase = 1;      // (a fresh barrier's previous phase counts as complete)
+        for (int t = first; t < total && ok; t += step) {
+            Share of;
+            int m0, n0;
+            tile_of(t, of, m0, n0);
+            for (int b = 0; b < p.blocks; ++b) {
+                if (!ptx::mbar_wait_quick_uniform(empty0 + s * 8, phase, &abort_flag, kMaxSpins)) {
+                    ok = false;
+                    break;
+                }
+                // (both CTAs' bytes are counted by rank 0)
+                const uint32_t dst = ring0 + s * kStageBytes;
+                if (is_w) {
+                    ptx::mbar_arrive_expect_tx_u32(full0 + s * 8, kPairN * kBlk, counts);
+                    ptx::tma_load_3d_pair(dst + 128 * kBlk, reinterpret_cast<uint64_t>(&p.tmW), full_lead + s * 8, b * kBlk, n0 + rank * (kPairN / 2), of.expert, leader);
+                } else {
+                    ptx::mbar_arrive_expect_tx_u32(full0 + s * 8, kPairM * kBlk, counts);
+                    ptx::tma_load_2d_pair(dst, reinterpret_cast<uint64_t>(&p.tmA), full_lead + s * 8, b * kBlk, m0 + rank * 128, leader);
+                }
+                __syncwarp();      // (see the other kernel's)
+                if (++s == kStages) {
+                    s = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        if (!ok && lane == 0) ptx::give_up(p.error, 1);
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0) {      // issues for both
+            const uint32_t leader = ptx::elect_one() ? 1u : 0u;
+            const uint64_t d0 = ptx::make_smem_desc(ring0, kBlk);
+            const uint32_t desc_hi = (uint32_t)(d0 >> 32);
+            bool ok = true;
+            int s = 0, buf = 0;
+            uint32_t phase = 0, acc_phase = 1;
+            for (int t = first; t < total && ok; t += step) {
+                if (!ptx::mbar_wait_quick_uniform(tempty0 + buf * 8, acc_phase, &abort_flag, kMaxSpins)) {
+                    ok = false;
+                    break;
+                }
+                ptx::tc_fence_after_sync();
+                for (int b = 0; b < p.blocks; ++b) {
+                    if (!ptx::mbar_wait_quick_uniform(full0 + s * 8, phase, &abort_flag, kMaxSpins)) {
+                        ok = false;
+                        break;
+                    }
+                    ptx::tc_fence_after_sync();
+                    const uint32_t a_lo = (uint32_t)d0 + ((uint32_t)(s * kStageBytes) >> 4), w_lo = a_lo + ((128 * kBlk) >> 4);
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+                        ptx::tc_mma_lohi_pair<kKind == kInt8>(tmem_base + buf * kPairN, a_lo + 2 * ks, w_lo + 2 * ks, desc_hi, p.idesc, b | ks ? 1u : 0u, leader);
+                    ptx::tc_commit_pair_u32(empty0 + s * 8, leader);
+                    __syncwarp();
+                    if (++s == kStages) {
+                        s = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                ptx::tc_commit_pair_u32(tfull0 + buf * 8, leader);
+                __syncwarp();
+                if (++buf == 2) {
+                    buf = 0;
+                    acc_phase ^= 1u;
+                }
+            }
+            if (!ok) ptx::give_up(p.error, 2);
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        const int q = warp & 3, half = (warp >> 2) - 1;
+        uint8_t* stage = out + (warp - 4) * kStageOut;
+        float* my_scales = scales + (warp - 4) * kPairN;      // kPairCols scales, kPairCols biases
+        const uint32_t taddr0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * kPairCols);
+        const uint32_t tempty_lead = ptx::map_to_cta(tempty0, 0);
+        bool ok = true;
+        int buf = 0;
+        uint32_t acc_phase = 0;
+        for (int t = first; t < total && ok; t += step) {
+            Share of;
+            int m0, n0;
+            tile_of(t, of, m0, n0);
+            const int row0 = m0 + rank * 128 + q * 32, col = n0 + half * kPairCols;
+            __syncwarp();
+#pragma unroll
+            for (int c = lane; c < kPairCols; c += 32) {
+                const bool is = col + c < p.N;
+                my_scales[c] = kKind == kInt8 && is ? p.w_scales[(int64_t)of.expert * p.N + col + c] : 0.f;
+                my_scales[kPairCols + c] = p.bias && is ? p.bias[(int64_t)of.expert * p.N + col + c] : 0.f;
+            }
+            const float as = kKind == kInt8 && row0 + lane < of.end ? p.a_scales[row0 + lane] : 0.f;
+            __syncwarp();
+            if (!ptx::mbar_wait_bounded_uniform(tfull0 + buf * 8, acc_phase, &abort_flag, kMaxSpins)) {
+                ok = false;
+                break;
+            }
+            __syncwarp();      // (what follows needs the warp together)
+            ptx::tc_fence_after_sync();
+            const uint32_t taddr = taddr0 + (uint32_t)(buf * kPairN);
+            constexpr int kPass = 64;      // columns at a time
+#pragma unroll 1
+            for (int c = 0; c < kPairCols; c += kPass) {
+                float2 acc[kPass / 2];
+                uint32_t raw[kPass / 16][16];
+#pragma unroll
+                for (int i = 0; i < kPass; i += 16) ptx::tmem_ld_32x32b_x16(taddr + c + i, raw[i / 16]);
+#pragma unroll
+                for (int i = 0; i < kPass; i += 16) ptx::tmem_ld_wait(raw[i / 16]);
+                if (c + kPass == kPairCols) {
+                    ptx::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive_cluster_u32(tempty_lead + buf * 8);
+                }
+#pragma unroll
+                for (int i = 0; i < kPass; i += 2) {
+                    const float2 b = *reinterpret_cast<const float2*>(my_scales + kPairCols + c + i);
+                    const float u = sum_of<kKind>(raw[i / 16][i % 16]), v = sum_of<kKind>(raw[i / 16][i % 16 + 1]);
+                    if (kKind == kInt8) {
+                        const float2 ws = *reinterpret_cast<const float2*>(my_scales + c + i);
+                        acc[i / 2] = make_float2(fmaf(u, as * ws.x, b.x), fmaf(v, as * ws.y, b.y));
+                    } else {
+                        acc[i / 2] = make_float2(u + b.x, v + b.y);
+                    }
+                }
+                if (p.y_dtype == EXB_F16) store_rows(acc, stage, static_cast<__half*>(p.y), p.y_stride, row0, col + c, of.end, p.N, p.vec, lane);
+                else if (p.y_dtype == EXB_BF16) store_rows(acc, stage, static_cast<__nv_bfloat16*>(p.y), p.y_stride, row0, col + c, of.end, p.N, p.vec, lane);
+                else store_rows(acc, stage, static_cast<float*>(p.y), p.y_stride, row0, col + c, of.end, p.N, p.vec, lane);
+            }
+            if (++buf == 2) {
+                buf = 0;
+                acc_phase ^= 1u;
+            }
+        }
+        if (!ok && lane == 0) atomicExch(p.error, 3);
+    }
+    __syncwarp();
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_sync();      // neither CTA leaves while its peer may still signal its barriers or read its TMEM
+    if (warp == 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc_pair(tmem_base, 2 * kPairN);
+    }
+}
+
+// Which kernel and how it divides the product.
+struct Plan {
+    bool few;
+    int tile, splits;      // rows of a (few) or of w (pairs) in a tile
+};
+Plan plan_for(int sms, int M, int N, int blocks, int experts) {
+    const int64_t n_tiles = ((int64_t)N + 127) / 128;
+    const int groups = std::max(1, std::min(experts, M));
+    const int each = (M + groups - 1) / groups;
+    auto tiles = [&](int rows) { return std::min<int64_t>(M, ((int64_t)M + (int64_t)groups * (rows - 1)) / rows) * n_tiles; };      // at most
+    auto parts = [&](int64_t t, bool two) {
+        auto within = [&](int64_t places) { return std::max<int64_t>(1, std::min<int64_t>({8, places / t, blocks / 2})); };
+        const int64_t s = within(sms * 9 / 10);
+        return (int)(two && t * s * 5 < sms * 4 ? within(sms * 33 / 20) : s);
+    };
+    const int rows = experts ? 2 * each : M;
+    if (rows <= 64) {
+        const int cols = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+        return {true, cols, parts(tiles(cols), true)};
+    }
+    if (rows <= 128) return {true, 128, parts(tiles(128), false)};
+    auto rounds = [](int64_t t, int64_t places) { return (double)((t + places - 1) / places); };
+    const int64_t m_pairs = ((int64_t)M + (int64_t)groups * (kPairM / 2)) / kPairM;
+    const double pair128 = 5.0 + 0.17 * rounds(m_pairs * n_tiles, sms / 2) * blocks;
+    const double pair256 = 5.0 + 0.28 * rounds(m_pairs * (((int64_t)N + 255) / 256), sms / 2) * blocks;
+    return {false, pair128 < pair256 ? 128 : 256, 1};
+}
+
+// Rows of `bytes` of each expert in boxes of 128 bytes x box_rows, 128-byte swizzle; zeros beyond the matrix.
+int encode_experts(const char* what, CUtensorMap* map, const void* base, int64_t rows, int64_t bytes, int64_t stride, int64_t experts, int64_t expert_stride,
+                   int box_rows) {
+    const auto fn = tensor_map_encoder();
+    if (!fn) return fail(EXB_ERR_CUDA, "%s: the driver has no cuTensorMapEncodeTiled", what);
+    cuuint64_t dims[3] = {(cuuint64_t)bytes, (cuuint64_t)rows, (cuuint64_t)experts}, strides[2] = {(cuuint64_t)stride, (cuuint64_t)expert_stride};
+    cuuint32_t box[3] = {(cuuint32_t)kBlk, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(EXB_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
+    return EXB_OK;
+}
+
+template <Kind kKind>
+int run(exb_ctx* ctx, const char* what, ProductParams& p, const Plan& plan, const void* a, int64_t a_bytes, const void* w, int64_t K_bytes, int64_t w_bytes,
+        int64_t expert_bytes, cudaStream_t st) {
+    const int64_t M = p.M, experts = std::max(p.experts, 1), groups = std::min<int64_t>(experts, M);
+    const size_t table = p.experts ? (size_t)p.experts * sizeof(int2) : 0;
+    const int box_a = plan.few ? plan.tile : 128, box_w = plan.few ? 128 : plan.tile / 2;
+    if (int rc = encode_rows(what, &p.tmA, static_cast<const uint8_t*>(a), M, (int)K_bytes, a_bytes, box_a)) return rc;
+    if (int rc = encode_experts(what, &p.tmW, w, p.N, K_bytes, w_bytes, experts, expert_bytes, box_w)) return rc;
+    const int rows = plan.few ? plan.tile : kPairM, width = plan.few ? 128 : plan.tile;
+    p.n_tiles = (p.N + width - 1) / width;
+    p.splits = plan.splits;
+    const int64_t tiles = std::min<int64_t>(M, (M + groups * (rows - 1)) / rows) * p.n_tiles;      // at most
+    if (tiles > INT32_MAX / 16) return fail(EXB_ERR_UNSUPPORTED, "%s: %lld x %d is too large for one call", what, (long long)M, p.N);
+    p.idesc = ptx::make_idesc(kKind == kInt8, plan.few ? 128 : kPairM, (uint32_t)plan.tile) | (kKind == kBfloat ? 1u << 7 | 1u << 10 : 0u);
+    if (plan.few) {
+        auto go = [&](auto c) {
+            constexpr int kCols = decltype(c)::value;
+            if (int rc = raise_smem_limit(ctx, product_few_kernel<kKind, kCols>)) return rc;
+            const int64_t places = (int64_t)ctx->sm_count * (kCols == 128 ? 1 : 2);
+            const int64_t grid = plan.splits > 1 ? tiles * plan.splits : std::min(tiles, places);
+            return launch_pdl_cluster(ctx, "product_few_kernel", product_few_kernel<kKind, kCols>, dim3((unsigned)grid), dim3(96 + few_epi_warps(kCols) * 32),
+                                      dim3(plan.splits), (size_t)few_smem(kCols) + table, st, p);
+        };
+        if (plan.tile == 16) return go(std::integral_constant<int, 16>());
+        if (plan.tile == 32) return go(std::integral_constant<int, 32>());
+        if (plan.tile == 64) return go(std::integral_constant<int, 64>());
+        return go(std::integral_constant<int, 128>());
+    }
+    const int64_t places = ctx->sm_count / 2;
+    auto go = [&](auto c) {
+        constexpr int kN = decltype(c)::value;
+        if (int rc = raise_smem_limit(ctx, product_pair_kernel<kKind, kN>)) return rc;
+        return launch_pdl_cluster(ctx, "product_pair_kernel", product_pair_kernel<kKind, kN>, dim3((unsigned)(2 * std::min(tiles, places))), dim3(kPairThreads), dim3(2),
+                                  (size_t)pair_smem(kN) + table, st, p);
+    };
+    return plan.tile == 256 ? go(std::integral_constant<int, 256>()) : go(std::integral_constant<int, 128>());
+}
+
+constexpr int kMostExperts = 1024;
+constexpr int kMostExactK = 131071;      // times 128^2: the largest sum of products below 2^31
+
+int product_fwd(exb_ctx* ctx, const char* what, const exb_grouped_desc& d, bool grouped, const void* a, const float* a_scales, const void* w,
+                const float* w_scales, const int32_t* ends, const float* bias, void* y, void* stream) {
+    const int64_t M = d.M;
+    const int N = d.N, K = d.K, experts = grouped ? d.experts : 1;
+    const size_t es = d.dtype == EXB_I8 ? 1 : d.dtype == EXB_F16 || d.dtype == EXB_BF16 ? 2 : 0, ys = rows::element_size(d.y_dtype);
+    EXB_REQUIRE(es != 0, "%s: a and w must be EXB_I8, EXB_F16 or EXB_BF16, got %d", what, d.dtype);
+    EXB_REQUIRE(ys != 0, "%s: y must be EXB_F16, EXB_BF16 or EXB_F32, got %d", what, d.y_dtype);
+    EXB_REQUIRE(M >= 0 && N >= 1 && K >= 1, "%s: bad shape (%lld x %d x %d)", what, (long long)M, N, K);
+    EXB_REQUIRE(experts >= 1, "%s: %d experts", what, experts);
+    if (experts > kMostExperts) return fail(EXB_ERR_UNSUPPORTED, "%s: at most %d experts, got %d", what, kMostExperts, experts);
+    if (es == 1 && K > kMostExactK) return fail(EXB_ERR_UNSUPPORTED, "%s: int32 sums of 8-bit products hold K up to %d, got %d", what, kMostExactK, K);
+    if (M > INT32_MAX - 256 || N > INT32_MAX - 256 || K > INT32_MAX / 2 - 256)
+        return fail(EXB_ERR_UNSUPPORTED, "%s: %lld x %d x %d is too large for one call", what, (long long)M, N, K);
+    if (M == 0) return EXB_OK;
+    EXB_REQUIRE(a && w && y && (!grouped || ends), "%s: null buffer", what);
+    EXB_REQUIRE((a_scales != nullptr) == (es == 1) && (w_scales != nullptr) == (es == 1), "%s: 8-bit integers have scales, other types none", what);
+    EXB_REQUIRE(d.a_stride >= K && d.w_stride >= K && d.y_stride >= N, "%s: row strides smaller than the rows", what);
+    const int64_t a_bytes = d.a_stride * (int64_t)es, w_bytes = d.w_stride * (int64_t)es;
+    const int64_t expert_stride = experts > 1 ? d.expert_stride : (int64_t)N * d.w_stride, expert_bytes = expert_stride * (int64_t)es;
+    EXB_REQUIRE(experts == 1 || expert_stride >= (N - 1) * d.w_stride + K, "%s: expert stride smaller than an expert", what);
+    EXB_REQUIRE(aligned16(a) && aligned16(w) && a_bytes % 16 == 0 && w_bytes % 16 == 0 && expert_bytes % 16 == 0,
+                "%s: the rows of a and w must start at multiples of 16 bytes", what);
+    if (a_bytes >= 1ll << 40 || w_bytes >= 1ll << 40 || expert_bytes >= 1ll << 40) return fail(EXB_ERR_UNSUPPORTED, "%s: strides of 2^40 bytes or more", what);
+    EXB_REQUIRE(rows::aligned_to(y, ys), "%s: y not aligned to its element", what);
+    for (const void* q : {static_cast<const void*>(a_scales), static_cast<const void*>(w_scales), static_cast<const void*>(bias), static_cast<const void*>(ends)})
+        EXB_REQUIRE(rows::aligned_to(q, 4), "%s: scales, bias or ends not aligned to their element", what);
+    const int64_t w_span = (experts - 1) * expert_stride + (N - 1) * d.w_stride + K;      // (between its rows y may not lie either)
+    const rows::Place in[] = {rows::place_of(a, M, K, d.a_stride, es),
+                              experts == 1 ? rows::place_of(w, N, K, d.w_stride, es) : rows::place_of(w, 1, w_span, w_span, es),
+                              rows::place_of(a_scales, 1, M, M, 4),
+                              rows::place_of(w_scales, 1, (int64_t)experts * N, (int64_t)experts * N, 4),
+                              rows::place_of(bias, 1, (int64_t)experts * N, (int64_t)experts * N, 4),
+                              rows::place_of(grouped ? ends : nullptr, 1, experts, experts, 4)};
+    const rows::Place out[] = {rows::place_of(y, M, N, d.y_stride, ys)};
+    EXB_REQUIRE(!rows::results_overlap(out, in), "%s: y lies over an input", what);
+    if (int rc = rows::check_device(ctx, what)) return rc;
+    ProductParams p;
+    p.a_scales = a_scales; p.w_scales = w_scales; p.bias = bias; p.ends = ends; p.y = y; p.y_stride = d.y_stride;
+    p.M = (int)M; p.N = N; p.experts = grouped ? experts : 0; p.y_dtype = d.y_dtype;
+    p.blocks = (int)(((int64_t)K * (int64_t)es + kBlk - 1) / kBlk);
+    p.vec = rows::vector_rows(y, d.y_stride, ys);
+    p.error = ctx->d_error;
+    const Plan plan = plan_for(ctx->sm_count, p.M, N, p.blocks, p.experts);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int64_t K_bytes = (int64_t)K * (int64_t)es;
+    if (d.dtype == EXB_I8) return run<kInt8>(ctx, what, p, plan, a, a_bytes, w, K_bytes, w_bytes, expert_bytes, st);
+    if (d.dtype == EXB_F16) return run<kHalf>(ctx, what, p, plan, a, a_bytes, w, K_bytes, w_bytes, expert_bytes, st);
+    return run<kBfloat>(ctx, what, p, plan, a, a_bytes, w, K_bytes, w_bytes, expert_bytes, st);
+}
+
+}  // namespace
+}  // namespace exb
+
+using namespace exb;
+
+extern "C" int exb_int8_matmul_fwd(exb_ctx* ctx, const exb_int8_desc* d, const int8_t* a, const float* a_scales, const int8_t* w, const float* w_scales,
+                                   const float* bias, void* y, void* stream) {
+    EXB_REQUIRE(ctx != nullptr && d != nullptr, "exb_int8_matmul_fwd: null context or descriptor");
+    exb_grouped_desc g = {};
+    g.M = d->M; g.N = d->N; g.K = d->K; g.dtype = EXB_I8; g.y_dtype = d->y_dtype; g.experts = 1;
+    g.a_stride = d->a_stride; g.w_stride = d->w_stride; g.y_stride = d->y_stride;
+    return product_fwd(ctx, "exb_int8_matmul_fwd", g, false, a, a_scales, w, w_scales, nullptr, bias, y, stream);
+}
+
+extern "C" int exb_grouped_matmul_fwd(exb_ctx* ctx, const exb_grouped_desc* d, const void* a, const float* a_scales, const void* w, const float* w_scales,
+                                      const int32_t* ends, const float* bias, void* y, void* stream) {
+    EXB_REQUIRE(ctx != nullptr && d != nullptr, "exb_grouped_matmul_fwd: null context or descriptor");
+    return product_fwd(ctx, "exb_grouped_matmul_fwd", *d, true, a, a_scales, w, w_scales, ends, bias, y, stream);
+}

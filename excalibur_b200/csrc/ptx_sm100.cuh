@@ -304,6 +304,20 @@ __device__ __forceinline__ void tma_load_2d_u32(uint32_t dst, uint64_t map, uint
         " [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(leader)
         : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_u32(uint32_t dst, uint64_t map, uint32_t bar, int c0, int c1, int c2, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, uint64_t map, uint32_t bar, int c0, int c1, int c2, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(leader)
+        : "memory");
+}
 __device__ __forceinline__ void mbar_arrive_expect_tx_u32(uint32_t bar, uint32_t bytes, uint32_t leader) {
     asm volatile(
         "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"

@@ -563,6 +563,59 @@ EXB_API int exb_token_logprobs_fwd(exb_ctx* ctx, const exb_logprobs_desc* d, con
                                    float* logprobs, float* entropy, float* top_logprobs, int32_t* top_tokens,
                                    void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Decoding in 8-bit integers, by experts and with beams: operators beside those above, under the same rules (types, strides, alignment, empty calls,
+ * results over inputs, devices).
+ *
+ * exb_quantize_rows_fwd: 8-bit integers with a scale for each row (a token of activations, an output channel of weights):
+ *   scale = max(max |x| / 127, 2^-126), q = the whole number nearest to x * (1 / scale), ties to the even one
+ * (scale and 1 / scale are rounded to fp32, the product is not), so that q * scale stands for x and q is -127 to 127.  A row with a
+ * NaN or an infinity has the scale NaN and q of 0: every product with it is NaN.
+ * q: [rows][C] with q_stride >= C, a multiple of 16, and a 16-byte aligned base, as exb_int8_matmul_fwd takes it (bytes between C and
+ * q_stride are left alone).  scales: fp32 [rows].
+ * ------------------------------------------------------------------------------------- */
+typedef struct exb_rows_desc {
+    int64_t rows;
+    int32_t C;
+    int32_t in_dtype;       /* of x */
+    int64_t x_stride, q_stride;
+} exb_rows_desc;
+EXB_API int exb_quantize_rows_fwd(exb_ctx* ctx, const exb_rows_desc* d, const void* x, int8_t* q, float* scales, void* stream);
+
+/* Matrix product of what exb_quantize_rows_fwd writes:
+ *   y[m][n] = (a_scales[m] * w_scales[n]) * sum_k a[m][k] * w[n][k]  (+ bias[n])
+ * a: [M][K], w: [N][K], 8-bit integers (-128 to 127), 16-byte aligned, strides multiples of 16 and >= K (what lies between K and the stride is not
+ * read); a_scales: fp32 [M], w_scales: fp32 [N]; bias: fp32 [N] or NULL; y: [M][N] in EXB_F16, EXB_BF16 or EXB_F32.  The sum is
+ * an int32, exact (K up to 131071); it and the product of the scales are rounded to fp32 before they are multiplied. */
+typedef struct exb_int8_desc {
+    int64_t M;
+    int32_t N, K;
+    int32_t y_dtype;
+    int32_t reserved;       /* 0 */
+    int64_t a_stride, w_stride, y_stride;
+} exb_int8_desc;
+EXB_API int exb_int8_matmul_fwd(exb_ctx* ctx, const exb_int8_desc* d, const int8_t* a, const float* a_scales, const int8_t* w,
+                                const float* w_scales, const float* bias, void* y, void* stream);
+
+/* Products grouped by expert: a's rows are sorted by expert, expert e's end before row ends[e] (int32 [experts], on the device):
+ *   y[m][n] = sum_k a[m][k] * w[e][n][k]  (+ bias[e][n]),   ends[e - 1] <= m < ends[e]  (ends[-1] = 0)
+ * in dtype EXB_F16 or EXB_BF16 (fp32 sums, no scales: NULL), or EXB_I8 with a_scales [M] and w_scales [experts][N] as exb_int8_matmul_fwd.
+ * a: [M][K], w: [experts][N][K], rows and experts (expert_stride elements apart) 16-byte aligned; bias: fp32 [experts][N] or NULL; y: [M][N] in y_dtype.
+ * Experts may be without rows; their weights are not read.  Rows of y from the last end on are left as they were.  ends should not fall and
+ * not exceed M: one below those before it counts as theirs, one above M as M.  Up to 1024 experts.  With several experts
+ * y may not lie between the rows of w either. */
+typedef struct exb_grouped_desc {
+    int64_t M;
+    int32_t N, K;
+    int32_t dtype;          /* of a and w */
+    int32_t y_dtype;
+    int32_t experts;
+    int32_t reserved;       /* 0 */
+    int64_t a_stride, w_stride, expert_stride, y_stride;      /* in elements */
+} exb_grouped_desc;
+EXB_API int exb_grouped_matmul_fwd(exb_ctx* ctx, const exb_grouped_desc* d, const void* a, const float* a_scales, const void* w,
+                                   const float* w_scales, const int32_t* ends, const float* bias, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
