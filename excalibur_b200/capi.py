@@ -27,7 +27,7 @@ EXPORTED_SYMBOLS = [
     "exb_dequantize_fwd", "exb_concat_fwd", "exb_concat_nearest_fwd", "exb_interp_nearest_fwd", "exb_channel_affine_fwd",
     "exb_conv_weights_set_slopes", "exb_dw_weights_set_slopes", "exb_depth_to_space_nchw_f32", "exb_deconv_few_f32", "exb_image_f32_to_nhwc_norm", "exb_nchw_f32_to_nhwc4_padded_norm", "exb_nhwc_f16_split_heads_f32", "exb_hardsigmoid_fwd", "exb_softmax_channels_f32", "exb_binaryop_channel_bcast_fwd", "exb_nchw_f16_to_nhwc4_padded", "exb_nchw_f32_focus_to_nhwc_f16", "exb_channel_affine_prelu_fwd", "exb_hardswish_fwd", "exb_focus_fwd", "exb_prelu_fwd", "exb_depth_to_space_fwd", "exb_transpose_hw_f32",
     "exb_quantize_blocks_fwd", "exb_fp8_matmul_fwd", "exb_residual_norm_fwd", "exb_token_logprobs_fwd",
-    "exb_quantize_rows_fwd", "exb_int8_matmul_fwd", "exb_grouped_matmul_fwd",
+    "exb_quantize_rows_fwd", "exb_int8_matmul_fwd", "exb_grouped_matmul_fwd", "exb_beam_select_fwd", "exb_reorder_beams_fwd",
 ]
 
 
@@ -88,6 +88,16 @@ class GroupedDesc(C.Structure):
         [(n, C.c_int64) for n in ("a_stride", "w_stride", "expert_stride", "y_stride")]
 
 
+class BeamDesc(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("sentences", "stride", "workspace_bytes")] + \
+        [(n, C.c_int32) for n in ("beams", "V", "dtype", "select", "end_token")] + [("scale", C.c_float)]
+
+
+class ReorderDesc(C.Structure):
+    _fields_ = [("sentences", C.c_int64)] + [(n, C.c_int32) for n in ("beams", "n_states")] + \
+        [(n, C.c_int64) for n in ("outer", "positions", "bytes", "row_stride", "outer_stride", "position_stride")]
+
+
 # The same layouts as bytes: packing costs 0.2 us, a ctypes structure 0.8, and an argument of its own 0.1 each.
 _pack_norm = struct.Struct("@q4i2f7q").pack
 _pack_blocks = struct.Struct("@q4i3q").pack
@@ -96,6 +106,8 @@ _pack_logprobs = struct.Struct("@2q4ifi").pack
 _pack_rows = struct.Struct("@q2i2q").pack
 _pack_int8 = struct.Struct("@q4i3q").pack
 _pack_grouped = struct.Struct("@q6i4q").pack
+_pack_beams = struct.Struct("@3q5if").pack
+_pack_reorder = struct.Struct("@q2i6q").pack
 
 
 class ExbError(RuntimeError):
@@ -177,6 +189,8 @@ def lib():
         L.exb_quantize_rows_fwd.argtypes = [vp] * 6
         L.exb_int8_matmul_fwd.argtypes = [vp] * 9
         L.exb_grouped_matmul_fwd.argtypes = [vp] * 10
+        L.exb_beam_select_fwd.argtypes = [vp] * 10
+        L.exb_reorder_beams_fwd.argtypes = [vp] * 6
         _LIB = L
     return _LIB
 
@@ -1060,3 +1074,115 @@ def grouped_matmul(ctx, a, w, ends, a_scales=None, w_scales=None, bias=None, out
     if rc:
         check(rc)
     return y
+
+
+def beam_select(ctx, logits, scores, select=None, scale=1.0, ended=None, end_token=0):
+    """(scores, parents, tokens), each (sentences, select): the best continuations of every sentence over its beams and the vocabulary.  logits:
+    (sentences * beams, V); scores: (sentences, beams) float32, minus infinity where there is no beam; ended: None or (sentences, beams) bool,
+    beams that go on with end_token alone, at their score.  select: as many as there are beams unless told otherwise, up to 32.  Where fewer are left,
+    scores are minus infinity, parents and tokens -1."""
+    t = _TORCH or _torch()
+    device, f32 = ctx.device, t.float32
+    if scores.dtype is not f32 or scores.dim() != 2 or scores.get_device() != device or not scores.is_contiguous():
+        _refuse("scores have to be (sentences, beams) float32, contiguous, on the context's device")
+    sentences, beams = scores.shape
+    shape = logits.shape
+    ls = shape[-1] if logits.is_contiguous() and logits.get_device() == device and len(shape) == 2 else _row_stride(logits, device, "logits")
+    rows, V = shape
+    if rows != sentences * beams:
+        _refuse("%d rows of logits for %d x %d beams", rows, sentences, beams)
+    ended_p = None
+    if ended is not None:
+        if ended.dtype not in (t.bool, t.uint8) or ended.shape != scores.shape or ended.get_device() != device or not ended.is_contiguous():
+            _refuse("ended has to be (%d, %d) bool, contiguous, on the context's device", sentences, beams)
+        ended_p = ended.data_ptr()
+    if select is None:
+        select = beams
+    out = scores.new_empty(sentences, max(select, 0))
+    parents = t.empty_like(out, dtype=t.int32)
+    tokens = t.empty_like(parents)
+    room = 8 * rows * (1 + min(max(select, 0), V))
+    workspace = scores.new_empty(room, dtype=t.uint8)
+    rc = lib().exb_beam_select_fwd(ctx._h, _pack_beams(sentences, ls, room, beams, V, _DTYPES.get(logits.dtype, -1), select, end_token, scale), logits.data_ptr(),
+                                   scores.data_ptr(), ended_p, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), workspace.data_ptr(), _stream())
+    if rc:
+        check(rc)
+    return out, parents, tokens
+
+
+def _state_layout(state, rows, by_length):
+    """(outer, positions, bytes, row stride, outer stride, position stride) of a state, strides in bytes; positions are its last dimension but one."""
+    es = state.element_size()
+    if state.dim() < (3 if by_length else 1) or state.shape[0] != rows:
+        _refuse("a state has to be (%d%s)", rows, ", ..., positions, channels" if by_length else ", ...")
+    dims = [(n, s * es) for n, s in zip(state.shape[1:], state.stride()[1:])]
+
+    def joined(dims):
+        out = []
+        for n, s in dims:
+            if n == 1:
+                continue
+            if out and out[-1][1] == n * s:
+                out[-1] = (out[-1][0] * n, s)
+            else:
+                out.append((n, s))
+        return out
+    at = [dims[:-2], [dims[-2]], [dims[-1]]] if by_length else [joined(dims)[:-2], joined(dims)[-2:-1], joined(dims)[-1:]]
+    outer, positions, inner = (joined(d) for d in at)
+    if inner and inner[0][1] != es:      # nothing lies side by side
+        if by_length or positions and outer:
+            _refuse("a state's channels have to be innermost")
+        outer, positions, inner = positions, inner, []
+    if len(outer) > 1:
+        _refuse("a state's dimensions between rows and positions have to lie behind one another")
+    (o, os_), (p, ps) = outer[0] if outer else (1, 0), positions[0] if positions else (1, 0)
+    if 0 in state.shape:
+        o = 0
+    size = extent = inner[0][0] * es if inner else es
+    for step, n in sorted(((state.stride(0) * es, rows), (os_, o), (ps, p))):
+        if n > 1:
+            if step < extent:
+                _refuse("some of a state's rows lie over others")
+            extent += (n - 1) * step
+    return o, p, size, state.stride(0) * es, os_, ps
+
+
+def reorder_beams(ctx, states, parents, lengths=None):
+    """Rows sentence * beams + j of each state become what rows sentence * beams + parents[sentence, j] were, in place.  states: a tensor or a list of
+    them, (sentences * beams, ...) of any type; parents: (sentences, beams) int32, -1 for rows that stay; lengths: None, or (sentences,) int32: of states
+    (sentences * beams, ..., positions, channels) only positions below the sentence's length change."""
+    t = _TORCH or _torch()
+    device, i32 = ctx.device, t.int32
+    if parents.dtype is not i32 or parents.dim() != 2 or parents.get_device() != device or not parents.is_contiguous():
+        _refuse("parents have to be (sentences, beams) int32, contiguous, on the context's device")
+    sentences, beams = parents.shape
+    lengths_p = None
+    if lengths is not None:
+        if lengths.dtype is not i32 or lengths.shape != (sentences,) or lengths.get_device() != device or not lengths.is_contiguous():
+            _refuse("lengths have to be (%d,) int32 on the context's device", sentences)
+        lengths_p = lengths.data_ptr()
+    if isinstance(states, t.Tensor):
+        states = (states,)
+    calls, pointers = [], []
+    like = states[0] if len(states) else None
+    if like is not None and like.is_contiguous():      # the usual states: all alike, told apart by a few looks each
+        shape, dtype = like.shape, like.dtype
+        pointers = [s.data_ptr() for s in states if s.shape == shape and s.dtype is dtype and s.is_contiguous() and s.get_device() == device]
+    if len(pointers) == len(states) and like is not None:
+        calls.append((like, pointers))
+    else:
+        same = {}      # states of one layout are moved together
+        for s in states:
+            if s.get_device() != device:
+                _refuse("a state is not on the context's device")
+            same.setdefault((s.shape, s.stride(), s.element_size()), []).append(s)
+        calls = [(group[0], [s.data_ptr() for s in group]) for group in same.values()]
+        spans = sorted((s.data_ptr(), s.data_ptr() + s.element_size() * (1 + sum((n - 1) * k for n, k in zip(s.shape, s.stride())))) for s in states if s.numel())
+        if len(same) > 1 and any(end > begin for (_, end), (begin, _) in zip(spans, spans[1:])):
+            _refuse("states of unlike layouts lie among each other")
+    rows = sentences * beams
+    packed = [(_pack_reorder(sentences, beams, len(at), *_state_layout(s, rows, lengths is not None)), struct.pack("%dQ" % len(at), *at)) for s, at in calls]
+    for d, at in packed:
+        rc = lib().exb_reorder_beams_fwd(ctx._h, d, at, parents.data_ptr(), lengths_p, _stream())
+        if rc:
+            check(rc)

@@ -1,0 +1,223 @@
+// The states of beams follow their parents, in place: after a step of beam search row j of a sentence's rows becomes what row parents[j] was.
+// A thread has the same few bytes of all of a sentence's rows: it reads those of the parents of beams that change, and only then writes, so that
+// no row is lost whatever the parents are, and no other thread is waited for.  Beams that are their own parents are neither read nor written
+// (but as another's parent), nor are positions from the sentence's length on.
+// Bound by memory: the beams that change, in and out once.
+#include <algorithm>
+#include <vector>
+
+#include "rows_common.cuh"
+
+namespace exb {
+namespace {
+
+constexpr int kMaxBeams = 32;
+constexpr int kThreads = 256;
+constexpr int kStates = 128;           // of one launch
+constexpr int kSentences = 256;        // the same
+
+struct ReorderArgs {
+    uint8_t* states[kStates];
+    const int32_t *parents, *lengths;
+    int64_t first;                     // sentence
+    int64_t positions, bytes;          // bytes of a position (of all where they follow one another: positions is 1)
+    int64_t row_stride, outer_stride, position_stride;
+    int64_t outer;
+    int64_t per_length;                // positions that follow one another: a sentence's length times this many bytes; otherwise 0
+    int n_states, sentences, beams;
+};
+
+// A sentence's columns (kUnit bytes of a position, of one state and outer index), in chunks of kThreads * kColumns.
+template <typename U, int kColumns>
+__device__ __forceinline__ int64_t columns_of(const ReorderArgs& a, int b) {
+    const int64_t whole = a.per_length ? a.bytes / a.per_length : a.positions;
+    const int64_t length = a.lengths ? min((int64_t)max(a.lengths[a.first + b], 0), whole) : whole;
+    return length * ((a.per_length ? a.per_length : a.bytes) / (int64_t)sizeof(U));
+}
+
+template <typename U, int kMoves, int kColumns>
+__global__ void __launch_bounds__(kThreads) reorder_beams_kernel(const __grid_constant__ ReorderArgs a) {
+    __shared__ int s_chunks[kSentences];                        // up to each sentence's end
+    __shared__ uint8_t s_to[kMaxBeams], s_from[kMaxBeams];
+    __shared__ int s_moves;
+    constexpr int kChunk = kThreads * kColumns;
+    pdl_enter();
+    const int tid = threadIdx.x, lane = tid & 31;
+    int mine = 0;
+    if (tid < a.sentences) {
+        bool moved = false;
+        const int32_t* parent = a.parents + (a.first + tid) * a.beams;
+        for (int j = 0; j < a.beams; ++j) moved |= parent[j] != j && parent[j] >= 0 && parent[j] < a.beams;
+        if (moved) mine = (int)((columns_of<U, kColumns>(a, tid) + kChunk - 1) / kChunk);
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, mine, o);
+        if (lane >= o) mine += u;
+    }
+    s_chunks[tid] = mine;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < tid >> 5; ++w) before += s_chunks[w * 32 + 31];
+    __syncthreads();
+    s_chunks[tid] = mine + before;
+    __syncthreads();
+    const int chunks = s_chunks[a.sentences - 1];
+    const int64_t items = (int64_t)chunks * a.n_states * a.outer;
+    int last = -1, moves = 0;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t which = item / chunks;
+        const int c = (int)(item - which * chunks);
+        int lo = 0, hi = a.sentences - 1;      // the first sentence with more chunks up to its end
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (s_chunks[mid] > c) hi = mid;
+            else lo = mid + 1;
+        }
+        if (lo != last) {
+            __syncthreads();
+            if (tid < 32) {
+                const int p = tid < a.beams ? a.parents[(a.first + lo) * a.beams + tid] : -1;
+                const bool moved = p >= 0 && p < a.beams && p != tid;
+                const uint32_t all = __ballot_sync(0xffffffffu, moved);
+                if (moved) {
+                    const int k = __popc(all & ((1u << tid) - 1));
+                    s_to[k] = (uint8_t)tid;
+                    s_from[k] = (uint8_t)p;
+                }
+                if (tid == 0) s_moves = __popc(all);
+            }
+            __syncthreads();
+            moves = s_moves;
+            last = lo;
+        }
+        const int64_t outer = which % a.outer;
+        uint8_t* base = a.states[which / a.outer] + outer * a.outer_stride + (a.first + lo) * a.beams * a.row_stride;
+        const int64_t columns = columns_of<U, kColumns>(a, lo), per = a.bytes / (int64_t)sizeof(U);
+        const int64_t column0 = (int64_t)(c - (lo ? s_chunks[lo - 1] : 0)) * kChunk + tid;
+        U v[kColumns][kMoves];
+        uint8_t* at[kColumns];
+#pragma unroll
+        for (int k = 0; k < kColumns; ++k) {
+            const int64_t column = column0 + k * kThreads;
+            at[k] = nullptr;
+            if (column < columns) {
+                const int64_t position = a.positions > 1 ? column / per : 0;
+                at[k] = base + position * a.position_stride + (column - position * per) * (int64_t)sizeof(U);
+#pragma unroll
+                for (int i = 0; i < kMoves; ++i)
+                    if (i < moves) v[k][i] = *reinterpret_cast<const U*>(at[k] + s_from[i] * a.row_stride);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kColumns; ++k)
+            if (at[k]) {
+#pragma unroll
+                for (int i = 0; i < kMoves; ++i)
+                    if (i < moves) *reinterpret_cast<U*>(at[k] + s_to[i] * a.row_stride) = v[k][i];
+            }
+    }
+}
+
+// ---- host: where states lie ----------------------------------------------------------------------
+struct Dim {
+    int64_t n, stride;
+};
+// A state's dimensions from the outermost in, each inside one step of the next outer one; false where some lie over others.
+bool nest(const exb_reorder_desc& d, std::vector<Dim>& dims, int64_t& extent) {
+    dims.clear();
+    for (const Dim& x : {Dim{d.sentences * d.beams, d.row_stride}, Dim{d.outer, d.outer_stride}, Dim{d.positions, d.position_stride}})
+        if (x.n > 1) dims.push_back(x);
+    std::sort(dims.begin(), dims.end(), [](const Dim& a, const Dim& b) { return a.stride > b.stride; });
+    extent = d.bytes;
+    for (size_t i = dims.size(); i-- > 0;) {
+        if (dims[i].stride < extent) return false;
+        extent += (dims[i].n - 1) * dims[i].stride;
+    }
+    return true;
+}
+// Whether two states whose first bytes are `d` apart share a byte: at each dimension the step at or before the distance and the one behind it can.
+bool meet(const std::vector<Dim>& dims, size_t i, int64_t bytes, int64_t d) {
+    if (i == dims.size()) return d < bytes && -d < bytes;
+    const int64_t at = d >= 0 ? d / dims[i].stride : -((-d + dims[i].stride - 1) / dims[i].stride);
+    for (int64_t s = at; s <= at + 1; ++s)
+        if (s < dims[i].n && -s < dims[i].n && meet(dims, i + 1, bytes, d - s * dims[i].stride)) return true;
+    return false;
+}
+
+template <typename U>
+int launch(const exb_ctx* ctx, const ReorderArgs& a, int beams, cudaStream_t st) {
+    const int64_t columns = a.positions * a.bytes / (int64_t)sizeof(U) * a.sentences * a.n_states * a.outer;
+    auto go = [&](auto kernel, int each) {
+        const int64_t chunks = std::max<int64_t>(1, (columns + each - 1) / each + (int64_t)a.sentences * a.n_states * a.outer);      // at most
+        const int64_t grid = std::min<int64_t>(chunks, (int64_t)ctx->sm_count * 8);
+        return launch_pdl(ctx, "reorder_beams_kernel", kernel, dim3((unsigned)grid), dim3(kThreads), 0, st, a);
+    };
+    if (beams <= 4) return go(reorder_beams_kernel<U, 4, 4>, kThreads * 4);
+    if (beams <= 8) return go(reorder_beams_kernel<U, 8, 2>, kThreads * 2);
+    if (beams <= 16) return go(reorder_beams_kernel<U, 16, 1>, kThreads);
+    return go(reorder_beams_kernel<U, 32, 1>, kThreads);
+}
+
+}  // namespace
+}  // namespace exb
+
+using namespace exb;
+
+extern "C" int exb_reorder_beams_fwd(exb_ctx* ctx, const exb_reorder_desc* d, void* const* states, const int32_t* parents, const int32_t* lengths, void* stream) {
+    EXB_REQUIRE(ctx != nullptr && d != nullptr, "exb_reorder_beams_fwd: null context or descriptor");
+    EXB_REQUIRE(d->sentences >= 0 && d->beams >= 1 && d->n_states >= 0 && d->outer >= 0 && d->positions >= 0 && d->bytes >= 0,
+                "exb_reorder_beams_fwd: bad shape (%lld x %d beams, %d states of %lld x %lld x %lld bytes)", (long long)d->sentences, d->beams, d->n_states,
+                (long long)d->outer, (long long)d->positions, (long long)d->bytes);
+    if (d->beams > kMaxBeams) return fail(EXB_ERR_UNSUPPORTED, "exb_reorder_beams_fwd: at most %d beams, got %d", kMaxBeams, d->beams);
+    if ((double)d->sentences * d->beams * (double)d->outer * (double)d->positions * (double)d->bytes > 274877906944.0)      // 256 GB
+        return fail(EXB_ERR_UNSUPPORTED, "exb_reorder_beams_fwd: states are too large for one call");
+    if (d->sentences == 0 || d->n_states == 0 || d->outer == 0 || d->positions == 0 || d->bytes == 0) return EXB_OK;
+    EXB_REQUIRE(states && parents, "exb_reorder_beams_fwd: null buffer");
+    EXB_REQUIRE(rows::aligned_to(parents, 4) && rows::aligned_to(lengths, 4), "exb_reorder_beams_fwd: parents or lengths not aligned to their element");
+    std::vector<Dim> dims;
+    int64_t extent;
+    EXB_REQUIRE(nest(*d, dims, extent), "exb_reorder_beams_fwd: some of a state's rows lie over others");
+    // states that share no memory with each other, nor have parents or lengths among them
+    std::vector<const uint8_t*> at(d->n_states);
+    uintptr_t bits = (uintptr_t)d->bytes;
+    for (int i = 0; i < d->n_states; ++i) {
+        EXB_REQUIRE(states[i], "exb_reorder_beams_fwd: null state");
+        at[i] = static_cast<const uint8_t*>(states[i]);
+        bits |= reinterpret_cast<uintptr_t>(states[i]);
+    }
+    for (const Dim& x : dims) bits |= (uintptr_t)x.stride;
+    std::sort(at.begin(), at.end());
+    for (int i = 0; i < d->n_states; ++i) {
+        for (int j = i + 1; j < d->n_states && at[j] < at[i] + extent; ++j)
+            EXB_REQUIRE(!meet(dims, 0, d->bytes, at[j] - at[i]), "exb_reorder_beams_fwd: two states share memory");
+        auto among = [&](const void* p, int64_t n) {
+            const uint8_t* b = static_cast<const uint8_t*>(p);
+            return p && b < at[i] + extent && b + n * 4 > at[i];
+        };
+        EXB_REQUIRE(!among(parents, d->sentences * d->beams) && !among(lengths, d->sentences), "exb_reorder_beams_fwd: parents or lengths lie among a state's rows");
+    }
+    if (int rc = rows::check_device(ctx, "exb_reorder_beams_fwd")) return rc;
+    ReorderArgs a;
+    a.parents = parents; a.lengths = lengths;
+    a.row_stride = d->row_stride; a.outer_stride = d->outer_stride; a.position_stride = d->position_stride;
+    a.outer = d->outer; a.beams = d->beams;
+    a.positions = d->positions; a.bytes = d->bytes; a.per_length = 0;
+    if (d->positions == 1 || d->position_stride == d->bytes) {      // positions that follow one another
+        a.per_length = d->bytes;
+        a.bytes = d->positions * d->bytes;
+        a.positions = 1;
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    for (a.first = 0; a.first < d->sentences; a.first += kSentences) {
+        a.sentences = (int)std::min<int64_t>(kSentences, d->sentences - a.first);
+        for (int s = 0; s < d->n_states; s += kStates) {
+            a.n_states = std::min(kStates, d->n_states - s);
+            for (int i = 0; i < a.n_states; ++i) a.states[i] = static_cast<uint8_t*>(states[s + i]);
+            const int rc = bits % 16 == 0 ? launch<uint4>(ctx, a, d->beams, st) : bits % 4 == 0 ? launch<uint32_t>(ctx, a, d->beams, st)
+                         : bits % 2 == 0 ? launch<uint16_t>(ctx, a, d->beams, st) : launch<uint8_t>(ctx, a, d->beams, st);
+            if (rc) return rc;
+        }
+    }
+    return EXB_OK;
+}

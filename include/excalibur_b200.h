@@ -616,6 +616,43 @@ typedef struct exb_grouped_desc {
 EXB_API int exb_grouped_matmul_fwd(exb_ctx* ctx, const exb_grouped_desc* d, const void* a, const float* a_scales, const void* w,
                                    const float* w_scales, const int32_t* ends, const float* bias, void* y, void* stream);
 
+/* A step of beam search: of every sentence's beams x V continuations the `select` best, in falling order of
+ *   score(j, v) = scores[j] + z[j][v] - lse[j],  z = scale * logits (scale between 1e-8 and 1e8), lse = log sum exp z
+ * compared in 64 bits, equal scores by the lower beam, a beam's by their logits, equal logits by the lower token.
+ * logits: [sentences * beams][V] with `stride` elements between rows; scores: fp32 [sentences][beams]; ended: NULL or a byte for each beam that is not 0
+ * where the beam has ended: it goes on with end_token alone, at its score.  A beam whose score is minus infinity is none, and minus infinity masks
+ * a token; neither is selected.  Rows of ended beams and of those that are none are not read.  A row with a NaN or plus infinity has NaN scores; NaN come before
+ * all others (and a beam's NaN logits before its other ones).
+ * Results, each [sentences][select]: out_scores fp32, parents (the beam, 0..beams) and tokens int32; where fewer than `select` are left,
+ * minus infinity, -1 and -1.  beams and select: 1..32.
+ * workspace: workspace_bytes of device memory, 8-byte aligned, at least 8 * sentences * beams * (1 + min(select, V)); what is in it
+ * before and after the call means nothing. */
+typedef struct exb_beam_desc {
+    int64_t sentences, stride, workspace_bytes;
+    int32_t beams, V;
+    int32_t dtype;          /* of logits */
+    int32_t select, end_token;
+    float scale;
+} exb_beam_desc;
+EXB_API int exb_beam_select_fwd(exb_ctx* ctx, const exb_beam_desc* d, const void* logits, const float* scores, const uint8_t* ended,
+                                float* out_scores, int32_t* parents, int32_t* tokens, void* workspace, void* stream);
+
+/* The states of beams follow their parents, in place: rows sentence * beams + j of each state become what rows sentence * beams + parents[sentence][j] were.
+ * Parents that are no beam's (below 0, or `beams` and above) leave a row as it is.  lengths: NULL, or int32 [sentences]: only positions below
+ * the sentence's length change (above `positions`: all).
+ * A state is [sentences * beams][outer][positions] of `bytes` bytes, whatever their type, with strides in bytes, in any order, as long as no two share a
+ * byte.  states: host array of n_states device pointers; all have the same sizes and strides, none shares memory with another; parents (int32
+ * [sentences][beams]) and lengths lie outside of the memory that each spans.  16-byte aligned states, strides and sizes are moved in vectors.
+ * beams: 1..32. */
+typedef struct exb_reorder_desc {
+    int64_t sentences;
+    int32_t beams, n_states;
+    int64_t outer, positions, bytes;
+    int64_t row_stride, outer_stride, position_stride;
+} exb_reorder_desc;
+EXB_API int exb_reorder_beams_fwd(exb_ctx* ctx, const exb_reorder_desc* d, void* const* states, const int32_t* parents,
+                                  const int32_t* lengths, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
