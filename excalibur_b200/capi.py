@@ -1101,10 +1101,13 @@ def beam_select(ctx, logits, scores, select=None, scale=1.0, ended=None, end_tok
     out = scores.new_empty(sentences, max(select, 0))
     parents = t.empty_like(out, dtype=t.int32)
     tokens = t.empty_like(parents)
-    room = 8 * rows * (1 + min(max(select, 0), V))
-    workspace = scores.new_empty(room, dtype=t.uint8)
-    rc = lib().exb_beam_select_fwd(ctx._h, _pack_beams(sentences, ls, room, beams, V, _DTYPES.get(logits.dtype, -1), select, end_token, scale), logits.data_ptr(),
-                                   scores.data_ptr(), ended_p, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), workspace.data_ptr(), _stream())
+    dt = _DTYPES.get(logits.dtype, -1)
+    at = logits.data_ptr(), scores.data_ptr(), ended_p, out.data_ptr(), parents.data_ptr(), tokens.data_ptr()
+    rc = lib().exb_beam_select_fwd(ctx._h, _pack_beams(sentences, ls, 0, beams, V, dt, select, end_token, scale), *at, None, _stream())
+    if rc == EXB_ERR_NOMEM:      # one of those calls that need a workspace
+        room = 8 * rows * (1 + min(select, V))
+        workspace = scores.new_empty(room, dtype=t.uint8)
+        rc = lib().exb_beam_select_fwd(ctx._h, _pack_beams(sentences, ls, room, beams, V, dt, select, end_token, scale), *at, workspace.data_ptr(), _stream())
     if rc:
         check(rc)
     return out, parents, tokens

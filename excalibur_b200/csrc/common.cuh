@@ -78,6 +78,20 @@ inline int raise_smem_limit(const exb_ctx* ctx, K kern) {
     return EXB_OK;
 }
 
+// Clusters of up to 16 CTAs, as every B200 has room for, must be asked for once.
+template <typename K>
+inline int allow_wide_clusters(const exb_ctx* ctx, K kern) {
+    static std::mutex attr_mutex;
+    static std::set<std::pair<const void*, int>> allowed;
+    const auto key = std::make_pair(reinterpret_cast<const void*>(kern), ctx->device);
+    std::lock_guard<std::mutex> lock(attr_mutex);
+    if (!allowed.count(key)) {
+        EXB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        allowed.insert(key);
+    }
+    return EXB_OK;
+}
+
 // Launch with programmatic stream serialization: the grid may be scheduled while the previous kernel of the stream
 // drains.  Every kernel launched this way calls pdl_wait() before it touches global memory that another kernel
 // writes or reads.

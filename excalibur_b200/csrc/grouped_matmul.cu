@@ -22,7 +22,7 @@ struct ProductParams {
     void* y;
     int64_t y_stride;
     int M, N, blocks, experts, y_dtype, vec;      // experts 0: all rows are one's, and there are no ends
-    int n_tiles, splits;
+    int n_tiles, splits, stages;
     uint32_t idesc;
     int* error;
 };
@@ -30,28 +30,43 @@ struct ProductParams {
 // ---- which rows are whose ------------------------------------------------------------------------
 // Where each expert's rows end, and its tiles (kRows rows by one of n_tiles).  Ends come from the device and nobody has looked at them: one
 // below those before it counts as theirs, one beyond the rows as their number, so that no row is two experts' and none is out of range.
+// By all threads of a CTA; a barrier has to follow.
 template <int kRows>
-__device__ __forceinline__ void list_experts(const ProductParams& p, int2* table, int lane) {
-    int end = 0, tiles = 0;
-    for (int e0 = 0; e0 < p.experts; e0 += 32) {
-        int v = e0 + lane < p.experts ? min(max(p.ends[e0 + lane], 0), p.M) : 0;
+__device__ __forceinline__ void list_experts(const ProductParams& p, int2* table) {
+    __shared__ int s_end[32], s_tiles[32];      // of each warp
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (int)blockDim.x >> 5;
+    int end = 0, tiles = 0;                      // of the experts before
+    for (int e0 = 0; e0 < p.experts; e0 += (int)blockDim.x) {
+        int v = e0 + tid < p.experts ? min(max(p.ends[e0 + tid], 0), p.M) : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v = max(v, u);
         }
-        v = max(v, end);
-        const int before = __shfl_up_sync(0xffffffffu, v, 1);
-        int t = (v - (lane ? before : end) + kRows - 1) / kRows * p.n_tiles;
+        __syncthreads();
+        if (lane == 31) s_end[warp] = v;
+        __syncthreads();
+        int before = end;
+        for (int w = 0; w < warps; ++w) {
+            if (w < warp) before = max(before, s_end[w]);
+            end = max(end, s_end[w]);
+        }
+        v = max(v, before);
+        const int begin = __shfl_up_sync(0xffffffffu, v, 1);
+        int t = (v - (lane ? begin : before) + kRows - 1) / kRows * p.n_tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, t, o);
             if (lane >= o) t += u;
         }
+        if (lane == 31) s_tiles[warp] = t;
+        __syncthreads();
         t += tiles;
-        if (e0 + lane < p.experts) table[e0 + lane] = make_int2(v, t);
-        end = __shfl_sync(0xffffffffu, v, 31);
-        tiles = __shfl_sync(0xffffffffu, t, 31);
+        for (int w = 0; w < warps; ++w) {
+            if (w < warp) t += s_tiles[w];
+            tiles += s_tiles[w];
+        }
+        if (e0 + tid < p.experts) table[e0 + tid] = make_int2(v, t);
     }
 }
 
@@ -86,32 +101,33 @@ __device__ __forceinline__ float sum_of(uint32_t raw) {
 // SMs a CTA works on one after the other, the next one's loads under way while it stores (two accumulators in turn).  With fewer, the K blocks
 // of a tile are divided over a cluster of up to 8 CTAs, so that enough of them ask for w at the same time; every CTA then
 // finishes a share of the columns: the others send it their sums in one bulk copy each, counted by a barrier of its own.
-constexpr int few_stages(int cols) { return cols == 128 ? 4 : cols == 64 ? 3 : cols == 32 ? 4 : 5; }      // (two CTAs fit an SM up to 64 columns)
+constexpr int kFewMostStages = 12;
 constexpr int few_epi_warps(int cols) { return cols == 128 ? 16 : cols == 64 ? 8 : 4; }                   // up to 32 columns each
 constexpr int few_stage_bytes(int cols) { return (128 + cols) * kBlk; }
 // (columns that a CTA gets, of 16 by 7 CTAs: 3 from each of 6 others)
 constexpr int few_received(int cols) { return cols == 16 ? 18 : cols; }
-constexpr int few_smem(int cols) { return few_stages(cols) * few_stage_bytes(cols) + few_received(cols) * 512 + 1024; }
+constexpr int few_smem(int cols, int stages, bool parts) { return stages * few_stage_bytes(cols) + (parts ? few_received(cols) * 512 : 0) + 1024; }
 
 template <Kind kKind, int kCols>
 __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ? 1 : 2) product_few_kernel(const __grid_constant__ ProductParams p) {
-    constexpr int kStages = few_stages(kCols), kStageBytes = few_stage_bytes(kCols), kEpi = few_epi_warps(kCols);
+    constexpr int kStageBytes = few_stage_bytes(kCols), kEpi = few_epi_warps(kCols);
+    const int stages = p.stages;
     constexpr int kMine = kCols * 4 / kEpi;      // columns of a warp
     constexpr int kTmem = 2 * kCols;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages], tfull_bar[2], tempty_bar[2], recv_bar;
+    __shared__ __align__(8) uint64_t full_bar[kFewMostStages], empty_bar[kFewMostStages], tfull_bar[2], tempty_bar[2], recv_bar;
     __shared__ uint32_t tmem_base_smem;
     __shared__ int abort_flag;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint32_t* part = reinterpret_cast<uint32_t*>(ring);                  // [column][128] behind the loop
-    uint32_t* recv = part + kStages * kStageBytes / 4;                   // [CTA, without this one][column of the share][128]
-    int2* table = reinterpret_cast<int2*>(recv + few_received(kCols) * 128);
+    uint32_t* recv = part + stages * kStageBytes / 4;                    // [CTA, without this one][column of the share][128]
+    int2* table = reinterpret_cast<int2*>(recv + (p.splits > 1 ? few_received(kCols) * 128 : 0));
     const int warp = ptx::uniform_warp(), lane = threadIdx.x & 31;
     const int rank = (int)blockIdx.x % p.splits, first = (int)blockIdx.x / p.splits, step = (int)gridDim.x / p.splits;
     const int b0 = (int)((int64_t)rank * p.blocks / p.splits), nb = (int)((int64_t)(rank + 1) * p.blocks / p.splits) - b0;
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int s = 0; s < kStages; ++s) {
+        for (int s = 0; s < stages; ++s) {
             ptx::mbar_init(&full_bar[s], 2);
             ptx::mbar_init(&empty_bar[s], 1);
         }
@@ -128,7 +144,7 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
     if (p.splits > 1) ptx::cluster_arrive();      // every CTA runs and its barriers are initialised: waited for before the first part is sent
     pdl_wait();
     if (p.experts) {
-        if (warp == 0) list_experts<kCols>(p, table, lane);
+        list_experts<kCols>(p, table);
         __syncthreads();
     }
     // TMEM is taken when the previous kernel is done, and the next one may start when it is taken (see kTmemOrder).  The loads do not wait
@@ -178,7 +194,7 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
                     ptx::tma_load_2d_u32(dst + 128 * kBlk, reinterpret_cast<uint64_t>(&p.tmA), full0 + s * 8, (b0 + b) * kBlk, m0, leader);
                 }
                 __syncwarp();      // (the elected lane may take a branch of its own; what follows is in registers of the whole warp)
-                if (++s == kStages) {
+                if (++s == stages) {
                     s = 0;
                     phase ^= 1u;
                 }
@@ -210,7 +226,7 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
                     ptx::tc_mma_lohi<kKind == kInt8>(tmem_base + buf * kCols, w_lo + 2 * ks, a_lo + 2 * ks, desc_hi, p.idesc, b | ks ? 1u : 0u, leader);
                 ptx::tc_commit_u32(empty0 + s * 8, leader);
                 __syncwarp();
-                if (++s == kStages) {
+                if (++s == stages) {
                     s = 0;
                     phase ^= 1u;
                 }
@@ -342,27 +358,43 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
 }
 
 // ---- CTA pairs ---------------------------------------------------------------------------------
-// Tiles of 256 rows of a by 256 or 128 of w by pairs of CTAs, persistent.  Each CTA keeps 128 rows of a and half of w's rows of a stage.  TMEM holds
-// two accumulators: the epilogue warps read one out, scale and store it while the MMAs fill the other.
-constexpr int kPairM = 256;
+// Tiles of 256 rows of w by up to kWide rows of a by pairs of CTAs, persistent, with the operands' roles exchanged here too: the MMA's columns are as many as the
+// tile has rows of a, in whole 32s, so that groups of any size cost what they need (256 rows of a as the MMA's rows took 704 us for 8192 x 14336 x 4096 bf16
+// over 8 experts, this takes 657); an expert's rows are divided evenly between its tiles.  Each CTA keeps 128 rows of w and half of a's rows of a stage.
+// TMEM holds two accumulators: the epilogue warps read one out, scale and store it while the MMAs fill the other.  A thread has a channel of all rows, and a
+// warp stores 32 neighbours of a row at a time.
 constexpr int kPairEpiWarps = 8;                 // two per TMEM lane quarter, half of the accumulator's columns each
-constexpr int pair_stage_bytes(int n) { return (kPairM + n) / 2 * kBlk; }      // of one of the two CTAs
-constexpr int pair_stages(int n) { return n == 256 ? 5 : 7; }
-constexpr int pair_scale_bytes(int n) { return kPairEpiWarps * n * 4; }         // each warp's columns' scales and biases
-constexpr int pair_smem(int n) { return pair_stages(n) * pair_stage_bytes(n) + kPairEpiWarps * kStageOut + pair_scale_bytes(n) + 1024; }
+constexpr int pair_stage_bytes(int wide) { return (128 + wide / 2) * kBlk; }      // of one of the two CTAs
+constexpr int pair_stages(int wide) { return wide == 256 ? 6 : 8; }
+constexpr int pair_smem(int wide) { return pair_stages(wide) * pair_stage_bytes(wide) + 1024; }
 constexpr int kPairThreads = 128 + kPairEpiWarps * 32;
 
-template <Kind kKind, int kPairN>
+// A thread's results of up to 32 rows from m on, in channel n.  (Neighbours put together in whole words took longer: 4048 x 7312 x 264 36.7 us, this way 29.0;
+// so did whole vectors through shared memory, 34.8.)
+template <typename T>
+__device__ __forceinline__ void store_columns_as(const ProductParams& p, const float (&v)[32], int m, int n, int left) {
+    T* y = static_cast<T*>(p.y) + (int64_t)m * p.y_stride + n;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        if (i < left && n < p.N) *y = rows::from_float<T>(v[i]);
+        y += p.y_stride;
+    }
+}
+__device__ __forceinline__ void store_columns(const ProductParams& p, const float (&v)[32], int m, int n, int left) {
+    if (p.y_dtype == EXB_F16) store_columns_as<__half>(p, v, m, n, left);
+    else if (p.y_dtype == EXB_BF16) store_columns_as<__nv_bfloat16>(p, v, m, n, left);
+    else store_columns_as<float>(p, v, m, n, left);
+}
+
+template <Kind kKind, int kWide>
 __global__ void __launch_bounds__(kPairThreads, 1) product_pair_kernel(const __grid_constant__ ProductParams p) {
-    constexpr int kStages = pair_stages(kPairN), kStageBytes = pair_stage_bytes(kPairN), kPairCols = kPairN / 2;
+    constexpr int kStages = pair_stages(kWide), kStageBytes = pair_stage_bytes(kWide);
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages], tfull_bar[2], tempty_bar[2];
     __shared__ uint32_t tmem_base_smem;
     __shared__ int abort_flag;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* out = ring + kStages * kStageBytes;
-    float* scales = reinterpret_cast<float*>(out + kPairEpiWarps * kStageOut);
-    int2* table = reinterpret_cast<int2*>(scales + pair_scale_bytes(kPairN) / 4);
+    int2* table = reinterpret_cast<int2*>(ring + kStages * kStageBytes);
     const int warp = ptx::uniform_warp(), lane = threadIdx.x & 31;
     const int rank = (int)__shfl_sync(0xffffffffu, ptx::cluster_ctarank(), 0);
     const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
@@ -380,12 +412,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) product_pair_kernel(const __g
         ptx::tma_prefetch_desc(&p.tmA);
         ptx::tma_prefetch_desc(&p.tmW);
     }
+    __syncwarp();
     pdl_wait();      // (before TMEM is taken: see kTmemOrder)
+    if (p.experts) list_experts<kWide>(p, table);
     if (warp == 1) {
-        ptx::tmem_alloc_pair(&tmem_base_smem, 2 * kPairN);
+        ptx::tmem_alloc_pair(&tmem_base_smem, 2 * kWide);
         ptx::tmem_relinquish_pair();
-    } else if (warp == 0 && p.experts) {
-        list_experts<kPairM>(p, table, lane);
     }
     ptx::tc_fence_before_sync();
     __syncthreads();
@@ -395,25 +427,28 @@ __global__ void __launch_bounds__(kPairThreads, 1) product_pair_kernel(const __g
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_smem, 0);
     const uint32_t ring0 = ptx::smem_u32(ring), full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
     const uint32_t tfull0 = ptx::smem_u32(tfull_bar), tempty0 = ptx::smem_u32(tempty_bar);
-    const int total = all_tiles<kPairM>(p, table);
-    auto tile_of = [&](int t, Share& s, int& m0, int& n0) {
-        s = share_of(p, table, t);
+    const int total = all_tiles<kWide>(p, table);
+    // rows [m0, m0 + rows) of a, `wide` columns of the MMA; rows [n0, n0 + 256) of w
+    struct Tile {
+        int expert, m0, rows, wide, n0;
+    };
+    auto tile_of = [&](int t) {
+        const Share s = share_of(p, table, t);
+        const int all = s.end - s.begin, tiles = (all + kWide - 1) / kWide, each = ((all + tiles - 1) / tiles + 31) & ~31;
         int m, n;
-        tile_at(s.tile, (s.end - s.begin + kPairM - 1) / kPairM, p.n_tiles, m, n);
-        m0 = s.begin + m * kPairM;
-        n0 = n * kPairN;
+        tile_at(s.tile, tiles, p.n_tiles, m, n);
+        const int rows = min(each, all - m * each);
+        return Tile{s.expert, s.begin + m * each, rows, (rows + 31) & ~31, n * 256};
     };
     if (warp == 0 || warp == 2) {      // a loading warp for each operand
-        const bool is_w = warp == 2;
+        const bool is_w = warp == 0;
         const uint32_t leader = ptx::elect_one() ? 1u : 0u, counts = rank == 0 ? leader : 0u;
         const uint32_t full_lead = ptx::map_to_cta(full0, 0);
         bool ok = true;
         int s = 0;
         uint32_t phase = 1;      // (a fresh barrier's previous phase counts as complete)
         for (int t = first; t < total && ok; t += step) {
-            Share of;
-            int m0, n0;
-            tile_of(t, of, m0, n0);
+            const Tile of = tile_of(t);
             for (int b = 0; b < p.blocks; ++b) {
                 if (!ptx::mbar_wait_quick_uniform(empty0 + s * 8, phase, &abort_flag, kMaxSpins)) {
                     ok = false;
@@ -422,11 +457,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) product_pair_kernel(const __g
                 // (both CTAs' bytes are counted by rank 0)
                 const uint32_t dst = ring0 + s * kStageBytes;
                 if (is_w) {
-                    ptx::mbar_arrive_expect_tx_u32(full0 + s * 8, kPairN * kBlk, counts);
-                    ptx::tma_load_3d_pair(dst + 128 * kBlk, reinterpret_cast<uint64_t>(&p.tmW), full_lead + s * 8, b * kBlk, n0 + rank * (kPairN / 2), of.expert, leader);
+                    ptx::mbar_arrive_expect_tx_u32(full0 + s * 8, 256 * kBlk, counts);
+                    ptx::tma_load_3d_pair(dst, reinterpret_cast<uint64_t>(&p.tmW), full_lead + s * 8, b * kBlk, of.n0 + rank * 128, of.expert, leader);
                 } else {
-                    ptx::mbar_arrive_expect_tx_u32(full0 + s * 8, kPairM * kBlk, counts);
-                    ptx::tma_load_2d_pair(dst, reinterpret_cast<uint64_t>(&p.tmA), full_lead + s * 8, b * kBlk, m0 + rank * 128, leader);
+                    ptx::mbar_arrive_expect_tx_u32(full0 + s * 8, kWide * kBlk, counts);
+                    ptx::tma_load_2d_pair(dst + 128 * kBlk, reinterpret_cast<uint64_t>(&p.tmA), full_lead + s * 8, b * kBlk, of.m0 + rank * (of.wide / 2), leader);
                 }
                 __syncwarp();      // (see the other kernel's)
                 if (++s == kStages) {
@@ -446,6 +481,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) product_pair_kernel(const __g
             int s = 0, buf = 0;
             uint32_t phase = 0, acc_phase = 1;
             for (int t = first; t < total && ok; t += step) {
+                const uint32_t idesc = p.idesc + ((uint32_t)(tile_of(t).wide >> 3) << 17);
                 if (!ptx::mbar_wait_quick_uniform(tempty0 + buf * 8, acc_phase, &abort_flag, kMaxSpins)) {
                     ok = false;
                     break;
@@ -457,10 +493,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) product_pair_kernel(const __g
                         break;
                     }
                     ptx::tc_fence_after_sync();
-                    const uint32_t a_lo = (uint32_t)d0 + ((uint32_t)(s * kStageBytes) >> 4), w_lo = a_lo + ((128 * kBlk) >> 4);
+                    const uint32_t w_lo = (uint32_t)d0 + ((uint32_t)(s * kStageBytes) >> 4), a_lo = w_lo + ((128 * kBlk) >> 4);
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks)
-                        ptx::tc_mma_lohi_pair<kKind == kInt8>(tmem_base + buf * kPairN, a_lo + 2 * ks, w_lo + 2 * ks, desc_hi, p.idesc, b | ks ? 1u : 0u, leader);
+                        ptx::tc_mma_lohi_pair<kKind == kInt8>(tmem_base + buf * kWide, w_lo + 2 * ks, a_lo + 2 * ks, desc_hi, idesc, b | ks ? 1u : 0u, leader);
                     ptx::tc_commit_pair_u32(empty0 + s * 8, leader);
                     __syncwarp();
                     if (++s == kStages) {
@@ -481,63 +517,51 @@ __global__ void __launch_bounds__(kPairThreads, 1) product_pair_kernel(const __g
         __syncwarp();
     } else if (warp >= 4) {
         const int q = warp & 3, half = (warp >> 2) - 1;
-        uint8_t* stage = out + (warp - 4) * kStageOut;
-        float* my_scales = scales + (warp - 4) * kPairN;      // kPairCols scales, kPairCols biases
-        const uint32_t taddr0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * kPairCols);
+        const uint32_t taddr0 = tmem_base + ((uint32_t)(q * 32) << 16);
         const uint32_t tempty_lead = ptx::map_to_cta(tempty0, 0);
         bool ok = true;
         int buf = 0;
         uint32_t acc_phase = 0;
         for (int t = first; t < total && ok; t += step) {
-            Share of;
-            int m0, n0;
-            tile_of(t, of, m0, n0);
-            const int row0 = m0 + rank * 128 + q * 32, col = n0 + half * kPairCols;
-            __syncwarp();
+            const Tile of = tile_of(t);
+            const int n = of.n0 + rank * 128 + q * 32 + lane, c0 = half * (of.wide / 2), c1 = min(c0 + of.wide / 2, of.rows);
+            // (asked for before there is anything to scale) this channel's scale and bias, and each row's scale in a lane of its own
+            const float ws = kKind == kInt8 && n < p.N ? p.w_scales[(int64_t)of.expert * p.N + n] : 0.f;
+            const float start = p.bias && n < p.N ? p.bias[(int64_t)of.expert * p.N + n] : 0.f;
+            float as[kWide / 64];
 #pragma unroll
-            for (int c = lane; c < kPairCols; c += 32) {
-                const bool is = col + c < p.N;
-                my_scales[c] = kKind == kInt8 && is ? p.w_scales[(int64_t)of.expert * p.N + col + c] : 0.f;
-                my_scales[kPairCols + c] = p.bias && is ? p.bias[(int64_t)of.expert * p.N + col + c] : 0.f;
-            }
-            const float as = kKind == kInt8 && row0 + lane < of.end ? p.a_scales[row0 + lane] : 0.f;
-            __syncwarp();
+            for (int k = 0; k < kWide / 64; ++k) as[k] = kKind == kInt8 && c0 + k * 32 + lane < c1 ? p.a_scales[of.m0 + c0 + k * 32 + lane] : 0.f;
             if (!ptx::mbar_wait_bounded_uniform(tfull0 + buf * 8, acc_phase, &abort_flag, kMaxSpins)) {
                 ok = false;
                 break;
             }
             __syncwarp();      // (what follows needs the warp together)
             ptx::tc_fence_after_sync();
-            const uint32_t taddr = taddr0 + (uint32_t)(buf * kPairN);
-            constexpr int kPass = 64;      // columns at a time
-#pragma unroll 1
-            for (int c = 0; c < kPairCols; c += kPass) {
-                float2 acc[kPass / 2];
-                uint32_t raw[kPass / 16][16];
 #pragma unroll
-                for (int i = 0; i < kPass; i += 16) ptx::tmem_ld_32x32b_x16(taddr + c + i, raw[i / 16]);
-#pragma unroll
-                for (int i = 0; i < kPass; i += 16) ptx::tmem_ld_wait(raw[i / 16]);
-                if (c + kPass == kPairCols) {
+            for (int k = 0; k < kWide / 64; ++k) {
+                const int c = c0 + k * 32, rows = c1 - c;
+                if (rows <= 0) break;
+                uint32_t raw[2][16];
+                const uint32_t taddr = taddr0 + (uint32_t)(buf * kWide + c);
+                ptx::tmem_ld_32x32b_x16(taddr, raw[0]);
+                if (rows > 16) ptx::tmem_ld_32x32b_x16(taddr + 16, raw[1]);
+                ptx::tmem_ld_wait(raw[0]);
+                ptx::tmem_ld_wait(raw[1]);
+                if (rows <= 32) {
                     ptx::tc_fence_before_sync();
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive_cluster_u32(tempty_lead + buf * 8);
                 }
+                float v[32];
 #pragma unroll
-                for (int i = 0; i < kPass; i += 2) {
-                    const float2 b = *reinterpret_cast<const float2*>(my_scales + kPairCols + c + i);
-                    const float u = sum_of<kKind>(raw[i / 16][i % 16]), v = sum_of<kKind>(raw[i / 16][i % 16 + 1]);
-                    if (kKind == kInt8) {
-                        const float2 ws = *reinterpret_cast<const float2*>(my_scales + c + i);
-                        acc[i / 2] = make_float2(fmaf(u, as * ws.x, b.x), fmaf(v, as * ws.y, b.y));
-                    } else {
-                        acc[i / 2] = make_float2(u + b.x, v + b.y);
-                    }
+                for (int i = 0; i < 32; ++i) {
+                    const float u = sum_of<kKind>(raw[i / 16][i % 16]);
+                    v[i] = kKind == kInt8 ? fmaf(u, __shfl_sync(0xffffffffu, as[k], i) * ws, start) : u + start;
                 }
-                if (p.y_dtype == EXB_F16) store_rows(acc, stage, static_cast<__half*>(p.y), p.y_stride, row0, col + c, of.end, p.N, p.vec, lane);
-                else if (p.y_dtype == EXB_BF16) store_rows(acc, stage, static_cast<__nv_bfloat16*>(p.y), p.y_stride, row0, col + c, of.end, p.N, p.vec, lane);
-                else store_rows(acc, stage, static_cast<float*>(p.y), p.y_stride, row0, col + c, of.end, p.N, p.vec, lane);
+                store_columns(p, v, of.m0 + c, n, rows);
             }
+            if (c0 >= c1 && lane == 0) ptx::mbar_arrive_cluster_u32(tempty_lead + buf * 8);      // (none of its columns has a row)
+            __syncwarp();
             if (++buf == 2) {
                 buf = 0;
                 acc_phase ^= 1u;
@@ -551,36 +575,48 @@ __global__ void __launch_bounds__(kPairThreads, 1) product_pair_kernel(const __g
     ptx::cluster_sync();      // neither CTA leaves while its peer may still signal its barriers or read its TMEM
     if (warp == 1) {
         ptx::tc_fence_after_sync();
-        ptx::tmem_dealloc_pair(tmem_base, 2 * kPairN);
+        ptx::tmem_dealloc_pair(tmem_base, 2 * kWide);
     }
 }
 
 // Which kernel and how it divides the product.
+//  - Up to 64 rows, or groups that have half as many on the average: the kernel for few rows, which has one tile for nearly every group.  (Groups of 32 on the
+//    average, 1024 x 2048 x 2048 bf16 over 32: 48.2 us with 64 columns, 48.3 in pairs; of 64, 4096 x 2048 x 2048 over 64: 99.4 with 128 columns, 93 in pairs.)
+//  - Otherwise the least of what was measured (8-bit and 16-bit alike: a K block has as many MMA cycles), us:
+//    few rows, 128 columns: 5 + 2.2 where K is divided + 0.45 a block (128 x 4096 x 4096 11 to 12, in pairs 13);
+//    pairs, 128 rows: 5 + 0.21 to 0.24 a block (512 x 4096 x 4096 11.8, 333 x 1000 x 1234 7.3);
+//    pairs, 256 rows: 5 + 0.345 a block (512 x 4096 x 4096 16, 2048 x 4096 x 4096 26.9 and with 128 rows 32).
 struct Plan {
     bool few;
-    int tile, splits;      // rows of a (few) or of w (pairs) in a tile
+    int tile, splits;      // rows of a in a tile, parts of K
+    int each;              // CTAs of an SM (few)
 };
 Plan plan_for(int sms, int M, int N, int blocks, int experts) {
-    const int64_t n_tiles = ((int64_t)N + 127) / 128;
-    const int groups = std::max(1, std::min(experts, M));
-    const int each = (M + groups - 1) / groups;
-    auto tiles = [&](int rows) { return std::min<int64_t>(M, ((int64_t)M + (int64_t)groups * (rows - 1)) / rows) * n_tiles; };      // at most
-    auto parts = [&](int64_t t, bool two) {
+    const int64_t n_tiles = ((int64_t)N + 127) / 128, n_pairs = ((int64_t)N + 255) / 256;
+    const int64_t groups = std::max(1, std::min(experts, M)), each = (M + groups - 1) / groups;
+    auto m_tiles = [&](int rows) { return std::min<int64_t>(M, (M + groups * (rows - 1)) / rows); };                      // at most
+    auto m_likely = [&](int rows) { return std::max<int64_t>(groups, (M + (groups > 1 ? groups * rows / 2 : rows - 1)) / rows); };
+    // Parts of K, of at least two blocks each.  Clusters of several CTAs do not fill the SMs to the last: up to nine tenths are counted on.  Of one CTA an SM
+    // as long as that leaves no more than three tenths of the SMs out; otherwise of two, and up to 1.65 an SM.  (64 rows, K = 4096, one and two CTAs an SM, each with
+    // its best number of parts: N = 1024 and K = 14336 8.3 and 9.7 us, N = 4096 8.2 and 8.6, N = 6144 (32 rows) 9.2 and 8.1, N = 14336 15.0 and 15.8; 1 row, N = 4096
+    // 6.5 and 6.4, N = 14336 12.3 and 13.4.)
+    auto few = [&](int cols) -> Plan {
+        const int64_t t = m_tiles(cols) * n_tiles;
         auto within = [&](int64_t places) { return std::max<int64_t>(1, std::min<int64_t>({8, places / t, blocks / 2})); };
-        const int64_t s = within(sms * 9 / 10);
-        return (int)(two && t * s * 5 < sms * 4 ? within(sms * 33 / 20) : s);
+        const int64_t one = t <= sms ? within(sms * 9 / 10) : 0;
+        if (cols == 128) return {true, cols, (int)std::max<int64_t>(one, 1), 1};
+        if (one && (t * one * 10 >= sms * 7 || one == 8)) return {true, cols, (int)one, 1};
+        return {true, cols, (int)within(sms * 33 / 20), 2};
     };
-    const int rows = experts ? 2 * each : M;
-    if (rows <= 64) {
-        const int cols = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-        return {true, cols, parts(tiles(cols), true)};
-    }
-    if (rows <= 128) return {true, 128, parts(tiles(128), false)};
+    const int64_t rows = experts ? 2 * each : M;
+    if (rows <= 64) return few(rows <= 16 ? 16 : rows <= 32 ? 32 : 64);
     auto rounds = [](int64_t t, int64_t places) { return (double)((t + places - 1) / places); };
-    const int64_t m_pairs = ((int64_t)M + (int64_t)groups * (kPairM / 2)) / kPairM;
-    const double pair128 = 5.0 + 0.17 * rounds(m_pairs * n_tiles, sms / 2) * blocks;
-    const double pair256 = 5.0 + 0.28 * rounds(m_pairs * (((int64_t)N + 255) / 256), sms / 2) * blocks;
-    return {false, pair128 < pair256 ? 128 : 256, 1};
+    const Plan narrow = few(128);
+    const double few128 = 5.0 + (narrow.splits > 1 ? 2.2 : 0.0) + 0.45 * rounds(m_likely(128) * n_tiles * narrow.splits, sms) * ((blocks + narrow.splits - 1) / narrow.splits);
+    const double rounds128 = rounds(m_likely(128) * n_pairs, sms / 2), pair128 = 5.0 + (rounds128 > 4 ? 0.235 : 0.212) * rounds128 * blocks;
+    const double pair256 = 5.0 + 0.345 * rounds(m_likely(256) * n_pairs, sms / 2) * blocks;
+    if (few128 < pair128 && few128 < pair256) return narrow;
+    return {false, pair128 < pair256 ? 128 : 256, 1, 1};
 }
 
 // Rows of `bytes` of each expert in boxes of 128 bytes x box_rows, 128-byte swizzle; zeros beyond the matrix.
@@ -601,23 +637,26 @@ int run(exb_ctx* ctx, const char* what, ProductParams& p, const Plan& plan, cons
         int64_t expert_bytes, cudaStream_t st) {
     const int64_t M = p.M, experts = std::max(p.experts, 1), groups = std::min<int64_t>(experts, M);
     const size_t table = p.experts ? (size_t)p.experts * sizeof(int2) : 0;
-    const int box_a = plan.few ? plan.tile : 128, box_w = plan.few ? 128 : plan.tile / 2;
+    const int box_a = plan.few ? plan.tile : plan.tile / 2;
     if (int rc = encode_rows(what, &p.tmA, static_cast<const uint8_t*>(a), M, (int)K_bytes, a_bytes, box_a)) return rc;
-    if (int rc = encode_experts(what, &p.tmW, w, p.N, K_bytes, w_bytes, experts, expert_bytes, box_w)) return rc;
-    const int rows = plan.few ? plan.tile : kPairM, width = plan.few ? 128 : plan.tile;
+    if (int rc = encode_experts(what, &p.tmW, w, p.N, K_bytes, w_bytes, experts, expert_bytes, 128)) return rc;
+    const int rows = plan.tile, width = plan.few ? 128 : 256;
     p.n_tiles = (p.N + width - 1) / width;
     p.splits = plan.splits;
     const int64_t tiles = std::min<int64_t>(M, (M + groups * (rows - 1)) / rows) * p.n_tiles;      // at most
     if (tiles > INT32_MAX / 16) return fail(EXB_ERR_UNSUPPORTED, "%s: %lld x %d is too large for one call", what, (long long)M, p.N);
-    p.idesc = ptx::make_idesc(kKind == kInt8, plan.few ? 128 : kPairM, (uint32_t)plan.tile) | (kKind == kBfloat ? 1u << 7 | 1u << 10 : 0u);
+    // (pairs: the columns are the tile's)
+    p.idesc = ptx::make_idesc(kKind == kInt8, plan.few ? 128 : 256, plan.few ? (uint32_t)plan.tile : 0u) | (kKind == kBfloat ? 1u << 7 | 1u << 10 : 0u);
     if (plan.few) {
         auto go = [&](auto c) {
             constexpr int kCols = decltype(c)::value;
             if (int rc = raise_smem_limit(ctx, product_few_kernel<kKind, kCols>)) return rc;
-            const int64_t places = (int64_t)ctx->sm_count * (kCols == 128 ? 1 : 2);
+            const int64_t places = (int64_t)ctx->sm_count * plan.each;
             const int64_t grid = plan.splits > 1 ? tiles * plan.splits : std::min(tiles, places);
+            const int room = (plan.each == 1 ? 220 : 108) * 1024 - (int)table - few_smem(kCols, 0, plan.splits > 1);
+            p.stages = std::min(kFewMostStages, room / few_stage_bytes(kCols));
             return launch_pdl_cluster(ctx, "product_few_kernel", product_few_kernel<kKind, kCols>, dim3((unsigned)grid), dim3(96 + few_epi_warps(kCols) * 32),
-                                      dim3(plan.splits), (size_t)few_smem(kCols) + table, st, p);
+                                      dim3(plan.splits), (size_t)few_smem(kCols, p.stages, plan.splits > 1) + table, st, p);
         };
         if (plan.tile == 16) return go(std::integral_constant<int, 16>());
         if (plan.tile == 32) return go(std::integral_constant<int, 32>());
@@ -626,10 +665,10 @@ int run(exb_ctx* ctx, const char* what, ProductParams& p, const Plan& plan, cons
     }
     const int64_t places = ctx->sm_count / 2;
     auto go = [&](auto c) {
-        constexpr int kN = decltype(c)::value;
-        if (int rc = raise_smem_limit(ctx, product_pair_kernel<kKind, kN>)) return rc;
-        return launch_pdl_cluster(ctx, "product_pair_kernel", product_pair_kernel<kKind, kN>, dim3((unsigned)(2 * std::min(tiles, places))), dim3(kPairThreads), dim3(2),
-                                  (size_t)pair_smem(kN) + table, st, p);
+        constexpr int kWide = decltype(c)::value;
+        if (int rc = raise_smem_limit(ctx, product_pair_kernel<kKind, kWide>)) return rc;
+        return launch_pdl_cluster(ctx, "product_pair_kernel", product_pair_kernel<kKind, kWide>, dim3((unsigned)(2 * std::min(tiles, places))), dim3(kPairThreads), dim3(2),
+                                  (size_t)pair_smem(kWide) + table, st, p);
     };
     return plan.tile == 256 ? go(std::integral_constant<int, 256>()) : go(std::integral_constant<int, 128>());
 }

@@ -164,7 +164,7 @@ struct Parts {
 template <typename T, bool kW>
 struct Seen {
     // vectors that are asked for at a time (16 bits: 4, 6 and 8 took 47.8, 47.1 and 49.8 us for 2048 rows of 50001)
-    static constexpr int kAhead = sizeof(T) == 4 ? 8 : 6;
+    static constexpr int kAhead = sizeof(T) == 4 || !kW ? 8 : 6;
     Sums r = {-INFINITY, 0.f, 0.f, -INFINITY};
     float2 s2 = {0.f, 0.f}, w2 = {0.f, 0.f};      // on top of r.s and r.w
     float c;
@@ -303,6 +303,26 @@ __device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
     return __reduce_min_sync(0xffffffffu, larger < n ? v : 0xffffffffu);
 }
 
+// A bound not above the n-th largest of 32 * kEach values: its upper 20 bits, found from the top (0 if there are fewer).  The more groups the threads' largest
+// are divided into, the nearer their n-th largest is to that of the threads themselves: of 32 groups the 32nd is the least, and 130 threads hold something not
+// below it; of 64 or 128 groups 44 or 37 do.
+constexpr int kFewTop = 16;
+template <int kEach>
+__device__ __forceinline__ uint32_t least_of_groups(const uint32_t* values, int n, int lane) {
+    uint32_t v[kEach], low = 0;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) v[k] = values[k * 32 + lane];
+#pragma unroll 1
+    for (int bit = 31; bit >= 12; --bit) {
+        const uint32_t at = low | 1u << bit;
+        int above = 0;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) above += v[k] >= at;
+        if ((int)__reduce_add_sync(0xffffffffu, above) >= n) low = at;
+    }
+    return low;
+}
+
 // How many of n keys are before (above) one.
 __device__ __forceinline__ int count_before(const unsigned long long* keys, int n, unsigned long long key) {
     int before = 0;
@@ -320,7 +340,7 @@ struct Shared {
     Sums part[kThreads / 32];
     Sums row[kSplitMax];                                   // (of the cluster's CTAs, in the first one)
     unsigned long long best[kSplitMax * kMaxTop];         // the same: the `top` best of each, in order
-    uint32_t largest[kThreads / 8];                        // of 8 threads each
+    uint32_t largest[kThreads / 4];                        // of 8 or 4 threads each
     unsigned long long list[kRoom > kThreads ? kRoom : kThreads];
     int threads[kThreads];
     unsigned long long tau;
@@ -366,6 +386,12 @@ struct Row {
 template <typename T>
 __device__ __forceinline__ bool row_known(const Sums& all, float c) {
     return all.s > 0.f && all.s < INFINITY && fabsf(all.w) < INFINITY && fmaf(Vec<T>::kLow, c, -all.e) < -150.f;
+}
+
+// Of sums that answer it (see row_known).
+__device__ __forceinline__ Row row_of(const Sums& all, float scale) {
+    const float log_s = log2f(all.s);
+    return {all.m, log_s - fmaf(all.m, scale * kLog2e, -all.e), max_nan((log_s - all.w / all.s) * kLn2, 0.f), false, scale};
 }
 
 template <typename T, int kThreads, typename Args>
@@ -457,15 +483,9 @@ __device__ __forceinline__ void rows_by_warps(const Args& a, int64_t n_rows) {
     seen.stream(part.body, lane, part.vecs, 32);
     if (lane < n_tail) seen.single(to_float<T>(x[part.tail0 + lane]));
     const Sums all = warp_sums<Args::kEntropy>(seen.r);
-    Row out;
-    out.scale = a.scale;
-    out.m = all.m;
-    out.empty = false;
+    Row out = row_of(all, a.scale);
     const bool known = row_known<T>(all, seen.c);
     if (known) {
-        const float log_s = log2f(all.s);
-        out.entropy = max_nan((log_s - all.w / all.s) * kLn2, 0.f);
-        out.log_s = log_s - fmaf(all.m, seen.c, -all.e);
         if (lane == 0) a.row_is(row, out);
         a.template given<T>(x, row, out, lane, 32);
     }
@@ -515,65 +535,51 @@ __device__ __forceinline__ void rows_by_warps(const Args& a, int64_t n_rows) {
     if (slow) slow_row<T, 32>(a, x, row, nullptr, &s_best[warp], known, out);
 }
 
-// gridDim.x = rows * splits, the CTAs of a row are a cluster (kNarrow threads: one CTA a row).
-template <typename T, int kThreads, typename Args>
-__device__ __forceinline__ void rows_by_ctas(const Args& a) {
-    __shared__ Shared<kThreads> sh;
+// What a CTA makes of its part of a row: the sums, alike in all threads, and its `top` largest elements' keys in order through put(place, key) (0 where there are
+// fewer), or too_many where it cannot tell.  Of the row's vectors it has [lo, hi) and a thread every kThreads-th; n_head and n_tail elements
+// before and behind them.  ready(): called by all before the first put.
+struct PartSeen {
+    Sums all;
+    bool too_many;
+};
+template <typename T, int kThreads, bool kW, typename Ready, typename Put>
+__device__ __forceinline__ PartSeen see_part(const T* x, const Parts<T>& part, float c, int top, int lo, int hi, int n_head, int n_tail, Shared<kThreads>& sh,
+                                             Ready&& ready, Put&& put) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int splits = kThreads == kWide ? a.splits : 1;
-    const int64_t row = blockIdx.x / splits;
-    const int rank = (int)(blockIdx.x - row * splits);
-    const T* x = static_cast<const T*>(a.logits) + row * a.stride;
-    // Of the row's vectors this CTA has [lo, hi) and a thread every kThreads-th; the head is with the first CTA, the tail with the last.
-    const Parts<T> part(x, a.V);
-    const int head = part.head, vecs = part.vecs, tail0 = part.tail0;
-    const uint4* body = part.body;
-    const int lo = (int)((int64_t)rank * vecs / splits), hi = (int)((int64_t)(rank + 1) * vecs / splits);
-    const int n_head = rank == 0 ? head : 0, n_tail = rank == splits - 1 ? a.V - tail0 : 0;
-    const float c = a.scale * kLog2e;
-    if (tid == 0) {
-        sh.n_list = 0;
-        sh.n_threads = 0;
-        sh.tau = 0;
-    }
-    if (splits > 1) ptx::cluster_arrive();      // (waited for before anything is written into the first CTA)
-    pdl_enter();
-    if (a.left_out(row)) {      // (alike in all of the row's CTAs)
-        if (splits > 1) {
-            __syncwarp();
-            ptx::cluster_wait();
-        }
-        return;
-    }
-
-    Seen<T, Args::kEntropy> seen;
+    Seen<T, kW> seen;
     seen.c = c;
     if (tid < n_head) seen.single(to_float<T>(x[tid]));
-    seen.stream(body, lo + tid, hi, kThreads);
-    if (tid < n_tail) seen.single(to_float<T>(x[tail0 + tid]));
+    seen.stream(part.body, lo + tid, hi, kThreads);
+    if (tid < n_tail) seen.single(to_float<T>(x[part.tail0 + tid]));
 
-    Sums all = warp_sums<Args::kEntropy>(seen.r);
+    const Sums all = warp_sums<kW>(seen.r);
     if (lane == 0) sh.part[warp] = all;
     const bool any = tid < n_head || lo + tid < hi || tid < n_tail;
     const uint32_t mine = any ? order_of(seen.r.m) : 0;
-    if (a.top) {
-        uint32_t g = mine;
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if ((lane & 7) == 0) sh.largest[tid >> 3] = g;
+    if (top) {      // of 8 threads each, or of 4 where many tokens are asked for (see least_of_groups)
+        uint32_t g = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+        g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
+        if (top > kFewTop) {
+            if ((lane & 3) == 0) sh.largest[tid >> 2] = g;
+        } else {
+            g = max(g, __shfl_xor_sync(0xffffffffu, g, 4));
+            if ((lane & 7) == 0) sh.largest[tid >> 3] = g;
+        }
     }
-    if (splits > 1) {
-        __syncwarp();
-        ptx::cluster_wait();
-    }
+    ready();
     __syncthreads();
     bool too_many = false;
     int n_best = 0;
-    if (a.top) {
+    if (top) {
         if (warp == 0) {      // (with 64 groups a lane has the larger of two: the bound is lower, and serves all the same)
-            uint32_t g = sh.largest[lane];
-            if constexpr (kThreads == kWide) g = max(g, sh.largest[lane + 32]);
-            g = nth_largest(g, a.top);
+            uint32_t g;
+            if (top > kFewTop) {
+                g = least_of_groups<kThreads / 128>(sh.largest, top, lane);
+            } else {
+                g = sh.largest[lane];
+                if constexpr (kThreads == kWide) g = max(g, sh.largest[lane + 32]);
+                g = nth_largest(g, top);
+            }
             if (lane == 0) sh.tau = (unsigned long long)g << 32;
         }
         __syncthreads();
@@ -607,29 +613,71 @@ __device__ __forceinline__ void rows_by_ctas(const Args& a) {
             }
             __syncthreads();
             const int before = count_before(sh.list, kThreads, key);
-            if (key && before == a.top - 1) sh.tau = key;
+            if (key && before == top - 1) sh.tau = key;
             __syncthreads();
             tau = sh.tau;
             looked = key != 0 && key >= tau;
             if (tid == 0) sh.n_list = 0;
         }
         too_many = n > kRoom;
-        n_best = min(n, a.top);
+        n_best = min(n, top);
         if (!too_many) {
-            unsigned long long* to = splits > 1 ? nullptr : sh.best;
             for (int k = tid; k < n; k += kThreads) {
                 const unsigned long long key = sh.list[k];
                 const int before = count_before(sh.list, n, key);
-                if (before < a.top) {
-                    if (to) to[before] = key;
-                    else ptx::st_cta_u64(ptx::map_to_cta(ptx::smem_u32(&sh.best[rank * a.top + before]), 0), key);
-                }
+                if (before < top) put(before, key);
             }
-            if (splits > 1 && tid >= n_best && tid < a.top) ptx::st_cta_u64(ptx::map_to_cta(ptx::smem_u32(&sh.best[rank * a.top + tid]), 0), 0);
+            if (tid >= n_best && tid < top) put(tid, 0ull);
         }
     }
     // (the warps' sums, in every warp for itself)
-    all = warp_sums<Args::kEntropy>(lane < kThreads / 32 ? sh.part[lane] : Sums{-INFINITY, 0.f, 0.f, -INFINITY});
+    return {warp_sums<kW>(lane < kThreads / 32 ? sh.part[lane] : Sums{-INFINITY, 0.f, 0.f, -INFINITY}), too_many};
+}
+
+// gridDim.x = rows * splits, the CTAs of a row are a cluster (kNarrow threads: one CTA a row).
+template <typename T, int kThreads, typename Args>
+__device__ __forceinline__ void rows_by_ctas(const Args& a) {
+    __shared__ Shared<kThreads> sh;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int splits = kThreads == kWide ? a.splits : 1;
+    const int64_t row = blockIdx.x / splits;
+    const int rank = (int)(blockIdx.x - row * splits);
+    const T* x = static_cast<const T*>(a.logits) + row * a.stride;
+    // (the head is with the first CTA, the tail with the last)
+    const Parts<T> part(x, a.V);
+    const int lo = (int)((int64_t)rank * part.vecs / splits), hi = (int)((int64_t)(rank + 1) * part.vecs / splits);
+    const int n_head = rank == 0 ? part.head : 0, n_tail = rank == splits - 1 ? a.V - part.tail0 : 0;
+    const float c = a.scale * kLog2e;
+    if (tid == 0) {
+        sh.n_list = 0;
+        sh.n_threads = 0;
+        sh.tau = 0;
+    }
+    if (splits > 1) ptx::cluster_arrive();      // (waited for before anything is written into the first CTA)
+    pdl_enter();
+    if (a.left_out(row)) {      // (alike in all of the row's CTAs)
+        if (splits > 1) {
+            __syncwarp();
+            ptx::cluster_wait();
+        }
+        return;
+    }
+
+    unsigned long long* best = sh.best;
+    const PartSeen seen = see_part<T, kThreads, Args::kEntropy>(
+        x, part, c, a.top, lo, hi, n_head, n_tail, sh,
+        [&] {
+            if (splits > 1) {
+                __syncwarp();
+                ptx::cluster_wait();
+            }
+        },
+        [&](int place, unsigned long long key) {
+            if (splits == 1) best[place] = key;
+            else ptx::st_cta_u64(ptx::map_to_cta(ptx::smem_u32(&best[rank * a.top + place]), 0), key);
+        });
+    Sums all = seen.all;
+    bool too_many = seen.too_many;
     if (splits > 1) {      // the first CTA finishes the row
         if (tid == 0) {
             const uint32_t to = ptx::map_to_cta(ptx::smem_u32(&sh.row[rank]), 0);
@@ -643,15 +691,9 @@ __device__ __forceinline__ void rows_by_ctas(const Args& a) {
         all = warp_sums<Args::kEntropy>(lane < splits ? sh.row[lane] : Sums{-INFINITY, 0.f, 0.f, -INFINITY});
         too_many = __any_sync(0xffffffffu, lane < splits && sh.too_many[lane] != 0);
     }
-    Row out;
-    out.scale = a.scale;
-    out.m = all.m;
-    out.empty = false;
+    Row out = row_of(all, a.scale);
     const bool known = row_known<T>(all, a.scale * kLog2e);
     if (known) {
-        const float log_s = log2f(all.s);
-        out.entropy = max_nan((log_s - all.w / all.s) * kLn2, 0.f);
-        out.log_s = log_s - fmaf(all.m, c, -all.e);
         if (tid == 0) a.row_is(row, out);
         a.template given<T>(x, row, out, tid, kThreads);
     }
@@ -665,9 +707,7 @@ __device__ __forceinline__ void rows_by_ctas(const Args& a) {
         for (int k = tid; k < n; k += kThreads) {
             const unsigned long long mine = sh.best[k];
             const int before = splits == 1 ? k : count_before(sh.best, n, mine);
-            if (before < a.top && mine) {
-                a.best_is(row, before, index_of(mine), logit_of(mine), out);
-            }
+            if (before < a.top && mine) a.best_is(row, before, index_of(mine), logit_of(mine), out);
         }
     }
 }

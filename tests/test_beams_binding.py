@@ -49,7 +49,7 @@ def test_a_good_call_gets_as_far_as_the_device(call, changed):
     (select, dict(beams=33), UNSUPPORTED), (select, dict(select=33), UNSUPPORTED), (select, dict(sentences=1 << 31), UNSUPPORTED), (select, dict(V=(1 << 30) + 1, stride=1 << 31), UNSUPPORTED),
     (select, dict(scale=0.0), BAD), (select, dict(scale=-1.0), BAD), (select, dict(scale=float("nan")), BAD), (select, dict(scale=float("inf")), BAD),
     (select, dict(end_token=-1), BAD), (select, dict(end_token=1000), BAD), (select, dict(stride=999), BAD), (select, dict(workspace_bytes=8 * 12 * 9 - 1), BAD),
-    *[(select, {k: None}, BAD) for k in ("logits", "scores", "out", "parents", "tokens", "workspace")],
+    *[(select, {k: None}, BAD) for k in ("logits", "scores", "out", "parents", "tokens")],
     (select, dict(logits=A + 1), BAD), (select, dict(scores=S + 2), BAD), (select, dict(out=O + 1), BAD), (select, dict(tokens=T + 2), BAD), (select, dict(workspace=W + 4), BAD),
     (select, dict(out=S), BAD), (select, dict(parents=A + 8), BAD), (select, dict(tokens=P + 4), BAD), (select, dict(workspace=A + 16), BAD), (select, dict(workspace=O), BAD),
     (select, dict(out=N), BAD),
@@ -63,6 +63,12 @@ def test_a_good_call_gets_as_far_as_the_device(call, changed):
 ])
 def test_bad_calls_are_refused(call, changed, code):
     assert call(**changed)[0] == code, changed
+
+
+@pytest.mark.skipif(not _no_gpu(), reason="the addresses are not real")
+def test_a_call_needs_a_workspace_or_none():
+    """(The device is looked for first: what this machine cannot show, the selection's own tests do.)"""
+    assert select(workspace=None, workspace_bytes=0)[0] == -3
 
 
 def test_empty_calls_are_no_error():
