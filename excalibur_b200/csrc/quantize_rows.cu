@@ -61,46 +61,54 @@ __device__ __forceinline__ void store_share(const Kept<T, kL>& k, int8_t* q, flo
     }
 }
 
-// kRowWarps warps of a CTA have a row, up to kShares shares each (every kRowWarps-th).
-template <typename T, Layout kL, int kRowWarps, int kShares>
-__global__ void __launch_bounds__(kThreads) quantize_whole_rows_kernel(const T* __restrict__ x, int64_t x_stride, int8_t* __restrict__ q, int64_t q_stride,
-                                                                       float* __restrict__ scales, int64_t rows, int C, Span span) {
-    __shared__ uint32_t s_max[kWarps];
+// kRowWarps warps of a CTA have kRows rows, up to kShares shares of each (every kRowWarps-th).
+template <typename T, Layout kL, int kRowWarps, int kShares, int kRows>
+__global__ void __launch_bounds__(kRowWarps > kWarps ? kRowWarps * 32 : kThreads)
+quantize_whole_rows_kernel(const T* __restrict__ x, int64_t x_stride, int8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int64_t rows, int C,
+                           Span span) {
+    static_assert(kRowWarps == 1 || kRows == 1, "several rows for a warp alone");
+    constexpr int kGroups = kRowWarps > kWarps ? 1 : kWarps / kRowWarps;      // of warps with rows of their own
+    __shared__ uint32_t s_max[kGroups * kRowWarps];
     pdl_enter();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kRowWarps;
-    const int64_t r = (int64_t)blockIdx.x * (kWarps / kRowWarps) + warp / kRowWarps;
-    const bool mine = r < rows;
-    const bool inside = r >= 8 && r < rows - 8;
-    const T* at = x + r * x_stride;
-    Kept<T, kL> k[kShares];
+    const int64_t r0 = ((int64_t)blockIdx.x * kGroups + warp / kRowWarps) * kRows;
+    const bool inside = r0 >= 8 && r0 + kRows <= rows - 8;
+    Kept<T, kL> k[kRows][kShares];
+    auto valid = [&](int r, int i) { return r0 + r < rows ? C - (i * kRowWarps + part) * kShare : 0; };      // elements of the share
+    auto at = [&](int r, int i) { return x + (r0 + r) * x_stride + (i * kRowWarps + part) * kShare; };
 #pragma unroll
-    for (int i = 0; i < kShares; ++i) {
-        const int c0 = (i * kRowWarps + part) * kShare;
-        if (mine && c0 < C) k[i].load(at + c0, C - c0, lane, span, inside);
-        else k[i].none();
-    }
-    uint32_t m = 0;
+    for (int r = 0; r < kRows; ++r)
 #pragma unroll
-    for (int i = 0; i < kShares; ++i) {
-        const int c0 = (i * kRowWarps + part) * kShare;
-        if (mine && c0 < C) k[i].settle(at + c0, C - c0, lane);
-        m = max(m, largest_bits(k[i]));
+        for (int i = 0; i < kShares; ++i) {
+            if (valid(r, i) > 0) k[r][i].load(at(r, i), valid(r, i), lane, span, inside);
+            else k[r][i].none();
+        }
+    uint32_t m[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        m[r] = 0;
+#pragma unroll
+        for (int i = 0; i < kShares; ++i) {
+            if (valid(r, i) > 0) k[r][i].settle(at(r, i), valid(r, i), lane);
+            m[r] = max(m[r], largest_bits(k[r][i]));
+        }
+        m[r] = __reduce_max_sync(0xffffffffu, m[r]);
     }
-    m = __reduce_max_sync(0xffffffffu, m);
     if constexpr (kRowWarps > 1) {
-        if (lane == 0) s_max[warp] = m;
+        if (lane == 0) s_max[warp] = m[0];
         __syncthreads();
         const int first = warp / kRowWarps * kRowWarps;
 #pragma unroll
-        for (int i = 0; i < kRowWarps; ++i) m = max(m, s_max[first + i]);
+        for (int i = 0; i < kRowWarps; ++i) m[0] = max(m[0], s_max[first + i]);
     }
-    if (!mine) return;
-    const Scale s = scale_of(m);
-    if (part == 0 && lane == 0) scales[r] = s.scale;
 #pragma unroll
-    for (int i = 0; i < kShares; ++i) {
-        const int c0 = (i * kRowWarps + part) * kShare;
-        if (c0 + lane * 8 < C) store_share(k[i], q + r * q_stride + c0 + lane * 8, s.inverse, C - c0 - lane * 8);
+    for (int r = 0; r < kRows; ++r) {
+        if (r0 + r >= rows) break;
+        const Scale s = scale_of(m[r]);
+        if (part == 0 && lane == 0) scales[r0 + r] = s.scale;
+#pragma unroll
+        for (int i = 0; i < kShares; ++i)
+            if (lane * 8 < valid(r, i)) store_share(k[r][i], q + (r0 + r) * q_stride + (i * kRowWarps + part) * kShare + lane * 8, s.inverse, valid(r, i) - lane * 8);
     }
 }
 
@@ -138,14 +146,20 @@ __global__ void __launch_bounds__(kThreads) quantize_long_rows_kernel(const T* _
 template <typename T, Layout kL>
 void launch(const exb_ctx* ctx, const T* x, int64_t x_stride, int8_t* q, int64_t q_stride, float* scales, int64_t rows, int C, const Span& span, cudaStream_t st) {
     const int64_t shares = ((int64_t)C + kShare - 1) / kShare;
-    auto go = [&](auto kernel, int rows_each) {
-        launch_overlapped(ctx, kernel, dim3((unsigned)((rows + rows_each - 1) / rows_each)), dim3(kThreads), st, x, x_stride, q, q_stride, scales, rows, C, span);
+    auto go = [&](auto kernel, int rows_each, int threads = kThreads) {
+        launch_overlapped(ctx, kernel, dim3((unsigned)((rows + rows_each - 1) / rows_each)), dim3(threads), st, x, x_stride, q, q_stride, scales, rows, C, span);
     };
-    if (shares <= 2) go(quantize_whole_rows_kernel<T, kL, 1, 2>, 8);
-    else if (shares <= 8) go(quantize_whole_rows_kernel<T, kL, 4, 2>, 2);
-    else if (shares <= 16) go(quantize_whole_rows_kernel<T, kL, 8, 2>, 1);
-    else if (shares <= 32) go(quantize_whole_rows_kernel<T, kL, 8, 4>, 1);
-    else if (shares <= 64) go(quantize_whole_rows_kernel<T, kL, 8, 8>, 1);
+    // Few rows are divided among as many warps as have something to do; of many a warp has four shares under way, of one row or of several short ones.
+    const bool many = rows * shares > 64 * (int64_t)ctx->sm_count;
+    constexpr int kLongest = sizeof(T) == 2 ? 128 : 64;
+    if (shares <= 1) many ? go(quantize_whole_rows_kernel<T, kL, 1, 1, 4>, 32) : go(quantize_whole_rows_kernel<T, kL, 1, 1, 1>, 8);
+    else if (shares <= 2) many ? go(quantize_whole_rows_kernel<T, kL, 1, 2, 2>, 16) : go(quantize_whole_rows_kernel<T, kL, 2, 1, 1>, 4);
+    else if (shares <= 4) many ? go(quantize_whole_rows_kernel<T, kL, 1, 4, 1>, 8) : go(quantize_whole_rows_kernel<T, kL, 4, 1, 1>, 2);
+    else if (shares <= 8) many ? go(quantize_whole_rows_kernel<T, kL, 2, 4, 1>, 4) : go(quantize_whole_rows_kernel<T, kL, 8, 1, 1>, 1);
+    else if (shares <= 16) many ? go(quantize_whole_rows_kernel<T, kL, 4, 4, 1>, 2) : go(quantize_whole_rows_kernel<T, kL, 8, 2, 1>, 1);
+    else if (shares <= 32) go(quantize_whole_rows_kernel<T, kL, 8, 4, 1>, 1);
+    else if (shares <= 64) go(quantize_whole_rows_kernel<T, kL, 8, 8, 1>, 1);
+    else if (shares <= kLongest) go(quantize_whole_rows_kernel<T, kL, 16, 8, 1>, 1, 512);
     else go(quantize_long_rows_kernel<T, kL>, 1);
 }
 
