@@ -948,6 +948,27 @@ def token_logprobs(ctx, logits, tokens=None, top=0, scale=1.0):
 
 
 # ---- decoding in 8-bit integers, by experts and with beams -----------------------------------------
+_EMPTY = False      # torch's shortest way to device memory, 0.8 us instead of 1.5; None where this torch does not have it
+
+
+def _room(like, dtype, rows, columns, pitch=None):
+    """Room for (rows, columns) beside `like`, rows `pitch` elements apart."""
+    global _EMPTY
+    if _EMPTY is False:
+        _EMPTY = getattr(getattr(getattr(_TORCH._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+    if pitch is None:
+        pitch = columns
+    if _EMPTY is not None and like.is_cuda:
+        return _EMPTY((rows, columns), (pitch, 1), dtype)      # (on the current device: the library refuses calls for another one)
+    return like.new_empty_strided((rows, columns), (pitch, 1), dtype=dtype)
+
+
+def _room1(like, dtype, n):
+    if _EMPTY and like.is_cuda:
+        return _EMPTY((n,), (1,), dtype)
+    return like.new_empty(n, dtype=dtype)
+
+
 def _int8_row_stride(q, device, what):
     """Row stride of an 8-bit integer matrix, whose rows have to start at multiples of 16 bytes."""
     if q.dtype is not _TORCH.int8:
@@ -968,15 +989,13 @@ def quantize_rows(ctx, x, q=None, scales=None):
     rows, channels = shape
     if q is None:
         qs = (channels + 15) & -16
-        q = x.new_empty(rows, qs, dtype=t.int8)
-        if qs != channels:
-            q = q.as_strided((rows, channels), (qs, 1))
+        q = _room(x, t.int8, rows, channels, qs)
     else:
         qs = _int8_row_stride(q, device, "q")
         if q.shape != shape:
             _refuse("q has to be of x's shape")
     if scales is None:
-        scales = x.new_empty(rows, dtype=t.float32)
+        scales = _room1(x, t.float32, rows)
         sp = scales.data_ptr()
     else:
         sp = _parameter(scales, device, rows, "scales")
@@ -997,7 +1016,7 @@ def int8_matmul(ctx, a, a_scales, w, w_scales, bias=None, out_dtype=EXB_F16, y=N
     if K != k:
         _refuse("a and w have %d and %d columns", K, k)
     if y is None:
-        y = a.new_empty(M, N, dtype=_DTYPES[out_dtype])
+        y = _room(a, _DTYPES[out_dtype], M, N)
         ys = N
     else:
         ys = _row_stride(y, device, "y")
@@ -1063,7 +1082,7 @@ def grouped_matmul(ctx, a, w, ends, a_scales=None, w_scales=None, bias=None, out
     if out_dtype is None:
         out_dtype = EXB_F16 if whole else dt
     if y is None:
-        y = a.new_empty(M, N, dtype=_DTYPES[out_dtype])
+        y = _room(a, _DTYPES[out_dtype], M, N)
         ys = N
     else:
         ys = _row_stride(y, device, "y")
@@ -1098,15 +1117,14 @@ def beam_select(ctx, logits, scores, select=None, scale=1.0, ended=None, end_tok
         ended_p = ended.data_ptr()
     if select is None:
         select = beams
-    out = scores.new_empty(sentences, max(select, 0))
-    parents = t.empty_like(out, dtype=t.int32)
-    tokens = t.empty_like(parents)
+    places = max(select, 0)
+    out, parents, tokens = _room(scores, f32, sentences, places), _room(scores, t.int32, sentences, places), _room(scores, t.int32, sentences, places)
     dt = _DTYPES.get(logits.dtype, -1)
     at = logits.data_ptr(), scores.data_ptr(), ended_p, out.data_ptr(), parents.data_ptr(), tokens.data_ptr()
     rc = lib().exb_beam_select_fwd(ctx._h, _pack_beams(sentences, ls, 0, beams, V, dt, select, end_token, scale), *at, None, _stream())
     if rc == EXB_ERR_NOMEM:      # one of those calls that need a workspace
         room = 8 * rows * (1 + min(select, V))
-        workspace = scores.new_empty(room, dtype=t.uint8)
+        workspace = _room1(scores, t.uint8, room)
         rc = lib().exb_beam_select_fwd(ctx._h, _pack_beams(sentences, ls, room, beams, V, dt, select, end_token, scale), *at, workspace.data_ptr(), _stream())
     if rc:
         check(rc)
