@@ -2,7 +2,9 @@
 // A thread has the same few bytes of all of a sentence's rows: it reads those of the parents of beams that change, and only then writes, so that
 // no row is lost whatever the parents are, and no other thread is waited for.  Beams that are their own parents are neither read nor written
 // (but as another's parent), nor are positions from the sentence's length on.
-// Bound by memory: the beams that change, in and out once.
+// Bound by memory: the beams that change, in and out once.  us (of them at the copy rate): 4 beams of which 2 change, 64 states of 8 x 512 positions x 128 fp16, 42
+// (41); 16 x 8 beams, 6 change, 16 states of 8 x 1024 to 2047 positions x 64 bf16, 665 (737: parents that several beams have are in L2); rows that start anywhere go
+// in units of what divides them: 2 x 5 beams, 43 channels in fp32, 75 (54), 4 x 8 beams, 37 channels in fp16, 15 (7).
 #include <algorithm>
 #include <vector>
 
@@ -38,7 +40,7 @@ __device__ __forceinline__ int64_t columns_of(const ReorderArgs& a, int b) {
 template <typename U, int kMoves, int kColumns>
 __global__ void __launch_bounds__(kThreads) reorder_beams_kernel(const __grid_constant__ ReorderArgs a) {
     __shared__ int s_chunks[kSentences];                        // up to each sentence's end
-    __shared__ uint8_t s_to[kMaxBeams], s_from[kMaxBeams];
+    __shared__ int64_t s_to[kMaxBeams], s_from[kMaxBeams];      // bytes from the sentence's first row
     __shared__ int s_moves;
     constexpr int kChunk = kThreads * kColumns;
     pdl_enter();
@@ -82,8 +84,8 @@ __global__ void __launch_bounds__(kThreads) reorder_beams_kernel(const __grid_co
                 const uint32_t all = __ballot_sync(0xffffffffu, moved);
                 if (moved) {
                     const int k = __popc(all & ((1u << tid) - 1));
-                    s_to[k] = (uint8_t)tid;
-                    s_from[k] = (uint8_t)p;
+                    s_to[k] = tid * a.row_stride;
+                    s_from[k] = p * a.row_stride;
                 }
                 if (tid == 0) s_moves = __popc(all);
             }
@@ -95,7 +97,6 @@ __global__ void __launch_bounds__(kThreads) reorder_beams_kernel(const __grid_co
         uint8_t* base = a.states[which / a.outer] + outer * a.outer_stride + (a.first + lo) * a.beams * a.row_stride;
         const int64_t columns = columns_of<U, kColumns>(a, lo), per = a.bytes / (int64_t)sizeof(U);
         const int64_t column0 = (int64_t)(c - (lo ? s_chunks[lo - 1] : 0)) * kChunk + tid;
-        U v[kColumns][kMoves];
         uint8_t* at[kColumns];
 #pragma unroll
         for (int k = 0; k < kColumns; ++k) {
@@ -104,18 +105,25 @@ __global__ void __launch_bounds__(kThreads) reorder_beams_kernel(const __grid_co
             if (column < columns) {
                 const int64_t position = a.positions > 1 ? column / per : 0;
                 at[k] = base + position * a.position_stride + (column - position * per) * (int64_t)sizeof(U);
-#pragma unroll
-                for (int i = 0; i < kMoves; ++i)
-                    if (i < moves) v[k][i] = *reinterpret_cast<const U*>(at[k] + s_from[i] * a.row_stride);
             }
         }
+        U v[kMoves][kColumns];
 #pragma unroll
-        for (int k = 0; k < kColumns; ++k)
-            if (at[k]) {
+        for (int i = 0; i < kMoves; ++i) {
+            if (i >= moves) break;
+            const int64_t from = s_from[i];
 #pragma unroll
-                for (int i = 0; i < kMoves; ++i)
-                    if (i < moves) *reinterpret_cast<U*>(at[k] + s_to[i] * a.row_stride) = v[k][i];
-            }
+            for (int k = 0; k < kColumns; ++k)
+                if (at[k]) v[i][k] = *reinterpret_cast<const U*>(at[k] + from);
+        }
+#pragma unroll
+        for (int i = 0; i < kMoves; ++i) {
+            if (i >= moves) break;
+            const int64_t to = s_to[i];
+#pragma unroll
+            for (int k = 0; k < kColumns; ++k)
+                if (at[k]) *reinterpret_cast<U*>(at[k] + to) = v[i][k];
+        }
     }
 }
 
@@ -148,15 +156,19 @@ bool meet(const std::vector<Dim>& dims, size_t i, int64_t bytes, int64_t d) {
 template <typename U>
 int launch(const exb_ctx* ctx, const ReorderArgs& a, int beams, cudaStream_t st) {
     const int64_t columns = a.positions * a.bytes / (int64_t)sizeof(U) * a.sentences * a.n_states * a.outer;
+    // Four CTAs an SM, which are there at once.  Bytes on their way: with 16 at a time four columns of up to 4 beams (two and one with more beams: their values are
+    // registers too); smaller units take more columns, and what is left is a load and a store for 32 of them.
     auto go = [&](auto kernel, int each) {
         const int64_t chunks = std::max<int64_t>(1, (columns + each - 1) / each + (int64_t)a.sentences * a.n_states * a.outer);      // at most
-        const int64_t grid = std::min<int64_t>(chunks, (int64_t)ctx->sm_count * 8);
+        const int64_t grid = std::min<int64_t>(chunks, (int64_t)ctx->sm_count * 4);
         return launch_pdl(ctx, "reorder_beams_kernel", kernel, dim3((unsigned)grid), dim3(kThreads), 0, st, a);
     };
-    if (beams <= 4) return go(reorder_beams_kernel<U, 4, 4>, kThreads * 4);
-    if (beams <= 8) return go(reorder_beams_kernel<U, 8, 2>, kThreads * 2);
-    if (beams <= 16) return go(reorder_beams_kernel<U, 16, 1>, kThreads);
-    return go(reorder_beams_kernel<U, 32, 1>, kThreads);
+    constexpr bool kVector = sizeof(U) == 16;
+    constexpr int c4 = kVector ? 4 : 8, c8 = kVector ? 2 : 8, c16 = kVector ? 1 : 4, c32 = kVector ? 1 : 2;
+    if (beams <= 4) return go(reorder_beams_kernel<U, 4, c4>, kThreads * c4);
+    if (beams <= 8) return go(reorder_beams_kernel<U, 8, c8>, kThreads * c8);
+    if (beams <= 16) return go(reorder_beams_kernel<U, 16, c16>, kThreads * c16);
+    return go(reorder_beams_kernel<U, 32, c32>, kThreads * c32);
 }
 
 }  // namespace
@@ -214,7 +226,7 @@ extern "C" int exb_reorder_beams_fwd(exb_ctx* ctx, const exb_reorder_desc* d, vo
         for (int s = 0; s < d->n_states; s += kStates) {
             a.n_states = std::min(kStates, d->n_states - s);
             for (int i = 0; i < a.n_states; ++i) a.states[i] = static_cast<uint8_t*>(states[s + i]);
-            const int rc = bits % 16 == 0 ? launch<uint4>(ctx, a, d->beams, st) : bits % 4 == 0 ? launch<uint32_t>(ctx, a, d->beams, st)
+            const int rc = bits % 16 == 0 ? launch<uint4>(ctx, a, d->beams, st) : bits % 8 == 0 ? launch<uint2>(ctx, a, d->beams, st) : bits % 4 == 0 ? launch<uint32_t>(ctx, a, d->beams, st)
                          : bits % 2 == 0 ? launch<uint16_t>(ctx, a, d->beams, st) : launch<uint8_t>(ctx, a, d->beams, st);
             if (rc) return rc;
         }
