@@ -956,11 +956,9 @@ def _room(like, dtype, rows, columns, pitch=None):
     global _EMPTY
     if _EMPTY is False:
         _EMPTY = getattr(getattr(getattr(_TORCH._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
-    if pitch is None:
-        pitch = columns
     if _EMPTY is not None and like.is_cuda:
-        return _EMPTY((rows, columns), (pitch, 1), dtype)      # (on the current device: the library refuses calls for another one)
-    return like.new_empty_strided((rows, columns), (pitch, 1), dtype=dtype)
+        return _EMPTY((rows, columns), (pitch or columns, 1), dtype)      # (on the current device: the library refuses calls for another one)
+    return like.new_empty_strided((rows, columns), (pitch or columns, 1), dtype=dtype)
 
 
 def _room1(like, dtype, n):
@@ -1008,11 +1006,13 @@ def quantize_rows(ctx, x, q=None, scales=None):
 def int8_matmul(ctx, a, a_scales, w, w_scales, bias=None, out_dtype=EXB_F16, y=None):
     """y (M, N) = a (M, K) @ w (N, K)^T (+ bias) of 8-bit integers, each row of a and each of w with its scale, as quantize_rows gives them."""
     t = _TORCH or _torch()
-    device = ctx.device
-    ast = _int8_row_stride(a, device, "a")
-    wst = _int8_row_stride(w, device, "w")
-    M, K = a.shape
-    N, k = w.shape
+    device, i8, a_shape, w_shape = ctx.device, t.int8, a.shape, w.shape
+    whole = len(a_shape) == 2 and not a_shape[1] & 15 and a.dtype is i8 and a.is_contiguous() and a.get_device() == device
+    ast = a_shape[1] if whole else _int8_row_stride(a, device, "a")
+    whole = len(w_shape) == 2 and not w_shape[1] & 15 and w.dtype is i8 and w.is_contiguous() and w.get_device() == device
+    wst = w_shape[1] if whole else _int8_row_stride(w, device, "w")
+    M, K = a_shape
+    N, k = w_shape
     if K != k:
         _refuse("a and w have %d and %d columns", K, k)
     if y is None:
