@@ -580,8 +580,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) product_pair_kernel(const __g
 }
 
 // Which kernel and how it divides the product.
-//  - Up to 64 rows, or groups that have half as many on the average: the kernel for few rows, which has one tile for nearly every group.  (Groups of 32 on the
-//    average, 1024 x 2048 x 2048 bf16 over 32: 48.2 us with 64 columns, 48.3 in pairs; of 64, 4096 x 2048 x 2048 over 64: 99.4 with 128 columns, 93 in pairs.)
+//  - Up to 64 rows, or groups that have half as many on the average: the kernel for few rows, which has one tile for nearly every group.  But pairs load half as many
+//    rows of a for each of w: with more than 24 rows, and tiles for three fifths of the pairs, they are the faster (K = 4096, us with few rows and in pairs: 17 x
+//    14336 13.9 and 15.1, 32 x 14336 15.1 and 13.7, 64 x 11008 13.9 and 12.3, 64 x 128256 86.9 and 83.9, 64 x 4096 8.3 and 10.5; 400 x 1024 x 2048 int8 over 16
+//    experts 13.3 and 11.5, 256 x 4096 x 4096 bf16 over 16 87 and 88).
 //  - Otherwise the least of what was measured (8-bit and 16-bit alike: a K block has as many MMA cycles), us:
 //    few rows, 128 columns: 5 + 2.2 where K is divided + 0.45 a block (128 x 4096 x 4096 11 to 12, in pairs 13);
 //    pairs, 128 rows: 5 + 0.21 to 0.24 a block (512 x 4096 x 4096 11.8, 333 x 1000 x 1234 7.3);
@@ -609,6 +611,7 @@ Plan plan_for(int sms, int M, int N, int blocks, int experts) {
         return {true, cols, (int)within(sms * 33 / 20), 2};
     };
     const int64_t rows = experts ? 2 * each : M;
+    if (rows <= 64 && rows > 24 && m_likely(128) * n_pairs * 5 >= sms / 2 * 3) return {false, 128, 1, 1};
     if (rows <= 64) return few(rows <= 16 ? 16 : rows <= 32 ? 32 : 64);
     auto rounds = [](int64_t t, int64_t places) { return (double)((t + places - 1) / places); };
     const Plan narrow = few(128);
