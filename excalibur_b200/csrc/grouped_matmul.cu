@@ -656,7 +656,8 @@ int run(exb_ctx* ctx, const char* what, ProductParams& p, const Plan& plan, cons
             if (int rc = raise_smem_limit(ctx, product_few_kernel<kKind, kCols>)) return rc;
             const int64_t places = (int64_t)ctx->sm_count * plan.each;
             const int64_t grid = plan.splits > 1 ? tiles * plan.splits : std::min(tiles, places);
-            const int room = (plan.each == 1 ? 220 : 108) * 1024 - (int)table - few_smem(kCols, 0, plan.splits > 1);
+            // (more for one CTA an SM would keep the next kernel's from starting: 1 x 14336 x 4096 with 108, 150 and 220 KB 12.4, 12.0 and 12.5 us)
+            const int room = (plan.each > 1 ? 108 : kCols == 128 ? 220 : 150) * 1024 - (int)table - few_smem(kCols, 0, plan.splits > 1);
             p.stages = std::min(kFewMostStages, room / few_stage_bytes(kCols));
             return launch_pdl_cluster(ctx, "product_few_kernel", product_few_kernel<kKind, kCols>, dim3((unsigned)grid), dim3(96 + few_epi_warps(kCols) * 32),
                                       dim3(plan.splits), (size_t)few_smem(kCols, p.stages, plan.splits > 1) + table, st, p);
