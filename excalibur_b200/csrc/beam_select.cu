@@ -5,7 +5,7 @@
 // rounding of scores, and the beams' lists are merged by a warp.  Beams that have ended or are none (a score of minus infinity) are not read.
 // The CTAs of a sentence are a cluster, whose first one has the lists in its shared memory and merges them; with more beams than a cluster has CTAs,
 // and for rows so short that a warp has one, the lists go through a workspace to a second kernel.
-// 128 x 8 rows of 131072 fp16 take 61.4 us with 8 selected (4370 GB/s; 53 without looking for candidates), 64 x 5 of 50001 bf16 19.1, 4 of 131072 fp32 9.3.  Bound by the waits
+// 128 x 8 rows of 131072 fp16 take 60.3 us with 8 selected (4450 GB/s; 53 without looking for candidates), 64 x 5 of 50001 bf16 19.1, 4 of 131072 fp32 9.3.  Bound by the waits
 // for a row's batches of logits and by its end: 29 % of the issue slots are used, 47 % of the exponentials' unit, half of the copy rate.
 #include "logit_rows.cuh"
 
@@ -326,10 +326,11 @@ extern "C" int exb_beam_select_fwd(exb_ctx* ctx, const exb_beam_desc* d, const v
     const RowPlan plan = plan_rows(ctx->sm_count, n_rows, (int64_t)V * (int64_t)es);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     int rc = EXB_OK;
-    // A cluster for a sentence saves a launch and what the second kernel waits for, but its CTAs wait for each other: with rows for several waves of CTAs, and short
-    // ones, that costs more (us, one kernel and two: 4 x 131072 fp32 9.3 and 9.4, 16 x 4 x 32000 bf16 9.4 and 11.3, 8 x 16 x 131072 fp16 with 32 selected 27.0
-    // and 32.9, 54 x 9 x 11037 fp16 15.1 and 17.5, 128 x 8 x 131072 fp16 61.6 and 66; 300 x 4 x 8000 fp16 22 and 16.5, 150 x 14 x 25884 fp32 62 and 50).
-    if (!plan.warps && beams <= kMostCtas && n_rows <= 7 * ctx->sm_count) {
+    // A cluster for a sentence saves a launch and what the second kernel waits for, but its CTAs wait for each other: with rows for more than one wave of CTAs that
+    // costs more (us, one kernel and two: 4 x 131072 fp32 9.3 and 9.4, 16 x 4 x 32000 bf16 9.7 and 11.3, 8 x 16 x 131072 fp16 with 32 selected 26.6 and 32.9, 54 x 9 x
+    // 11037 fp16 15.2 and 15.7, 64 x 8 x 131072 fp32 58 and 60; 80 x 8 x 131072 fp16 49.5 and 45.9, 100 x 8 x 50000 30.1 and 27.4, 128 x 8 x 131072 61.5 and 60.3, 60 x 16
+    // x 32000 bf16 with 32 selected 45 and 37).
+    if (!plan.warps && beams <= kMostCtas && 2 * n_rows <= 7 * ctx->sm_count) {
         SentenceArgs a = {logits, scores, ended, stride, V, top, 1, d->scale, to};
         while (a.splits < plan.splits && a.splits * 2 * beams <= kMostCtas) a.splits *= 2;
         const unsigned ctas = (unsigned)(beams * a.splits);

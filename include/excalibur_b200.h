@@ -627,7 +627,7 @@ EXB_API int exb_grouped_matmul_fwd(exb_ctx* ctx, const exb_grouped_desc* d, cons
  * minus infinity, -1 and -1.  beams and select: 1..32.
  * workspace: NULL, or workspace_bytes of device memory, 8-byte aligned, at least 8 * sentences * beams * (1 + min(select, V)); what is in it
  * before and after the call means nothing.  It is needed with more than 16 beams, for rows of up to 2048 bytes, and for more than
- * 7 rows an SM: without one such calls return EXB_ERR_NOMEM and do nothing. */
+ * 3.5 rows an SM: without one such calls return EXB_ERR_NOMEM and do nothing. */
 typedef struct exb_beam_desc {
     int64_t sentences, stride, workspace_bytes;
     int32_t beams, V;
