@@ -1136,6 +1136,12 @@ def _state_layout(state, rows, by_length):
     es = state.element_size()
     if state.dim() < (3 if by_length else 1) or state.shape[0] != rows:
         _refuse("a state has to be (%d%s)", rows, ", ..., positions, channels" if by_length else ", ...")
+    if state.is_contiguous() and state.numel():      # the usual states
+        row = state.numel() // rows * es
+        if not by_length:
+            return 1, 1, row, row, 0, 0
+        p, inner = state.shape[-2], state.shape[-1] * es
+        return row // (p * inner), p, inner, row, p * inner, inner
     dims = [(n, s * es) for n, s in zip(state.shape[1:], state.stride()[1:])]
 
     def joined(dims):

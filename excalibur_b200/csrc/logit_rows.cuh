@@ -602,7 +602,8 @@ __device__ __forceinline__ PartSeen see_part(const T* x, const Parts<T>& part, f
                 n = kRoom + 1;
             }
             if (n <= kRoom || tries) break;
-            // too many of equal value, or no bound: of so few tokens that fewer groups of threads hold any than are asked for.  The top-th largest of the threads' keys is one.  (256 x 1100 fp16 with 20 came this way with groups of 8: 15.8 us, 8.4 now.)
+            // too many of equal value, or no bound: of so few tokens that fewer groups of threads hold any than are asked for.  The top-th largest of
+            // the threads' keys is one.  (256 x 1100 fp16 with 20 came this way with groups of 8 alone: 15.8 us, 8.4 now.)
             const unsigned long long key = best_key<T>(x, part, tid, n_head, n_tail, lo + tid, hi, kThreads);
             __syncthreads();
             sh.list[tid] = key;
