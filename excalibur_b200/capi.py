@@ -1192,9 +1192,12 @@ def reorder_beams(ctx, states, parents, lengths=None):
         states = (states,)
     calls, pointers = [], []
     like = states[0] if len(states) else None
-    if like is not None and like.is_contiguous():      # the usual states: all alike, told apart by a few looks each
-        shape, dtype = like.shape, like.dtype
-        pointers = [s.data_ptr() for s in states if s.shape == shape and s.dtype is dtype and s.is_contiguous() and s.get_device() == device]
+    if like is not None:      # the usual states: all alike, told apart by a few looks each
+        shape, dtype, stride = like.shape, like.dtype, like.stride()
+        if like.is_contiguous():
+            pointers = [s.data_ptr() for s in states if s.shape == shape and s.dtype is dtype and s.is_contiguous() and s.get_device() == device]
+        else:
+            pointers = [s.data_ptr() for s in states if s.shape == shape and s.dtype is dtype and s.stride() == stride and s.get_device() == device]
     if len(pointers) == len(states) and like is not None:
         calls.append((like, pointers))
     else:

@@ -6,6 +6,7 @@
 // (41); 16 x 8 beams, 6 change, 16 states of 8 x 1024 to 2047 positions x 64 bf16, 665 (737: parents that several beams have are in L2); rows that start anywhere go
 // in units of what divides them: 2 x 5 beams, 43 channels in fp32, 75 (54), 4 x 8 beams, 37 channels in fp16, 15 (7).
 #include <algorithm>
+#include <new>
 #include <vector>
 
 #include "rows_common.cuh"
@@ -14,6 +15,7 @@ namespace exb {
 namespace {
 
 constexpr int kMaxBeams = 32;
+constexpr int kMostStates = 1 << 20;
 constexpr int kThreads = 256;
 constexpr int kStates = 128;           // of one launch
 constexpr int kSentences = 256;        // the same
@@ -153,6 +155,16 @@ bool meet(const std::vector<Dim>& dims, size_t i, int64_t bytes, int64_t d) {
     return false;
 }
 
+// Whether all of them (sorted) lie side by side within one step of the outermost dimension, as layers inside rows do: then none needs to be looked at with each
+// other one.
+bool side_by_side(const std::vector<Dim>& dims, int64_t extent, const std::vector<const uint8_t*>& at) {
+    if (dims.empty()) return false;
+    const int64_t inner = extent - (dims[0].n - 1) * dims[0].stride;
+    for (size_t i = 1; i < at.size(); ++i)
+        if (at[i] - at[i - 1] < inner) return false;
+    return at.back() - at.front() + inner <= dims[0].stride;
+}
+
 template <typename U>
 int launch(const exb_ctx* ctx, const ReorderArgs& a, int beams, cudaStream_t st) {
     const int64_t columns = a.positions * a.bytes / (int64_t)sizeof(U) * a.sentences * a.n_states * a.outer;
@@ -176,12 +188,13 @@ int launch(const exb_ctx* ctx, const ReorderArgs& a, int beams, cudaStream_t st)
 
 using namespace exb;
 
-extern "C" int exb_reorder_beams_fwd(exb_ctx* ctx, const exb_reorder_desc* d, void* const* states, const int32_t* parents, const int32_t* lengths, void* stream) {
+extern "C" int exb_reorder_beams_fwd(exb_ctx* ctx, const exb_reorder_desc* d, void* const* states, const int32_t* parents, const int32_t* lengths, void* stream) try {
     EXB_REQUIRE(ctx != nullptr && d != nullptr, "exb_reorder_beams_fwd: null context or descriptor");
     EXB_REQUIRE(d->sentences >= 0 && d->beams >= 1 && d->n_states >= 0 && d->outer >= 0 && d->positions >= 0 && d->bytes >= 0,
                 "exb_reorder_beams_fwd: bad shape (%lld x %d beams, %d states of %lld x %lld x %lld bytes)", (long long)d->sentences, d->beams, d->n_states,
                 (long long)d->outer, (long long)d->positions, (long long)d->bytes);
-    if (d->beams > kMaxBeams) return fail(EXB_ERR_UNSUPPORTED, "exb_reorder_beams_fwd: at most %d beams, got %d", kMaxBeams, d->beams);
+    if (d->beams > kMaxBeams || d->n_states > kMostStates)
+        return fail(EXB_ERR_UNSUPPORTED, "exb_reorder_beams_fwd: at most %d beams and %d states, got %d and %d", kMaxBeams, kMostStates, d->beams, d->n_states);
     if ((double)d->sentences * d->beams * (double)d->outer * (double)d->positions * (double)d->bytes > 274877906944.0)      // 256 GB
         return fail(EXB_ERR_UNSUPPORTED, "exb_reorder_beams_fwd: states are too large for one call");
     if (d->sentences == 0 || d->n_states == 0 || d->outer == 0 || d->positions == 0 || d->bytes == 0) return EXB_OK;
@@ -200,8 +213,9 @@ extern "C" int exb_reorder_beams_fwd(exb_ctx* ctx, const exb_reorder_desc* d, vo
     }
     for (const Dim& x : dims) bits |= (uintptr_t)x.stride;
     std::sort(at.begin(), at.end());
+    const bool apart = side_by_side(dims, extent, at);
     for (int i = 0; i < d->n_states; ++i) {
-        for (int j = i + 1; j < d->n_states && at[j] < at[i] + extent; ++j)
+        for (int j = i + 1; !apart && j < d->n_states && at[j] < at[i] + extent; ++j)
             EXB_REQUIRE(!meet(dims, 0, d->bytes, at[j] - at[i]), "exb_reorder_beams_fwd: two states share memory");
         auto among = [&](const void* p, int64_t n) {
             const uint8_t* b = static_cast<const uint8_t*>(p);
@@ -232,4 +246,6 @@ extern "C" int exb_reorder_beams_fwd(exb_ctx* ctx, const exb_reorder_desc* d, vo
         }
     }
     return EXB_OK;
+} catch (const std::bad_alloc&) {
+    return fail(EXB_ERR_NOMEM, "exb_reorder_beams_fwd: no memory for the list of %d states", d->n_states);
 }

@@ -644,7 +644,7 @@ EXB_API int exb_beam_select_fwd(exb_ctx* ctx, const exb_beam_desc* d, const void
  * A state is [sentences * beams][outer][positions] of `bytes` bytes, whatever their type, with strides in bytes, in any order, as long as no two share a
  * byte.  states: host array of n_states device pointers; all have the same sizes and strides, none shares memory with another; parents (int32
  * [sentences][beams]) and lengths lie outside of the memory that each spans.  16-byte aligned states, strides and sizes are moved in vectors.
- * beams: 1..32. */
+ * beams: 1..32; up to 2^20 states. */
 typedef struct exb_reorder_desc {
     int64_t sentences;
     int32_t beams, n_states;

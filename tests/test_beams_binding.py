@@ -54,7 +54,7 @@ def test_a_good_call_gets_as_far_as_the_device(call, changed):
     (select, dict(out=S), BAD), (select, dict(parents=A + 8), BAD), (select, dict(tokens=P + 4), BAD), (select, dict(workspace=A + 16), BAD), (select, dict(workspace=O), BAD),
     (select, dict(out=N), BAD),
     (reorder, dict(sentences=-1), BAD), (reorder, dict(beams=0), BAD), (reorder, dict(n_states=-1), BAD), (reorder, dict(outer=-1), BAD), (reorder, dict(bytes=-1), BAD),
-    (reorder, dict(beams=33), UNSUPPORTED), (reorder, dict(sentences=1 << 40), UNSUPPORTED),
+    (reorder, dict(beams=33), UNSUPPORTED), (reorder, dict(n_states=(1 << 20) + 1), UNSUPPORTED), (reorder, dict(sentences=1 << 40), UNSUPPORTED),
     (reorder, dict(parents=None), BAD), (reorder, dict(states=(A, None)), BAD), (reorder, dict(parents=P + 2), BAD), (reorder, dict(lengths=L + 1), BAD),
     (reorder, dict(states=(A, A)), BAD), (reorder, dict(states=(A, A + 63)), BAD), (reorder, dict(states=(A + 8 * 3 * 16 * 64 - 1, A)), BAD),
     (reorder, dict(states=(A, A + 32), row_stride=3 * 16 * 128, outer_stride=16 * 128, position_stride=128), BAD),
