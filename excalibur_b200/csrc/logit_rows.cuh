@@ -9,9 +9,9 @@
 // A thread keeps an integer e near the largest value that it has seen, so that x * scale * log2(e) - e is one multiply-add with one
 // rounding and a change of e scales its sums by a power of two, exactly.
 //
-// The most probable tokens come out of the same pass: a thread also keeps its largest logit.  The top-th largest of these (of groups
-// of 8 threads in a CTA) is a lower bound tau of the answer, and only threads whose largest is not below tau hold anything
-// that is not: about as many as tokens are asked for.  Their elements are read again (out of L2), those from tau on are put in
+// The most probable tokens come out of the same pass: a thread also keeps its largest logit.  The top-th largest of these (in a CTA of groups of 8
+// threads, or for more than kFewTop tokens of groups of 4, cut to its upper bits) is a lower bound tau of the answer, and only threads whose largest is
+// not below tau hold anything that is not: about as many as tokens are asked for.  Their elements are read again (out of L2), those from tau on are put in
 // order by counting for each how many are before it.  Logits and indexes make keys that are all different.  Where there are too many
 // elements of equal value from tau on (masks, constant rows), the threads find out where their largest is, and the same
 // is done with keys.
@@ -43,6 +43,7 @@ __device__ __forceinline__ float logit_of(unsigned long long key) {      // (not
     return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o);
 }
 __device__ __forceinline__ int index_of(unsigned long long key) { return (int)~(uint32_t)key; }
+constexpr uint32_t kFiniteOrder = 0x00800000u;      // of the lowest finite logit; the one below is minus infinity's, and what is lower still a NaN's bits
 
 __device__ __forceinline__ float exp2_fast(float t) {
     float p;
@@ -270,7 +271,7 @@ __device__ __noinline__ unsigned long long best_key(const T* x, const Parts<T>& 
 template <typename T>
 __device__ __forceinline__ void collect(const T* x, const Parts<T>& part, unsigned long long tau, int thread, int n_head, int n_tail, int first, int end, int step,
                                         int lane, int lanes, unsigned long long* list, int* n_list, int room) {
-    const float low = tau >> 32 ? logit_of(tau) : -INFINITY;
+    const float low = tau >> 32 >= kFiniteOrder ? logit_of(tau) : -INFINITY;      // (what a bound was cut to below that is no logit)
     auto offer = [&](float v, int index) {
         if (!(v >= low)) return;
         const unsigned long long k = key_of(v, index);
@@ -303,7 +304,8 @@ __device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
     return __reduce_min_sync(0xffffffffu, larger < n ? v : 0xffffffffu);
 }
 
-// A bound not above the n-th largest of 32 * kEach values: its upper 20 bits, found from the top (0 if there are fewer).  The more groups the threads' largest
+// A bound not above the n-th largest of 32 * kEach values: its upper 20 bits, found from the top (0 if there are fewer).  No logit need have that order, nor is
+// it always a number's: minus infinity's is cut to one below it (see kFiniteOrder).  Finite ones stay so.  The more groups the threads' largest
 // are divided into, the nearer their n-th largest is to that of the threads themselves: of 32 groups the 32nd is the least, and 130 threads hold something not
 // below it; of 64 or 128 groups 44 or 37 do.
 constexpr int kFewTop = 16;
