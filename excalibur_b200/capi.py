@@ -27,7 +27,7 @@ EXPORTED_SYMBOLS = [
     "exb_dequantize_fwd", "exb_concat_fwd", "exb_concat_nearest_fwd", "exb_interp_nearest_fwd", "exb_channel_affine_fwd",
     "exb_conv_weights_set_slopes", "exb_dw_weights_set_slopes", "exb_depth_to_space_nchw_f32", "exb_deconv_few_f32", "exb_image_f32_to_nhwc_norm", "exb_nchw_f32_to_nhwc4_padded_norm", "exb_nhwc_f16_split_heads_f32", "exb_hardsigmoid_fwd", "exb_softmax_channels_f32", "exb_binaryop_channel_bcast_fwd", "exb_nchw_f16_to_nhwc4_padded", "exb_nchw_f32_focus_to_nhwc_f16", "exb_channel_affine_prelu_fwd", "exb_hardswish_fwd", "exb_focus_fwd", "exb_prelu_fwd", "exb_depth_to_space_fwd", "exb_transpose_hw_f32",
     "exb_quantize_blocks_fwd", "exb_fp8_matmul_fwd", "exb_residual_norm_fwd", "exb_token_logprobs_fwd",
-    "exb_quantize_rows_fwd", "exb_int8_matmul_fwd", "exb_grouped_matmul_fwd", "exb_beam_select_fwd", "exb_reorder_beams_fwd",
+    "exb_quantize_rows_fwd", "exb_int8_matmul_fwd", "exb_grouped_matmul_fwd", "exb_beam_select_fwd", "exb_reorder_beams_fwd", "exb_reorder_beams_check",
 ]
 
 
@@ -191,6 +191,7 @@ def lib():
         L.exb_grouped_matmul_fwd.argtypes = [vp] * 10
         L.exb_beam_select_fwd.argtypes = [vp] * 10
         L.exb_reorder_beams_fwd.argtypes = [vp] * 6
+        L.exb_reorder_beams_check.argtypes = [vp, C.c_int32, vp, vp, vp]
         _LIB = L
     return _LIB
 
@@ -1212,6 +1213,10 @@ def reorder_beams(ctx, states, parents, lengths=None):
             _refuse("states of unlike layouts lie among each other")
     rows = sentences * beams
     packed = [(_pack_reorder(sentences, beams, len(at), *_state_layout(s, rows, lengths is not None)), struct.pack("%dQ" % len(at), *at)) for s, at in calls]
+    if len(packed) > 1:      # what the library would refuse of a later layout it refuses before the first one moves
+        rc = lib().exb_reorder_beams_check(b"".join(d for d, _ in packed), len(packed), (C.c_char_p * len(packed))(*[at for _, at in packed]), parents.data_ptr(), lengths_p)
+        if rc:
+            check(rc)
     for d, at in packed:
         rc = lib().exb_reorder_beams_fwd(ctx._h, d, at, parents.data_ptr(), lengths_p, _stream())
         if rc:

@@ -165,6 +165,46 @@ bool side_by_side(const std::vector<Dim>& dims, int64_t extent, const std::vecto
     return at.back() - at.front() + inner <= dims[0].stride;
 }
 
+// What can be wrong with a call.  bits: of all addresses, sizes and strides (0: there is nothing to do).
+int look_over(const char* what, const exb_reorder_desc& d, void* const* states, const int32_t* parents, const int32_t* lengths, uintptr_t& bits) {
+    bits = 0;
+    EXB_REQUIRE(d.sentences >= 0 && d.beams >= 1 && d.n_states >= 0 && d.outer >= 0 && d.positions >= 0 && d.bytes >= 0,
+                "%s: bad shape (%lld x %d beams, %d states of %lld x %lld x %lld bytes)", what, (long long)d.sentences, d.beams, d.n_states, (long long)d.outer,
+                (long long)d.positions, (long long)d.bytes);
+    if (d.beams > kMaxBeams || d.n_states > kMostStates)
+        return fail(EXB_ERR_UNSUPPORTED, "%s: at most %d beams and %d states, got %d and %d", what, kMaxBeams, kMostStates, d.beams, d.n_states);
+    if ((double)d.sentences * d.beams * (double)d.outer * (double)d.positions * (double)d.bytes > 274877906944.0)      // 256 GB
+        return fail(EXB_ERR_UNSUPPORTED, "%s: states are too large for one call", what);
+    if (d.sentences == 0 || d.n_states == 0 || d.outer == 0 || d.positions == 0 || d.bytes == 0) return EXB_OK;
+    EXB_REQUIRE(states && parents, "%s: null buffer", what);
+    EXB_REQUIRE(rows::aligned_to(parents, 4) && rows::aligned_to(lengths, 4), "%s: parents or lengths not aligned to their element", what);
+    std::vector<Dim> dims;
+    int64_t extent;
+    EXB_REQUIRE(nest(d, dims, extent), "%s: some of a state's rows lie over others", what);
+    // states that share no memory with each other, nor have parents or lengths among them
+    std::vector<const uint8_t*> at(d.n_states);
+    uintptr_t all = (uintptr_t)d.bytes;
+    for (int i = 0; i < d.n_states; ++i) {
+        EXB_REQUIRE(states[i], "%s: null state", what);
+        at[i] = static_cast<const uint8_t*>(states[i]);
+        all |= reinterpret_cast<uintptr_t>(states[i]);
+    }
+    for (const Dim& x : dims) all |= (uintptr_t)x.stride;
+    std::sort(at.begin(), at.end());
+    const bool apart = side_by_side(dims, extent, at);
+    for (int i = 0; i < d.n_states; ++i) {
+        for (int j = i + 1; !apart && j < d.n_states && at[j] < at[i] + extent; ++j)
+            EXB_REQUIRE(!meet(dims, 0, d.bytes, at[j] - at[i]), "%s: two states share memory", what);
+        auto among = [&](const void* p, int64_t n) {
+            const uint8_t* b = static_cast<const uint8_t*>(p);
+            return p && b < at[i] + extent && b + n * 4 > at[i];
+        };
+        EXB_REQUIRE(!among(parents, d.sentences * d.beams) && !among(lengths, d.sentences), "%s: parents or lengths lie among a state's rows", what);
+    }
+    bits = all;
+    return EXB_OK;
+}
+
 template <typename U>
 int launch(const exb_ctx* ctx, const ReorderArgs& a, int beams, cudaStream_t st) {
     const int64_t columns = a.positions * a.bytes / (int64_t)sizeof(U) * a.sentences * a.n_states * a.outer;
@@ -188,41 +228,22 @@ int launch(const exb_ctx* ctx, const ReorderArgs& a, int beams, cudaStream_t st)
 
 using namespace exb;
 
+extern "C" int exb_reorder_beams_check(const exb_reorder_desc* d, int32_t n, void* const* const* states, const int32_t* parents, const int32_t* lengths) try {
+    EXB_REQUIRE(n >= 0 && (n == 0 || (d && states)), "exb_reorder_beams_check: null descriptors or states");
+    for (int32_t i = 0; i < n; ++i) {
+        uintptr_t bits;
+        if (int rc = look_over("exb_reorder_beams_check", d[i], states[i], parents, lengths, bits)) return rc;
+    }
+    return EXB_OK;
+} catch (const std::bad_alloc&) {
+    return fail(EXB_ERR_NOMEM, "exb_reorder_beams_check: no memory for the list of states");
+}
+
 extern "C" int exb_reorder_beams_fwd(exb_ctx* ctx, const exb_reorder_desc* d, void* const* states, const int32_t* parents, const int32_t* lengths, void* stream) try {
     EXB_REQUIRE(ctx != nullptr && d != nullptr, "exb_reorder_beams_fwd: null context or descriptor");
-    EXB_REQUIRE(d->sentences >= 0 && d->beams >= 1 && d->n_states >= 0 && d->outer >= 0 && d->positions >= 0 && d->bytes >= 0,
-                "exb_reorder_beams_fwd: bad shape (%lld x %d beams, %d states of %lld x %lld x %lld bytes)", (long long)d->sentences, d->beams, d->n_states,
-                (long long)d->outer, (long long)d->positions, (long long)d->bytes);
-    if (d->beams > kMaxBeams || d->n_states > kMostStates)
-        return fail(EXB_ERR_UNSUPPORTED, "exb_reorder_beams_fwd: at most %d beams and %d states, got %d and %d", kMaxBeams, kMostStates, d->beams, d->n_states);
-    if ((double)d->sentences * d->beams * (double)d->outer * (double)d->positions * (double)d->bytes > 274877906944.0)      // 256 GB
-        return fail(EXB_ERR_UNSUPPORTED, "exb_reorder_beams_fwd: states are too large for one call");
-    if (d->sentences == 0 || d->n_states == 0 || d->outer == 0 || d->positions == 0 || d->bytes == 0) return EXB_OK;
-    EXB_REQUIRE(states && parents, "exb_reorder_beams_fwd: null buffer");
-    EXB_REQUIRE(rows::aligned_to(parents, 4) && rows::aligned_to(lengths, 4), "exb_reorder_beams_fwd: parents or lengths not aligned to their element");
-    std::vector<Dim> dims;
-    int64_t extent;
-    EXB_REQUIRE(nest(*d, dims, extent), "exb_reorder_beams_fwd: some of a state's rows lie over others");
-    // states that share no memory with each other, nor have parents or lengths among them
-    std::vector<const uint8_t*> at(d->n_states);
-    uintptr_t bits = (uintptr_t)d->bytes;
-    for (int i = 0; i < d->n_states; ++i) {
-        EXB_REQUIRE(states[i], "exb_reorder_beams_fwd: null state");
-        at[i] = static_cast<const uint8_t*>(states[i]);
-        bits |= reinterpret_cast<uintptr_t>(states[i]);
-    }
-    for (const Dim& x : dims) bits |= (uintptr_t)x.stride;
-    std::sort(at.begin(), at.end());
-    const bool apart = side_by_side(dims, extent, at);
-    for (int i = 0; i < d->n_states; ++i) {
-        for (int j = i + 1; !apart && j < d->n_states && at[j] < at[i] + extent; ++j)
-            EXB_REQUIRE(!meet(dims, 0, d->bytes, at[j] - at[i]), "exb_reorder_beams_fwd: two states share memory");
-        auto among = [&](const void* p, int64_t n) {
-            const uint8_t* b = static_cast<const uint8_t*>(p);
-            return p && b < at[i] + extent && b + n * 4 > at[i];
-        };
-        EXB_REQUIRE(!among(parents, d->sentences * d->beams) && !among(lengths, d->sentences), "exb_reorder_beams_fwd: parents or lengths lie among a state's rows");
-    }
+    uintptr_t bits;
+    if (int rc = look_over("exb_reorder_beams_fwd", *d, states, parents, lengths, bits)) return rc;
+    if (!bits) return EXB_OK;
     if (int rc = rows::check_device(ctx, "exb_reorder_beams_fwd")) return rc;
     ReorderArgs a;
     a.parents = parents; a.lengths = lengths;
