@@ -1208,12 +1208,9 @@ def reorder_beams(ctx, states, parents, lengths=None):
                 _refuse("a state is not on the context's device")
             same.setdefault((s.shape, s.stride(), s.element_size()), []).append(s)
         calls = [(group[0], [s.data_ptr() for s in group]) for group in same.values()]
-        spans = sorted((s.data_ptr(), s.data_ptr() + s.element_size() * (1 + sum((n - 1) * k for n, k in zip(s.shape, s.stride())))) for s in states if s.numel())
-        if len(same) > 1 and any(end > begin for (_, end), (begin, _) in zip(spans, spans[1:])):
-            _refuse("states of unlike layouts lie among each other")
     rows = sentences * beams
     packed = [(_pack_reorder(sentences, beams, len(at), *_state_layout(s, rows, lengths is not None)), struct.pack("%dQ" % len(at), *at)) for s, at in calls]
-    if len(packed) > 1:      # what the library would refuse of a later layout it refuses before the first one moves
+    if len(packed) > 1:      # what the library would refuse of a later layout, or of two together, it refuses before the first one moves
         rc = lib().exb_reorder_beams_check(b"".join(d for d, _ in packed), len(packed), (C.c_char_p * len(packed))(*[at for _, at in packed]), parents.data_ptr(), lengths_p)
         if rc:
             check(rc)

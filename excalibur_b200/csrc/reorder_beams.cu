@@ -133,75 +133,110 @@ __global__ void __launch_bounds__(kThreads) reorder_beams_kernel(const __grid_co
 struct Dim {
     int64_t n, stride;
 };
-// A state's dimensions from the outermost in, each inside one step of the next outer one; false where some lie over others.
-bool nest(const exb_reorder_desc& d, std::vector<Dim>& dims, int64_t& extent) {
-    dims.clear();
+// Sizes and strides that states of a call have, from the outermost in, each dimension inside one step of the next outer one.
+struct Layout {
+    std::vector<Dim> dims;
+    int64_t bytes, extent;      // side by side; from the first byte to behind the last
+};
+struct State {
+    const uint8_t* at;
+    int32_t layout;
+};
+// false where some rows lie over others
+bool nest(const exb_reorder_desc& d, Layout& to) {
+    to.dims.clear();
     for (const Dim& x : {Dim{d.sentences * d.beams, d.row_stride}, Dim{d.outer, d.outer_stride}, Dim{d.positions, d.position_stride}})
-        if (x.n > 1) dims.push_back(x);
-    std::sort(dims.begin(), dims.end(), [](const Dim& a, const Dim& b) { return a.stride > b.stride; });
-    extent = d.bytes;
-    for (size_t i = dims.size(); i-- > 0;) {
-        if (dims[i].stride < extent) return false;
-        extent += (dims[i].n - 1) * dims[i].stride;
+        if (x.n > 1) to.dims.push_back(x);
+    std::sort(to.dims.begin(), to.dims.end(), [](const Dim& a, const Dim& b) { return a.stride > b.stride; });
+    to.bytes = to.extent = d.bytes;
+    for (size_t i = to.dims.size(); i-- > 0;) {
+        if (to.dims[i].stride < to.extent) return false;
+        to.extent += (to.dims[i].n - 1) * to.dims[i].stride;
     }
     return true;
 }
-// Whether two states whose first bytes are `d` apart share a byte: at each dimension the step at or before the distance and the one behind it can.
-bool meet(const std::vector<Dim>& dims, size_t i, int64_t bytes, int64_t d) {
-    if (i == dims.size()) return d < bytes && -d < bytes;
-    const int64_t at = d >= 0 ? d / dims[i].stride : -((-d + dims[i].stride - 1) / dims[i].stride);
-    for (int64_t s = at; s <= at + 1; ++s)
-        if (s < dims[i].n && -s < dims[i].n && meet(dims, i + 1, bytes, d - s * dims[i].stride)) return true;
+
+// Whether two states share a byte whose first ones are `d` apart.  Steps of either are taken from the longest stride on (one that both have: as many as one is
+// ahead of the other), in every number that leaves them within reach of each other: two at most where their dimensions lie inside each other's steps.
+// Where they do not, that can be many: states that `steps` do not suffice for count as sharing memory.
+bool meet(const Layout& a, size_t i, const Layout& b, size_t j, int64_t a_extent, int64_t b_extent, int64_t d, int& steps) {
+    if (d >= a_extent || -d >= b_extent) return false;
+    if (i == a.dims.size() && j == b.dims.size()) return true;      // (the extents are the bytes)
+    if (--steps < 0) return true;
+    const bool of_a = i < a.dims.size() && (j == b.dims.size() || a.dims[i].stride >= b.dims[j].stride);
+    const bool of_b = j < b.dims.size() && (i == a.dims.size() || b.dims[j].stride >= a.dims[i].stride);
+    const int64_t stride = of_a ? a.dims[i].stride : b.dims[j].stride, n_a = of_a ? a.dims[i].n : 1, n_b = of_b ? b.dims[j].n : 1;
+    a_extent -= (n_a - 1) * stride;
+    b_extent -= (n_b - 1) * stride;
+    auto floor_of = [&](int64_t v) { return v >= 0 ? v / stride : -((-v + stride - 1) / stride); };
+    const int64_t from = std::max(-(n_b - 1), floor_of(d - a_extent) + 1), to = std::min(n_a - 1, floor_of(d + b_extent - 1));      // d - s * stride below a_extent, above -b_extent
+    for (int64_t s = from; s <= to; ++s)
+        if (meet(a, i + of_a, b, j + of_b, a_extent, b_extent, d - s * stride, steps)) return true;
     return false;
 }
+constexpr int kMostSteps = 4096;
 
-// Whether all of them (sorted) lie side by side within one step of the outermost dimension, as layers inside rows do: then none needs to be looked at with each
+// Whether all of them (sorted) lie side by side within one step of their outermost dimension, as layers inside rows do: then none needs to be looked at with each
 // other one.
-bool side_by_side(const std::vector<Dim>& dims, int64_t extent, const std::vector<const uint8_t*>& at) {
-    if (dims.empty()) return false;
-    const int64_t inner = extent - (dims[0].n - 1) * dims[0].stride;
-    for (size_t i = 1; i < at.size(); ++i)
-        if (at[i] - at[i - 1] < inner) return false;
-    return at.back() - at.front() + inner <= dims[0].stride;
+bool side_by_side(const std::vector<Layout>& layouts, const std::vector<State>& states) {
+    const Layout& first = layouts[states[0].layout];
+    if (first.dims.empty()) return false;
+    const int64_t step = first.dims[0].stride;
+    const uint8_t* end = states[0].at;
+    for (const State& s : states) {
+        const Layout& of = layouts[s.layout];
+        if (of.dims.empty() || of.dims[0].stride != step || s.at < end) return false;
+        end = s.at + of.extent - (of.dims[0].n - 1) * step;
+    }
+    return end - states[0].at <= step;
 }
 
-// What can be wrong with a call.  bits: of all addresses, sizes and strides (0: there is nothing to do).
-int look_over(const char* what, const exb_reorder_desc& d, void* const* states, const int32_t* parents, const int32_t* lengths, uintptr_t& bits) {
+// What can be wrong with n calls.  bits: of all addresses, sizes and strides (0: there is nothing to do).
+int look_over(const char* what, const exb_reorder_desc* descs, int32_t n, void* const* const* lists, const int32_t* parents, const int32_t* lengths, uintptr_t& bits) {
     bits = 0;
-    EXB_REQUIRE(d.sentences >= 0 && d.beams >= 1 && d.n_states >= 0 && d.outer >= 0 && d.positions >= 0 && d.bytes >= 0,
-                "%s: bad shape (%lld x %d beams, %d states of %lld x %lld x %lld bytes)", what, (long long)d.sentences, d.beams, d.n_states, (long long)d.outer,
-                (long long)d.positions, (long long)d.bytes);
-    if (d.beams > kMaxBeams || d.n_states > kMostStates)
-        return fail(EXB_ERR_UNSUPPORTED, "%s: at most %d beams and %d states, got %d and %d", what, kMaxBeams, kMostStates, d.beams, d.n_states);
-    if ((double)d.sentences * d.beams * (double)d.outer * (double)d.positions * (double)d.bytes > 274877906944.0)      // 256 GB
-        return fail(EXB_ERR_UNSUPPORTED, "%s: states are too large for one call", what);
-    if (d.sentences == 0 || d.n_states == 0 || d.outer == 0 || d.positions == 0 || d.bytes == 0) return EXB_OK;
-    EXB_REQUIRE(states && parents, "%s: null buffer", what);
-    EXB_REQUIRE(rows::aligned_to(parents, 4) && rows::aligned_to(lengths, 4), "%s: parents or lengths not aligned to their element", what);
-    std::vector<Dim> dims;
-    int64_t extent;
-    EXB_REQUIRE(nest(d, dims, extent), "%s: some of a state's rows lie over others", what);
-    // states that share no memory with each other, nor have parents or lengths among them
-    std::vector<const uint8_t*> at(d.n_states);
-    uintptr_t all = (uintptr_t)d.bytes;
-    for (int i = 0; i < d.n_states; ++i) {
-        EXB_REQUIRE(states[i], "%s: null state", what);
-        at[i] = static_cast<const uint8_t*>(states[i]);
-        all |= reinterpret_cast<uintptr_t>(states[i]);
+    std::vector<Layout> layouts;
+    std::vector<State> states;
+    for (int32_t k = 0; k < n; ++k) {
+        const exb_reorder_desc& d = descs[k];
+        EXB_REQUIRE(d.sentences >= 0 && d.beams >= 1 && d.n_states >= 0 && d.outer >= 0 && d.positions >= 0 && d.bytes >= 0,
+                    "%s: bad shape (%lld x %d beams, %d states of %lld x %lld x %lld bytes)", what, (long long)d.sentences, d.beams, d.n_states, (long long)d.outer,
+                    (long long)d.positions, (long long)d.bytes);
+        if (d.beams > kMaxBeams || d.n_states > kMostStates)
+            return fail(EXB_ERR_UNSUPPORTED, "%s: at most %d beams and %d states, got %d and %d", what, kMaxBeams, kMostStates, d.beams, d.n_states);
+        if ((double)d.sentences * d.beams * (double)d.outer * (double)d.positions * (double)d.bytes > 274877906944.0)      // 256 GB
+            return fail(EXB_ERR_UNSUPPORTED, "%s: states are too large for one call", what);
+        if (d.sentences == 0 || d.n_states == 0 || d.outer == 0 || d.positions == 0 || d.bytes == 0) continue;
+        EXB_REQUIRE(lists[k] && parents, "%s: null buffer", what);
+        EXB_REQUIRE(rows::aligned_to(parents, 4) && rows::aligned_to(lengths, 4), "%s: parents or lengths not aligned to their element", what);
+        Layout of;
+        EXB_REQUIRE(nest(d, of), "%s: some of a state's rows lie over others", what);
+        bits |= (uintptr_t)d.bytes;
+        for (const Dim& x : of.dims) bits |= (uintptr_t)x.stride;
+        for (int i = 0; i < d.n_states; ++i) {
+            const uint8_t* at = static_cast<const uint8_t*>(lists[k][i]);
+            EXB_REQUIRE(at, "%s: null state", what);
+            auto among = [&](const void* p, int64_t count) {
+                const uint8_t* b = static_cast<const uint8_t*>(p);
+                return p && b < at + of.extent && b + count * 4 > at;
+            };
+            EXB_REQUIRE(!among(parents, d.sentences * d.beams) && !among(lengths, d.sentences), "%s: parents or lengths lie among a state's rows", what);
+            bits |= reinterpret_cast<uintptr_t>(at);
+            states.push_back({at, (int32_t)layouts.size()});
+        }
+        layouts.push_back(std::move(of));
     }
-    for (const Dim& x : dims) all |= (uintptr_t)x.stride;
-    std::sort(at.begin(), at.end());
-    const bool apart = side_by_side(dims, extent, at);
-    for (int i = 0; i < d.n_states; ++i) {
-        for (int j = i + 1; !apart && j < d.n_states && at[j] < at[i] + extent; ++j)
-            EXB_REQUIRE(!meet(dims, 0, d.bytes, at[j] - at[i]), "%s: two states share memory", what);
-        auto among = [&](const void* p, int64_t n) {
-            const uint8_t* b = static_cast<const uint8_t*>(p);
-            return p && b < at[i] + extent && b + n * 4 > at[i];
-        };
-        EXB_REQUIRE(!among(parents, d.sentences * d.beams) && !among(lengths, d.sentences), "%s: parents or lengths lie among a state's rows", what);
+    if (states.empty()) return EXB_OK;
+    // no two share memory
+    std::sort(states.begin(), states.end(), [](const State& a, const State& b) { return a.at < b.at; });
+    if (side_by_side(layouts, states)) return EXB_OK;
+    for (size_t i = 0; i < states.size(); ++i) {
+        const Layout& a = layouts[states[i].layout];
+        for (size_t j = i + 1; j < states.size() && states[j].at < states[i].at + a.extent; ++j) {
+            const Layout& b = layouts[states[j].layout];
+            int steps = kMostSteps;
+            EXB_REQUIRE(!meet(a, 0, b, 0, a.extent, b.extent, states[j].at - states[i].at, steps), "%s: two states share memory", what);
+        }
     }
-    bits = all;
     return EXB_OK;
 }
 
@@ -230,11 +265,8 @@ using namespace exb;
 
 extern "C" int exb_reorder_beams_check(const exb_reorder_desc* d, int32_t n, void* const* const* states, const int32_t* parents, const int32_t* lengths) try {
     EXB_REQUIRE(n >= 0 && (n == 0 || (d && states)), "exb_reorder_beams_check: null descriptors or states");
-    for (int32_t i = 0; i < n; ++i) {
-        uintptr_t bits;
-        if (int rc = look_over("exb_reorder_beams_check", d[i], states[i], parents, lengths, bits)) return rc;
-    }
-    return EXB_OK;
+    uintptr_t bits;
+    return look_over("exb_reorder_beams_check", d, n, states, parents, lengths, bits);
 } catch (const std::bad_alloc&) {
     return fail(EXB_ERR_NOMEM, "exb_reorder_beams_check: no memory for the list of states");
 }
@@ -242,7 +274,7 @@ extern "C" int exb_reorder_beams_check(const exb_reorder_desc* d, int32_t n, voi
 extern "C" int exb_reorder_beams_fwd(exb_ctx* ctx, const exb_reorder_desc* d, void* const* states, const int32_t* parents, const int32_t* lengths, void* stream) try {
     EXB_REQUIRE(ctx != nullptr && d != nullptr, "exb_reorder_beams_fwd: null context or descriptor");
     uintptr_t bits;
-    if (int rc = look_over("exb_reorder_beams_fwd", *d, states, parents, lengths, bits)) return rc;
+    if (int rc = look_over("exb_reorder_beams_fwd", d, 1, &states, parents, lengths, bits)) return rc;
     if (!bits) return EXB_OK;
     if (int rc = rows::check_device(ctx, "exb_reorder_beams_fwd")) return rc;
     ReorderArgs a;

@@ -654,7 +654,9 @@ typedef struct exb_reorder_desc {
 EXB_API int exb_reorder_beams_fwd(exb_ctx* ctx, const exb_reorder_desc* d, void* const* states, const int32_t* parents,
                                   const int32_t* lengths, void* stream);
 /* Whether exb_reorder_beams_fwd would refuse one of n calls for what it is given, asked before the first of them moves anything (states of several layouts are moved by
- * a call each): n descriptors, and for each the array of its states.  Reads no device memory and needs no device. */
+ * a call each), and whether a state of one of them shares memory with one of another: n descriptors, and for each the array of its states.  States
+ * of unlike layouts may lie among each other (keys beside wider values); where finding out takes thousands of steps they count as sharing memory.  Reads no
+ * device memory and needs no device. */
 EXB_API int exb_reorder_beams_check(const exb_reorder_desc* d, int32_t n, void* const* const* states, const int32_t* parents,
                                     const int32_t* lengths);
 
