@@ -93,3 +93,46 @@ def test_selection_from_short_masked_rows(ctx, dtype, V, beams, select):
     sure = gap & torch.cat([torch.ones_like(gap[:, :1]), gap[:, :-1]], 1) & ~none
     assert sure.float().mean() > 0.5 * (~none).float().mean()
     assert torch.equal((parents.long() * V + tokens.long())[sure], at[:, :select][sure])
+
+
+def _sure(scores, parents, near, select):
+    """The places that have to hold the reference's very candidate: the next score is further away than twice what sums may be off, or all that lie within that are one
+    beam's, whose order is that of its logits."""
+    sure, first = [False] * select, 0
+    for i in range(1, len(scores) + 1):
+        if i == len(scores) or scores[i - 1] - scores[i] > 2 * near:
+            whole = i < len(scores) and len(set(parents[first:i])) == 1
+            for k in range(first, min(i, select)):
+                sure[k] = whole
+            first = i
+    return sure
+
+
+@pytest.mark.parametrize("sentences,beams,V,select", [(1, 1, 50001, 32), (1, 4, 131072, 8), (1, 8, 262144, 16), (64, 5, 50001, 10), (2, 16, 131072, 32), (4, 32, 50000, 32),
+                                                      (40, 8, 131072, 8), (300, 4, 2050, 20), (500, 4, 8000, 17), (700, 3, 1000, 32)])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+def test_selection_is_the_references_where_scores_are_apart(ctx, sentences, beams, V, select, dtype):
+    """Scores within what sums and roundings may be off (4e-5 at 131072 tokens), and the reference's own candidates in its order."""
+    import torch
+    from excalibur_b200 import capi
+    g = _gen(V + select)
+    x = (torch.randn((sentences * beams, V), device="cuda", generator=g) * 2.5).to(getattr(torch, dtype))
+    scores = -3 * torch.rand((sentences, beams), device="cuda", generator=g)
+    got = capi.beam_select(ctx, x, scores, select)
+    ctx.sync_check()
+    more = select + 24
+    rows = []
+    for r in range(0, sentences * beams, 64):      # (the rows' best `more` are all that can be among a sentence's)
+        z = x[r:r + 64].double()
+        best, at = z.sort(dim=1, descending=True, stable=True)
+        rows.append((best[:, :more] - torch.logsumexp(z, 1, keepdim=True), at[:, :more]))
+    each, at = (torch.cat([row[k] for row in rows]).view(sentences, beams * more) for k in (0, 1))
+    each = each + scores.double().repeat_interleave(more, 1)
+    best, order = each.sort(dim=1, descending=True, stable=True)
+    best, order = best[:, :more], order[:, :more]
+    parents, tokens = order // more, at.gather(1, order)
+    near = float(_near(V, torch.zeros(())))
+    assert ((got[0].double() - best[:, :select]).abs() <= near + best[:, :select].abs() * 2.0 ** -21).all()
+    sure = torch.tensor([_sure(s, p, near + 2.0 ** -21 * abs(s[-1]), select) for s, p in zip(best.tolist(), parents.tolist())], device="cuda")
+    assert sure.float().mean() > 0.5
+    assert torch.equal(got[1][sure].long(), parents[:, :select][sure]) and torch.equal(got[2][sure].long(), tokens[:, :select][sure])
