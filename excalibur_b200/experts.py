@@ -40,4 +40,4 @@ class Experts:
         y = self._product(h, self.down, ends, capi.EXB_F32)
         each = torch.empty_like(y)
         each[order] = y
-        return (each.view(rows, k, -1) * gates.float()[..., None]).sum(1).to(x.dtype)
+        return (each.view(rows, k, y.shape[1]) * gates.float()[..., None]).sum(1).to(x.dtype)
