@@ -28,10 +28,11 @@ class BeamSearch:
         capi.reorder_beams takes them).  Returns the chosen tokens, (sentences * beams,) int32, -1 where there is no beam (its score is minus infinity)."""
         if self.length == self.tokens.shape[1]:
             raise ValueError("there is room for %d tokens" % self.length)
-        self.scores, parents, chosen = capi.beam_select(self.ctx, logits, self.scores, scale=self.scale, ended=self.ended, end_token=self.end_token)
-        capi.reorder_beams(self.ctx, self.tokens, parents)
-        if len(states):
+        scores, parents, chosen = capi.beam_select(self.ctx, logits, self.scores, scale=self.scale, ended=self.ended, end_token=self.end_token)
+        if len(states):      # (the caller's first: where they are refused, nothing has changed)
             capi.reorder_beams(self.ctx, states, parents, lengths)
+        capi.reorder_beams(self.ctx, self.tokens, parents)
+        self.scores = scores
         self.tokens[:, self.length] = chosen.view(-1)
         self.length += 1
         self.ended = chosen == self.end_token      # (a beam that had ended goes on with that token)
