@@ -5,7 +5,7 @@
 // rounding of scores, and the beams' lists are merged by a warp.  Beams that have ended or are none (a score of minus infinity) are not read.
 // The CTAs of a sentence are a cluster, whose first one has the lists in its shared memory and merges them; with more beams than a cluster has CTAs,
 // and for rows so short that a warp has one, the lists go through a workspace to a second kernel.
-// 128 x 8 rows of 131072 fp16 take 60.3 us with 8 selected (4450 GB/s; 53 without looking for candidates), 64 x 5 of 50001 bf16 19.1, 4 of 131072 fp32 9.3.  Bound by the waits
+// 128 x 8 rows of 131072 fp16 take 58.8 us with 8 selected (4570 GB/s; 53 without looking for candidates), 64 x 5 of 50001 bf16 18.8, 4 of 131072 fp32 9.4.  Bound by the waits
 // for a row's batches of logits and by its end: 31 % of the issue slots are used, 50 % of the exponentials' unit, two thirds of the copy rate.
 #include <algorithm>
 
