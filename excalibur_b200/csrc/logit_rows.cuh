@@ -9,9 +9,9 @@
 // A thread keeps an integer e near the largest value that it has seen, so that x * scale * log2(e) - e is one multiply-add with one
 // rounding and a change of e scales its sums by a power of two, exactly.
 //
-// The most probable tokens come out of the same pass: a thread also keeps its largest logit.  The top-th largest of these (in a CTA of groups of 8
-// threads, or for more than kFewTop tokens of groups of 4, cut to its upper bits) is a lower bound tau of the answer, and only threads whose largest is
-// not below tau hold anything that is not: about as many as tokens are asked for.  Their elements are read again (out of L2), those from tau on are put in
+// The most probable tokens come out of the same pass: a thread also keeps its largest logit.  The top-th largest of these (in a CTA of 32 groups' of threads, for
+// more than kFewTop tokens of 64 groups') is a lower bound tau of the answer, and only threads whose largest is not below tau hold anything that is
+// not: about as many as tokens are asked for.  Their elements are read again (out of L2), those from tau on are put in
 // order by counting for each how many are before it.  Logits and indexes make keys that are all different.  Where there are too many
 // elements of equal value from tau on (masks, constant rows), the threads find out where their largest is, and the same
 // is done with keys.
@@ -43,7 +43,6 @@ __device__ __forceinline__ float logit_of(unsigned long long key) {      // (not
     return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o);
 }
 __device__ __forceinline__ int index_of(unsigned long long key) { return (int)~(uint32_t)key; }
-constexpr uint32_t kFiniteOrder = 0x00800000u;      // of the lowest finite logit; the one below is minus infinity's, and what is lower still a NaN's bits
 
 __device__ __forceinline__ float exp2_fast(float t) {
     float p;
@@ -273,7 +272,7 @@ __device__ __forceinline__ unsigned long long best_key(const T* x, const Parts<T
 template <typename T>
 __device__ __forceinline__ void collect(const T* x, const Parts<T>& part, unsigned long long tau, int thread, int n_head, int n_tail, int first, int end, int step,
                                         int lane, int lanes, unsigned long long* list, int* n_list, int room) {
-    const float low = tau >> 32 >= kFiniteOrder ? logit_of(tau) : -INFINITY;      // (what a bound was cut to below that is no logit)
+    const float low = tau >> 32 ? logit_of(tau) : -INFINITY;      // (a bound's upper half is 0 or a logit's)
     auto offer = [&](float v, int index) {
         if (!(v >= low)) return;
         const unsigned long long k = key_of(v, index);
@@ -306,27 +305,19 @@ __device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
     return __reduce_min_sync(0xffffffffu, larger < n ? v : 0xffffffffu);
 }
 
-// A bound not above the n-th largest of 32 * kEach values: its upper 20 bits, found from the top (0 if there are fewer).  No logit need have that order, nor is
-// it always a number's: minus infinity's is cut to one below it (see kFiniteOrder).  Finite ones stay so.  The more groups the threads' largest
-// are divided into, the nearer their n-th largest is to that of the threads themselves: of 32 groups the 32nd is the least, and 130 threads hold something not
-// below it; of 64 or 128 groups 44 or 37 do.
+// The same of 64 values, two a lane.  The more groups the threads' largest are divided into, the nearer their n-th largest is to that of the threads themselves: of
+// 32 groups the 32nd is the least, and 130 threads hold something not below it; of 64 44 do.  (Of 128, found bit by bit from the top, 37 do, but that takes longer:
+// one row of 131072 fp32 with 20 7.8 us, 7.1 this way.)
 constexpr int kFewTop = 16;
-template <int kEach>
-__device__ __forceinline__ uint32_t least_of_groups(const uint32_t* values, int n, int lane) {
-    uint32_t v[kEach], low = 0;
+__device__ __forceinline__ uint32_t nth_largest(uint32_t v, uint32_t w, int n) {
+    int above_v = w > v, above_w = v > w;
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) v[k] = values[k * 32 + lane];
-#pragma unroll 1
-    for (int bit = 30; bit >= 12; bit -= 2) {      // two bits at a step (one row of 131072 fp32 with 20: 7.8 us bit by bit, 7.7)
-        int above[3] = {0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < kEach; ++k)
-#pragma unroll
-            for (int j = 0; j < 3; ++j) above[j] += v[k] >= (low | (uint32_t)(j + 1) << bit);
-        const int a1 = (int)__reduce_add_sync(0xffffffffu, above[0]), a2 = (int)__reduce_add_sync(0xffffffffu, above[1]), a3 = (int)__reduce_add_sync(0xffffffffu, above[2]);
-        low |= (uint32_t)((a1 >= n) + (a2 >= n) + (a3 >= n)) << bit;
+    for (int j = 1; j < 32; ++j) {
+        const uint32_t x = __shfl_xor_sync(0xffffffffu, v, j), y = __shfl_xor_sync(0xffffffffu, w, j);
+        above_v += (x > v) + (y > v);
+        above_w += (x > w) + (y > w);
     }
-    return low;
+    return __reduce_min_sync(0xffffffffu, min(above_v < n ? v : 0xffffffffu, above_w < n ? w : 0xffffffffu));
 }
 
 // How many of n keys are before (above) one.
@@ -346,7 +337,7 @@ struct Shared {
     Sums part[kThreads / 32];
     Sums row[kSplitMax];                                   // (of the cluster's CTAs, in the first one)
     unsigned long long best[kSplitMax * kMaxTop];         // the same: the `top` best of each, in order
-    uint32_t largest[kThreads / 4];                        // of 8 or 4 threads each
+    uint32_t largest[64];                                  // of groups of threads
     unsigned long long list[kRoom > kThreads ? kRoom : kThreads];
     int threads[kThreads];
     unsigned long long tau;
@@ -562,14 +553,15 @@ __device__ __forceinline__ PartSeen see_part(const T* x, const Parts<T>& part, f
     if (lane == 0) sh.part[warp] = all;
     const bool any = tid < n_head || lo + tid < hi || tid < n_tail;
     const uint32_t mine = any ? order_of(seen.r.m) : 0;
-    if (top) {      // of 8 threads each, or of 4 where many tokens are asked for (see least_of_groups)
+    constexpr int kSmall = kThreads / 64;      // threads of a group where many tokens are asked for; otherwise 8
+    if (top) {
         uint32_t g = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
         g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
-        if (top > kFewTop) {
+        if (kSmall == 8 || top <= kFewTop) g = max(g, __shfl_xor_sync(0xffffffffu, g, 4));
+        if (kSmall == 4 && top > kFewTop) {
             if ((lane & 3) == 0) sh.largest[tid >> 2] = g;
-        } else {
-            g = max(g, __shfl_xor_sync(0xffffffffu, g, 4));
-            if ((lane & 7) == 0) sh.largest[tid >> 3] = g;
+        } else if ((lane & 7) == 0) {
+            sh.largest[tid >> 3] = g;
         }
     }
     ready();
@@ -578,11 +570,10 @@ __device__ __forceinline__ PartSeen see_part(const T* x, const Parts<T>& part, f
     int n_best = 0;
     if (top) {
         if (warp == 0) {      // (with 64 groups a lane has the larger of two: the bound is lower, and serves all the same)
-            uint32_t g;
+            uint32_t g = sh.largest[lane];
             if (top > kFewTop) {
-                g = least_of_groups<kThreads / 128>(sh.largest, top, lane);
+                g = nth_largest(g, sh.largest[lane + 32], top);
             } else {
-                g = sh.largest[lane];
                 if constexpr (kThreads == kWide) g = max(g, sh.largest[lane + 32]);
                 g = nth_largest(g, top);
             }
@@ -609,7 +600,7 @@ __device__ __forceinline__ PartSeen see_part(const T* x, const Parts<T>& part, f
             }
             if (n <= kRoom || tries) break;
             // too many of equal value, or no bound: of so few tokens that fewer groups of threads hold any than are asked for.  The top-th largest of
-            // the threads' keys is one.  (256 x 1100 fp16 with 20 came this way with groups of 8 alone: 15.8 us, 8.4 now.)
+            // the threads' keys is one.  (256 x 1100 fp16 with 20 came this way with groups of 8 alone: 15.4 us, 7.9 now.)
             const unsigned long long key = best_key<T>(x, part, tid, n_head, n_tail, lo + tid, hi, kThreads);
             __syncthreads();
             sh.list[tid] = key;
