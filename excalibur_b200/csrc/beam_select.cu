@@ -5,7 +5,7 @@
 // rounding of scores, and the beams' lists are merged by a warp.  Beams that have ended or are none (a score of minus infinity) are not read.
 // The CTAs of a sentence are a cluster, whose first one has the lists in its shared memory and merges them; with more beams than a cluster has CTAs,
 // and for rows so short that a warp has one, the lists go through a workspace to a second kernel.
-// 128 x 8 rows of 131072 fp16 take 58.8 us with 8 selected (4570 GB/s; 53 without looking for candidates), 64 x 5 of 50001 bf16 18.8, 4 of 131072 fp32 9.4.  Bound by the waits
+// 128 x 8 rows of 131072 fp16 take 58.8 us with 8 selected (4570 GB/s), 64 x 5 of 50001 bf16 18.8, 4 of 131072 fp32 9.4.  Bound by the waits
 // for a row's batches of logits and by its end: 31 % of the issue slots are used, 50 % of the exponentials' unit, two thirds of the copy rate.
 #include <algorithm>
 
@@ -334,7 +334,7 @@ extern "C" int exb_beam_select_fwd(exb_ctx* ctx, const exb_beam_desc* d, const v
     // x 32000 bf16 with 32 selected 45 and 37).
     // Few rows with many beams have fewer and longer parts in a cluster: 100 KB more in each cost about what the second kernel does (rows of 524 KB,
     // 131072 fp32, in one kernel and in two: 4 beams 131 and 66 KB 9.2 and 10.1, 5 beams 175 and 66 KB 10.8 and 10.7, 8 beams 262 and 66 KB 13.8 and 12.9, 10 beams 524
-    // and 66 KB 19.8 and 16.0), on the device; a call of two kernels is 4 us longer.
+    // and 66 KB 19.8 and 16.0), on the device.  60 KB more are allowed for: a call of two kernels takes the host 4 us longer, though not one that has been captured.
     const int64_t bytes = (int64_t)V * (int64_t)es;
     const int parts = std::min(plan.splits, std::max(1, kMostCtas / beams));
     if (!plan.warps && beams <= kMostCtas && 2 * n_rows <= 7 * ctx->sm_count && bytes / parts - bytes / plan.splits <= 160000) {

@@ -361,8 +361,8 @@ __global__ void __launch_bounds__(96 + few_epi_warps(kCols) * 32, kCols == 128 ?
 
 // ---- CTA pairs ---------------------------------------------------------------------------------
 // Tiles of 256 rows of w by up to kWide rows of a by pairs of CTAs, persistent, with the operands' roles exchanged here too: the MMA's columns are as many as the
-// tile has rows of a, in whole 32s, so that groups of any size cost what they need (256 rows of a as the MMA's rows took 704 us for 8192 x 14336 x 4096 bf16
-// over 8 experts, this takes 657); an expert's rows are divided evenly between its tiles.  Each CTA keeps 128 rows of w and half of a's rows of a stage.
+// tile has rows of a, in whole 32s, so that groups of any size cost the MMAs that they need (256 rows of a as the MMA's rows took 704 us for 8192 x 14336 x 4096 bf16
+// over 8 experts, this takes 657); their loads are kWide / 2 rows of a for each CTA whatever the tile has.  An expert's rows are divided evenly between its tiles.  Each CTA keeps 128 rows of w and half of a's rows of a stage.
 // TMEM holds two accumulators: the epilogue warps read one out, scale and store it while the MMAs fill the other.  A thread has a channel of all rows, and a
 // warp stores 32 neighbours of a row at a time.
 // 8 bits: 8192^3 takes 334 us from a cool GPU (3290 TOP/s; 390 when repeated for seconds, where the power limit sets the clock), 4096^3 49, of which the tensor pipe is

@@ -243,8 +243,8 @@ int look_over(const char* what, const exb_reorder_desc* descs, int32_t n, void* 
 template <typename U>
 int launch(const exb_ctx* ctx, const ReorderArgs& a, int beams, cudaStream_t st) {
     const int64_t columns = a.positions * a.bytes / (int64_t)sizeof(U) * a.sentences * a.n_states * a.outer;
-    // Four CTAs an SM (64 states with 2 of 4 beams changed, 4, 6, 8 and 16: 42.1, 46.6, 43.8, 48.7 us).  Values on their way are registers: with 16 bytes each, four
-    // columns of up to 4 beams, two of 8, one of more; smaller units take more columns (43 channels in fp32, 1, 2, 4 and 8 columns: 231, 98, 105, 78 us).
+    // A grid of four CTAs an SM (64 states with 2 of 4 beams changed, 4, 6, 8 and 16: 42.1, 46.6, 43.8, 48.7 us), of which their 90 to 194 registers a thread let two, or one,
+    // be there at a time.  Values on their way are registers: with 16 bytes each, four columns of up to 4 beams, two of 8, one of more; smaller units take more columns (43 channels in fp32, 1, 2, 4 and 8 columns: 231, 98, 105, 78 us).
     auto go = [&](auto kernel, int each) {
         const int64_t chunks = std::max<int64_t>(1, (columns + each - 1) / each + (int64_t)a.sentences * a.n_states * a.outer);      // at most
         const int64_t grid = std::min<int64_t>(chunks, (int64_t)ctx->sm_count * 4);

@@ -586,7 +586,8 @@ EXB_API int exb_quantize_rows_fwd(exb_ctx* ctx, const exb_rows_desc* d, const vo
  *   y[m][n] = (a_scales[m] * w_scales[n]) * sum_k a[m][k] * w[n][k]  (+ bias[n])
  * a: [M][K], w: [N][K], 8-bit integers (-128 to 127), 16-byte aligned, strides multiples of 16 and >= K (what lies between K and the stride is not
  * read); a_scales: fp32 [M], w_scales: fp32 [N]; bias: fp32 [N] or NULL; y: [M][N] in EXB_F16, EXB_BF16 or EXB_F32.  The sum is
- * an int32, exact (K up to 131071); it and the product of the scales are rounded to fp32 before they are multiplied. */
+ * an int32, exact (K up to 131071); it and the product of the scales are rounded to fp32 before they are multiplied: where fp32 holds no number as large as that
+ * product, results are infinite, or NaN where the sum is 0, and where it is subnormal they have its precision. */
 typedef struct exb_int8_desc {
     int64_t M;
     int32_t N, K;
@@ -599,7 +600,7 @@ EXB_API int exb_int8_matmul_fwd(exb_ctx* ctx, const exb_int8_desc* d, const int8
 
 /* Products grouped by expert: a's rows are sorted by expert, expert e's end before row ends[e] (int32 [experts], on the device):
  *   y[m][n] = sum_k a[m][k] * w[e][n][k]  (+ bias[e][n]),   ends[e - 1] <= m < ends[e]  (ends[-1] = 0)
- * in dtype EXB_F16 or EXB_BF16 (fp32 sums, no scales: NULL), or EXB_I8 with a_scales [M] and w_scales [experts][N] as exb_int8_matmul_fwd.
+ * in dtype EXB_F16 or EXB_BF16 (fp32 sums, no scales: NULL), or EXB_I8 with a_scales [M] and w_scales [experts][N], multiplied as exb_int8_matmul_fwd does.
  * a: [M][K], w: [experts][N][K], rows and experts (expert_stride elements apart) 16-byte aligned; bias: fp32 [experts][N] or NULL; y: [M][N] in y_dtype.
  * Experts may be without rows; their weights are not read.  Rows of y from the last end on are left as they were.  ends should not fall and
  * not exceed M: one below those before it counts as theirs, one above M as M.  Up to 1024 experts.  With several experts
