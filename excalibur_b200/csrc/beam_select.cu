@@ -6,7 +6,7 @@
 // The CTAs of a sentence are a cluster, whose first one has the lists in its shared memory and merges them; with more beams than a cluster has CTAs,
 // and for rows so short that a warp has one, the lists go through a workspace to a second kernel.
 // 128 x 8 rows of 131072 fp16 take 58.8 us with 8 selected (4570 GB/s), 64 x 5 of 50001 bf16 18.8, 4 of 131072 fp32 9.4.  Bound by the waits
-// for a row's batches of logits and by its end: 31 % of the issue slots are used, 50 % of the exponentials' unit, two thirds of the copy rate.
+// for a row's batches of logits and by its end: 39 % of the issue slots are used, 64 % of the exponentials' unit, 70 % of the copy rate.
 #include <algorithm>
 
 #include "logit_rows.cuh"
@@ -331,7 +331,7 @@ extern "C" int exb_beam_select_fwd(exb_ctx* ctx, const exb_beam_desc* d, const v
     // A cluster for a sentence saves a launch and what the second kernel waits for, but its CTAs wait for each other: with rows for more than one wave of CTAs that
     // costs more (us, one kernel and two: 4 x 131072 fp32 9.3 and 9.4, 16 x 4 x 32000 bf16 9.7 and 11.3, 8 x 16 x 131072 fp16 with 32 selected 26.6 and 32.9, 54 x 9 x
     // 11037 fp16 15.2 and 15.7, 64 x 8 x 131072 fp32 58 and 60; 80 x 8 x 131072 fp16 49.5 and 45.9, 100 x 8 x 50000 30.1 and 27.4, 128 x 8 x 131072 61.5 and 60.3, 60 x 16
-    // x 32000 bf16 with 32 selected 45 and 37).
+    // x 32000 bf16 with 32 selected 45 and 37; since a row's second look is in place both take 1 to 3 % less).
     // Few rows with many beams have fewer and longer parts in a cluster: 100 KB more in each cost about what the second kernel does (rows of 524 KB,
     // 131072 fp32, in one kernel and in two: 4 beams 131 and 66 KB 9.2 and 10.1, 5 beams 175 and 66 KB 10.8 and 10.7, 8 beams 262 and 66 KB 13.8 and 12.9, 10 beams 524
     // and 66 KB 19.8 and 16.0), on the device.  60 KB more are allowed for: a call of two kernels takes the host 4 us longer, though not one that has been captured.

@@ -2,7 +2,7 @@
 //
 // z = scale * x, p = exp(z - lse), lse = log sum exp z.  With any e, t = x * scale * log2(e) - e, s = sum 2^t, w = sum 2^t * t:
 //   log p(v) = ln 2 * (t_v - log2 s),  entropy = ln 2 * (log2 s - w / s).
-// One pass over the row, bound by its reading and, in 16 bits, by the latency of its loads (46 to 49 % of the issue slots are used, 40 to
+// One pass over the row, bound by its reading and, in 16 bits, by the latency of its loads (50 % of the issue slots are used, 40 to
 // 46 % of the warps' stalls are waits for logits, and a CTA's loads drain at its row's end): 2048 rows of 50001 fp16 take 42.4 us with the
 // top 5 (4830 GB/s), 37.0 without, 49.6 with 20; 1024 rows of 50000 fp32 without 33.5 (6110 GB/s); one row of 131072 fp32 with 20 7.1.
 #include "logit_rows.cuh"
