@@ -625,7 +625,7 @@ EXB_API int exb_grouped_matmul_fwd(exb_ctx* ctx, const exb_grouped_desc* d, cons
  * a token; neither is selected.  Rows of ended beams and of those that are none are not read.  A row with a NaN or plus infinity has NaN scores; NaN come before
  * all others (and a beam's NaN logits before its other ones).
  * Results, each [sentences][select]: out_scores fp32, parents (the beam, 0..beams) and tokens int32; where fewer than `select` are left,
- * minus infinity, -1 and -1.  beams and select: 1..32.
+ * minus infinity, -1 and -1.  A score below what fp32 holds is minus infinity too, beside its parent and token.  beams and select: 1..32.
  * workspace: NULL, or workspace_bytes of device memory, 8-byte aligned, at least 8 * sentences * beams * (1 + min(select, V)); what is in it
  * before and after the call means nothing.  Some calls need it (more than 16 beams, rows of up to 2048 bytes, more than 3.5 rows an SM, many beams of few long
  * rows): without one these return EXB_ERR_NOMEM and do nothing. */
